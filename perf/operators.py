@@ -119,11 +119,11 @@ def _codes(x, store, dtype):
     """(codes, exponent bytes) of rows of fp32 values [..., D]."""
     amax = x.abs().amax(-1)
     m, e = torch.frexp(amax / TOP[store])                    # amax / top = m * 2^e, m in [0.5, 1)
-    e = torch.where(m == 0.5, e - 1, e).clamp(-126, 127)     # the smallest with top * 2^e >= amax; exact: see below
+    e = torch.where(m == 0.5, e - 1, e).clamp(-96, 127)     # the smallest with top * 2^e >= amax; exact: see below
     # frexp of a rounded quotient may sit one off at the border: settled by comparing in 64 bits
     two = _two(e)
     e = torch.where(TOP[store] * two < amax.double(), e + 1, e)
-    e = torch.where((TOP[store] * two * 0.5 >= amax.double()) & (e > -126), e - 1, e)
+    e = torch.where((TOP[store] * two * 0.5 >= amax.double()) & (e > -96), e - 1, e)
     e = torch.where(amax == 0, torch.zeros_like(e), e)
     y = x.clamp(-MOST[store, dtype], MOST[store, dtype]).double() * _two(-e)[..., None]
     codes = y.round().to(torch.int8) if store == "int8" else y.float().to(torch.float8_e4m3fn)
@@ -305,9 +305,9 @@ def work(case):
 def _exact_codes(x, store, dtype):
     """64 bits: what the rows [..., D] stand for once stored."""
     amax = x.abs().amax(-1, keepdim=True)
-    e = torch.ceil(torch.log2(amax.clamp(min=1e-300) / TOP[store])).clamp(-126, 127)
+    e = torch.ceil(torch.log2(amax.clamp(min=1e-300) / TOP[store])).clamp(-96, 127)
     for d in (1, -1):                                         # log2 is rounded: the neighbours decide
-        near = (e + d).clamp(-126, 127)
+        near = (e + d).clamp(-96, 127)
         e = torch.where((TOP[store] * _two(near) >= amax) & ((near < e) | (TOP[store] * _two(e) < amax)), near, e)
     e = torch.where(amax == 0, torch.zeros_like(e), e)
     y = x.clamp(-MOST[store, dtype], MOST[store, dtype]) / _two(e)
