@@ -27,7 +27,12 @@ SYMBOLS = (
     "moba_attend", "moba_merge", "moba_attend_tile_rows", "moba_attend_tile_rows_for", "moba_problem_tile_rows", "moba_problem_attend_kernel", "moba_route_static",
     "moba_backward_workspace_size", "moba_backward",
     "moba_cp_workspace_size", "moba_cp_forward", "moba_cp_poll", "moba_cp_abort", "moba_selftest_bounded_wait",
+    "moba_paged_check", "moba_paged_store", "moba_paged_load", "moba_paged_workspace_size", "moba_paged_attention",
 )
+
+#: MOBA_DTYPE_*, MOBA_STORE_*
+DTYPE_BF16, DTYPE_FP16 = 0, 1
+STORE_SAME, STORE_E4M3, STORE_INT8 = range(3)
 
 
 class Problem(C.Structure):
@@ -42,6 +47,21 @@ class Problem(C.Structure):
         ("o_stride_token", C.c_int64), ("o_stride_head", C.c_int64),
         ("q_token_begin", C.c_int64), ("q_tokens", C.c_int64),
         ("dtype", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
+class Paged(C.Structure):
+    """struct moba_paged"""
+    _fields_ = [
+        ("total_tokens", C.c_int64),
+        ("batch", C.c_int32), ("num_q_heads", C.c_int32), ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("num_pages", C.c_int32), ("page_size", C.c_int32), ("pages_per_seq", C.c_int32), ("max_new", C.c_int32),
+        ("dtype", C.c_int32), ("store", C.c_int32), ("softmax_scale", C.c_float), ("reserved", C.c_int32),
+        ("q_stride_token", C.c_int64), ("q_stride_head", C.c_int64), ("o_stride_token", C.c_int64), ("o_stride_head", C.c_int64),
+        ("k_stride_token", C.c_int64), ("k_stride_head", C.c_int64), ("v_stride_token", C.c_int64), ("v_stride_head", C.c_int64),
+        ("k_page_stride", C.c_int64), ("k_page_token", C.c_int64), ("k_page_head", C.c_int64),
+        ("v_page_stride", C.c_int64), ("v_page_token", C.c_int64), ("v_page_head", C.c_int64),
+        ("table_stride", C.c_int64),
     ]
 
 
@@ -106,6 +126,12 @@ def lib() -> C.CDLL:
         handle.moba_cp_poll.argtypes = [vp, C.POINTER(C.c_int32)]
         handle.moba_cp_abort.argtypes = [vp]
         handle.moba_selftest_bounded_wait.argtypes = [i32p, C.c_uint32, vp]
+        pg = C.POINTER(Paged)
+        handle.moba_paged_check.argtypes = [pg]
+        handle.moba_paged_store.argtypes = [pg, vp, vp, i32p, i32p, i32p, vp, vp, vp, vp, vp]
+        handle.moba_paged_load.argtypes = [pg, i32p, i32p, i32p, vp, vp, vp, vp, vp, vp, vp]
+        handle.moba_paged_workspace_size.argtypes = [pg, C.POINTER(sz)]
+        handle.moba_paged_attention.argtypes = [pg, vp, i32p, i32p, i32p, vp, vp, vp, vp, vp, vp, vp, sz, vp]
         _lib = handle
     return _lib
 

@@ -1,0 +1,630 @@
+// Attention over pages for sequences with few new tokens (decode steps, drafted tokens), with mma.sync.
+//
+// Rows of an item are the (new token, query head) pairs of one sequence and kv head, token by token, 16 at a time: the M of one
+// m16n8k16.  With so few rows the bytes of K and V bound the call (2 * 16 rows of products a key against 4 D bytes of it), so what
+// counts is that many bytes are always on their way, and the tensor work only has to keep up: no tcgen05 here, whose 128
+// lanes would be mostly empty and whose tiles would have to be handed from warp to warp.
+//   - A warp is on its own: it copies (cp.async) blocks of 16 keys (32 of 8-bit pages) of K and V into its own ring of
+//     shared memory and runs Q.K^T, the softmax step and P.V on them in registers.  Nothing is waited for but its copies.
+//   - The keys of all items are one line of units (a block for each warp of a CTA), cut into equal pieces, one for each CTA: whatever
+//     the lengths in the batch are, all SMs read the same number of bytes.  A CTA has at most two items that others share; their
+//     results (maximum, sum, unnormalised output, fp32) go through the workspace, and a second kernel joins them in the order of
+//     the keys.  No atomics: a call gives the same bits every time.
+//   - 8-bit codes become fp16, which holds them exactly, on their way from shared memory to the tensor core.  Scales are applied to
+//     scores and probabilities, of which there are fewer than elements of K and V.  The power of two 2^e of a V row is part of its
+//     weight: with x = score * log2(e) and M the running maximum of x + e, a key weighs w = 2^(x + e - M) <= 1, so that w fits
+//     fp16 whatever the scales are; the output is sum(w * code) / sum(w * 2^-e).  bf16 queries become fp16 with a power of two for
+//     each row, the largest magnitude in [2^14, 2^15): fp16 then keeps three bits more of them than bf16 has.
+//   - P is rounded to the 16-bit type that V has (or fp16): 2^-9 (2^-12) relative at most, as in the dense stage of the prefill.
+// The maximum that weights refer to is only moved when it grows by more than 8 (a factor of 256).
+#include "paged.cuh"
+#include "sm100_ptx.cuh"
+
+namespace moba {
+namespace {
+
+constexpr int kFewWarps = 4, kFewThreads = kFewWarps * 32;
+constexpr int kRowsM = 16;
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <int D, int kStore> struct FewShape {
+  static constexpr int kElem = kStore == MOBA_STORE_SAME ? 2 : 1;
+  static constexpr int kRowBytes = D * kElem;
+  static constexpr int kKeys = kStore == MOBA_STORE_SAME ? 16 : 32;              // of a warp's block
+  static constexpr int kBlockBytes = kKeys * kRowBytes;                          // of K, and of V
+  static constexpr int kScaleBytes = kStore == MOBA_STORE_SAME ? 0 : 2 * kKeys;  // bytes of K, then of V
+  static constexpr int kStageBytes = 2 * kBlockBytes + kScaleBytes;
+  // about 24 KB a warp: two CTAs, eight warps, have 150 KB on their way to an SM
+  static constexpr int kStages = D == 256 ? 2 : D == 128 ? 3 : D == 96 ? 4 : 6;
+  static constexpr int kWarpBytes = kStages * kStageBytes;
+  static constexpr int kUnit = kKeys * kFewWarps;                                // keys of a CTA's unit
+  static constexpr size_t kSmem = (size_t)kFewWarps * kWarpBytes;
+  static_assert(kWarpBytes >= kRowsM * D * 4, "the output of a warp fits its ring");
+};
+
+// 16-byte pieces of a row are moved by its number so that eight rows of one piece lie in different banks.
+template <int kRowBytes> __device__ __forceinline__ int swizzled(int row, int piece) {
+  if (kRowBytes % 128 == 0) return piece ^ (row & 7);
+  if (kRowBytes % 64 == 0) return piece ^ ((row >> 1) & 3);                      // 64 and 192
+  return piece ^ ((row >> 2) & 1);                                               // 96
+}
+
+__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void* src, bool on) {
+  const int bytes = on ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool kHalf>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (kHalf)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Four codes, of which the bytes of `kA` and `kB` (a prmt selector each) are wanted as pairs of fp16.
+template <int kStore, uint32_t kLo, uint32_t kHi>
+__device__ __forceinline__ void codes_to_half(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  if (kStore == MOBA_STORE_E4M3) {
+    const uint32_t y = kLo == 0x10 && kHi == 0x32 ? x : __byte_perm(x, 0, kLo | kHi << 8);
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(y));
+  } else {
+    // u = code + 128 under the exponent of 1024 is 1024 + u: taking 1152 off leaves the code
+    const uint32_t u = x ^ 0x80808080u;
+    constexpr uint32_t kSelLo = 0x4040 | (kLo & 0xf) | (kLo & 0xf0) << 4, kSelHi = 0x4040 | (kHi & 0xf) | (kHi & 0xf0) << 4;
+    const uint32_t a = __byte_perm(u, 0x64u, kSelLo), b = __byte_perm(u, 0x64u, kSelHi);
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));                  // 1152
+    const __half2 ra = __hsub2(*reinterpret_cast<const __half2*>(&a), off), rb = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&ra);
+    hi = *reinterpret_cast<const uint32_t*>(&rb);
+  }
+}
+
+// ---- the line of units -------------------------------------------------------
+// Sequence b has tiles(b) row tiles of 16, each of units(b) units of keys, for every kv head: in the order
+// sequence, kv head, row tile, unit.  (Units behind the last key that a tile sees are empty: they differ by the few new tokens.)
+struct FewPlan {
+  int64_t begin[kPagedBatch + 1];          // first unit of a sequence
+  int64_t scan[kFewThreads / 32];
+};
+struct FewItem {
+  int b, h, tile;
+  int u0, u1, units;                       // this piece's units of the item's
+};
+
+__device__ __forceinline__ int few_tiles(const PagedParams& p, const PagedSeq& s) { return (int)(((int64_t)s.n * p.G + kRowsM - 1) / kRowsM); }
+
+// All threads; returns the number of units of the batch.
+template <int kUnit, int kThreads>
+__device__ __forceinline__ int64_t few_plan(const PagedParams& p, FewPlan& plan) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t carry = 0;
+  for (int base = 0; base < p.B; base += kThreads) {
+    const int b = base + threadIdx.x;
+    int64_t w = 0;
+    if (b < p.B) {
+      const PagedSeq s = paged_seq(p, b);
+      // (rows without a key need an item too: they are written as zeros)
+      const int units = max((s.len + kUnit - 1) / kUnit, 1);
+      w = (int64_t)few_tiles(p, s) * units * p.Hkv;
+    }
+    int64_t x = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) plan.scan[warp] = x;
+    __syncthreads();
+    int64_t before = carry;
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) {
+      if (i < warp) before += plan.scan[i];
+      carry += plan.scan[i];
+    }
+    if (b < p.B) plan.begin[b] = before + x - w;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) plan.begin[p.B] = carry;
+  __syncthreads();
+  return carry;
+}
+
+// The item that has unit `u` of the line, from there on up to `end`.
+template <int kUnit>
+__device__ __forceinline__ FewItem few_item(const PagedParams& p, const FewPlan& plan, int64_t u, int64_t end, PagedSeq& s) {
+  int lo = 0, n = p.B;
+  while (n > 1) {                                           // last b with begin[b] <= u: one with units
+    const int half = n >> 1;
+    const bool up = plan.begin[lo + half] <= u;
+    lo = up ? lo + half : lo;
+    n = up ? n - half : half;
+  }
+  s = paged_seq(p, lo);
+  FewItem it;
+  it.b = lo;
+  it.units = max((s.len + kUnit - 1) / kUnit, 1);
+  const int64_t at = u - plan.begin[lo], item = at / it.units;
+  const int tiles = few_tiles(p, s);
+  it.h = (int)(item / tiles);
+  it.tile = (int)(item - (int64_t)it.h * tiles);
+  it.u0 = (int)(at - item * it.units);
+  it.u1 = (int)min((int64_t)it.units, it.u0 + (end - u));
+  return it;
+}
+
+// Units [first, last) of CTA c of n.
+__device__ __forceinline__ int64_t few_cut(int64_t units, int n, int c) { return units / n * c + units % n * c / n; }
+// CTAs that share the line: a piece is two units at least, so that short lines are joined from fewer pieces.
+__device__ __forceinline__ int few_ctas(int64_t units, int grid) { return (int)max(min((units + 1) / 2, (int64_t)grid), (int64_t)1); }
+
+struct FewArgs {
+  const void* q;
+  const void *kp, *vp;
+  const uint8_t *ks, *vs;
+  void* out;
+  float* lse;
+  float* part;                             // [2 * CTAs][16][D]: outputs of shared items, by CTA: 0 one that others began, 1 one that others end
+  float2* part_ml;                         // [2 * CTAs][16]: {maximum, sum}
+};
+
+// Packed row (token, head) of row r of a tile, or -1.
+__device__ __forceinline__ bool few_row(const PagedParams& p, const PagedSeq& s, int h, int tile, int r, int64_t& token, int& head, int& i) {
+  const int64_t at = (int64_t)tile * kRowsM + r;
+  i = (int)(at / p.G);
+  head = h * p.G + (int)(at - (int64_t)i * p.G);
+  token = (int64_t)s.row0 + i;
+  return i < s.n;
+}
+
+template <bool kHalf, int D, int kStore>
+__global__ void __launch_bounds__(kFewThreads, 2) paged_few_kernel(const PagedParams p, const FewArgs a) {
+  using S = FewShape<D, kStore>;
+  constexpr bool kCodes = kStore != MOBA_STORE_SAME;
+  constexpr bool kF16 = kHalf || kCodes;                    // operands of the MMAs
+  constexpr int kSteps = D / 16;                            // k-steps of Q.K^T
+  constexpr int kBlocksN = S::kKeys / 8;                    // 8-key blocks of scores
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ FewPlan plan;
+  __shared__ float2 warp_ml[kFewWarps][kRowsM];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t4 = lane & 3;
+  pdl_wait();
+  pdl_trigger();
+  const int64_t units = few_plan<S::kUnit, kFewThreads>(p, plan);
+  const int ctas = few_ctas(units, gridDim.x);
+  if ((int)blockIdx.x >= ctas) return;
+  const int64_t first = few_cut(units, ctas, blockIdx.x), last = few_cut(units, ctas, blockIdx.x + 1);
+  unsigned char* ring = smem + warp * S::kWarpBytes;
+  const uint32_t sring = ptx::smem_u32(ring);
+
+  for (int64_t u = first; u < last;) {
+    PagedSeq s;
+    const FewItem it = few_item<S::kUnit>(p, plan, u, last, s);
+    u += it.u1 - it.u0;
+    // ---- rows of this thread: g and g + 8
+    int lim[2];                                             // keys below are visible
+    float rs[2];                                            // factor of the scores
+    uint32_t qa[kSteps][4];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      int64_t token;
+      int head, i;
+      const bool on = few_row(p, s, it.h, it.tile, g + 8 * e, token, head, i);
+      lim[e] = on ? (int)min(max((int64_t)s.pos0 + i + 1, (int64_t)0), (int64_t)s.len) : 0;
+      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + token * p.sq_t + head * p.sq_h;
+      rs[e] = p.sl2;
+      if (!kCodes) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          qa[k][e] = on ? __ldg(reinterpret_cast<const uint32_t*>(q + 16 * k + 2 * t4)) : 0;
+          qa[k][2 + e] = on ? __ldg(reinterpret_cast<const uint32_t*>(q + 16 * k + 8 + 2 * t4)) : 0;
+        }
+      } else {
+        // the dims that a lane's four codes of a step are of: 4 t4 .. 4 t4 + 3 of its 16
+        uint2 x[kSteps];
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) x[k] = on ? __ldg(reinterpret_cast<const uint2*>(q + 16 * k + 4 * t4)) : make_uint2(0, 0);
+        float f = 1.f;
+        if (!kHalf) {
+          float amax = 0.f;
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k) {
+            const float2 u0 = unpack2<false>(x[k].x), u1 = unpack2<false>(x[k].y);
+            amax = fmaxf(fmaxf(fmaxf(amax, fabsf(u0.x)), fabsf(u0.y)), fmaxf(fabsf(u1.x), fabsf(u1.y)));
+          }
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+          // 2^(14 - k), between 2^-113 and 2^100 (rows of next to nothing score next to nothing)
+          const int k14 = min(max(14 - ((int)(__float_as_uint(amax) >> 23) - 127), -113), 100);
+          f = __uint_as_float((uint32_t)(127 + k14) << 23);
+          rs[e] = p.sl2 * __uint_as_float((uint32_t)(127 - k14) << 23);
+        }
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          if (kHalf) {
+            qa[k][e] = x[k].x;
+            qa[k][2 + e] = x[k].y;
+          } else {
+            const float2 u0 = unpack2<false>(x[k].x), u1 = unpack2<false>(x[k].y);
+            qa[k][e] = pack2_half(u0.x * f, u0.y * f);
+            qa[k][2 + e] = pack2_half(u1.x * f, u1.y * f);
+          }
+        }
+      }
+    }
+    float o[D / 8][4];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    // keys that some row of the tile sees: rows of the last new token see the most
+    const int64_t tile_last = min((int64_t)s.n - 1, ((int64_t)(it.tile + 1) * kRowsM - 1) / p.G);
+    const int end = (int)min(max((int64_t)s.pos0 + tile_last + 1, (int64_t)0), (int64_t)s.len);
+    const int key_of_warp = warp * S::kKeys;
+    // this warp's blocks: unit v of [u0, u1) has keys v * kUnit + key_of_warp ..
+    int blocks = 0;
+    if (end > key_of_warp) blocks = min(it.u1, (end - key_of_warp + S::kUnit - 1) / S::kUnit) - it.u0;
+    blocks = max(blocks, 0);
+
+    // ---- copies: the pages of a block are looked up one block ahead of its copies
+    constexpr int kGroups = S::kKeys / 16;                  // groups of 16 keys, each in one page
+    int page[kGroups];
+    auto lookup = [&](int j) {
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr) {
+        const int key = (it.u0 + j) * S::kUnit + key_of_warp + 16 * gr;
+        page[gr] = j < blocks && key < end ? paged_page(p, it.b, key) : -1;
+      }
+    };
+    auto copy = [&](int j) {                                // block j into its stage; `page` is the block's
+      const uint32_t dst = sring + (j % S::kStages) * S::kStageBytes;
+      const int key0 = (it.u0 + j) * S::kUnit + key_of_warp;
+      constexpr int kPieces = S::kRowBytes / 16;            // of a row
+      constexpr int kElemPiece = 16 / S::kElem;
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr) {
+        const int id = page[gr];
+        const int slot0 = (key0 + 16 * gr) & ((1 << p.page_shift) - 1);
+        const int64_t kb = id * p.kp_p + slot0 * p.kp_t + it.h * p.kp_h, vb = id * p.vp_p + slot0 * p.vp_t + it.h * p.vp_h;
+#pragma unroll
+        for (int i = 0; i < (16 * kPieces + 31) / 32; ++i) {
+          const int n = lane + 32 * i;
+          const int r = n / kPieces, c = n % kPieces;
+          if ((16 * kPieces) % 32 != 0 && r >= 16) break;
+          // rows nobody sees are zeros: whatever the page holds there, 0 * it stays out of P.V
+          const bool on = id >= 0 && key0 + 16 * gr + r < end;
+          const uint32_t at = (uint32_t)((16 * gr + r) * S::kRowBytes + swizzled<S::kRowBytes>(r, c) * 16);
+          const int64_t off = r * p.kp_t + c * kElemPiece, voff = r * p.vp_t + c * kElemPiece;
+          cp_async_16_or_zero(dst + at, static_cast<const unsigned char*>(a.kp) + (on ? (kb + off) * S::kElem : 0), on);
+          cp_async_16_or_zero(dst + S::kBlockBytes + at, static_cast<const unsigned char*>(a.vp) + (on ? (vb + voff) * S::kElem : 0), on);
+        }
+        if (kCodes && lane < 2) {
+          const int64_t at = id >= 0 ? (((int64_t)id * p.Hkv + it.h) << p.page_shift) + slot0 : 0;
+          cp_async_16_or_zero(dst + 2 * S::kBlockBytes + lane * S::kKeys + 16 * gr, (lane ? a.vs : a.ks) + at, id >= 0);
+        }
+      }
+    };
+    lookup(0);
+#pragma unroll
+    for (int j = 0; j < S::kStages - 1; ++j) {
+      if (j < blocks) copy(j);
+      lookup(j + 1);
+      cp_async_commit();
+    }
+
+    for (int j = 0; j < blocks; ++j) {
+      if (j + S::kStages - 1 < blocks) copy(j + S::kStages - 1);
+      lookup(j + S::kStages);
+      cp_async_commit();
+      cp_async_wait<S::kStages - 1>();
+      __syncwarp();
+      const uint32_t sk = sring + (j % S::kStages) * S::kStageBytes, sv = sk + S::kBlockBytes;
+      const int key0 = (it.u0 + j) * S::kUnit + key_of_warp;
+      // ---- S = Q.K^T
+      float sc[kBlocksN][4];
+#pragma unroll
+      for (int n = 0; n < kBlocksN; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
+      const int mrow = lane & 7, mi = lane >> 3;            // ldmatrix: row and matrix of this lane's address
+      if (!kCodes) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {                  // matrices: keys 0-7 pieces 2k, 2k + 1, keys 8-15 the same
+          uint32_t b[4];
+          const int r = mrow + 8 * (mi >> 1);
+          ldsm4(sk + r * S::kRowBytes + swizzled<S::kRowBytes>(r, 2 * k + (mi & 1)) * 16, b);
+          mma_16816<kF16>(sc[0], qa[k], b[0], b[1]);
+          mma_16816<kF16>(sc[1], qa[k], b[2], b[3]);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {                  // matrices: piece k (16 dims) of keys 0-7, 8-15, 16-23, 24-31
+          uint32_t b[4];
+          const int r = mrow + 8 * mi;
+          ldsm4(sk + r * S::kRowBytes + swizzled<S::kRowBytes>(r & 15, k) * 16, b);
+#pragma unroll
+          for (int n = 0; n < kBlocksN; ++n) {
+            uint32_t b0, b1;
+            codes_to_half<kStore, 0x10, 0x32>(b[n], b0, b1);
+            mma_16816<kF16>(sc[n], qa[k], b0, b1);
+          }
+        }
+      }
+      // ---- x = scores in powers of two (+ the exponent of the V row); running maximum
+      float vinv[kBlocksN][2];
+      if (kCodes) {
+        const unsigned char* sb = ring + (j % S::kStages) * S::kStageBytes + 2 * S::kBlockBytes;
+#pragma unroll
+        for (int n = 0; n < kBlocksN; ++n) {
+          const uint32_t kb = *reinterpret_cast<const uint16_t*>(sb + 8 * n + 2 * t4), vb = *reinterpret_cast<const uint16_t*>(sb + S::kKeys + 8 * n + 2 * t4);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t ke = (kb >> (8 * c)) & 255, ve = (vb >> (8 * c)) & 255;
+            const float kf = paged_scale(ke), vf = (float)((int)ve - 127);
+            vinv[n][c] = ve == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((254u - ve) << 23);
+            sc[n][c] = fmaf(sc[n][c], rs[0] * kf, vf);
+            sc[n][2 + c] = fmaf(sc[n][2 + c], rs[1] * kf, vf);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < kBlocksN; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[n][e] *= p.sl2;
+      }
+      int there[kGroups];
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr) there[gr] = key0 + 16 * gr < end && paged_page(p, it.b, key0 + 16 * gr) >= 0;
+#pragma unroll
+      for (int n = 0; n < kBlocksN; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int key = key0 + 8 * n + 2 * t4 + c;
+          if (key >= lim[0] || !there[n >> 1]) sc[n][c] = -INFINITY;
+          if (key >= lim[1] || !there[n >> 1]) sc[n][2 + c] = -INFINITY;
+        }
+      float alpha[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < kBlocksN; ++n) mx = fmaxf(mx, fmaxf(sc[n][2 * e], sc[n][2 * e + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        alpha[e] = 1.f;
+        if (mx > m[e] + 8.f) {
+          alpha[e] = exp2f(m[e] - mx);                      // (0 the first time)
+          m[e] = mx;
+        }
+      }
+      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          o[i][0] *= alpha[0]; o[i][1] *= alpha[0];
+          o[i][2] *= alpha[1]; o[i][3] *= alpha[1];
+        }
+        l[0] *= alpha[0];
+        l[1] *= alpha[1];
+      }
+      uint32_t pa[kGroups][4];
+      // a row that has seen nothing yet has no reference: any finite one leaves its weights at 0
+      const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
+#pragma unroll
+      for (int n = 0; n < kBlocksN; ++n) {
+        const float w0 = ptx::ex2_approx(sc[n][0] - m0), w1 = ptx::ex2_approx(sc[n][1] - m0);
+        const float w2 = ptx::ex2_approx(sc[n][2] - m1), w3 = ptx::ex2_approx(sc[n][3] - m1);
+        if (kCodes) {
+          l[0] += w0 == 0.f ? 0.f : w0 * vinv[n][0];
+          l[0] += w1 == 0.f ? 0.f : w1 * vinv[n][1];
+          l[1] += w2 == 0.f ? 0.f : w2 * vinv[n][0];
+          l[1] += w3 == 0.f ? 0.f : w3 * vinv[n][1];
+        } else {
+          l[0] += w0 + w1;
+          l[1] += w2 + w3;
+        }
+        pa[n >> 1][(n & 1) * 2] = pack2_16<kF16>(w0, w1);
+        pa[n >> 1][(n & 1) * 2 + 1] = pack2_16<kF16>(w2, w3);
+      }
+      // ---- O += P.V
+      if (!kCodes) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {                  // matrices: keys 0-7, 8-15 of pieces 2i, the same of 2i + 1
+          uint32_t b[4];
+          const int r = mrow + 8 * (mi & 1);
+          ldsm4_t(sv + r * S::kRowBytes + swizzled<S::kRowBytes>(r, 2 * i + (mi >> 1)) * 16, b);
+          mma_16816<kF16>(o[2 * i], pa[0], b[0], b[1]);
+          mma_16816<kF16>(o[2 * i + 1], pa[0], b[2], b[3]);
+        }
+      } else {
+        // pairs of dims are the 16-bit elements of a matrix: piece i gives the even dims of 16, and the odd ones
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {                  // matrices: keys 0-7, 8-15, 16-23, 24-31 of piece i
+          uint32_t b[4];
+          const int r = mrow + 8 * mi;
+          ldsm4_t(sv + r * S::kRowBytes + swizzled<S::kRowBytes>(r & 15, i) * 16, b);
+#pragma unroll
+          for (int gr = 0; gr < kGroups; ++gr) {
+            uint32_t e0, o0, e1, o1;
+            codes_to_half<kStore, 0x20, 0x31>(b[2 * gr], e0, o0);
+            codes_to_half<kStore, 0x20, 0x31>(b[2 * gr + 1], e1, o1);
+            mma_16816<kF16>(o[2 * i], pa[gr], e0, e1);
+            mma_16816<kF16>(o[2 * i + 1], pa[gr], o0, o1);
+          }
+        }
+      }
+      __syncwarp();
+    }
+
+    // ---- the warps' results, joined by all threads
+    cp_async_wait<0>();
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+      // a row with a score that is not a number has no maximum to speak of: with this one it stays NaN in every join
+      if (l[e] != l[e]) m[e] = INFINITY;
+      if (t4 == 0) warp_ml[warp][g + 8 * e] = make_float2(m[e], l[e]);
+    }
+    __syncwarp();
+    float* so = reinterpret_cast<float*>(ring);             // [16][D]
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (!kCodes) {
+          *reinterpret_cast<float2*>(so + (g + 8 * e) * D + 8 * i + 2 * t4) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
+        } else {                                            // column c of blocks 2i, 2i + 1: dims 2c, 2c + 1 of 16
+          float* at = so + (g + 8 * e) * D + 16 * (i >> 1) + (i & 1);
+          at[2 * (2 * t4)] = o[i][2 * e];
+          at[2 * (2 * t4 + 1)] = o[i][2 * e + 1];
+        }
+      }
+    __syncthreads();
+    const bool whole = it.u0 == 0 && it.u1 == it.units;
+    const int64_t slot = 2 * (int64_t)blockIdx.x + (it.u0 == 0 ? 1 : 0);
+    for (int n = threadIdx.x; n < kRowsM * (D / 4); n += kFewThreads) {
+      const int r = n / (D / 4), c = n % (D / 4) * 4;
+      int64_t token;
+      int head, i;
+      if (!few_row(p, s, it.h, it.tile, r, token, head, i)) continue;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kFewWarps; ++w) mx = fmaxf(mx, warp_ml[w][r].x);
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      float sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kFewWarps; ++w) {
+        const float f = exp2f(warp_ml[w][r].x - ref);
+        const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * S::kWarpBytes) + r * D + c);
+        if (f == 0.f) continue;
+        sum += f * warp_ml[w][r].y;
+        x[0] += f * v.x; x[1] += f * v.y; x[2] += f * v.z; x[3] += f * v.w;
+      }
+      if (whole) {
+        const float inv = mx == -INFINITY ? 0.f : 1.f / sum;
+        uint2 y;
+        y.x = pack2_16<kHalf>(x[0] * inv, x[1] * inv);
+        y.y = pack2_16<kHalf>(x[2] * inv, x[3] * inv);
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + token * p.so_t + head * p.so_h + c) = y;
+        if (a.lse != nullptr && c == 0) a.lse[(int64_t)head * p.T + token] = (mx + log2f(sum)) * kLn2;
+      } else {
+        *reinterpret_cast<float4*>(a.part + (slot * kRowsM + r) * D + c) = make_float4(x[0], x[1], x[2], x[3]);
+        if (c == 0) a.part_ml[slot * kRowsM + r] = make_float2(mx, sum);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Joins the pieces of the items that several CTAs share.  Block c: the item that CTA c began and did not end.
+template <bool kHalf, int D, int kStore>
+__global__ void __launch_bounds__(kFewThreads) paged_few_join_kernel(const PagedParams p, const FewArgs a, int grid) {
+  using S = FewShape<D, kStore>;
+  __shared__ FewPlan plan;
+  pdl_wait();
+  pdl_trigger();
+  const int64_t units = few_plan<S::kUnit, kFewThreads>(p, plan);
+  const int ctas = few_ctas(units, grid);
+  const int c0 = blockIdx.x;
+  if (c0 >= ctas) return;
+  const int64_t first = few_cut(units, ctas, c0), last = few_cut(units, ctas, c0 + 1);
+  if (last <= first || last >= units) return;
+  PagedSeq s;
+  const FewItem it = few_item<S::kUnit>(p, plan, last - 1, last, s);
+  const int64_t begin = last - 1 - it.u0, end = begin + it.units;
+  if (begin < first || end <= last) return;                 // begun before, or ended here
+  int c1 = c0 + 1;                                          // the CTA that ends it
+  while (few_cut(units, ctas, c1 + 1) < end) ++c1;
+  for (int n = threadIdx.x; n < kRowsM * (D / 4); n += kFewThreads) {
+    const int r = n / (D / 4), c = n % (D / 4) * 4;
+    int64_t token;
+    int head, i;
+    if (!few_row(p, s, it.h, it.tile, r, token, head, i)) continue;
+    float mx = -INFINITY, sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int cc = c0; cc <= c1; ++cc) {
+      const int64_t slot = 2 * (int64_t)cc + (cc == c0 ? 1 : 0);
+      const float2 ml = __ldcg(a.part_ml + slot * kRowsM + r);
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part + (slot * kRowsM + r) * D + c));
+      if (ml.x == -INFINITY) continue;
+      const float up = fmaxf(mx, ml.x), f0 = exp2f(mx - up), f1 = exp2f(ml.x - up);
+      mx = up;
+      sum = sum * f0 + ml.y * f1;
+      x[0] = x[0] * f0 + v.x * f1; x[1] = x[1] * f0 + v.y * f1;
+      x[2] = x[2] * f0 + v.z * f1; x[3] = x[3] * f0 + v.w * f1;
+    }
+    const float inv = mx == -INFINITY ? 0.f : 1.f / sum;
+    uint2 y;
+    y.x = pack2_16<kHalf>(x[0] * inv, x[1] * inv);
+    y.y = pack2_16<kHalf>(x[2] * inv, x[3] * inv);
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + token * p.so_t + head * p.so_h + c) = y;
+    if (a.lse != nullptr && c == 0) a.lse[(int64_t)head * p.T + token] = (mx + log2f(sum)) * kLn2;
+  }
+}
+
+struct FewKernels {
+  void (*attend)(const PagedParams, const FewArgs);
+  void (*join)(const PagedParams, const FewArgs, int);
+  size_t smem;
+};
+template <bool kHalf, int D, int kStore>
+FewKernels few_kernels() {
+  return FewKernels{paged_few_kernel<kHalf, D, kStore>, paged_few_join_kernel<kHalf, D, kStore>, FewShape<D, kStore>::kSmem};
+}
+template <bool kHalf, int D>
+FewKernels pick_few(int store) {
+  return store == MOBA_STORE_SAME ? few_kernels<kHalf, D, MOBA_STORE_SAME>() : store == MOBA_STORE_E4M3 ? few_kernels<kHalf, D, MOBA_STORE_E4M3>()
+                                                                             : few_kernels<kHalf, D, MOBA_STORE_INT8>();
+}
+template <bool kHalf>
+FewKernels pick_few_dim(int D, int store) {
+  return D == 64 ? pick_few<kHalf, 64>(store) : D == 96 ? pick_few<kHalf, 96>(store) : D == 128 ? pick_few<kHalf, 128>(store)
+                                                                                               : pick_few<kHalf, 256>(store);
+}
+
+constexpr int kFewMaxCtas = 148 * 2;
+
+}  // namespace
+
+size_t paged_few_workspace(const PagedParams& p) { return (size_t)2 * kFewMaxCtas * kRowsM * (p.D * sizeof(float) + sizeof(float2)); }
+
+cudaError_t launch_paged_few(const PagedParams& all, const void* q, const void* kp, const void* vp, const uint8_t* ks,
+                             const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st) {
+  const FewKernels k = all.fp16 ? pick_few_dim<true>(all.D, all.store) : pick_few_dim<false>(all.D, all.store);
+  FewArgs a{q, kp, vp, ks, vs, out, lse, nullptr, nullptr};
+  a.part_ml = static_cast<float2*>(workspace);
+  a.part = reinterpret_cast<float*>(a.part_ml + 2 * kFewMaxCtas * kRowsM);
+  cudaError_t e = prepare_kernel(k.attend, k.smem, nullptr, true);
+  if (e != cudaSuccess) return e;
+  const int sms = device_info().sms;
+  const int grid = 2 * sms < kFewMaxCtas ? 2 * sms : kFewMaxCtas;
+  for (int b = 0; b < all.B; b += kPagedBatch) {
+    PagedParams p = all;
+    p.B = all.B - b < kPagedBatch ? all.B - b : kPagedBatch;
+    p.cu += b;
+    p.lens += b;
+    p.table += b * all.table_stride;
+    if ((e = launch_pdl(k.attend, dim3(grid), kFewThreads, k.smem, st, p, a)) != cudaSuccess) return e;
+    if ((e = launch_pdl(k.join, dim3(grid), kFewThreads, 0, st, p, a, grid)) != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace moba

@@ -375,6 +375,66 @@ enum {
 };
 int moba_problem_attend_kernel(const moba_problem_t* p);
 
+/* ---- keys and values of many sequences in pages ------------------------------------------------
+ *
+ * For a server: the K and V rows of any number of growing sequences live in one pool of pages (no counterpart in the reference,
+ * whose operator takes whole packed sequences).  A call concerns a packed batch of new tokens:
+ *   cu_seqlens  int32[batch+1] on the device, from 0, never decreasing: sequence b has the rows cu[b] .. cu[b+1]-1 of the
+ *               packed tensors.  Rows from cu[batch] on are not touched.  A sequence may have no row.
+ *   seq_lens    int32[batch] on the device: the sequence's tokens, the packed ones, which are its last, included.  Row i of
+ *               sequence b is at position seq_lens[b] - (cu[b+1] - cu[b]) + i.
+ *   page_table  int32[batch, pages_per_seq] on the device, rows `table_stride` apart: position x is slot x % page_size of page
+ *               page_table[b][x / page_size].  An entry outside 0 .. num_pages-1 is a page that is not there: rows for it are
+ *               not stored, load as zeros, and take no part in attention; so do positions behind the table, and below 0.
+ * Neither is read back to the host.  Pages hold rows of the 16-bit type `dtype` (MOBA_STORE_SAME), or 8-bit codes
+ * (MOBA_STORE_E4M3, MOBA_STORE_INT8) and one byte per row and head: code c with byte s stands for c * 2^(s - 127), which both 16-bit types
+ * hold exactly (a power of two costs e4m3 next to nothing and int8 half a bit on average; nothing is rounded twice, and
+ * codes do not depend on how a division is rounded).  The byte is that of the least power of two, from 2^-96, whose product with the
+ * largest code (448, 127) reaches the row's largest magnitude; a row of zeros has 127; a row with an infinity or a NaN has
+ * 255 and reads back as NaN.  A value whose code would stand for an infinity of `dtype` is stored as the largest finite one.
+ * A pool's element (page, slot, head, dim) is at page * page_stride + slot * token_stride + head * head_stride + dim, in
+ * elements; the bytes of the codes are [num_pages, num_kv_heads, page_size]. */
+enum {
+  MOBA_STORE_SAME = 0,
+  MOBA_STORE_E4M3 = 1,
+  MOBA_STORE_INT8 = 2
+};
+typedef struct moba_paged {
+  int64_t total_tokens;     /* rows of the packed tensors                                          */
+  int32_t batch, num_q_heads, num_kv_heads, head_dim;
+  int32_t num_pages, page_size;            /* page_size: a power of two, at least 16               */
+  int32_t pages_per_seq;    /* columns of page_table                                               */
+  int32_t max_new;          /* most rows of a sequence, which the kernel is chosen by (a wrong one costs time only) */
+  int32_t dtype, store;     /* MOBA_DTYPE_*, MOBA_STORE_*                                          */
+  float softmax_scale;      /* factor of the scores; 0: head_dim^-0.5                              */
+  int32_t reserved;         /* must be 0                                                           */
+  int64_t q_stride_token, q_stride_head;   /* elements; of the packed q ...                        */
+  int64_t o_stride_token, o_stride_head;   /* ... and out                                          */
+  int64_t k_stride_token, k_stride_head;   /* of the packed k (new rows, or rows read back) ...    */
+  int64_t v_stride_token, v_stride_head;   /* ... and v                                            */
+  int64_t k_page_stride, k_page_token, k_page_head;
+  int64_t v_page_stride, v_page_token, v_page_head;
+  int64_t table_stride;
+} moba_paged_t;
+
+int moba_paged_check(const moba_paged_t* p);
+/* k, v -> pages.  A slot that two rows of a call are for (pages shared by sequences) holds one of them. */
+int moba_paged_store(const moba_paged_t* p, const void* k, const void* v, const int32_t* cu_seqlens, const int32_t* seq_lens,
+                     const int32_t* page_table, void* k_pages, void* v_pages, uint8_t* k_scales, uint8_t* v_scales, void* stream);
+/* pages -> k, v: the same rows back, in `dtype`. */
+int moba_paged_load(const moba_paged_t* p, const int32_t* cu_seqlens, const int32_t* seq_lens, const int32_t* page_table,
+                    const void* k_pages, const void* v_pages, const uint8_t* k_scales, const uint8_t* v_scales, void* k, void* v,
+                    void* stream);
+/* Softmax attention of every packed row to the positions of its sequence up to its own, each kv head for its group of query
+ * heads.  A row that sees nothing is zeros, its LSE -inf.  lse_out: optional fp32 [Hq, T], natural log.  Sums, maxima and the
+ * accumulated output are fp32; probabilities are rounded to 16 bits before the product with V.
+ * The workspace needs no clearing. */
+int moba_paged_workspace_size(const moba_paged_t* p, size_t* bytes);
+int moba_paged_attention(const moba_paged_t* p, const void* q, const int32_t* cu_seqlens, const int32_t* seq_lens,
+                         const int32_t* page_table, const void* k_pages, const void* v_pages, const uint8_t* k_scales,
+                         const uint8_t* v_scales, void* out, float* lse_out, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif
