@@ -61,6 +61,13 @@ cudaError_t launch_paged_load(const PagedParams& p, const void* kp, const void* 
 // Sequences that one launch of an attention kernel takes: their work is added up in shared memory.
 constexpr int kPagedBatch = 1024;
 
+// Items of more rows run on tcgen05.
+constexpr int kPagedFewRows = 16;
+inline bool paged_few_rows(const PagedParams& p) { return (int64_t)p.max_new * p.G <= kPagedFewRows || p.D == 256; }
+
+size_t paged_rows_workspace(const PagedParams& p);
+cudaError_t launch_paged_rows(const PagedParams& p, const void* q, const void* kp, const void* vp, const uint8_t* ks,
+                              const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st);
 size_t paged_few_workspace(const PagedParams& p);
 cudaError_t launch_paged_few(const PagedParams& p, const void* q, const void* kp, const void* vp, const uint8_t* ks,
                              const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st);

@@ -74,6 +74,8 @@ int check_pointers(const moba_paged_t* p, const void* a, const void* b, const in
   return MOBA_OK;
 }
 
+size_t workspace_of(const PagedParams& p) { return paged_few_rows(p) ? paged_few_workspace(p) : paged_rows_workspace(p); }
+
 }  // namespace
 
 extern "C" {
@@ -100,7 +102,7 @@ int moba_paged_workspace_size(const moba_paged_t* p, size_t* bytes) {
   const int rc = check_paged(p);
   if (rc != MOBA_OK) return rc;
   if (bytes == nullptr) return MOBA_E_NULL;
-  *bytes = paged_few_workspace(paged_params(p, nullptr, nullptr, nullptr));
+  *bytes = workspace_of(paged_params(p, nullptr, nullptr, nullptr));
   return MOBA_OK;
 }
 
@@ -112,9 +114,9 @@ int moba_paged_attention(const moba_paged_t* p, const void* q, const int32_t* cu
   if (rc != MOBA_OK) return rc;
   if ((uintptr_t)lse_out & 3) return MOBA_E_ALIGN;
   const PagedParams r = paged_params(p, cu, lens, table);
-  if (workspace == nullptr || workspace_bytes < paged_few_workspace(r)) return MOBA_E_WORKSPACE;
-  if ((uintptr_t)workspace & 15) return MOBA_E_ALIGN;
-  return (int)launch_paged_few(r, q, kp, vp, ks, vs, out, lse_out, workspace, (cudaStream_t)stream);
+  if (workspace == nullptr || workspace_bytes < workspace_of(r)) return MOBA_E_WORKSPACE;
+  if ((uintptr_t)workspace & 31) return MOBA_E_ALIGN;
+  return (int)(paged_few_rows(r) ? launch_paged_few : launch_paged_rows)(r, q, kp, vp, ks, vs, out, lse_out, workspace, (cudaStream_t)stream);
 }
 
 }  // extern "C"

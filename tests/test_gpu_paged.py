@@ -10,6 +10,8 @@ from tests.paged_util import Batch, quantise, values
 pytestmark = pytest.mark.gpu
 
 E4M3, INT8 = torch.float8_e4m3fn, torch.int8
+#: `max_new` decides between the kernel for few rows and the one for many, whatever the batch holds
+FEW, MANY = 1, 4096
 #: (new, length): a fresh sequence, one without new tokens, an empty one, one token, page borders from both sides
 RAGGED = [(5, 5), (0, 40), (0, 0), (1, 1), (1, 17), (16, 64), (3, 65), (33, 100), (1, 128), (2, 129)]
 
@@ -77,40 +79,43 @@ def test_codes_of_unusual_rows(store, dtype):
     assert torch.isfinite(k[finite]).all() and torch.isnan(k[~finite]).all()
 
 
+@pytest.mark.parametrize("kernel", [FEW, MANY])
 @pytest.mark.parametrize("hq,hkv", [(4, 4), (8, 2), (6, 2), (16, 1), (40, 1)])
 @pytest.mark.parametrize("dim,page,dtype,store", [
     (64, 16, torch.float16, None), (64, 64, torch.bfloat16, E4M3), (64, 128, torch.float16, INT8),
     (96, 32, torch.bfloat16, None), (96, 16, torch.float16, E4M3), (96, 16, torch.bfloat16, INT8),
     (128, 64, torch.bfloat16, None), (128, 16, torch.bfloat16, E4M3), (128, 32, torch.float16, INT8), (128, 256, torch.float16, E4M3),
     (256, 16, torch.bfloat16, None), (256, 64, torch.float16, E4M3), (256, 32, torch.bfloat16, INT8)])
-def test_attention_of_a_ragged_batch(dim, page, dtype, store, hq, hkv):
+def test_attention_of_a_ragged_batch(dim, page, dtype, store, hq, hkv, kernel):
     b = Batch(RAGGED, hq, hkv, dim, page, dtype, store, seed=dim + hq, layout="heads" if hq % 3 else "tokens")
     b.fill()
-    got, lse = paged_attention(b.q, b.k, b.v, *b.where, b.max_new, return_lse=True, **b.scales)
+    got, lse = paged_attention(b.q, b.k, b.v, *b.where, kernel, return_lse=True, **b.scales)
     b.check(got, lse)
-    again = paged_attention(b.q, b.k, b.v, *b.where, b.max_new, **b.scales)
+    again = paged_attention(b.q, b.k, b.v, *b.where, kernel, **b.scales)
     assert torch.equal(got, again)
 
 
 @pytest.mark.parametrize("store", [None, E4M3, INT8])
 @pytest.mark.parametrize("seqs", [[(1, n)] for n in (1, 2, 15, 16, 17, 127, 128, 129, 1000, 4097)] +
                          [[(1, 3000), (1, 1), (1, 700), (2, 2), (1, 5000)], [(7, 2500), (1, 9)], [(200, 200)], [(150, 1300), (1, 77)]])
-def test_attention_over_lengths(seqs, store):
+@pytest.mark.parametrize("kernel", [FEW, MANY])
+def test_attention_over_lengths(seqs, store, kernel):
     b = Batch(seqs, 8, 2, 128, 16, torch.bfloat16, store, seed=len(seqs) + seqs[0][1])
     b.fill()
-    got, lse = paged_attention(b.q, b.k, b.v, *b.where, b.max_new, return_lse=True, **b.scales)
+    got, lse = paged_attention(b.q, b.k, b.v, *b.where, kernel, return_lse=True, **b.scales)
     b.check(got, lse)
 
 
 @pytest.mark.parametrize("store", [None, E4M3])
 @pytest.mark.parametrize("new", [3, 70])
-def test_rows_that_see_nothing(store, new):
+@pytest.mark.parametrize("kernel", [FEW, MANY])
+def test_rows_that_see_nothing(store, new, kernel):
     """Positions below zero, pages that are not there (all of a sequence's, its first, one in the middle), a table too short."""
     seqs = [(new, new - 2), (new, 0), (new, -4), (new, 300), (new, 300), (new, 300), (1, 40)]
     missing = [(3, i) for i in range(19)] + [(4, 0)] + [(5, 7)]
     b = Batch(seqs, 4, 2, 64, 16, torch.float16, store, seed=new, missing=missing)
     b.fill()
-    got, lse = paged_attention(b.q, b.k, b.v, *b.where, b.max_new, return_lse=True, **b.scales)
+    got, lse = paged_attention(b.q, b.k, b.v, *b.where, kernel, return_lse=True, **b.scales)
     b.check(got, lse)
     empty = torch.isinf(lse).t()
     assert empty[:2].all() == (new > 2) and empty[new:3 * new].all() and (got[empty] == 0).all()
@@ -159,20 +164,21 @@ def test_strides_and_scale():
     b.check(got, want=b.attention(0.2))
 
 
+@pytest.mark.parametrize("kernel", [FEW, MANY])
 @pytest.mark.parametrize("store", [None, E4M3])
-def test_numbers_that_are_none(store):
+def test_numbers_that_are_none(store, kernel):
     """A NaN in a token's query reaches its own row only; a key or value row with one reaches the rows that see it, and not the
     sequences that do not."""
     seqs = [(2, 200), (1, 77), (1, 40)]
     b = Batch(seqs, 4, 2, 64, 16, torch.bfloat16, store, seed=1)
     clean = Batch(seqs, 4, 2, 64, 16, torch.bfloat16, store, seed=1)
     clean.fill()
-    want = paged_attention(clean.q, clean.k, clean.v, *clean.where, 2, **clean.scales)
+    want = paged_attention(clean.q, clean.k, clean.v, *clean.where, kernel, **clean.scales)
     b.q[2, 1, 5] = math.nan
     b.hist[0][0][30, 0, 3] = math.inf
     b.hist[2][1][7, 1] = math.nan
     b.fill()
-    got, lse = paged_attention(b.q, b.k, b.v, *b.where, 2, return_lse=True, **b.scales)
+    got, lse = paged_attention(b.q, b.k, b.v, *b.where, kernel, return_lse=True, **b.scales)
     bad = torch.isnan(got).any(-1)
     # an infinite key scores +inf or -inf, as the query's element there has it: the first makes NaN (inf - inf), the second a weight
     # of 0.  Quantised, the key is NaN and so is every score of it.
@@ -184,31 +190,34 @@ def test_numbers_that_are_none(store):
 
 
 @pytest.mark.parametrize("store,scale", [(None, 1e3), (E4M3, 1e3), (E4M3, 1e-3), (INT8, 1e-3), (INT8, 3e4), (E4M3, 2.0 ** 60), (INT8, 2.0 ** -60)])
-def test_large_and_small_values(store, scale):
+@pytest.mark.parametrize("kernel", [FEW, MANY])
+def test_large_and_small_values(store, scale, kernel):
     """Rows of any size, scores that run from one key to a single one: weights stay in range whatever the powers of two are."""
     b = Batch([(1, 500), (4, 900), (40, 300)], 4, 2, 128, 16, torch.bfloat16, store, seed=4, scale=scale, q_scale=1.0 / scale)
     b.fill()
-    got, lse = paged_attention(b.q, b.k, b.v, *b.where, 40, return_lse=True, **b.scales)
+    got, lse = paged_attention(b.q, b.k, b.v, *b.where, kernel, return_lse=True, **b.scales)
     b.check(got, lse)
 
 
-def test_v_rows_of_very_different_sizes():
+@pytest.mark.parametrize("kernel", [FEW, MANY])
+def test_v_rows_of_very_different_sizes(kernel):
     """Powers of two of V rows that differ by 2^20: the weights follow their product with the probabilities."""
     b = Batch([(1, 400), (3, 777)], 4, 2, 128, 16, torch.float16, E4M3, seed=5)
     for k, v in b.hist:
         v[::3] *= 2.0 ** -12
         v[1::3] *= 2.0 ** 8
     b.fill()
-    got, lse = paged_attention(b.q, b.k, b.v, *b.where, 3, return_lse=True, **b.scales)
+    got, lse = paged_attention(b.q, b.k, b.v, *b.where, kernel, return_lse=True, **b.scales)
     b.check(got, lse)
 
 
-def test_many_sequences():
+@pytest.mark.parametrize("kernel", [FEW, MANY])
+def test_many_sequences(kernel):
     """More sequences than one launch adds up, most of them without new tokens."""
     seqs = [(1, 3 + i % 40) if i % 3 == 0 else (0, i % 7) for i in range(2500)]
     b = Batch(seqs, 2, 1, 64, 16, torch.float16, seed=6)
     b.fill()
-    got, lse = paged_attention(b.q, b.k, b.v, *b.where, 1, return_lse=True)
+    got, lse = paged_attention(b.q, b.k, b.v, *b.where, kernel, return_lse=True)
     b.check(got, lse)
     k, v = paged_load(b.k, b.v, *b.where, b.rows)
     assert torch.equal(k, b.k_new) and torch.equal(v, b.v_new)

@@ -58,7 +58,7 @@ def test_pointers_are_checked_before_any_launch(lib):
     assert attend(p, None, ok) == -4 and attend(p, ok, None) == -4 and attend(q, ok, ok) == -4
     assert attend(p, off, ok) == -6 and attend(p, ok, ok, out=off) == -6 and attend(p, ok, ok, lse=0x10002) == -6
     assert attend(p, ok, ok, ws=None) == -3 and attend(p, ok, ok, size=need.value - 1) == -3
-    assert attend(p, ok, ok, ws=off) == -6
+    assert attend(p, ok, ok, ws=0x10010) == -6
 
 
 def _tensors(**kw):
