@@ -1529,18 +1529,20 @@ bool make_kv_map(CUtensorMap* m, bool fp16, int D, const __nv_bfloat16* base, in
   return make_tile_map(m, fp16, D, base, T, Hkv, st, sh, 1, box_rows);
 }
 
-// a pool of pages, [pages][slots][H][D] with element strides (sp, st, sh, 1): boxes of `box_rows` slots of one page and head x 64 dims
-bool make_page_map(CUtensorMap* m, bool fp16, int D, const void* base, int pages, int slots, int H, int64_t sp, int64_t st, int64_t sh,
+// a pool of pages, [pages][slots][H][D] with element strides (sp, st, sh, 1): boxes of `box_rows` slots of one page and head x 128 bytes.
+// `elem`: 1 bytes, 2 fp16, 3 bf16
+bool make_page_map(CUtensorMap* m, int elem, int D, const void* base, int pages, int slots, int H, int64_t sp, int64_t st, int64_t sh,
                    int box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return false;
+  const cuuint64_t bytes = elem == 1 ? 1 : 2;
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)slots, (cuuint64_t)H, (cuuint64_t)pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)st * 2, (cuuint64_t)sh * 2, (cuuint64_t)sp * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+  const cuuint64_t strides[3] = {(cuuint64_t)st * bytes, (cuuint64_t)sh * bytes, (cuuint64_t)sp * bytes};
+  const cuuint32_t box[4] = {(cuuint32_t)(128 / bytes), (cuuint32_t)box_rows, 1, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
-  return fn(m, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return fn(m, elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 cudaError_t launch_bounded_wait_probe(int32_t* status, unsigned long long limit_ns, cudaStream_t st) {

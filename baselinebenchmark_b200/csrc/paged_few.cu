@@ -4,8 +4,9 @@
 // m16n8k16.  With so few rows the bytes of K and V bound the call (2 * 16 rows of products a key against 4 D bytes of it), so what
 // counts is that many bytes are always on their way, and the tensor work only has to keep up: no tcgen05 here, whose 128
 // lanes would be mostly empty and whose tiles would have to be handed from warp to warp.
-//   - A warp is on its own: it copies (cp.async) blocks of 16 keys (32 of 8-bit pages) of K and V into its own ring of
-//     shared memory and runs Q.K^T, the softmax step and P.V on them in registers.  Nothing is waited for but its copies.
+//   - A warp is on its own: TMA brings it blocks of 16 keys (32 of 8-bit pages) of K and V into its own ring of swizzled shared memory, and it
+//     runs Q.K^T, the softmax step and P.V on them in registers.  Nothing is waited for but its copies.  (With a copy instruction
+//     and its addresses for every 16 bytes a block was 490 instructions, and a decode step of 48 requests 188 us.)
 //   - The keys of all items are one line of units (a block for each warp of a CTA), cut into equal pieces, one for each CTA: whatever
 //     the lengths in the batch are, all SMs read the same number of bytes.  A CTA has at most two items that others share; their
 //     results (maximum, sum, unnormalised output, fp32) go through the workspace, and a second kernel joins them in the order of
@@ -21,41 +22,39 @@
 #include "sm100_ptx.cuh"
 
 namespace moba {
+
+bool make_page_map(CUtensorMap* m, int elem, int D, const void* base, int pages, int slots, int H, int64_t sp, int64_t st, int64_t sh,
+                   int box_rows);
+
 namespace {
 
+using namespace ptx;
+
 constexpr int kFewWarps = 4, kFewThreads = kFewWarps * 32;
-constexpr int kRowsM = 16;
 constexpr float kLn2 = 0.6931471805599453f;
 
 template <int D, int kStore> struct FewShape {
-  static constexpr int kElem = kStore == MOBA_STORE_SAME ? 2 : 1;
-  static constexpr int kRowBytes = D * kElem;
-  static constexpr int kKeys = kStore == MOBA_STORE_SAME ? 16 : 32;              // of a warp's block
-  static constexpr int kBlockBytes = kKeys * kRowBytes;                          // of K, and of V
-  static constexpr int kScaleBytes = kStore == MOBA_STORE_SAME ? 0 : 2 * kKeys;  // bytes of K, then of V
-  static constexpr int kStageBytes = 2 * kBlockBytes + kScaleBytes;
-  // about 24 KB a warp: two CTAs, eight warps, have 150 KB on their way to an SM
-  static constexpr int kStages = D == 256 ? 2 : D == 128 ? 3 : D == 96 ? 4 : 6;
+  static constexpr bool kCodes = kStore != MOBA_STORE_SAME;
+  static constexpr int kKeys = kCodes ? 32 : 16;                     // of a warp's block
+  static constexpr int kSpan = kCodes ? 128 : 64;                    // elements of 128 bytes
+  static constexpr int kSubs = (D + kSpan - 1) / kSpan;              // sub-blocks [keys][128 bytes] of K, and of V
+  static constexpr int kSubBytes = kKeys * 128;
+  static constexpr int kSideBytes = kSubs * kSubBytes;               // K; V behind it
+  static constexpr int kStageBytes = 2 * kSideBytes;
+  // about 24 KB a warp: two CTAs, eight warps, have 130 KB and more on their way to an SM
+  static constexpr int kStages = kStageBytes == 16384 ? 3 : kStageBytes == 8192 ? 3 : 6;
   static constexpr int kWarpBytes = kStages * kStageBytes;
-  static constexpr int kUnit = kKeys * kFewWarps;                                // keys of a CTA's unit
-  static constexpr size_t kSmem = (size_t)kFewWarps * kWarpBytes;
-  static_assert(kWarpBytes >= kRowsM * D * 4, "the output of a warp fits its ring");
+  static constexpr int kUnit = kKeys * kFewWarps;                    // keys of a CTA's unit
+  static constexpr size_t kSmem = 1024 + (size_t)kFewWarps * kWarpBytes;
+  static_assert(kWarpBytes >= 16 * D * 4, "the output of a warp fits its ring");
 };
 
-// 16-byte pieces of a row are moved by its number so that eight rows of one piece lie in different banks.
-template <int kRowBytes> __device__ __forceinline__ int swizzled(int row, int piece) {
-  if (kRowBytes % 128 == 0) return piece ^ (row & 7);
-  if (kRowBytes % 64 == 0) return piece ^ ((row >> 1) & 3);                      // 64 and 192
-  return piece ^ ((row >> 2) & 1);                                               // 96
+// `bytes` (a multiple of 16) to shared memory, counted on the barrier
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+               "r"(bar)
+               : "memory");
 }
-
-__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void* src, bool on) {
-  const int bytes = on ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -96,7 +95,7 @@ __device__ __forceinline__ void codes_to_half(uint32_t x, uint32_t& lo, uint32_t
 }
 
 // ---- the line of units -------------------------------------------------------
-// Sequence b has tiles(b) row tiles of 16, each of units(b) units of keys, for every kv head: in the order
+// Sequence b has tiles(b) row tiles of kM, each of units(b) units of keys, for every kv head: in the order
 // sequence, kv head, row tile, unit.  (Units behind the last key that a tile sees are empty: they differ by the few new tokens.)
 struct FewPlan {
   int64_t begin[kPagedBatch + 1];          // first unit of a sequence
@@ -107,10 +106,11 @@ struct FewItem {
   int u0, u1, units;                       // this piece's units of the item's
 };
 
-__device__ __forceinline__ int few_tiles(const PagedParams& p, const PagedSeq& s) { return (int)(((int64_t)s.n * p.G + kRowsM - 1) / kRowsM); }
+template <int kM>
+__device__ __forceinline__ int few_tiles(const PagedParams& p, const PagedSeq& s) { return (int)(((int64_t)s.n * p.G + kM - 1) / kM); }
 
 // All threads; returns the number of units of the batch.
-template <int kUnit, int kThreads>
+template <int kM, int kUnit, int kThreads>
 __device__ __forceinline__ int64_t few_plan(const PagedParams& p, FewPlan& plan) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t carry = 0;
@@ -121,7 +121,7 @@ __device__ __forceinline__ int64_t few_plan(const PagedParams& p, FewPlan& plan)
       const PagedSeq s = paged_seq(p, b);
       // (rows without a key need an item too: they are written as zeros)
       const int units = max((s.len + kUnit - 1) / kUnit, 1);
-      w = (int64_t)few_tiles(p, s) * units * p.Hkv;
+      w = (int64_t)few_tiles<kM>(p, s) * units * p.Hkv;
     }
     int64_t x = w;
 #pragma unroll
@@ -146,7 +146,7 @@ __device__ __forceinline__ int64_t few_plan(const PagedParams& p, FewPlan& plan)
 }
 
 // The item that has unit `u` of the line, from there on up to `end`.
-template <int kUnit>
+template <int kM, int kUnit>
 __device__ __forceinline__ FewItem few_item(const PagedParams& p, const FewPlan& plan, int64_t u, int64_t end, PagedSeq& s) {
   int lo = 0, n = p.B;
   while (n > 1) {                                           // last b with begin[b] <= u: one with units
@@ -160,7 +160,7 @@ __device__ __forceinline__ FewItem few_item(const PagedParams& p, const FewPlan&
   it.b = lo;
   it.units = max((s.len + kUnit - 1) / kUnit, 1);
   const int64_t at = u - plan.begin[lo], item = at / it.units;
-  const int tiles = few_tiles(p, s);
+  const int tiles = few_tiles<kM>(p, s);
   it.h = (int)(item / tiles);
   it.tile = (int)(item - (int64_t)it.h * tiles);
   it.u0 = (int)(at - item * it.units);
@@ -179,53 +179,148 @@ struct FewArgs {
   const uint8_t *ks, *vs;
   void* out;
   float* lse;
-  float* part;                             // [2 * CTAs][16][D]: outputs of shared items, by CTA: 0 one that others began, 1 one that others end
-  float2* part_ml;                         // [2 * CTAs][16]: {maximum, sum}
+  float* part;                             // [2 * CTAs][kM][D]: outputs of shared items, by CTA: 0 one that others began, 1 one that others end
+  float2* part_ml;                         // [2 * CTAs][kM]: {maximum, sum}
 };
 
 // Packed row (token, head) of row r of a tile, or -1.
+template <int kM>
 __device__ __forceinline__ bool few_row(const PagedParams& p, const PagedSeq& s, int h, int tile, int r, int64_t& token, int& head, int& i) {
-  const int64_t at = (int64_t)tile * kRowsM + r;
+  const int64_t at = (int64_t)tile * kM + r;
   i = (int)(at / p.G);
   head = h * p.G + (int)(at - (int64_t)i * p.G);
   token = (int64_t)s.row0 + i;
   return i < s.n;
 }
 
-template <bool kHalf, int D, int kStore>
-__global__ void __launch_bounds__(kFewThreads, 2) paged_few_kernel(const PagedParams p, const FewArgs a) {
+// kM: rows of a tile, 8 or 16 (the upper half of the MMA's rows is empty with 8, and its exponentials are left out)
+template <bool kHalf, int D, int kStore, int kM>
+__global__ void __launch_bounds__(kFewThreads, FewShape<D, kStore>::kStageBytes > 8192 ? 1 : 2)
+paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const FewArgs a) {
   using S = FewShape<D, kStore>;
-  constexpr bool kCodes = kStore != MOBA_STORE_SAME;
+  constexpr bool kCodes = S::kCodes;
   constexpr bool kF16 = kHalf || kCodes;                    // operands of the MMAs
   constexpr int kSteps = D / 16;                            // k-steps of Q.K^T
   constexpr int kBlocksN = S::kKeys / 8;                    // 8-key blocks of scores
-  extern __shared__ __align__(128) unsigned char smem[];
+  constexpr int kGroups = S::kKeys / 16;                    // groups of 16 keys, each in one page
+  constexpr int kE = kM / 8;                                // rows of this thread: g, and g + 8
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ FewPlan plan;
-  __shared__ float2 warp_ml[kFewWarps][kRowsM];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ float2 warp_ml[kFewWarps][kM];
+  __shared__ uint64_t full[kFewWarps][S::kStages];
+  __shared__ __align__(16) uint8_t scales[kFewWarps][S::kStages][2][32];
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < kFewWarps; ++w)
+      for (int i = 0; i < S::kStages; ++i) mbar_init(smem_u32(&full[w][i]), 1);
+    fence_barrier_init();
+    prefetch_tmap(&tmap_k);
+    prefetch_tmap(&tmap_v);
+  }
   pdl_wait();
   pdl_trigger();
-  const int64_t units = few_plan<S::kUnit, kFewThreads>(p, plan);
+  const int64_t units = few_plan<kM, S::kUnit, kFewThreads>(p, plan);
   const int ctas = few_ctas(units, gridDim.x);
   if ((int)blockIdx.x >= ctas) return;
   const int64_t first = few_cut(units, ctas, blockIdx.x), last = few_cut(units, ctas, blockIdx.x + 1);
-  unsigned char* ring = smem + warp * S::kWarpBytes;
-  const uint32_t sring = ptx::smem_u32(ring);
+  const uint32_t ring = smem_u32(smem) + warp * S::kWarpBytes;
+  // addresses of ldmatrix within a sub-block: row of this lane, pieces in the order of the swizzle
+  const int mrow = lane & 7, mi = lane >> 3;
+  const uint32_t k_row = (uint32_t)((mrow + 8 * (kCodes ? mi : mi >> 1)) * 128), v_row = (uint32_t)((mrow + 8 * (kCodes ? mi : mi & 1)) * 128);
+  constexpr int kPer = kCodes ? 8 : 4;                      // k-steps, or pairs of pieces, of a sub-block
+  uint32_t k_at[kPer], v_at[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    k_at[i] = k_row + (uint32_t)(((kCodes ? i : 2 * i + (mi & 1)) ^ mrow) << 4);
+    v_at[i] = v_row + (uint32_t)(((kCodes ? i : 2 * i + (mi >> 1)) ^ mrow) << 4);
+  }
+  const uint32_t full0 = smem_u32(&full[warp][0]);
+  int st_in = 0, st_out = 0;                                // stages that come next: to be filled, to be read
+  uint32_t phase = 0;                                       // of st_out
+  uint32_t there = 0;                                       // groups in flight that have a page, the oldest block's lowest
+  bool ok = true;
 
   for (int64_t u = first; u < last;) {
     PagedSeq s;
-    const FewItem it = few_item<S::kUnit>(p, plan, u, last, s);
+    const FewItem it = few_item<kM, S::kUnit>(p, plan, u, last, s);
     u += it.u1 - it.u0;
-    // ---- rows of this thread: g and g + 8
-    int lim[2];                                             // keys below are visible
-    float rs[2];                                            // factor of the scores
+    // keys that some row of the tile sees: rows of the last new token see the most, the first row sees the least
+    const int64_t tile_last = min((int64_t)s.n - 1, ((int64_t)(it.tile + 1) * kM - 1) / p.G);
+    const int end = (int)min(max((int64_t)s.pos0 + tile_last + 1, (int64_t)0), (int64_t)s.len);
+    const int all_see = (int)min(max((int64_t)s.pos0 + (int64_t)it.tile * kM / p.G + 1, (int64_t)0), (int64_t)s.len);
+    const int key_of_warp = warp * S::kKeys;
+    // this warp's blocks: unit v of [u0, u1) has keys v * kUnit + key_of_warp ..
+    int blocks = 0;
+    if (end > key_of_warp) blocks = min(it.u1, (end - key_of_warp + S::kUnit - 1) / S::kUnit) - it.u0;
+    blocks = ok ? max(blocks, 0) : 0;
+
+    // ---- copies: the pages of a block are looked up one block ahead of its copies
+    int page[kGroups];
+    auto lookup = [&](int j) {
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr) {
+        const int key = (it.u0 + j) * S::kUnit + key_of_warp + 16 * gr;
+        page[gr] = j < blocks && key < end ? paged_page(p, it.b, key) : -1;
+      }
+    };
+    int waiting = 0;                                        // blocks asked for and not read yet
+    auto copy = [&](int j) {                                // block j into stage st_in; `page` is the block's
+      const uint32_t dst = ring + st_in * S::kStageBytes, bar = full0 + 8 * st_in;
+      const int key0 = (it.u0 + j) * S::kUnit + key_of_warp;
+      // 32 keys in one page come as one box
+      const bool one = kGroups == 2 && p.page_shift > 4;
+      uint32_t got = 0;
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr) got |= (page[gr] >= 0 ? 1u : 0u) << gr;
+      if (lane == 0) {
+        const uint32_t boxes = one ? (got ? 2 : 0) : __popc(got);
+        mbar_expect_tx(bar, boxes * (2 * S::kSubs * 16 * 128 + (kCodes ? 2 * 16 : 0)));
+#pragma unroll
+        for (int gr = 0; gr < kGroups; ++gr) {
+          if (!((got >> gr) & 1) || (one && gr > 0)) continue;
+          const int slot = (key0 + 16 * gr) & ((1 << p.page_shift) - 1);
+#pragma unroll
+          for (int i = 0; i < S::kSubs; ++i) {
+            tma_load_4d(dst + i * S::kSubBytes + gr * 2048, &tmap_k, bar, i * S::kSpan, slot, it.h, page[gr]);
+            tma_load_4d(dst + S::kSideBytes + i * S::kSubBytes + gr * 2048, &tmap_v, bar, i * S::kSpan, slot, it.h, page[gr]);
+          }
+          if (kCodes) {
+            const int64_t at = (((int64_t)page[gr] * p.Hkv + it.h) << p.page_shift) + slot;
+            bulk_load(smem_u32(&scales[warp][st_in][0][16 * gr]), a.ks + at, one ? 32 : 16, bar);
+            bulk_load(smem_u32(&scales[warp][st_in][1][16 * gr]), a.vs + at, one ? 32 : 16, bar);
+          }
+        }
+      }
+      // (both groups of one page; the second may lie behind the keys that are seen, and is masked then)
+      if (one && got) got = 3;
+      there |= got << (kGroups * waiting);
+      ++waiting;
+      st_in = st_in + 1 == S::kStages ? 0 : st_in + 1;
+    };
+    there = 0;
+    lookup(0);
+#pragma unroll
+    for (int j = 0; j < S::kStages - 1; ++j) {
+      if (j < blocks) copy(j);
+      lookup(j + 1);
+    }
+
+    // ---- rows of this thread
+    int lim[kE];                                            // keys below are visible
+    float rs[kE];                                           // factor of the scores
     uint32_t qa[kSteps][4];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
+      if (e >= kE) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) qa[k][e] = qa[k][2 + e] = 0;
+        continue;
+      }
       int64_t token;
       int head, i;
-      const bool on = few_row(p, s, it.h, it.tile, g + 8 * e, token, head, i);
+      const bool on = few_row<kM>(p, s, it.h, it.tile, g + 8 * e, token, head, i);
       lim[e] = on ? (int)min(max((int64_t)s.pos0 + i + 1, (int64_t)0), (int64_t)s.len) : 0;
       const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + token * p.sq_t + head * p.sq_h;
       rs[e] = p.sl2;
@@ -273,93 +368,51 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_few_kernel(const PagedPa
     for (int i = 0; i < D / 8; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
-    // keys that some row of the tile sees: rows of the last new token see the most
-    const int64_t tile_last = min((int64_t)s.n - 1, ((int64_t)(it.tile + 1) * kRowsM - 1) / p.G);
-    const int end = (int)min(max((int64_t)s.pos0 + tile_last + 1, (int64_t)0), (int64_t)s.len);
-    const int key_of_warp = warp * S::kKeys;
-    // this warp's blocks: unit v of [u0, u1) has keys v * kUnit + key_of_warp ..
-    int blocks = 0;
-    if (end > key_of_warp) blocks = min(it.u1, (end - key_of_warp + S::kUnit - 1) / S::kUnit) - it.u0;
-    blocks = max(blocks, 0);
-
-    // ---- copies: the pages of a block are looked up one block ahead of its copies
-    constexpr int kGroups = S::kKeys / 16;                  // groups of 16 keys, each in one page
-    int page[kGroups];
-    auto lookup = [&](int j) {
+    float m[kE], l[kE];
 #pragma unroll
-      for (int gr = 0; gr < kGroups; ++gr) {
-        const int key = (it.u0 + j) * S::kUnit + key_of_warp + 16 * gr;
-        page[gr] = j < blocks && key < end ? paged_page(p, it.b, key) : -1;
-      }
-    };
-    auto copy = [&](int j) {                                // block j into its stage; `page` is the block's
-      const uint32_t dst = sring + (j % S::kStages) * S::kStageBytes;
-      const int key0 = (it.u0 + j) * S::kUnit + key_of_warp;
-      constexpr int kPieces = S::kRowBytes / 16;            // of a row
-      constexpr int kElemPiece = 16 / S::kElem;
-#pragma unroll
-      for (int gr = 0; gr < kGroups; ++gr) {
-        const int id = page[gr];
-        const int slot0 = (key0 + 16 * gr) & ((1 << p.page_shift) - 1);
-        const int64_t kb = id * p.kp_p + slot0 * p.kp_t + it.h * p.kp_h, vb = id * p.vp_p + slot0 * p.vp_t + it.h * p.vp_h;
-#pragma unroll
-        for (int i = 0; i < (16 * kPieces + 31) / 32; ++i) {
-          const int n = lane + 32 * i;
-          const int r = n / kPieces, c = n % kPieces;
-          if ((16 * kPieces) % 32 != 0 && r >= 16) break;
-          // rows nobody sees are zeros: whatever the page holds there, 0 * it stays out of P.V
-          const bool on = id >= 0 && key0 + 16 * gr + r < end;
-          const uint32_t at = (uint32_t)((16 * gr + r) * S::kRowBytes + swizzled<S::kRowBytes>(r, c) * 16);
-          const int64_t off = r * p.kp_t + c * kElemPiece, voff = r * p.vp_t + c * kElemPiece;
-          cp_async_16_or_zero(dst + at, static_cast<const unsigned char*>(a.kp) + (on ? (kb + off) * S::kElem : 0), on);
-          cp_async_16_or_zero(dst + S::kBlockBytes + at, static_cast<const unsigned char*>(a.vp) + (on ? (vb + voff) * S::kElem : 0), on);
-        }
-        if (kCodes && lane < 2) {
-          const int64_t at = id >= 0 ? (((int64_t)id * p.Hkv + it.h) << p.page_shift) + slot0 : 0;
-          cp_async_16_or_zero(dst + 2 * S::kBlockBytes + lane * S::kKeys + 16 * gr, (lane ? a.vs : a.ks) + at, id >= 0);
-        }
-      }
-    };
-    lookup(0);
-#pragma unroll
-    for (int j = 0; j < S::kStages - 1; ++j) {
-      if (j < blocks) copy(j);
-      lookup(j + 1);
-      cp_async_commit();
-    }
+    for (int e = 0; e < kE; ++e) { m[e] = -INFINITY; l[e] = 0.f; }
 
     for (int j = 0; j < blocks; ++j) {
       if (j + S::kStages - 1 < blocks) copy(j + S::kStages - 1);
       lookup(j + S::kStages);
-      cp_async_commit();
-      cp_async_wait<S::kStages - 1>();
-      __syncwarp();
-      const uint32_t sk = sring + (j % S::kStages) * S::kStageBytes, sv = sk + S::kBlockBytes;
+      ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * st_out, phase));
+      if (!ok) {                                            // copies that are under way get time to land
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+        break;
+      }
+      const uint32_t sk = ring + st_out * S::kStageBytes, sv = sk + S::kSideBytes;
       const int key0 = (it.u0 + j) * S::kUnit + key_of_warp;
+      const uint32_t mine = there & ((1u << kGroups) - 1);
+      there >>= kGroups;
+      --waiting;
+      const bool plain = key0 + S::kKeys <= all_see && mine == (1u << kGroups) - 1;
+      if (!plain) {
+        // rows of V that nobody may see are zeros: whatever the page, or the stage, holds there, 0 * it stays out of P.V
+        for (int n = lane; n < S::kKeys * 8; n += 32) {
+          const int r = n >> 3;
+          if (key0 + r < end && ((mine >> (r >> 4)) & 1)) continue;
+#pragma unroll
+          for (int i = 0; i < S::kSubs; ++i)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sv + i * S::kSubBytes + n * 16), "r"(0) : "memory");
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
       // ---- S = Q.K^T
       float sc[kBlocksN][4];
 #pragma unroll
       for (int n = 0; n < kBlocksN; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
-      const int mrow = lane & 7, mi = lane >> 3;            // ldmatrix: row and matrix of this lane's address
-      if (!kCodes) {
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) {                  // matrices: keys 0-7 pieces 2k, 2k + 1, keys 8-15 the same
-          uint32_t b[4];
-          const int r = mrow + 8 * (mi >> 1);
-          ldsm4(sk + r * S::kRowBytes + swizzled<S::kRowBytes>(r, 2 * k + (mi & 1)) * 16, b);
+      for (int k = 0; k < kSteps; ++k) {
+        uint32_t b[4];
+        ldsm4(sk + k_at[k % kPer] + (k / kPer) * S::kSubBytes, b);
+        if (!kCodes) {                                      // matrices: keys 0-7 pieces 2k, 2k + 1, keys 8-15 the same
           mma_16816<kF16>(sc[0], qa[k], b[0], b[1]);
           mma_16816<kF16>(sc[1], qa[k], b[2], b[3]);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {                  // matrices: piece k (16 dims) of keys 0-7, 8-15, 16-23, 24-31
-          uint32_t b[4];
-          const int r = mrow + 8 * mi;
-          ldsm4(sk + r * S::kRowBytes + swizzled<S::kRowBytes>(r & 15, k) * 16, b);
+        } else {                                            // matrices: piece k (16 dims) of keys 0-7, 8-15, 16-23, 24-31
 #pragma unroll
           for (int n = 0; n < kBlocksN; ++n) {
             uint32_t b0, b1;
@@ -368,42 +421,46 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_few_kernel(const PagedPa
           }
         }
       }
-      // ---- x = scores in powers of two (+ the exponent of the V row); running maximum
+      // ---- x = scores in powers of two (+ the exponent of the V row)
       float vinv[kBlocksN][2];
       if (kCodes) {
-        const unsigned char* sb = ring + (j % S::kStages) * S::kStageBytes + 2 * S::kBlockBytes;
+        const uint8_t(*sb)[32] = scales[warp][st_out];
 #pragma unroll
         for (int n = 0; n < kBlocksN; ++n) {
-          const uint32_t kb = *reinterpret_cast<const uint16_t*>(sb + 8 * n + 2 * t4), vb = *reinterpret_cast<const uint16_t*>(sb + S::kKeys + 8 * n + 2 * t4);
+          const uint32_t kb = *reinterpret_cast<const uint16_t*>(sb[0] + 8 * n + 2 * t4), vb = *reinterpret_cast<const uint16_t*>(sb[1] + 8 * n + 2 * t4);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const uint32_t ke = (kb >> (8 * c)) & 255, ve = (vb >> (8 * c)) & 255;
             const float kf = paged_scale(ke), vf = (float)((int)ve - 127);
             vinv[n][c] = ve == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((254u - ve) << 23);
-            sc[n][c] = fmaf(sc[n][c], rs[0] * kf, vf);
-            sc[n][2 + c] = fmaf(sc[n][2 + c], rs[1] * kf, vf);
+#pragma unroll
+            for (int e = 0; e < kE; ++e) sc[n][2 * e + c] = fmaf(sc[n][2 * e + c], rs[e] * kf, vf);
           }
         }
       } else {
 #pragma unroll
         for (int n = 0; n < kBlocksN; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[n][e] *= p.sl2;
+          for (int e = 0; e < 2 * kE; ++e) sc[n][e] *= p.sl2;
       }
-      int there[kGroups];
+      if (!plain) {
 #pragma unroll
-      for (int gr = 0; gr < kGroups; ++gr) there[gr] = key0 + 16 * gr < end && paged_page(p, it.b, key0 + 16 * gr) >= 0;
+        for (int n = 0; n < kBlocksN; ++n)
 #pragma unroll
-      for (int n = 0; n < kBlocksN; ++n)
+          for (int c = 0; c < 2; ++c) {
+            const int key = key0 + 8 * n + 2 * t4 + c;
+            const bool here = (mine >> (n >> 1)) & 1;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int key = key0 + 8 * n + 2 * t4 + c;
-          if (key >= lim[0] || !there[n >> 1]) sc[n][c] = -INFINITY;
-          if (key >= lim[1] || !there[n >> 1]) sc[n][2 + c] = -INFINITY;
-        }
-      float alpha[2];
+            for (int e = 0; e < kE; ++e)
+              if (key >= lim[e] || !here) sc[n][2 * e + c] = -INFINITY;
+            if (key >= end || !here) vinv[n][c] = 0.f;
+          }
+      }
+      // ---- running maximum
+      bool moved = false;
+      float alpha[kE];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < kE; ++e) {
         float mx = -INFINITY;
 #pragma unroll
         for (int n = 0; n < kBlocksN; ++n) mx = fmaxf(mx, fmaxf(sc[n][2 * e], sc[n][2 * e + 1]));
@@ -413,53 +470,47 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_few_kernel(const PagedPa
         if (mx > m[e] + 8.f) {
           alpha[e] = exp2f(m[e] - mx);                      // (0 the first time)
           m[e] = mx;
+          moved = true;
         }
       }
-      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+      if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          o[i][0] *= alpha[0]; o[i][1] *= alpha[0];
-          o[i][2] *= alpha[1]; o[i][3] *= alpha[1];
+        for (int e = 0; e < kE; ++e) {
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            o[i][2 * e] *= alpha[e];
+            o[i][2 * e + 1] *= alpha[e];
+          }
+          l[e] *= alpha[e];
         }
-        l[0] *= alpha[0];
-        l[1] *= alpha[1];
       }
       uint32_t pa[kGroups][4];
-      // a row that has seen nothing yet has no reference: any finite one leaves its weights at 0
-      const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
 #pragma unroll
-      for (int n = 0; n < kBlocksN; ++n) {
-        const float w0 = ptx::ex2_approx(sc[n][0] - m0), w1 = ptx::ex2_approx(sc[n][1] - m0);
-        const float w2 = ptx::ex2_approx(sc[n][2] - m1), w3 = ptx::ex2_approx(sc[n][3] - m1);
-        if (kCodes) {
-          l[0] += w0 == 0.f ? 0.f : w0 * vinv[n][0];
-          l[0] += w1 == 0.f ? 0.f : w1 * vinv[n][1];
-          l[1] += w2 == 0.f ? 0.f : w2 * vinv[n][0];
-          l[1] += w3 == 0.f ? 0.f : w3 * vinv[n][1];
-        } else {
-          l[0] += w0 + w1;
-          l[1] += w2 + w3;
+      for (int e = 0; e < 2; ++e) {
+        if (e >= kE) {
+#pragma unroll
+          for (int gr = 0; gr < kGroups; ++gr) pa[gr][1] = pa[gr][3] = 0;
+          continue;
         }
-        pa[n >> 1][(n & 1) * 2] = pack2_16<kF16>(w0, w1);
-        pa[n >> 1][(n & 1) * 2 + 1] = pack2_16<kF16>(w2, w3);
+        // a row that has seen nothing yet has no reference: any finite one leaves its weights at 0
+        const float ref = m[e] == -INFINITY ? 0.f : m[e];
+#pragma unroll
+        for (int n = 0; n < kBlocksN; ++n) {
+          const float w0 = ex2_approx(sc[n][2 * e] - ref), w1 = ex2_approx(sc[n][2 * e + 1] - ref);
+          l[e] += kCodes ? w0 * vinv[n][0] + w1 * vinv[n][1] : w0 + w1;
+          pa[n >> 1][(n & 1) * 2 + e] = pack2_16<kF16>(w0, w1);
+        }
       }
       // ---- O += P.V
-      if (!kCodes) {
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {                  // matrices: keys 0-7, 8-15 of pieces 2i, the same of 2i + 1
-          uint32_t b[4];
-          const int r = mrow + 8 * (mi & 1);
-          ldsm4_t(sv + r * S::kRowBytes + swizzled<S::kRowBytes>(r, 2 * i + (mi >> 1)) * 16, b);
+      for (int i = 0; i < D / 16; ++i) {
+        uint32_t b[4];
+        ldsm4_t(sv + v_at[i % kPer] + (i / kPer) * S::kSubBytes, b);
+        if (!kCodes) {                                      // matrices: keys 0-7, 8-15 of pieces 2i, the same of 2i + 1
           mma_16816<kF16>(o[2 * i], pa[0], b[0], b[1]);
           mma_16816<kF16>(o[2 * i + 1], pa[0], b[2], b[3]);
-        }
-      } else {
-        // pairs of dims are the 16-bit elements of a matrix: piece i gives the even dims of 16, and the odd ones
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {                  // matrices: keys 0-7, 8-15, 16-23, 24-31 of piece i
-          uint32_t b[4];
-          const int r = mrow + 8 * mi;
-          ldsm4_t(sv + r * S::kRowBytes + swizzled<S::kRowBytes>(r & 15, i) * 16, b);
+        } else {
+          // matrices: keys 0-7, 8-15, 16-23, 24-31 of piece i; pairs of dims are their 16-bit elements: the even dims of 16, and the odd ones
 #pragma unroll
           for (int gr = 0; gr < kGroups; ++gr) {
             uint32_t e0, o0, e1, o1;
@@ -470,25 +521,22 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_few_kernel(const PagedPa
           }
         }
       }
+      if (++st_out == S::kStages) { st_out = 0; phase ^= 1; }
       __syncwarp();
     }
 
     // ---- the warps' results, joined by all threads
-    cp_async_wait<0>();
+    float* so = reinterpret_cast<float*>(smem + warp * S::kWarpBytes);                            // [kM][D]
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int e = 0; e < kE; ++e) {
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-      // a row with a score that is not a number has no maximum to speak of: with this one it stays NaN in every join
-      if (l[e] != l[e]) m[e] = INFINITY;
+      // a row with a score that is not a number has no maximum to speak of: with this one it stays NaN in every join (so does one whose
+      // copies did not arrive in time)
+      if (l[e] != l[e] || !ok) { m[e] = INFINITY; l[e] = __uint_as_float(0x7fc00000u); }
       if (t4 == 0) warp_ml[warp][g + 8 * e] = make_float2(m[e], l[e]);
-    }
-    __syncwarp();
-    float* so = reinterpret_cast<float*>(ring);             // [16][D]
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int i = 0; i < D / 8; ++i) {
         if (!kCodes) {
           *reinterpret_cast<float2*>(so + (g + 8 * e) * D + 8 * i + 2 * t4) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
         } else {                                            // column c of blocks 2i, 2i + 1: dims 2c, 2c + 1 of 16
@@ -497,14 +545,15 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_few_kernel(const PagedPa
           at[2 * (2 * t4 + 1)] = o[i][2 * e + 1];
         }
       }
+    }
     __syncthreads();
     const bool whole = it.u0 == 0 && it.u1 == it.units;
     const int64_t slot = 2 * (int64_t)blockIdx.x + (it.u0 == 0 ? 1 : 0);
-    for (int n = threadIdx.x; n < kRowsM * (D / 4); n += kFewThreads) {
+    for (int n = threadIdx.x; n < kM * (D / 4); n += kFewThreads) {
       const int r = n / (D / 4), c = n % (D / 4) * 4;
       int64_t token;
       int head, i;
-      if (!few_row(p, s, it.h, it.tile, r, token, head, i)) continue;
+      if (!few_row<kM>(p, s, it.h, it.tile, r, token, head, i)) continue;
       float mx = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kFewWarps; ++w) mx = fmaxf(mx, warp_ml[w][r].x);
@@ -526,43 +575,44 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_few_kernel(const PagedPa
         *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + token * p.so_t + head * p.so_h + c) = y;
         if (a.lse != nullptr && c == 0) a.lse[(int64_t)head * p.T + token] = (mx + log2f(sum)) * kLn2;
       } else {
-        *reinterpret_cast<float4*>(a.part + (slot * kRowsM + r) * D + c) = make_float4(x[0], x[1], x[2], x[3]);
-        if (c == 0) a.part_ml[slot * kRowsM + r] = make_float2(mx, sum);
+        *reinterpret_cast<float4*>(a.part + (slot * kM + r) * D + c) = make_float4(x[0], x[1], x[2], x[3]);
+        if (c == 0) a.part_ml[slot * kM + r] = make_float2(mx, sum);
       }
     }
+    fence_proxy_async_smem();                               // the ring is copied to again
     __syncthreads();
   }
 }
 
 // Joins the pieces of the items that several CTAs share.  Block c: the item that CTA c began and did not end.
-template <bool kHalf, int D, int kStore>
+template <bool kHalf, int D, int kStore, int kM>
 __global__ void __launch_bounds__(kFewThreads) paged_few_join_kernel(const PagedParams p, const FewArgs a, int grid) {
   using S = FewShape<D, kStore>;
   __shared__ FewPlan plan;
   pdl_wait();
   pdl_trigger();
-  const int64_t units = few_plan<S::kUnit, kFewThreads>(p, plan);
+  const int64_t units = few_plan<kM, S::kUnit, kFewThreads>(p, plan);
   const int ctas = few_ctas(units, grid);
   const int c0 = blockIdx.x;
   if (c0 >= ctas) return;
   const int64_t first = few_cut(units, ctas, c0), last = few_cut(units, ctas, c0 + 1);
   if (last <= first || last >= units) return;
   PagedSeq s;
-  const FewItem it = few_item<S::kUnit>(p, plan, last - 1, last, s);
+  const FewItem it = few_item<kM, S::kUnit>(p, plan, last - 1, last, s);
   const int64_t begin = last - 1 - it.u0, end = begin + it.units;
   if (begin < first || end <= last) return;                 // begun before, or ended here
   int c1 = c0 + 1;                                          // the CTA that ends it
   while (few_cut(units, ctas, c1 + 1) < end) ++c1;
-  for (int n = threadIdx.x; n < kRowsM * (D / 4); n += kFewThreads) {
+  for (int n = threadIdx.x; n < kM * (D / 4); n += kFewThreads) {
     const int r = n / (D / 4), c = n % (D / 4) * 4;
     int64_t token;
     int head, i;
-    if (!few_row(p, s, it.h, it.tile, r, token, head, i)) continue;
+    if (!few_row<kM>(p, s, it.h, it.tile, r, token, head, i)) continue;
     float mx = -INFINITY, sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
     for (int cc = c0; cc <= c1; ++cc) {
       const int64_t slot = 2 * (int64_t)cc + (cc == c0 ? 1 : 0);
-      const float2 ml = __ldcg(a.part_ml + slot * kRowsM + r);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part + (slot * kRowsM + r) * D + c));
+      const float2 ml = __ldcg(a.part_ml + slot * kM + r);
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part + (slot * kM + r) * D + c));
       if (ml.x == -INFINITY) continue;
       const float up = fmaxf(mx, ml.x), f0 = exp2f(mx - up), f1 = exp2f(ml.x - up);
       mx = up;
@@ -580,48 +630,58 @@ __global__ void __launch_bounds__(kFewThreads) paged_few_join_kernel(const Paged
 }
 
 struct FewKernels {
-  void (*attend)(const PagedParams, const FewArgs);
+  void (*attend)(const PagedParams, const CUtensorMap, const CUtensorMap, const FewArgs);
   void (*join)(const PagedParams, const FewArgs, int);
   size_t smem;
+  int per_sm;
 };
-template <bool kHalf, int D, int kStore>
+template <bool kHalf, int D, int kStore, int kM>
 FewKernels few_kernels() {
-  return FewKernels{paged_few_kernel<kHalf, D, kStore>, paged_few_join_kernel<kHalf, D, kStore>, FewShape<D, kStore>::kSmem};
+  using S = FewShape<D, kStore>;
+  return FewKernels{paged_few_kernel<kHalf, D, kStore, kM>, paged_few_join_kernel<kHalf, D, kStore, kM>, S::kSmem, S::kStageBytes > 8192 ? 1 : 2};
 }
-template <bool kHalf, int D>
+template <bool kHalf, int D, int kM>
 FewKernels pick_few(int store) {
-  return store == MOBA_STORE_SAME ? few_kernels<kHalf, D, MOBA_STORE_SAME>() : store == MOBA_STORE_E4M3 ? few_kernels<kHalf, D, MOBA_STORE_E4M3>()
-                                                                             : few_kernels<kHalf, D, MOBA_STORE_INT8>();
+  return store == MOBA_STORE_SAME ? few_kernels<kHalf, D, MOBA_STORE_SAME, kM>() : store == MOBA_STORE_E4M3 ? few_kernels<kHalf, D, MOBA_STORE_E4M3, kM>()
+                                                                                 : few_kernels<kHalf, D, MOBA_STORE_INT8, kM>();
 }
-template <bool kHalf>
+template <bool kHalf, int kM>
 FewKernels pick_few_dim(int D, int store) {
-  return D == 64 ? pick_few<kHalf, 64>(store) : D == 96 ? pick_few<kHalf, 96>(store) : D == 128 ? pick_few<kHalf, 128>(store)
-                                                                                               : pick_few<kHalf, 256>(store);
+  return D == 64 ? pick_few<kHalf, 64, kM>(store) : D == 96 ? pick_few<kHalf, 96, kM>(store) : D == 128 ? pick_few<kHalf, 128, kM>(store)
+                                                                                                       : pick_few<kHalf, 256, kM>(store);
 }
 
 constexpr int kFewMaxCtas = 148 * 2;
 
 }  // namespace
 
-size_t paged_few_workspace(const PagedParams& p) { return (size_t)2 * kFewMaxCtas * kRowsM * (p.D * sizeof(float) + sizeof(float2)); }
+size_t paged_few_workspace(const PagedParams& p) { return (size_t)2 * kFewMaxCtas * 16 * (p.D * sizeof(float) + sizeof(float2)); }
 
 cudaError_t launch_paged_few(const PagedParams& all, const void* q, const void* kp, const void* vp, const uint8_t* ks,
                              const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st) {
-  const FewKernels k = all.fp16 ? pick_few_dim<true>(all.D, all.store) : pick_few_dim<false>(all.D, all.store);
+  const bool eight = (int64_t)all.max_new * all.G <= 8;
+  const FewKernels k = all.fp16 ? (eight ? pick_few_dim<true, 8>(all.D, all.store) : pick_few_dim<true, 16>(all.D, all.store))
+                                : (eight ? pick_few_dim<false, 8>(all.D, all.store) : pick_few_dim<false, 16>(all.D, all.store));
   FewArgs a{q, kp, vp, ks, vs, out, lse, nullptr, nullptr};
   a.part_ml = static_cast<float2*>(workspace);
-  a.part = reinterpret_cast<float*>(a.part_ml + 2 * kFewMaxCtas * kRowsM);
+  a.part = reinterpret_cast<float*>(a.part_ml + 2 * kFewMaxCtas * 16);
+  const int slots = 1 << all.page_shift, box = all.store == MOBA_STORE_SAME || slots < 32 ? 16 : 32;
+  const int elem = all.store != MOBA_STORE_SAME ? 1 : all.fp16 ? 2 : 3;
+  CUtensorMap mk, mv;
+  if (!make_page_map(&mk, elem, all.D, kp, all.pages, slots, all.Hkv, all.kp_p, all.kp_t, all.kp_h, box) ||
+      !make_page_map(&mv, elem, all.D, vp, all.pages, slots, all.Hkv, all.vp_p, all.vp_t, all.vp_h, box))
+    return cudaErrorNotSupported;
   cudaError_t e = prepare_kernel(k.attend, k.smem, nullptr, true);
   if (e != cudaSuccess) return e;
   const int sms = device_info().sms;
-  const int grid = 2 * sms < kFewMaxCtas ? 2 * sms : kFewMaxCtas;
+  const int grid = k.per_sm * sms < kFewMaxCtas ? k.per_sm * sms : kFewMaxCtas;
   for (int b = 0; b < all.B; b += kPagedBatch) {
     PagedParams p = all;
     p.B = all.B - b < kPagedBatch ? all.B - b : kPagedBatch;
     p.cu += b;
     p.lens += b;
     p.table += b * all.table_stride;
-    if ((e = launch_pdl(k.attend, dim3(grid), kFewThreads, k.smem, st, p, a)) != cudaSuccess) return e;
+    if ((e = launch_pdl(k.attend, dim3(grid), kFewThreads, k.smem, st, p, mk, mv, a)) != cudaSuccess) return e;
     if ((e = launch_pdl(k.join, dim3(grid), kFewThreads, 0, st, p, a, grid)) != cudaSuccess) return e;
   }
   return cudaSuccess;

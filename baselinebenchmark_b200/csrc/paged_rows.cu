@@ -24,7 +24,7 @@
 
 namespace moba {
 
-bool make_page_map(CUtensorMap* m, bool fp16, int D, const void* base, int pages, int slots, int H, int64_t sp, int64_t st, int64_t sh,
+bool make_page_map(CUtensorMap* m, int elem, int D, const void* base, int pages, int slots, int H, int64_t sp, int64_t st, int64_t sh,
                    int box_rows);
 
 namespace {
@@ -1074,8 +1074,8 @@ cudaError_t launch_paged_rows(const PagedParams& all, const void* q, const void*
   CUtensorMap mk{}, mv{};
   if (all.store == MOBA_STORE_SAME) {
     const int slots = 1 << all.page_shift, box = slots < kBN ? slots : kBN;
-    if (!make_page_map(&mk, all.fp16 != 0, all.D, kp, all.pages, slots, all.Hkv, all.kp_p, all.kp_t, all.kp_h, box) ||
-        !make_page_map(&mv, all.fp16 != 0, all.D, vp, all.pages, slots, all.Hkv, all.vp_p, all.vp_t, all.vp_h, box))
+    if (!make_page_map(&mk, all.fp16 ? 2 : 3, all.D, kp, all.pages, slots, all.Hkv, all.kp_p, all.kp_t, all.kp_h, box) ||
+        !make_page_map(&mv, all.fp16 ? 2 : 3, all.D, vp, all.pages, slots, all.Hkv, all.vp_p, all.vp_t, all.vp_h, box))
       return cudaErrorNotSupported;
   }
   const int sms = device_info().sms;
