@@ -1545,6 +1545,21 @@ bool make_page_map(CUtensorMap* m, int elem, int D, const void* base, int pages,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// the same pool with its dims in `subs` parts of 128 bytes, [pages][H][subs][slots][128 bytes]: a box has all parts of its slots
+bool make_page_parts_map(CUtensorMap* m, int elem, int subs, const void* base, int pages, int slots, int H, int64_t sp, int64_t st,
+                         int64_t sh, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t bytes = elem == 1 ? 1 : 2;
+  const cuuint64_t dims[5] = {128 / bytes, (cuuint64_t)slots, (cuuint64_t)subs, (cuuint64_t)H, (cuuint64_t)pages};
+  const cuuint64_t strides[4] = {(cuuint64_t)st * bytes, 128, (cuuint64_t)sh * bytes, (cuuint64_t)sp * bytes};
+  const cuuint32_t box[5] = {(cuuint32_t)(128 / bytes), (cuuint32_t)box_rows, (cuuint32_t)subs, 1, 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return fn(m, elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
+            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 cudaError_t launch_bounded_wait_probe(int32_t* status, unsigned long long limit_ns, cudaStream_t st) {
   bounded_wait_probe_kernel<<<1, 32, 0, st>>>(status, limit_ns);
   return cudaGetLastError();

@@ -25,6 +25,8 @@ namespace moba {
 
 bool make_page_map(CUtensorMap* m, int elem, int D, const void* base, int pages, int slots, int H, int64_t sp, int64_t st, int64_t sh,
                    int box_rows);
+bool make_page_parts_map(CUtensorMap* m, int elem, int subs, const void* base, int pages, int slots, int H, int64_t sp, int64_t st,
+                         int64_t sh, int box_rows);
 
 namespace {
 
@@ -41,8 +43,11 @@ template <int D, int kStore> struct FewShape {
   static constexpr int kSubBytes = kKeys * 128;
   static constexpr int kSideBytes = kSubs * kSubBytes;               // K; V behind it
   static constexpr int kStageBytes = 2 * kSideBytes;
-  // about 24 KB a warp: two CTAs, eight warps, have 130 KB and more on their way to an SM
-  static constexpr int kStages = kStageBytes == 16384 ? 3 : kStageBytes == 8192 ? 3 : 6;
+  static constexpr bool kParts = !kCodes && kSubs > 1 && D % kSpan == 0;   // one box has all sub-blocks (not of head dim 96: a row's would end in the next)
+  // three CTAs, twelve warps, an SM with 16 KB of stages each (one CTA with 48 KB at head dim 256): what a warp waits for is its own chain of
+  // instructions, and there have to be others meanwhile
+  static constexpr int kCtas = kStageBytes == 16384 ? 1 : 3;
+  static constexpr int kStages = kStageBytes == 16384 ? 3 : kStageBytes == 8192 ? 2 : 4;
   static constexpr int kWarpBytes = kStages * kStageBytes;
   static constexpr int kUnit = kKeys * kFewWarps;                    // keys of a CTA's unit
   static constexpr size_t kSmem = 1024 + (size_t)kFewWarps * kWarpBytes;
@@ -195,7 +200,7 @@ __device__ __forceinline__ bool few_row(const PagedParams& p, const PagedSeq& s,
 
 // kM: rows of a tile, 8 or 16 (the upper half of the MMA's rows is empty with 8, and its exponentials are left out)
 template <bool kHalf, int D, int kStore, int kM>
-__global__ void __launch_bounds__(kFewThreads, FewShape<D, kStore>::kStageBytes > 8192 ? 1 : 2)
+__global__ void __launch_bounds__(kFewThreads, FewShape<D, kStore>::kCtas)
 paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const FewArgs a) {
   using S = FewShape<D, kStore>;
   constexpr bool kCodes = S::kCodes;
@@ -257,12 +262,14 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
     blocks = ok ? max(blocks, 0) : 0;
 
     // ---- copies: the pages of a block are looked up one block ahead of its copies
-    int page[kGroups];
+    int page[kGroups];                                      // as the table has them: they are looked at when the copies are asked for
+    const int32_t* row = p.table + (int64_t)it.b * p.table_stride;
     auto lookup = [&](int j) {
 #pragma unroll
       for (int gr = 0; gr < kGroups; ++gr) {
         const int key = (it.u0 + j) * S::kUnit + key_of_warp + 16 * gr;
-        page[gr] = j < blocks && key < end ? paged_page(p, it.b, key) : -1;
+        page[gr] = -1;
+        if (j < blocks && key < end) page[gr] = __ldg(row + (key >> p.page_shift));   // (end <= the table's reach)
       }
     };
     int waiting = 0;                                        // blocks asked for and not read yet
@@ -273,7 +280,7 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
       const bool one = kGroups == 2 && p.page_shift > 4;
       uint32_t got = 0;
 #pragma unroll
-      for (int gr = 0; gr < kGroups; ++gr) got |= (page[gr] >= 0 ? 1u : 0u) << gr;
+      for (int gr = 0; gr < kGroups; ++gr) got |= ((unsigned)page[gr] < (unsigned)p.pages ? 1u : 0u) << gr;
       if (lane == 0) {
         const uint32_t boxes = one ? (got ? 2 : 0) : __popc(got);
         mbar_expect_tx(bar, boxes * (2 * S::kSubs * 16 * 128 + (kCodes ? 2 * 16 : 0)));
@@ -281,10 +288,15 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
         for (int gr = 0; gr < kGroups; ++gr) {
           if (!((got >> gr) & 1) || (one && gr > 0)) continue;
           const int slot = (key0 + 16 * gr) & ((1 << p.page_shift) - 1);
+          if constexpr (S::kParts) {
+            tma_load_5d(dst, &tmap_k, bar, 0, slot, 0, it.h, page[gr]);
+            tma_load_5d(dst + S::kSideBytes, &tmap_v, bar, 0, slot, 0, it.h, page[gr]);
+          } else {
 #pragma unroll
-          for (int i = 0; i < S::kSubs; ++i) {
-            tma_load_4d(dst + i * S::kSubBytes + gr * 2048, &tmap_k, bar, i * S::kSpan, slot, it.h, page[gr]);
-            tma_load_4d(dst + S::kSideBytes + i * S::kSubBytes + gr * 2048, &tmap_v, bar, i * S::kSpan, slot, it.h, page[gr]);
+            for (int i = 0; i < S::kSubs; ++i) {
+              tma_load_4d(dst + i * S::kSubBytes + gr * 2048, &tmap_k, bar, i * S::kSpan, slot, it.h, page[gr]);
+              tma_load_4d(dst + S::kSideBytes + i * S::kSubBytes + gr * 2048, &tmap_v, bar, i * S::kSpan, slot, it.h, page[gr]);
+            }
           }
           if (kCodes) {
             const int64_t at = (((int64_t)page[gr] * p.Hkv + it.h) << p.page_shift) + slot;
@@ -634,11 +646,12 @@ struct FewKernels {
   void (*join)(const PagedParams, const FewArgs, int);
   size_t smem;
   int per_sm;
+  bool parts;                              // of the tensor maps
 };
 template <bool kHalf, int D, int kStore, int kM>
 FewKernels few_kernels() {
   using S = FewShape<D, kStore>;
-  return FewKernels{paged_few_kernel<kHalf, D, kStore, kM>, paged_few_join_kernel<kHalf, D, kStore, kM>, S::kSmem, S::kStageBytes > 8192 ? 1 : 2};
+  return FewKernels{paged_few_kernel<kHalf, D, kStore, kM>, paged_few_join_kernel<kHalf, D, kStore, kM>, S::kSmem, S::kCtas, S::kParts};
 }
 template <bool kHalf, int D, int kM>
 FewKernels pick_few(int store) {
@@ -651,7 +664,7 @@ FewKernels pick_few_dim(int D, int store) {
                                                                                                        : pick_few<kHalf, 256, kM>(store);
 }
 
-constexpr int kFewMaxCtas = 148 * 2;
+constexpr int kFewMaxCtas = 148 * 3;
 
 }  // namespace
 
@@ -668,8 +681,11 @@ cudaError_t launch_paged_few(const PagedParams& all, const void* q, const void* 
   const int slots = 1 << all.page_shift, box = all.store == MOBA_STORE_SAME || slots < 32 ? 16 : 32;
   const int elem = all.store != MOBA_STORE_SAME ? 1 : all.fp16 ? 2 : 3;
   CUtensorMap mk, mv;
-  if (!make_page_map(&mk, elem, all.D, kp, all.pages, slots, all.Hkv, all.kp_p, all.kp_t, all.kp_h, box) ||
-      !make_page_map(&mv, elem, all.D, vp, all.pages, slots, all.Hkv, all.vp_p, all.vp_t, all.vp_h, box))
+  const bool ok = k.parts ? make_page_parts_map(&mk, elem, all.D / 64, kp, all.pages, slots, all.Hkv, all.kp_p, all.kp_t, all.kp_h, box) &&
+                                make_page_parts_map(&mv, elem, all.D / 64, vp, all.pages, slots, all.Hkv, all.vp_p, all.vp_t, all.vp_h, box)
+                          : make_page_map(&mk, elem, all.D, kp, all.pages, slots, all.Hkv, all.kp_p, all.kp_t, all.kp_h, box) &&
+                                make_page_map(&mv, elem, all.D, vp, all.pages, slots, all.Hkv, all.vp_p, all.vp_t, all.vp_h, box);
+  if (!ok)
     return cudaErrorNotSupported;
   cudaError_t e = prepare_kernel(k.attend, k.smem, nullptr, true);
   if (e != cudaSuccess) return e;
