@@ -126,7 +126,7 @@ def lib() -> C.CDLL:
         handle.moba_cp_poll.argtypes = [vp, C.POINTER(C.c_int32)]
         handle.moba_cp_abort.argtypes = [vp]
         handle.moba_selftest_bounded_wait.argtypes = [i32p, C.c_uint32, vp]
-        pg = C.POINTER(Paged)
+        pg = vp                              # a Paged by reference, or its bytes
         handle.moba_paged_check.argtypes = [pg]
         handle.moba_paged_store.argtypes = [pg, vp, vp, i32p, i32p, i32p, vp, vp, vp, vp, vp]
         handle.moba_paged_load.argtypes = [pg, i32p, i32p, i32p, vp, vp, vp, vp, vp, vp, vp]

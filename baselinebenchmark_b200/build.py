@@ -22,7 +22,7 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     deps = srcs + list((PKG / "csrc").glob("*.cuh")) + [ROOT / "include" / "moba_b200.h"]
     if not force and LIB.exists() and all(LIB.stat().st_mtime >= d.stat().st_mtime for d in deps):
         return LIB
-    cmd = [nvcc(), "-shared", "-Xcompiler", "-fPIC", "-O3", "-std=c++17", "-lineinfo",
+    cmd = [nvcc(), "-shared", "-Xcompiler", "-fPIC", "-O3", "-std=c++17", "-lineinfo", "--threads", "0",
            "-gencode", "arch=compute_100a,code=sm_100a",
            "-I", str(ROOT / "include"), "-I", str(PKG / "csrc"),
            "-o", str(LIB)] + [str(s) for s in srcs] + ["-ldl"]

@@ -33,6 +33,7 @@ namespace {
 using namespace ptx;
 
 constexpr int kFewWarps = 4, kFewThreads = kFewWarps * 32;
+constexpr int kFewMaxCtas = 148 * 3;
 constexpr float kLn2 = 0.6931471805599453f;
 
 template <int D, int kStore> struct FewShape {
@@ -104,7 +105,7 @@ __device__ __forceinline__ void codes_to_half(uint32_t x, uint32_t& lo, uint32_t
 // sequence, kv head, row tile, unit.  (Units behind the last key that a tile sees are empty: they differ by the few new tokens.)
 struct FewPlan {
   int64_t begin[kPagedBatch + 1];          // first unit of a sequence
-  int64_t scan[kFewThreads / 32];
+  int64_t scan[16];
 };
 struct FewItem {
   int b, h, tile;
@@ -596,14 +597,19 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
   }
 }
 
-// Joins the pieces of the items that several CTAs share.  Block c: the item that CTA c began and did not end.
+// Joins the pieces of the items that several CTAs share.  Block c: the item that CTA c began and did not end.  A few long sequences
+// have a hundred pieces an item: threads in groups take every so many of them, their sums are added in the order of the groups.
+constexpr int kJoinThreads = 512;
 template <bool kHalf, int D, int kStore, int kM>
-__global__ void __launch_bounds__(kFewThreads) paged_few_join_kernel(const PagedParams p, const FewArgs a, int grid) {
+__global__ void __launch_bounds__(kJoinThreads) paged_few_join_kernel(const PagedParams p, const FewArgs a, int grid) {
   using S = FewShape<D, kStore>;
   __shared__ FewPlan plan;
+  __shared__ float weight[kFewMaxCtas][kM];
+  __shared__ float most[kM], total[kM];
+  __shared__ float4 sums[kJoinThreads];
   pdl_wait();
   pdl_trigger();
-  const int64_t units = few_plan<kM, S::kUnit, kFewThreads>(p, plan);
+  const int64_t units = few_plan<kM, S::kUnit, kJoinThreads>(p, plan);
   const int ctas = few_ctas(units, grid);
   const int c0 = blockIdx.x;
   if (c0 >= ctas) return;
@@ -613,31 +619,68 @@ __global__ void __launch_bounds__(kFewThreads) paged_few_join_kernel(const Paged
   const FewItem it = few_item<kM, S::kUnit>(p, plan, last - 1, last, s);
   const int64_t begin = last - 1 - it.u0, end = begin + it.units;
   if (begin < first || end <= last) return;                 // begun before, or ended here
-  int c1 = c0 + 1;                                          // the CTA that ends it
-  while (few_cut(units, ctas, c1 + 1) < end) ++c1;
-  for (int n = threadIdx.x; n < kM * (D / 4); n += kFewThreads) {
+  // CTAs that begin before the item's end: [c0, c0 + pieces)
+  int lo = c0 + 1, hi = ctas;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (few_cut(units, ctas, mid) < end) lo = mid; else hi = mid;
+  }
+  const int pieces = lo - c0 + 1;
+  auto slot = [&](int k) { return 2 * (int64_t)(c0 + k) + (k == 0 ? 1 : 0); };
+  const int rows = (int)min((int64_t)kM, (int64_t)s.n * p.G - (int64_t)it.tile * kM);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // ---- weights of the pieces, a warp a row
+  for (int r = warp; r < rows; r += kJoinThreads / 32) {
+    float mx = -INFINITY;
+    for (int k = lane; k < pieces; k += 32) mx = fmaxf(mx, __ldcg(a.part_ml + slot(k) * kM + r).x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    float sum = 0.f;
+    for (int k = lane; k < pieces; k += 32) {
+      const float2 ml = __ldcg(a.part_ml + slot(k) * kM + r);
+      const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mx);
+      weight[k][r] = f;
+      if (f != 0.f) sum += f * ml.y;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) { most[r] = mx; total[r] = sum; }
+  }
+  __syncthreads();
+  const int outputs = rows * (D / 4);
+  const int groups = outputs >= kJoinThreads ? 1 : kJoinThreads / outputs;
+  const int group = outputs >= kJoinThreads ? 0 : threadIdx.x / outputs;
+  for (int n = outputs >= kJoinThreads ? threadIdx.x : threadIdx.x % outputs; n < outputs; n += kJoinThreads) {
     const int r = n / (D / 4), c = n % (D / 4) * 4;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (group < groups) {
+#pragma unroll 4
+      for (int k = group; k < pieces; k += groups) {
+        const float f = weight[k][r];
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part + (slot(k) * kM + r) * D + c));
+        // (a piece that saw nothing has no weight; what it holds is no number that counts)
+        x[0] += f == 0.f ? 0.f : f * v.x; x[1] += f == 0.f ? 0.f : f * v.y;
+        x[2] += f == 0.f ? 0.f : f * v.z; x[3] += f == 0.f ? 0.f : f * v.w;
+      }
+    }
+    if (groups > 1) {
+      sums[threadIdx.x] = make_float4(x[0], x[1], x[2], x[3]);
+      __syncthreads();
+      if (group != 0) break;
+      for (int k = 1; k < groups; ++k) {
+        const float4 v = sums[k * outputs + n];
+        x[0] += v.x; x[1] += v.y; x[2] += v.z; x[3] += v.w;
+      }
+    }
     int64_t token;
     int head, i;
-    if (!few_row<kM>(p, s, it.h, it.tile, r, token, head, i)) continue;
-    float mx = -INFINITY, sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int cc = c0; cc <= c1; ++cc) {
-      const int64_t slot = 2 * (int64_t)cc + (cc == c0 ? 1 : 0);
-      const float2 ml = __ldcg(a.part_ml + slot * kM + r);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part + (slot * kM + r) * D + c));
-      if (ml.x == -INFINITY) continue;
-      const float up = fmaxf(mx, ml.x), f0 = exp2f(mx - up), f1 = exp2f(ml.x - up);
-      mx = up;
-      sum = sum * f0 + ml.y * f1;
-      x[0] = x[0] * f0 + v.x * f1; x[1] = x[1] * f0 + v.y * f1;
-      x[2] = x[2] * f0 + v.z * f1; x[3] = x[3] * f0 + v.w * f1;
-    }
-    const float inv = mx == -INFINITY ? 0.f : 1.f / sum;
+    few_row<kM>(p, s, it.h, it.tile, r, token, head, i);
+    const float inv = most[r] == -INFINITY ? 0.f : 1.f / total[r];
     uint2 y;
     y.x = pack2_16<kHalf>(x[0] * inv, x[1] * inv);
     y.y = pack2_16<kHalf>(x[2] * inv, x[3] * inv);
     *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + token * p.so_t + head * p.so_h + c) = y;
-    if (a.lse != nullptr && c == 0) a.lse[(int64_t)head * p.T + token] = (mx + log2f(sum)) * kLn2;
+    if (a.lse != nullptr && c == 0) a.lse[(int64_t)head * p.T + token] = (most[r] + log2f(total[r])) * kLn2;
   }
 }
 
@@ -664,7 +707,6 @@ FewKernels pick_few_dim(int D, int store) {
                                                                                                        : pick_few<kHalf, 256, kM>(store);
 }
 
-constexpr int kFewMaxCtas = 148 * 3;
 
 }  // namespace
 
@@ -698,7 +740,7 @@ cudaError_t launch_paged_few(const PagedParams& all, const void* q, const void* 
     p.lens += b;
     p.table += b * all.table_stride;
     if ((e = launch_pdl(k.attend, dim3(grid), kFewThreads, k.smem, st, p, mk, mv, a)) != cudaSuccess) return e;
-    if ((e = launch_pdl(k.join, dim3(grid), kFewThreads, 0, st, p, a, grid)) != cudaSuccess) return e;
+    if ((e = launch_pdl(k.join, dim3(grid), kJoinThreads, 0, st, p, a, grid)) != cudaSuccess) return e;
   }
   return cudaSuccess;
 }

@@ -18,12 +18,13 @@ with other numbers in the same tensors.  include/moba_b200.h has the rules in fu
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from .parallel import HEAD_DIMS, _on_device, _workspace
+from .parallel import HEAD_DIMS, _workspace
 
 __all__ = ["PagedKV", "paged_store", "paged_load", "paged_attention", "paged_append"]
 
@@ -92,46 +93,91 @@ def _check_rows(name, x, k_pages, heads: Optional[int], tokens: Optional[int]) -
         raise NotImplementedError(f"{name} requires grad: a paged cache is state of a server, its operators have no backward")
 
 
-def _problem(k_pages, v_pages, page_table, cu_seqlens, tokens: int, q_heads: int, dtype, max_new: int = 1, scale: float = 0.0):
-    pages, size, heads, dim = k_pages.shape
-    (kp, kt, kh, _), (vp, vt, vh, _) = k_pages.stride(), v_pages.stride()
-    # a dimension of one page, slot or head may have any stride: it is never stepped over
-    row = heads * size * dim
-    kp, vp = (kp, vp) if pages > 1 else (row, row)
-    kh, vh = (kh, vh) if heads > 1 else (size * dim, size * dim)
-    return _lib.Paged(
-        total_tokens=tokens, batch=cu_seqlens.numel() - 1, num_q_heads=q_heads, num_kv_heads=heads, head_dim=dim,
-        num_pages=pages, page_size=size, pages_per_seq=page_table.shape[1], max_new=max_new,
-        dtype=_lib.DTYPE_FP16 if dtype == torch.float16 else _lib.DTYPE_BF16, store=_STORES.get(k_pages.dtype, _lib.STORE_SAME),
-        softmax_scale=scale, k_page_stride=kp, k_page_token=kt, k_page_head=kh, v_page_stride=vp, v_page_token=vt,
-        v_page_head=vh, table_stride=page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1])
+#: struct moba_paged, field by field (filling a ctypes structure by name takes ten times as long)
+_PAGED = struct.Struct("@q10ifi15q")
+assert _PAGED.size == C.sizeof(_lib.Paged)
+_STORE_OF = {torch.bfloat16: _lib.STORE_SAME, torch.float16: _lib.STORE_SAME, **_STORES}
+_DTYPE_OF = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 
 
-def _ptr(x: Optional[torch.Tensor]):
-    return None if x is None else x.data_ptr()
+class _Pages:
+    """The tensors that describe a call, checked, with what the C structure needs of them; each attribute is read once, because this
+    runs on every call of a decode step."""
+    __slots__ = ("index", "shape", "dtype", "store", "batch", "per_seq", "strides", "pointers", "scales")
+
+    def __init__(self, k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales):
+        shape, dtype, index = k_pages.shape, k_pages.dtype, k_pages.get_device()
+        store = _STORE_OF.get(dtype)
+        table, batch = page_table.shape, cu_seqlens.shape[0] - 1 if cu_seqlens.dim() == 1 else 0
+        sk, sv, i32 = k_pages.stride(), v_pages.stride(), torch.int32
+        good = (index >= 0 and store is not None and len(shape) == 4 and v_pages.shape == shape and v_pages.dtype == dtype
+                and v_pages.get_device() == index and shape[3] in HEAD_DIMS and sk[3] == 1 == sv[3] and batch > 0
+                and len(table) == 2 and table[0] == batch and page_table.dtype == i32 and page_table.get_device() == index
+                and cu_seqlens.dtype == i32 and cu_seqlens.get_device() == index and cu_seqlens.stride(0) == 1
+                and seq_lens.dtype == i32 and seq_lens.get_device() == index and seq_lens.shape == (batch,)
+                and shape[0] > 0 and shape[2] > 0 and shape[1] >= 16 and not shape[1] & (shape[1] - 1))
+        ts = page_table.stride() if good else (0, 0)
+        if good:
+            good = table[1] > 0 and (ts[1] == 1 or table[1] == 1) and (batch == 1 or seq_lens.stride(0) == 1)
+        if good and store != _lib.STORE_SAME:
+            want = (shape[0], shape[2], shape[1])
+            good = (k_scales is not None and v_scales is not None and k_scales.shape == want and v_scales.shape == want
+                    and k_scales.dtype == torch.uint8 == v_scales.dtype and k_scales.get_device() == index
+                    and v_scales.get_device() == index and k_scales.is_contiguous() and v_scales.is_contiguous())
+        elif good:
+            good = k_scales is None and v_scales is None
+        if not good:
+            _check_pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
+        pages, size, heads, dim = shape
+        (kp, kt, kh, _), (vp, vt, vh, _) = sk, sv
+        # a dimension of one page or head may have any stride: it is never stepped over
+        if pages == 1:
+            kp = vp = heads * size * dim
+        if heads == 1:
+            kh = vh = size * dim
+        self.index, self.shape, self.dtype, self.store, self.batch, self.per_seq = index, shape, dtype, store, batch, table[1]
+        self.strides = (kp, kt, kh, vp, vt, vh, ts[0] if batch > 1 else table[1])
+        self.pointers = (k_pages.data_ptr(), v_pages.data_ptr())
+        self.scales = (None, None) if k_scales is None else (k_scales.data_ptr(), v_scales.data_ptr())
+
+    def pack(self, tokens, q_heads, max_new, dtype, scale, q=(0, 0), o=(0, 0), k=(0, 0), v=(0, 0)) -> bytes:
+        pages, size, heads, dim = self.shape
+        return _PAGED.pack(tokens, self.batch, q_heads, heads, dim, pages, size, self.per_seq, max_new, _DTYPE_OF[dtype], self.store,
+                           scale, 0, *q, *o, *k, *v, *self.strides)
+
+    def run(self, call) -> None:
+        """`call(stream)` with the pages' device current."""
+        index = self.index
+        if index != torch.cuda.current_device():
+            with torch.cuda.device(index):
+                _lib.check(call(torch._C._cuda_getCurrentRawStream(index)))
+        else:
+            _lib.check(call(torch._C._cuda_getCurrentRawStream(index)))
 
 
-def _rows_strides(x) -> Tuple[int, int]:
-    """Token and head stride; a single token or head may have any, and it is never stepped over."""
-    t, h, _ = x.stride()
-    return (t if x.shape[0] > 1 else 0), (h if x.shape[1] > 1 else 0)
-
-
-def _store(prob, k, v, k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales) -> None:
-    (prob.k_stride_token, prob.k_stride_head), (prob.v_stride_token, prob.v_stride_head) = _rows_strides(k), _rows_strides(v)
-    _lib.check(_on_device(k.device, lambda stream: _lib.lib().moba_paged_store(
-        C.byref(prob), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(),
-        k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales), stream)))
-    written = [x for x in (k_pages, v_pages, k_scales, v_scales) if x is not None and not x.is_inference()]
-    torch.autograd.graph.increment_version(written)          # as after an in-place torch operation
+def _rows(name, x, g: _Pages, heads: Optional[int], tokens: Optional[int], k_pages) -> Tuple[int, int]:
+    """A packed tensor, checked; its strides of tokens and heads (one token or head may have any, it is never stepped over)."""
+    shape, dtype, (t, h, d) = x.shape, x.dtype, x.stride() if x.dim() == 3 else (0, 0, 0)
+    if not (d == 1 and shape[2] == g.shape[3] and shape[1] > 0 and (heads is None or shape[1] == heads) and (tokens is None or shape[0] == tokens)
+            and dtype in _DTYPE_OF and (g.store != _lib.STORE_SAME or dtype == g.dtype) and x.get_device() == g.index
+            and not (x.requires_grad and torch.is_grad_enabled())):
+        _check_rows(name, x, k_pages, heads, tokens)
+    return t if shape[0] > 1 else 0, h if shape[1] > 1 else 0
 
 
 def _check_written(*tensors) -> None:
+    inference = torch.is_inference_mode_enabled()
     for x in tensors:
-        if x is not None and x.is_inference() and not torch.is_inference_mode_enabled():
-            raise RuntimeError("pages made in inference mode can only be written in inference mode")
-        if x is not None and x.requires_grad:
-            raise NotImplementedError("pages that require grad cannot be written")
+        if x is not None:
+            if not inference and x.is_inference():
+                raise RuntimeError("tensors made in inference mode can only be written in inference mode")
+            if x.requires_grad:
+                raise NotImplementedError("tensors that require grad cannot be written")
+
+
+def _written(*tensors) -> None:
+    """As after an in-place torch operation: what autograd saved of them is stale."""
+    torch.autograd.graph.increment_version([x for x in tensors if x is not None and not x.is_inference()])
 
 
 def paged_store(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -139,16 +185,20 @@ def paged_store(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages
                 v_scales: Optional[torch.Tensor] = None) -> None:
     """Writes the packed rows k, v [T, Hkv, D] into the pages of their sequences; 8-bit pages are quantised to, each row
     and head with a power of two of its own.  Rows behind the last sequence, and rows whose page is not there, are not written."""
-    _check_pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
-    _check_rows("k", k, k_pages, k_pages.shape[2], None)
-    _check_rows("v", v, k_pages, k_pages.shape[2], k.shape[0])
+    g = _Pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
+    heads, tokens = g.shape[2], k.shape[0] if k.dim() else None
+    ks = _rows("k", k, g, heads, None, k_pages)
+    vs = _rows("v", v, g, heads, tokens, k_pages)
     if k.dtype != v.dtype:
         raise TypeError("k and v must have the same dtype")
     _check_written(k_pages, v_pages, k_scales, v_scales)
-    if k.shape[0] == 0:
+    if tokens == 0:
         return
-    prob = _problem(k_pages, v_pages, page_table, cu_seqlens, k.shape[0], k.shape[1], k.dtype)
-    _store(prob, k, v, k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
+    prob = g.pack(tokens, heads, 1, k.dtype, 0.0, k=ks, v=vs)
+    g.run(lambda stream: _lib.lib().moba_paged_store(
+        prob, k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(), *g.pointers,
+        *g.scales, stream))
+    _written(k_pages, v_pages, k_scales, v_scales)
 
 
 def paged_load(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -158,69 +208,85 @@ def paged_load(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
     """Reads rows back: (k, v), each [total_tokens, Hkv, D] packed as cu_seqlens says, of `dtype` (8-bit pages: bfloat16 unless
     given).  With seq_lens the lengths of whole sequences this is the packed batch that `parallel_moba` takes.  Rows whose page is not
     there are zeros; rows behind the last sequence are left as they were (undefined without `out`)."""
-    _check_pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
+    g = _Pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
     if not isinstance(total_tokens, int) or total_tokens < 0:
         raise ValueError(f"total_tokens must be an int that is not negative, got {total_tokens}")
+    same = g.store == _lib.STORE_SAME
     if dtype is None:
-        dtype = k_pages.dtype if k_pages.dtype in _ROWS else out[0].dtype if out is not None else torch.bfloat16
-    heads, dim = k_pages.shape[2:]
+        dtype = g.dtype if same else out[0].dtype if out is not None else torch.bfloat16
+    _, _, heads, dim = g.shape
     if out is None:
-        if dtype not in _ROWS:
+        if dtype not in _DTYPE_OF:
             raise TypeError(f"only float16 and bfloat16 are supported, got {dtype}")
-        if k_pages.dtype in _ROWS and dtype != k_pages.dtype:
-            raise TypeError(f"rows of {k_pages.dtype} pages are {k_pages.dtype}, got {dtype}")
-        k, v = (torch.empty(total_tokens, heads, dim, dtype=dtype, device=k_pages.device) for _ in range(2))
+        if same and dtype != g.dtype:
+            raise TypeError(f"rows of {g.dtype} pages are {g.dtype}, got {dtype}")
+        k = torch.empty((total_tokens, heads, dim), dtype=dtype, device=k_pages.device)
+        v = torch.empty_like(k)
+        ks = vs = (heads * dim, dim)
     else:
         k, v = out
-        _check_rows("out[0]", k, k_pages, heads, total_tokens)
-        _check_rows("out[1]", v, k_pages, heads, total_tokens)
+        ks = _rows("out[0]", k, g, heads, total_tokens, k_pages)
+        vs = _rows("out[1]", v, g, heads, total_tokens, k_pages)
         if k.dtype != dtype or v.dtype != dtype:
             raise TypeError(f"out must be of {dtype}, got {k.dtype} and {v.dtype}")
         _check_written(k, v)
     if total_tokens == 0:
         return k, v
-    prob = _problem(k_pages, v_pages, page_table, cu_seqlens, total_tokens, heads, dtype)
-    (prob.k_stride_token, prob.k_stride_head), (prob.v_stride_token, prob.v_stride_head) = _rows_strides(k), _rows_strides(v)
-    _lib.check(_on_device(k.device, lambda stream: _lib.lib().moba_paged_load(
-        C.byref(prob), cu_seqlens.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(), k_pages.data_ptr(),
-        v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales), k.data_ptr(), v.data_ptr(), stream)))
+    prob = g.pack(total_tokens, heads, 1, dtype, 0.0, k=ks, v=vs)
+    g.run(lambda stream: _lib.lib().moba_paged_load(
+        prob, cu_seqlens.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(), *g.pointers, *g.scales, k.data_ptr(),
+        v.data_ptr(), stream))
     if out is not None:
-        torch.autograd.graph.increment_version([x for x in out if not x.is_inference()])
+        _written(*out)
     return k, v
 
 
-def _attention(q, k_pages, v_pages, page_table, cu_seqlens, seq_lens, prob, k_scales, v_scales, return_lse, out):
-    given = out is not None
-    if not given:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if return_lse else None
-    if q.shape[0] > 0:
-        (prob.q_stride_token, prob.q_stride_head), (prob.o_stride_token, prob.o_stride_head) = _rows_strides(q), _rows_strides(out)
-        lib, need = _lib.lib(), C.c_size_t(0)
-        _lib.check(lib.moba_paged_workspace_size(C.byref(prob), C.byref(need)))
-        ws = _workspace(q.device, need.value)
-        _lib.check(_on_device(q.device, lambda stream: lib.moba_paged_attention(
-            C.byref(prob), q.data_ptr(), cu_seqlens.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(),
-            k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales), out.data_ptr(), _ptr(lse),
-            ws.data_ptr(), need.value, stream)))
-        if given and not out.is_inference():
-            torch.autograd.graph.increment_version(out)
-    return (out, lse) if return_lse else out
-
-
 def _check_attention(q, k_pages, max_new, scale, out) -> None:
-    _check_rows("q", q, k_pages, None, None)
     if q.shape[1] % k_pages.shape[2] != 0:
         raise ValueError(f"q heads ({q.shape[1]}) must be divisible by kv heads ({k_pages.shape[2]})")
     if not isinstance(max_new, int) or max_new <= 0:
         raise ValueError(f"max_new must be a positive int, got {max_new}")
     if scale is not None and not 0.0 < float(scale) < 3e38:
         raise ValueError(f"scale must be a positive number, got {scale}")
-    if out is not None:
-        _check_rows("out", out, k_pages, q.shape[1], q.shape[0])
-        if out.dtype != q.dtype:
-            raise TypeError(f"out must be of {q.dtype}, got {out.dtype}")
+    if out is not None and out.dtype != q.dtype:
+        raise TypeError(f"out must be of {q.dtype}, got {out.dtype}")
+
+
+def _attention(g: _Pages, q, kv, k_pages, page_table, cu_seqlens, seq_lens, max_new, scale, return_lse, out):
+    """Attention of q; with `kv` the rows of k and v are stored first."""
+    qs = _rows("q", q, g, None, None, k_pages)
+    tokens, heads, _ = q.shape
+    _check_attention(q, k_pages, max_new, scale, out)
+    dtype, given, ks, vs = q.dtype, out is not None, (0, 0), (0, 0)
+    if given:
+        os = _rows("out", out, g, heads, tokens, k_pages)
         _check_written(out)
+    else:
+        out = torch.empty(q.shape, dtype=dtype, device=q.device)
+        os = (heads * g.shape[3], g.shape[3])
+    if kv is not None:
+        k, v = kv
+        ks = _rows("k", k, g, g.shape[2], tokens, k_pages)
+        vs = _rows("v", v, g, g.shape[2], tokens, k_pages)
+        if k.dtype != dtype or v.dtype != dtype:
+            raise TypeError("q, k, and v must have the same dtype")
+    lse = torch.empty((heads, tokens), dtype=torch.float32, device=q.device) if return_lse else None
+    if tokens > 0:
+        lib, need = _lib.lib(), C.c_size_t(0)
+        prob = g.pack(tokens, heads, max_new, dtype, 0.0 if scale is None else float(scale), qs, os, ks, vs)
+        _lib.check(lib.moba_paged_workspace_size(prob, C.byref(need)))
+        where = (cu_seqlens.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(), *g.pointers, *g.scales)
+
+        def call(stream):
+            ws = _workspace(q.device, need.value)
+            rc = 0 if kv is None else lib.moba_paged_store(prob, k.data_ptr(), v.data_ptr(), *where, stream)
+            return rc or lib.moba_paged_attention(prob, q.data_ptr(), *where, out.data_ptr(), None if lse is None else lse.data_ptr(),
+                                                  ws.data_ptr(), need.value, stream)
+
+        g.run(call)
+        if given:
+            _written(out)
+    return (out, lse) if return_lse else out
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -236,10 +302,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     log).  A token that sees nothing is zeros and -inf.  `out`: a tensor to write to; rows behind the last sequence are left as
     they were (undefined without it).  8-bit pages are attended to as the rows that `paged_load` gives; they take float16 and
     bfloat16 queries whatever they were written from."""
-    _check_pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
-    _check_attention(q, k_pages, max_new, scale, out)
-    prob = _problem(k_pages, v_pages, page_table, cu_seqlens, q.shape[0], q.shape[1], q.dtype, max_new, float(scale or 0.0))
-    return _attention(q, k_pages, v_pages, page_table, cu_seqlens, seq_lens, prob, k_scales, v_scales, return_lse, out)
+    g = _Pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
+    return _attention(g, q, None, k_pages, page_table, cu_seqlens, seq_lens, max_new, scale, return_lse, out)
 
 
 def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -247,17 +311,11 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
                  scale: Optional[float] = None, k_scales: Optional[torch.Tensor] = None,
                  v_scales: Optional[torch.Tensor] = None, return_lse: bool = False, out: Optional[torch.Tensor] = None):
     """`paged_store` of the new tokens' k and v, then `paged_attention` of their q: a layer's step of a server."""
-    _check_pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
-    _check_attention(q, k_pages, max_new, scale, out)
-    _check_rows("k", k, k_pages, k_pages.shape[2], q.shape[0])
-    _check_rows("v", v, k_pages, k_pages.shape[2], q.shape[0])
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError("q, k, and v must have the same dtype")
+    g = _Pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
     _check_written(k_pages, v_pages, k_scales, v_scales)
-    prob = _problem(k_pages, v_pages, page_table, cu_seqlens, q.shape[0], q.shape[1], q.dtype, max_new, float(scale or 0.0))
-    if q.shape[0] > 0:
-        _store(prob, k, v, k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
-    return _attention(q, k_pages, v_pages, page_table, cu_seqlens, seq_lens, prob, k_scales, v_scales, return_lse, out)
+    got = _attention(g, q, (k, v), k_pages, page_table, cu_seqlens, seq_lens, max_new, scale, return_lse, out)
+    _written(k_pages, v_pages, k_scales, v_scales)
+    return got
 
 
 class PagedKV:
