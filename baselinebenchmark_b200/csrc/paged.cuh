@@ -63,7 +63,7 @@ constexpr int kPagedBatch = 1024;
 
 // Items of more rows run on tcgen05.
 constexpr int kPagedFewRows = 16;
-inline bool paged_few_rows(const PagedParams& p) { return (int64_t)p.max_new * p.G <= kPagedFewRows || p.D == 256; }
+inline bool paged_few_rows(const PagedParams& p) { return (int64_t)p.max_new * p.G <= kPagedFewRows; }
 
 size_t paged_rows_workspace(const PagedParams& p);
 cudaError_t launch_paged_rows(const PagedParams& p, const void* q, const void* kp, const void* vp, const uint8_t* ks,

@@ -29,7 +29,10 @@ bool make_page_map(CUtensorMap* m, int elem, int D, const void* base, int pages,
 
 namespace {
 
-constexpr int kItemRows = 2 * kTileM;
+// Head dim 256 has one row tile an item; its K, V and Q are handled in halves of 128 dims, which take the places of the two stages and of the two
+// row tiles: S = Q_lo.K_lo^T + Q_hi.K_hi^T in one of two accumulators, O_lo += P.V_lo and O_hi += P.V_hi.
+constexpr int kMostRows = 2 * kTileM;
+__host__ __device__ constexpr int item_rows(int D) { return D == 256 ? kTileM : kMostRows; }
 constexpr int kCodeWarps = 8;              // that turn codes into operand tiles: warp 3, which has no V to bring, and warps 12-18
 template <int kStore> constexpr int kRowsThreads = kStore == MOBA_STORE_SAME ? 384 : 384 + 32 * (kCodeWarps - 1);
 constexpr int kMostSlots = 8 * 148;        // results of pieces that the workspace has room for
@@ -46,10 +49,13 @@ struct RowsPlan {
   int32_t piece[kPagedBatch];              // key tiles of a piece
 };
 
-__device__ __forceinline__ int rows_tiles(const PagedParams& p, int n) { return (int)(((int64_t)n * p.G + kItemRows - 1) / kItemRows); }
+__device__ __forceinline__ int rows_tiles(const PagedParams& p, int n) {
+  const int rows = item_rows(p.D);
+  return (int)(((int64_t)n * p.G + rows - 1) / rows);
+}
 // Keys that the rows of tile t see at most, and their tiles.
 __device__ __forceinline__ int rows_end(const PagedParams& p, const PagedSeq& s, int t) {
-  const int64_t last = min((int64_t)s.n - 1, ((int64_t)(t + 1) * kItemRows - 1) / p.G);
+  const int64_t last = min((int64_t)s.n - 1, ((int64_t)(t + 1) * item_rows(p.D) - 1) / p.G);
   return (int)min(max((int64_t)s.pos0 + last + 1, (int64_t)0), (int64_t)s.len);
 }
 // (an item without a key has one tile, all masked: its rows are written as zeros)
@@ -181,7 +187,8 @@ struct RowsCtrl {
   RowsItem item[2];
   int32_t done[2];
   uint32_t there[4];                       // [key tile mod 4]: which groups of 16 keys have a page
-  int64_t qoff[2][kItemRows], ooff[2][kItemRows];   // of a row in q and out; -1: no row
+  int64_t qoff[2][kMostRows], ooff[2][kMostRows];   // of a row in q and out; -1: no row
+  float row_inv[kTileM];                   // head dim 256: the row's factor (0: nothing is seen), for the warps that write the second half of O
   TileInfo info[kInfoSlots];
 };
 constexpr size_t kRowsSmem = 1024 + 6 * kTileBytes + sizeof(RowsCtrl);
@@ -193,8 +200,8 @@ struct RowsArgs {
   __nv_bfloat16* out;
   float* lse;
   RowsPlan* plan;
-  float* part;                             // [slots][256][D]
-  float2* part_ml;                         // [slots][256]: {maximum, sum}
+  float* part;                             // [slots][rows of an item][D]
+  float2* part_ml;                         // the same rows: {maximum, sum}
   FastDiv by_group;
 };
 
@@ -221,7 +228,8 @@ __device__ __forceinline__ void rows_prefetch(const PagedParams& p, const RowsAr
     it.j0 = cut * piece;
     it.ntiles = min(key_tiles(it.end) - it.j0, piece);
     if (it.ntiles <= 0) continue;
-    it.nrows = (int)min((int64_t)s.n * p.G - (int64_t)it.tile * kItemRows, (int64_t)kItemRows);
+    const int rows = item_rows(p.D);
+    it.nrows = (int)min((int64_t)s.n * p.G - (int64_t)it.tile * rows, (int64_t)rows);
     it.row0 = s.row0;
     it.n = s.n;
     it.pos0 = s.pos0;
@@ -232,16 +240,20 @@ __device__ __forceinline__ void rows_prefetch(const PagedParams& p, const RowsAr
   if (lane == 0) { c.item[at] = it; c.done[at] = done; }
   if (!done) {
 #pragma unroll
-    for (int u = 0; u < kItemRows / 32; ++u) {
+    for (int u = 0; u < kMostRows / 32; ++u) {
       const int r = lane + 32 * u;
       int64_t qo = -1, oo = -1;
       if (r < it.nrows) {
-        const int row = it.tile * kItemRows + r, i = row / a.by_group, head = it.h * p.G + row - i * p.G;
+        const int row = it.tile * item_rows(p.D) + r, i = row / a.by_group, head = it.h * p.G + row - i * p.G;
         const int64_t token = (int64_t)it.row0 + i;
         qo = token * p.sq_t + (int64_t)head * p.sq_h;
         oo = token * p.so_t + (int64_t)head * p.so_h;
         asm volatile("prefetch.global.L2 [%0];" ::"l"(a.q + qo));
         if (p.D > 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.q + qo + 64));
+        if (p.D > 128) {
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(a.q + qo + 128));
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(a.q + qo + 192));
+        }
       }
       c.qoff[at][r] = qo;
       c.ooff[at][r] = oo;
@@ -251,6 +263,7 @@ __device__ __forceinline__ void rows_prefetch(const PagedParams& p, const RowsAr
   if (lane == 0) mbar_arrive(smem_u32(&c.item_ready[at]));
 }
 
+__device__ __forceinline__ void rows_pair_barrier() { asm volatile("bar.sync 2, 256;" ::: "memory"); }   // warps 4-11
 // The warps that go item by item: all but those that turn codes into tiles.
 template <bool kCodes>
 __device__ __forceinline__ void rows_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kCodes ? 352 : 384) : "memory"); }
@@ -261,7 +274,7 @@ __device__ __forceinline__ bool rows_next(const RowsArgs& a, const RowsCtrl& c, 
   if (c.done[at]) return false;
   if (kGather) {
     constexpr int kChunks = D / 8;
-    constexpr int kPieces = kItemRows * kChunks / 256;
+    constexpr int kPieces = item_rows(D) * kChunks / 256;
     const int t = threadIdx.x - 128;
     uint4 val[kPieces];
 #pragma unroll
@@ -276,7 +289,9 @@ __device__ __forceinline__ bool rows_next(const RowsArgs& a, const RowsCtrl& c, 
     for (int u = 0; u < kPieces; ++u) {
       const int i = t + u * 256;
       const int r = i / kChunks, ch = i % kChunks;
-      const uint32_t dst = (uint32_t)((r >> 7) * kTileBytes + (ch >> 3) * kHalfBytes + (r & 127) * 128 + (((ch & 7) ^ (r & 7)) << 4));
+      // row tile, or half of the dims
+      const int tile = D == 256 ? ch >> 4 : r >> 7;
+      const uint32_t dst = (uint32_t)(tile * kTileBytes + ((ch >> 3) & 1) * kHalfBytes + (r & 127) * 128 + (((ch & 7) ^ (r & 7)) << 4));
       *reinterpret_cast<uint4*>(smem + dst) = val[u];
     }
   }
@@ -441,8 +456,9 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
-template <bool kMasked, bool kHalf, int D, bool kTwice>
-__device__ __forceinline__ bool rows_softmax(uint32_t tS, uint32_t tO, bool first, int rem, uint32_t there, float sl2, RowRef& row) {
+// `quiet` runs (the warp as one) before O is touched: where the P.V of the tile before may still be executing it waits for that.
+template <bool kMasked, bool kHalf, int D, bool kTwice, typename F>
+__device__ __forceinline__ bool rows_softmax(uint32_t tS, uint32_t tO, bool first, int rem, uint32_t there, float sl2, RowRef& row, F&& quiet) {
   constexpr int kW = kTwice ? 16 : 128, kP = kTwice ? 8 : 16;   // columns, and words of P, at a time
   uint32_t v[kTwice ? 2 : 1][kW];
   // runs `step(columns, first column)` over the scores; twice as it says: 16 columns travel while the 16 before them are worked on
@@ -496,6 +512,7 @@ __device__ __forceinline__ bool rows_softmax(uint32_t tS, uint32_t tO, bool firs
     float alpha = up ? ex2_approx(row.ref - ref) : 1.f;
     if (kMasked && up && fabsf(ref) > kLarge) alpha = ex2_approx((row.raw - raw) * sl2);
     if (!first) {
+      quiet();
       uint32_t o[32];
 #pragma unroll 1
       for (int ch = 0; ch < D / 32; ++ch) {
@@ -536,19 +553,19 @@ __device__ __forceinline__ bool rows_softmax(uint32_t tS, uint32_t tO, bool firs
   return true;
 }
 
+// D dims (at most 128): S at `d` (+)= the Q tile X . K^T; O at `d` (+)= P . V
 template <int X, bool kHalf, int D>
-__device__ __forceinline__ void rows_qk(uint32_t tmem, uint32_t dq, uint32_t dk) {
+__device__ __forceinline__ void rows_qk(uint32_t d, uint32_t dq, uint32_t dk, bool more = false) {
 #pragma unroll
   for (int ks = 0; ks < D / 16; ++ks) {
     const uint32_t koff = (uint32_t)((ks >> 2) * (kHalfBytes >> 4) + (ks & 3) * 2);
-    mma_ss(tmem + X * kBN, desc64(dq + X * (kTileBytes >> 4) + koff), desc64(dk + koff), kIdescQK<kHalf>, ks > 0);
+    mma_ss(d, desc64(dq + X * (kTileBytes >> 4) + koff), desc64(dk + koff), kIdescQK<kHalf>, more || ks > 0);
   }
 }
-template <int X, bool kHalf, int D>
-__device__ __forceinline__ void rows_pv(uint32_t tmem, uint32_t dv, bool first) {
+template <bool kHalf, int D>
+__device__ __forceinline__ void rows_pv(uint32_t d, uint32_t tp, uint32_t dv, bool first) {
 #pragma unroll
-  for (int ks = 0; ks < 8; ++ks)
-    mma_ts(tmem + 256 + X * 128, tmem + X * kBN + ks * 8, desc64(dv + ks * (2048 >> 4)), kIdescPV<kHalf, D>, (!first) || ks > 0);
+  for (int ks = 0; ks < 8; ++ks) mma_ts(d, tp + ks * 8, desc64(dv + ks * (2048 >> 4)), kIdescPV<kHalf, D>, (!first) || ks > 0);
 }
 
 // Rows of V that nobody may see become zeros: slots behind the sequence's end, and groups without a page.  One warp.
@@ -571,7 +588,10 @@ __global__ void __launch_bounds__(kRowsThreads<kStore>, 1)
 paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                   const RowsArgs a) {
   constexpr bool kCodes = kStore != MOBA_STORE_SAME;
-  constexpr int kBlocks = (D + 63) / 64;
+  constexpr bool kWide = D == 256;
+  constexpr int kParts = kWide ? 2 : 1, kPart = D / kParts;   // parts of the dims, each a tile of its own
+  constexpr int kBlocks = (kPart + 63) / 64;
+  constexpr int kRows = item_rows(D);
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sQ = smem_u32(smem), sK = sQ + 2 * kTileBytes, sV = sK + 2 * kTileBytes;
@@ -616,8 +636,9 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
   if (warp < (kCodes ? 3 : 4)) {
     // ---- warps 0-3: K (TMA, or where its codes are), MMA, items, V (TMA)
     if (!kCodes) setmaxnreg_dec<72>();
-    uint32_t kc = 0, vc = 0;               // K / V tiles produced (warps 0, 3) or consumed (warp 1) so far
+    uint32_t kc = 0, vc = 0;               // K / V tiles (of a part of the dims) produced (warps 0, 3) or consumed (warp 1) so far
     uint32_t pph0 = 0, pph1 = 0, raw = 0;
+    uint32_t gq = 0, gp = 0;               // head dim 256: tiles whose Q.K^T, whose P.V has been issued
     int pre = 0;                           // tiles of the coming item already requested
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     const uint32_t dq = __shfl_sync(0xffffffffu, desc_lo(sQ, 16), 0);
@@ -679,7 +700,8 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
       } else if (!kCodes && (warp == 0 || warp == 3)) {
         // a tile's pages: lanes 0 .. boxes - 1 have one each
         const int box_rows = min(1 << p.page_shift, kBN), boxes = kBN / box_rows;
-        auto load_tile = [&](const RowsItem& w, int j) -> bool {
+        auto load_tile = [&](const RowsItem& w, int jj) -> bool {
+          const int j = jj / kParts, dim0 = jj % kParts * kPart;
           const int key0 = (w.j0 + j) * kBN, key = key0 + lane * box_rows;
           const int id = lane < boxes && key < w.len ? paged_page(p, w.b, key) : -1;
           const uint32_t got = __ballot_sync(0xffffffffu, id >= 0);
@@ -694,13 +716,13 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
             const uint32_t bar = smem_u32(&c.k_full[s]);
             // (tiles of the other parity may still be in use, and one more softmax may read its word: hence four)
             if (lane == 0) {
-              c.there[kc & 3] = there;
+              c.there[kc / kParts & 3] = there;
               mbar_expect_tx(bar, bytes);
             }
             __syncwarp();
             if (id >= 0) {
 #pragma unroll
-              for (int blk = 0; blk < kBlocks; ++blk) tma_load_4d(at + blk * kHalfBytes, &tmap_k, bar, 64 * blk, slot, w.h, id);
+              for (int blk = 0; blk < kBlocks; ++blk) tma_load_4d(at + blk * kHalfBytes, &tmap_k, bar, dim0 + 64 * blk, slot, w.h, id);
             }
             ++kc;
           } else {
@@ -711,12 +733,12 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
             __syncwarp();
             if (id >= 0) {
 #pragma unroll
-              for (int blk = 0; blk < kBlocks; ++blk) tma_load_4d(at + blk * kHalfBytes, &tmap_v, bar, 64 * blk, slot, w.h, id);
+              for (int blk = 0; blk < kBlocks; ++blk) tma_load_4d(at + blk * kHalfBytes, &tmap_v, bar, dim0 + 64 * blk, slot, w.h, id);
             }
             if (!whole) {
               if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&c.v_raw), raw))) return false;
               raw ^= 1;
-              zero_rows<D>(smem + 4 * kTileBytes + s * kTileBytes, w, key0, there);
+              zero_rows<kPart>(smem + 4 * kTileBytes + s * kTileBytes, w, key0, there);
               fence_proxy_async_smem();
               __syncwarp();
               if (lane == 0) mbar_arrive(smem_u32(&c.v_full[s]));
@@ -726,18 +748,60 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
           return true;
         };
         bool alive = true;
-        for (int j = pre; alive && j < it.ntiles; ++j) alive = load_tile(it, j);
+        for (int j = pre; alive && j < it.ntiles * kParts; ++j) alive = load_tile(it, j);
         pre = 0;
         // the first tiles of the next item, as soon as stages free up
         if (alive) {
           const int s1 = (n + 1) & 1;
           alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(&c.item_ready[s1]), ((n + 1) >> 1) & 1));
           if (alive && !c.done[s1]) {
-            const int nt = min(2, c.item[s1].ntiles);
+            const int nt = min(2, c.item[s1].ntiles * kParts);
             for (; alive && pre < nt; ++pre) alive = load_tile(c.item[s1], pre);
           }
         }
         if (!alive && lane == 0) { atomicExch(&a.plan->status, RS_PRODUCER); c.abort = 1; }
+      } else if (kWide && warp == 1) {
+        // QK(0) QK(1) PV(0) QK(2) PV(1) ...: S of tile g of the CTA in accumulator g & 1
+        const int ntiles = it.ntiles;
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity)); };
+        tc_fence_after();
+        auto qk = [&]() -> bool {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (!wait(&c.k_full[h], (kc >> 1) & 1)) return false;
+            tc_fence_after();
+            if (el) {
+              if (h == 0) rows_qk<0, kHalf, kPart>(tm + (gq & 1) * kBN, dq, dk);
+              else rows_qk<1, kHalf, kPart>(tm + (gq & 1) * kBN, dq, dk + (kTileBytes >> 4), true);
+              tc_commit(smem_u32(&c.k_empty[h]));
+              if (h == 1) tc_commit(smem_u32(&c.s_full[gq & 1]));
+            }
+            __syncwarp();
+            ++kc;
+          }
+          ++gq;
+          return true;
+        };
+        bool ok = qk();
+        if (ok && ntiles > 1) ok = qk();
+        for (int j = 0; ok && j < ntiles; ++j) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            ok = ok && wait(&c.v_full[h], (vc >> 1) & 1) && (h == 1 || wait(&c.p_full[0], gp & 1));
+            if (!ok) break;
+            tc_fence_after();
+            if (el) {
+              rows_pv<kHalf, kPart>(tm + 256 + 128 * h, tm + (gp & 1) * kBN, dv + h * (kTileBytes >> 4), j == 0);
+              tc_commit(smem_u32(&c.v_empty[h]));
+              if (h == 1) tc_commit(smem_u32(&c.o_full[0]));
+            }
+            __syncwarp();
+            ++vc;
+          }
+          ++gp;
+          if (ok && j + 2 < ntiles) ok = qk();
+        }
+        if (!ok && lane == 0) { atomicExch(&a.plan->status, RS_MMA); c.abort = 1; }
       } else if (warp == 1) {
         const bool two = it.nrows > kTileM;                // tile B has rows
         const int ntiles = it.ntiles;
@@ -749,10 +813,10 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
         if (ok) {
           tc_fence_after();
           if (el) {
-            rows_qk<0, kHalf, D>(tm, dq, kd(kc & 1));
+            rows_qk<0, kHalf, kPart>(tm, dq, kd(kc & 1));
             tc_commit(smem_u32(&c.s_full[0]));
             if (two) {
-              rows_qk<1, kHalf, D>(tm, dq, kd(kc & 1));
+              rows_qk<1, kHalf, kPart>(tm + kBN, dq, kd(kc & 1));
               tc_commit(smem_u32(&c.s_full[1]));
             }
             tc_commit(smem_u32(&c.k_empty[kc & 1]));
@@ -768,7 +832,7 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
           pph0 ^= 1;
           tc_fence_after();
           if (el) {
-            rows_pv<0, kHalf, D>(tm, vd(vs), j == 0);
+            rows_pv<kHalf, kPart>(tm + 256, tm, vd(vs), j == 0);
             if (!two) tc_commit(smem_u32(&c.v_empty[vs]));
           }
           __syncwarp();
@@ -777,7 +841,7 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
             if (!ok) break;
             tc_fence_after();
             if (el) {
-              rows_qk<0, kHalf, D>(tm, dq, kd(ks));
+              rows_qk<0, kHalf, kPart>(tm, dq, kd(ks));
               tc_commit(smem_u32(&c.s_full[0]));
               if (!two) tc_commit(smem_u32(&c.k_empty[ks]));
             }
@@ -791,10 +855,10 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
             pph1 ^= 1;
             tc_fence_after();
             if (el) {
-              rows_pv<1, kHalf, D>(tm, vd(vs), j == 0);
+              rows_pv<kHalf, kPart>(tm + 384, tm + kBN, vd(vs), j == 0);
               tc_commit(smem_u32(&c.v_empty[vs]));
               if (more) {
-                rows_qk<1, kHalf, D>(tm, dq, kd(ks));
+                rows_qk<1, kHalf, kPart>(tm + kBN, dq, kd(ks));
                 tc_commit(smem_u32(&c.s_full[1]));
                 tc_commit(smem_u32(&c.k_empty[ks]));
               } else {
@@ -817,20 +881,56 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
     const int x = (warp - 4) >> 2;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + lane_base + x * kBN, tO = tmem + lane_base + 256 + x * 128;
+    const uint32_t tS = tmem + lane_base + x * kBN, tO = tmem + lane_base + 256 + (kWide ? 0 : x * 128);
     uint32_t sph = 0, oph = 0, kt = 0;     // kt: key tiles of this CTA before the item's
+    // head dim 256: the softmax of an item, by warps 4-7; all eight leave when its last P.V has executed
+    auto wide_rows = [&](const RowsItem& it, int ntiles, int j0, int lim, int lim_first, int x, uint32_t kt, RowRef& rr, bool& ok) {
+      uint32_t g = kt;                                      // the CTA's tiles before this one
+      if (x == 0) {
+        for (int j = 0; ok && j < ntiles; ++j, ++g) {
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&c.s_full[g & 1]), (g >> 1) & 1));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t tSg = tmem + lane_base + (g & 1) * kBN;
+          const int key0 = (j0 + j) * kBN;
+          const uint32_t there = c.there[g & 3];
+          // the P.V of tile g - 1 must have executed before O is touched (that of tile g - 2 has)
+          auto quiet = [&] {
+            if (!mbar_wait(smem_u32(&c.o_full[0]), (g - 1) & 1)) ok = false;
+            tc_fence_after();
+          };
+          if (key0 + kBN > lim_first || there != 0xff || !rows_softmax<false, kHalf, D, kCodes>(tSg, tO, j == 0, 0, 0, p.sl2, rr, quiet))
+            rows_softmax<true, kHalf, D, kCodes>(tSg, tO, j == 0, lim - key0, there, p.sl2, rr, quiet);
+          // completions of o_full stay at most one behind: the parity of a tile never answers for an older one
+          if (j > 0 && !mbar_wait(smem_u32(&c.o_full[0]), (g - 1) & 1)) ok = false;
+          ok = __all_sync(0xffffffffu, ok);
+          tc_fence_before();
+          mbar_arrive(smem_u32(&c.p_full[0]));
+        }
+      } else {
+        g += (uint32_t)ntiles;
+      }
+      rows_pair_barrier();                                  // the last P has been published
+      if (ok) ok = mbar_wait(smem_u32(&c.o_full[0]), (g - 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (x == 0) c.row_inv[row] = rr.ref == -INFINITY && rr.l == 0.f ? 0.f : 1.f / rr.l;
+      rows_pair_barrier();                                  // the rows' factors are visible to warps 8-11
+      (void)it;
+    };
     for (int n = 0; rows_next<true, D, kCodes>(a, c, smem, n & 1); ++n) {
       const RowsItem& it = c.item[n & 1];
       const int ntiles = it.ntiles, j0 = it.j0;
-      const int at = it.tile * kItemRows + x * kTileM;      // first row of the tile
-      const bool busy = x * kTileM < it.nrows;
+      const int at = it.tile * kRows + (kWide ? 0 : x * kTileM);   // first row of the tile
+      const bool busy = kWide || x * kTileM < it.nrows;
       const int i_row = (at + row) / a.by_group, i_first = at / a.by_group;
-      const bool on = x * kTileM + row < it.nrows;
+      const bool on = (kWide ? 0 : x * kTileM) + row < it.nrows;
       const int lim = on ? min(max(it.pos0 + i_row + 1, 0), it.len) : 0;
       const int lim_first = min(max(it.pos0 + i_first + 1, 0), it.len);
       RowRef rr{-INFINITY, -INFINITY, 0.f};
       bool ok = true;
-      if (busy) {
+      if constexpr (kWide) {
+        wide_rows(it, ntiles, j0, lim, lim_first, x, kt, rr, ok);
+      } else if (busy) {
         for (int j = 0; ok && j < ntiles; ++j) {
           ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&c.s_full[x]), sph));
           if (!ok) break;
@@ -838,8 +938,8 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
           tc_fence_after();
           const int key0 = (j0 + j) * kBN;
           const uint32_t there = c.there[(kt + j) & 3];
-          if (key0 + kBN > lim_first || there != 0xff || !rows_softmax<false, kHalf, D, kCodes>(tS, tO, j == 0, 0, 0, p.sl2, rr))
-            rows_softmax<true, kHalf, D, kCodes>(tS, tO, j == 0, lim - key0, there, p.sl2, rr);
+          if (key0 + kBN > lim_first || there != 0xff || !rows_softmax<false, kHalf, D, kCodes>(tS, tO, j == 0, 0, 0, p.sl2, rr, [] {}))
+            rows_softmax<true, kHalf, D, kCodes>(tS, tO, j == 0, lim - key0, there, p.sl2, rr, [] {});
           tc_fence_before();
           mbar_arrive(smem_u32(&c.p_full[x]));
         }
@@ -852,16 +952,19 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
         tc_fence_after();
         float m_ref = rr.ref;
         const float l = rr.l;
-        const bool empty = m_ref == -INFINITY && l == 0.f;
+        const float row_inv = kWide ? c.row_inv[row] : 0.f;
+        const bool empty = kWide ? row_inv == 0.f : m_ref == -INFINITY && l == 0.f;
         // a sum that is not a number stays one whatever it is joined with
         if (l != l) m_ref = INFINITY;
+        const int col0 = kWide ? x * kPart : 0;              // this warp's columns of O
         if (it.slot >= 0) {
-          if (on) a.part_ml[(int64_t)it.slot * kItemRows + x * kTileM + row] = make_float2(m_ref, l);
-          float* dst = a.part + ((int64_t)it.slot * kItemRows + x * kTileM + row) * D;
+          const int64_t part_row = (int64_t)it.slot * kRows + (kWide ? 0 : x * kTileM) + row;
+          if (on && col0 == 0) a.part_ml[part_row] = make_float2(m_ref, l);
+          float* dst = a.part + part_row * D + col0;
 #pragma unroll 1
-          for (int ch = 0; ch < D; ch += 32) {
+          for (int ch = 0; ch < kPart; ch += 32) {
             uint32_t v[32];
-            tmem_ld32(tO + ch, v);
+            tmem_ld32(tO + col0 + ch, v);
             tmem_wait_ld();
             if (on) {
 #pragma unroll
@@ -870,17 +973,17 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
             __syncwarp();
           }
         } else {
-          const float inv = empty ? 0.f : 1.f / l;
+          const float inv = kWide ? row_inv : empty ? 0.f : 1.f / l;
           // rows pass through this warp's 8 KB of the idle Q tile: 64 columns at a time, rows 144 bytes apart
           unsigned char* stage = smem + x * kTileBytes + (warp & 3) * 8192;
-          const int64_t* ooff = c.ooff[n & 1] + x * kTileM + (warp & 3) * 32;
+          const int64_t* ooff = c.ooff[n & 1] + (kWide ? 0 : x * kTileM) + (warp & 3) * 32;
 #pragma unroll 1
-          for (int ch = 0; ch < D; ch += 64) {
-            const int cols = min(D - ch, 64);
+          for (int ch = 0; ch < kPart; ch += 64) {
+            const int cols = min(kPart - ch, 64);
 #pragma unroll 1
             for (int half = 0; half < cols; half += 32) {
               uint32_t v[32];
-              tmem_ld32(tO + ch + half, v);
+              tmem_ld32(tO + col0 + ch + half, v);
               tmem_wait_ld();
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
@@ -900,11 +1003,11 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
               const int rl = i * 4 + (lane >> 3), c16 = lane & 7;
               const int64_t off = ooff[rl];
               if (off >= 0 && c16 * 8 < cols)
-                *reinterpret_cast<uint4*>(a.out + off + ch + c16 * 8) = *reinterpret_cast<const uint4*>(stage + rl * 144 + c16 * 16);
+                *reinterpret_cast<uint4*>(a.out + off + col0 + ch + c16 * 8) = *reinterpret_cast<const uint4*>(stage + rl * 144 + c16 * 16);
             }
             __syncwarp();
           }
-          if (a.lse != nullptr && on) {
+          if (a.lse != nullptr && on && col0 == 0) {
             const int head = it.h * p.G + (at + row) - i_row * p.G;
             a.lse[(int64_t)head * p.T + it.row0 + i_row] = empty ? -INFINITY : (m_ref + log2f(l)) * kLn2;
           }
@@ -918,39 +1021,64 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
   } else {
     // ---- warps 3 and 12-18: codes into operand tiles, one stream of tiles whatever the items are
     const int group = warp == 3 ? 7 : warp - 12;   // of 16 keys
-    RawTile<D> rk, rv;
+    RawTile<kPart> ra, rb;                 // two parts of operands: one on its way while the other is turned
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity));
       return ok;
     };
-    // the K codes of a tile are asked for while the V codes of the one before it are turned, its V codes in front of its K codes
-    auto ask_k = [&](uint32_t t) {                          // false: no more tiles
+    // a tile's parts in order: K, V; K_lo, K_hi, V_lo, V_hi.  The first of the next tile is asked for while the last one is turned.
+    auto ask_k = [&](uint32_t t, int part, RawTile<kPart>& raw) {
       const TileInfo& info = c.info[t % kInfoSlots];
-      if (!wait(&c.info_full[t % kInfoSlots], (t / kInfoSlots) & 1) || info.keys == 0) return false;
-      raw_load<D>(a.kp, a.ks, info.k[group], info.scale[group], p.kp_t, info.keys - 16 * group, lane, rk);
+      raw_load<kPart>(a.kp + part * kPart, a.ks, info.k[group], info.scale[group], p.kp_t, info.keys - 16 * group, lane, raw);
+    };
+    auto ask_v = [&](uint32_t t, int part, RawTile<kPart>& raw) {
+      const TileInfo& info = c.info[t % kInfoSlots];
+      raw_load<kPart>(a.vp + part * kPart, a.vs, info.v[group], info.scale[group], p.vp_t, info.keys - 16 * group, lane, raw);
+    };
+    auto more_tiles = [&](uint32_t t) {                     // false: there are no more
+      return wait(&c.info_full[t % kInfoSlots], (t / kInfoSlots) & 1) && c.info[t % kInfoSlots].keys != 0;
+    };
+    // into stage s, of which this is use number `use`
+    auto turn = [&](const RawTile<kPart>& raw, uint64_t* empty, uint64_t* full, uint32_t base, uint32_t s, uint32_t use) {
+      if (!wait(&empty[s], (use & 1) ^ 1)) return false;
+      raw_store<kHalf, kPart, kStore>(raw, base + s * kTileBytes + group * 2048, lane);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&full[s]));
       return true;
     };
-    bool more = ask_k(0);
+    bool more = more_tiles(0);
+    if (more) ask_k(0, 0, ra);
     for (uint32_t t = 0; more; ++t) {
-      const uint32_t s = t & 1, parity = ((t >> 1) & 1) ^ 1;
-      const TileInfo& info = c.info[t % kInfoSlots];
-      raw_load<D>(a.vp, a.vs, info.v[group], info.scale[group], p.vp_t, info.keys - 16 * group, lane, rv);
-      const uint32_t there = info.there;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&c.info_empty[t % kInfoSlots]));
-      if (!wait(&c.k_empty[s], parity)) break;
-      if (group == 0 && lane == 0) c.there[t & 3] = there;
-      raw_store<kHalf, D, kStore>(rk, sK + s * kTileBytes + group * 2048, lane);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&c.k_full[s]));
-      more = ask_k(t + 1);
-      if (!wait(&c.v_empty[s], parity)) break;
-      raw_store<kHalf, D, kStore>(rv, sV + s * kTileBytes + group * 2048, lane);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&c.v_full[s]));
+      const uint32_t there = c.info[t % kInfoSlots].there;
+      auto asked = [&] {                                    // for all of the tile: its description may go
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&c.info_empty[t % kInfoSlots]));
+      };
+      // (in front of the arrival on k_full, behind the wait that frees the stage)
+      auto tell = [&] { if (group == 0 && lane == 0) c.there[t & 3] = there; };
+      if constexpr (kWide) {
+        ask_k(t, 1, rb);
+        if (!wait(&c.k_empty[0], (t & 1) ^ 1)) break;
+        tell();
+        if (!turn(ra, c.k_empty, c.k_full, sK, 0, t)) break;
+        ask_v(t, 0, ra);
+        if (!turn(rb, c.k_empty, c.k_full, sK, 1, t)) break;
+        ask_v(t, 1, rb);
+        asked();
+        if (!turn(ra, c.v_empty, c.v_full, sV, 0, t)) break;
+        if ((more = more_tiles(t + 1))) ask_k(t + 1, 0, ra);
+        if (!turn(rb, c.v_empty, c.v_full, sV, 1, t)) break;
+      } else {
+        ask_v(t, 0, rb);
+        asked();
+        if (!wait(&c.k_empty[t & 1], ((t >> 1) & 1) ^ 1)) break;
+        tell();
+        if (!turn(ra, c.k_empty, c.k_full, sK, t & 1, t >> 1)) break;
+        if ((more = more_tiles(t + 1))) ask_k(t + 1, 0, ra);
+        if (!turn(rb, c.v_empty, c.v_full, sV, t & 1, t >> 1)) break;
+      }
     }
     if (!ok && lane == 0) { atomicExch(&a.plan->status, RS_PRODUCER); c.abort = 1; }
     __syncwarp();
@@ -997,16 +1125,20 @@ __global__ void __launch_bounds__(kJoinThreads) paged_rows_join_kernel(const Pag
     const int tiles = rows_tiles(p, s.n), piece = __ldcg(a.plan->piece + b);
     const int cuts = (key_tiles(rows_end(p, s, tiles - 1)) + piece - 1) / piece;
     const int h = head / p.G;
-    const int row = i * p.G + head - h * p.G, tile = row / kItemRows, r = row - tile * kItemRows;
+    constexpr int kRows = item_rows(D);
+    const int row = i * p.G + head - h * p.G, tile = row / kRows, r = row - tile * kRows;
     const int mine = (key_tiles(rows_end(p, s, tile)) + piece - 1) / piece;
     for (int k = 0; k < mine; ++k) {
-      const int64_t at = ((int64_t)slot0 + ((int64_t)h * cuts + k) * tiles + tiles - 1 - tile) * kItemRows + r;
+      const int64_t at = ((int64_t)slot0 + ((int64_t)h * cuts + k) * tiles + tiles - 1 - tile) * kRows + r;
       const float2 ml = __ldcg(a.part_ml + at);
       float v[kPer];
       const float* src = a.part + at * D + lane * kPer;
-      if constexpr (kPer == 4) {
-        const float4 f = __ldcg(reinterpret_cast<const float4*>(src));
-        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+      if constexpr (kPer % 4 == 0) {
+#pragma unroll
+        for (int u = 0; u < kPer; u += 4) {
+          const float4 f = __ldcg(reinterpret_cast<const float4*>(src + u));
+          v[u] = f.x; v[u + 1] = f.y; v[u + 2] = f.z; v[u + 3] = f.w;
+        }
       } else {
 #pragma unroll
         for (int u = 0; u < kPer; ++u) v[u] = __ldcg(src + u);
@@ -1054,7 +1186,7 @@ constexpr size_t kPlanBytes = (sizeof(RowsPlan) + 255) / 256 * 256;
 }  // namespace
 
 size_t paged_rows_workspace(const PagedParams& p) {
-  return kPlanBytes + (size_t)kMostSlots * kItemRows * (sizeof(float2) + p.D * sizeof(float));
+  return kPlanBytes + (size_t)kMostSlots * item_rows(p.D) * (sizeof(float2) + p.D * sizeof(float));
 }
 
 cudaError_t launch_paged_rows(const PagedParams& all, const void* q, const void* kp, const void* vp, const uint8_t* ks,
@@ -1069,7 +1201,7 @@ cudaError_t launch_paged_rows(const PagedParams& all, const void* q, const void*
   a.lse = lse;
   a.plan = static_cast<RowsPlan*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + kPlanBytes);
-  a.part = reinterpret_cast<float*>(a.part_ml + (size_t)kMostSlots * kItemRows);
+  a.part = reinterpret_cast<float*>(a.part_ml + (size_t)kMostSlots * item_rows(all.D));
   a.by_group = fast_div(all.G);
   CUtensorMap mk{}, mv{};
   if (all.store == MOBA_STORE_SAME) {
@@ -1087,7 +1219,8 @@ cudaError_t launch_paged_rows(const PagedParams& all, const void* q, const void*
     p.table += b * all.table_stride;
     const cudaError_t e = p.D == 64 ? (p.fp16 ? launch_rows_dim<true, 64>(p, mk, mv, a, sms, st) : launch_rows_dim<false, 64>(p, mk, mv, a, sms, st))
                         : p.D == 96 ? (p.fp16 ? launch_rows_dim<true, 96>(p, mk, mv, a, sms, st) : launch_rows_dim<false, 96>(p, mk, mv, a, sms, st))
-                                    : (p.fp16 ? launch_rows_dim<true, 128>(p, mk, mv, a, sms, st) : launch_rows_dim<false, 128>(p, mk, mv, a, sms, st));
+                        : p.D == 128 ? (p.fp16 ? launch_rows_dim<true, 128>(p, mk, mv, a, sms, st) : launch_rows_dim<false, 128>(p, mk, mv, a, sms, st))
+                                     : (p.fp16 ? launch_rows_dim<true, 256>(p, mk, mv, a, sms, st) : launch_rows_dim<false, 256>(p, mk, mv, a, sms, st));
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
