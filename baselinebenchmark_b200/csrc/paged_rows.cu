@@ -9,6 +9,8 @@
 //   - 8-bit pages: four more warps read the codes, multiply by the row's power of two (exact: see moba_b200.h) and store the operand
 //     tiles in the rows' 16-bit type; from there on nothing differs.  That is 2.5 instructions an element of bf16 (1 to 1.75 of fp16), 5
 //     of an SM's 8 thousand issue slots of a tile's MMAs with the softmax's, in place of a pass over the cache that would write it out in 16 bits.
+//   - An item of at most 128 rows (drafted tokens, a small group) has them in both row tiles: A takes every other key tile, B the ones between,
+//     each with its own output, and the two are joined at the end.  One softmax at a time left the copies waiting.
 //   - Pieces: a first kernel (one CTA) adds up the work of the batch and picks how many pieces an item is cut into, so that
 //     the waves of items on the SMs are full; pieces of a sequence and kv head lie next to one another in the order in which CTAs draw
 //     them, row tiles fastest, so that those that run together read the same K and V and find them in L2.  Cut items
@@ -188,6 +190,7 @@ struct RowsCtrl {
   int32_t done[2];
   uint32_t there[4];                       // [key tile mod 4]: which groups of 16 keys have a page
   int64_t qoff[2][kMostRows], ooff[2][kMostRows];   // of a row in q and out; -1: no row
+  float2 pair_ml[2][kTileM];               // {maximum, sum} of a row in tiles A and B, where both have it
   float row_inv[kTileM];                   // head dim 256: the row's factor (0: nothing is seen), for the warps that write the second half of O
   TileInfo info[kInfoSlots];
 };
@@ -204,6 +207,9 @@ struct RowsArgs {
   float2* part_ml;                         // the same rows: {maximum, sum}
   FastDiv by_group;
 };
+
+// Both row tiles have the item's rows, and the key tiles by turns.
+__device__ __forceinline__ bool rows_twice(int D, const RowsItem& it) { return D != 256 && it.nrows <= kTileM; }
 
 // Warp 2, one item ahead of the others.
 __device__ __forceinline__ void rows_prefetch(const PagedParams& p, const RowsArgs& a, RowsCtrl& c, int at) {
@@ -243,8 +249,9 @@ __device__ __forceinline__ void rows_prefetch(const PagedParams& p, const RowsAr
     for (int u = 0; u < kMostRows / 32; ++u) {
       const int r = lane + 32 * u;
       int64_t qo = -1, oo = -1;
-      if (r < it.nrows) {
-        const int row = it.tile * item_rows(p.D) + r, i = row / a.by_group, head = it.h * p.G + row - i * p.G;
+      const int rt = rows_twice(p.D, it) ? r & (kTileM - 1) : r;
+      if (rt < it.nrows) {
+        const int row = it.tile * item_rows(p.D) + rt, i = row / a.by_group, head = it.h * p.G + row - i * p.G;
         const int64_t token = (int64_t)it.row0 + i;
         qo = token * p.sq_t + (int64_t)head * p.sq_h;
         oo = token * p.so_t + (int64_t)head * p.so_h;
@@ -803,22 +810,56 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
         }
         if (!ok && lane == 0) { atomicExch(&a.plan->status, RS_MMA); c.abort = 1; }
       } else if (warp == 1) {
-        const bool two = it.nrows > kTileM;                // tile B has rows
         const int ntiles = it.ntiles;
         auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity)); };
         auto kd = [&](uint32_t s) { return dk + s * (kTileBytes >> 4); };
         auto vd = [&](uint32_t s) { return dv + s * (kTileBytes >> 4); };
         tc_fence_after();
-        bool ok = wait(&c.k_full[kc & 1], (kc >> 1) & 1);
+        bool ok = true;
+        if (rows_twice(D, it)) {
+          auto qk = [&](int t) -> bool {
+            const uint32_t s = kc & 1;
+            if (!wait(&c.k_full[s], (kc >> 1) & 1)) return false;
+            tc_fence_after();
+            if (el) {
+              if (t & 1) rows_qk<1, kHalf, kPart>(tm + kBN, dq, kd(s)); else rows_qk<0, kHalf, kPart>(tm, dq, kd(s));
+              tc_commit(smem_u32(&c.s_full[t & 1]));
+              tc_commit(smem_u32(&c.k_empty[s]));
+            }
+            __syncwarp();
+            ++kc;
+            return true;
+          };
+          ok = qk(0);
+          if (ok && ntiles > 1) ok = qk(1);
+          for (int t = 0; ok && t < ntiles; ++t) {
+            const int x = t & 1;
+            const uint32_t vs = vc & 1;
+            ok = wait(&c.v_full[vs], (vc >> 1) & 1) && wait(&c.p_full[x], x ? pph1 : pph0);
+            if (!ok) break;
+            if (x) pph1 ^= 1; else pph0 ^= 1;
+            tc_fence_after();
+            if (el) {
+              rows_pv<kHalf, kPart>(tm + 256 + 128 * x, tm + x * kBN, vd(vs), t < 2);
+              tc_commit(smem_u32(&c.v_empty[vs]));
+              if (t + 2 >= ntiles) tc_commit(smem_u32(&c.o_full[x]));
+            }
+            __syncwarp();
+            ++vc;
+            if (t + 2 < ntiles) ok = qk(t + 2);
+          }
+          if (!ok && lane == 0) { atomicExch(&a.plan->status, RS_MMA); c.abort = 1; }
+          __syncwarp();
+          continue;
+        }
+        ok = wait(&c.k_full[kc & 1], (kc >> 1) & 1);
         if (ok) {
           tc_fence_after();
           if (el) {
             rows_qk<0, kHalf, kPart>(tm, dq, kd(kc & 1));
             tc_commit(smem_u32(&c.s_full[0]));
-            if (two) {
-              rows_qk<1, kHalf, kPart>(tm + kBN, dq, kd(kc & 1));
-              tc_commit(smem_u32(&c.s_full[1]));
-            }
+            rows_qk<1, kHalf, kPart>(tm + kBN, dq, kd(kc & 1));
+            tc_commit(smem_u32(&c.s_full[1]));
             tc_commit(smem_u32(&c.k_empty[kc & 1]));
           }
           __syncwarp();
@@ -833,7 +874,6 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
           tc_fence_after();
           if (el) {
             rows_pv<kHalf, kPart>(tm + 256, tm, vd(vs), j == 0);
-            if (!two) tc_commit(smem_u32(&c.v_empty[vs]));
           }
           __syncwarp();
           if (more) {
@@ -843,30 +883,27 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
             if (el) {
               rows_qk<0, kHalf, kPart>(tm, dq, kd(ks));
               tc_commit(smem_u32(&c.s_full[0]));
-              if (!two) tc_commit(smem_u32(&c.k_empty[ks]));
             }
           } else if (el) {
             tc_commit(smem_u32(&c.o_full[0]));
           }
           __syncwarp();
-          if (two) {
-            ok = wait(&c.p_full[1], pph1);
-            if (!ok) break;
-            pph1 ^= 1;
-            tc_fence_after();
-            if (el) {
-              rows_pv<kHalf, kPart>(tm + 384, tm + kBN, vd(vs), j == 0);
-              tc_commit(smem_u32(&c.v_empty[vs]));
-              if (more) {
-                rows_qk<1, kHalf, kPart>(tm + kBN, dq, kd(ks));
-                tc_commit(smem_u32(&c.s_full[1]));
-                tc_commit(smem_u32(&c.k_empty[ks]));
-              } else {
-                tc_commit(smem_u32(&c.o_full[1]));
-              }
+          ok = wait(&c.p_full[1], pph1);
+          if (!ok) break;
+          pph1 ^= 1;
+          tc_fence_after();
+          if (el) {
+            rows_pv<kHalf, kPart>(tm + 384, tm + kBN, vd(vs), j == 0);
+            tc_commit(smem_u32(&c.v_empty[vs]));
+            if (more) {
+              rows_qk<1, kHalf, kPart>(tm + kBN, dq, kd(ks));
+              tc_commit(smem_u32(&c.s_full[1]));
+              tc_commit(smem_u32(&c.k_empty[ks]));
+            } else {
+              tc_commit(smem_u32(&c.o_full[1]));
             }
-            __syncwarp();
           }
+          __syncwarp();
           ++vc;
           if (more) ++kc;
         }
@@ -920,35 +957,89 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
     for (int n = 0; rows_next<true, D, kCodes>(a, c, smem, n & 1); ++n) {
       const RowsItem& it = c.item[n & 1];
       const int ntiles = it.ntiles, j0 = it.j0;
-      const int at = it.tile * kRows + (kWide ? 0 : x * kTileM);   // first row of the tile
-      const bool busy = kWide || x * kTileM < it.nrows;
+      const bool twice = rows_twice(D, it);
+      const int base = kWide || twice ? 0 : x * kTileM;    // first row of the item in this row tile
+      const int at = it.tile * kRows + base;
       const int i_row = (at + row) / a.by_group, i_first = at / a.by_group;
-      const bool on = (kWide ? 0 : x * kTileM) + row < it.nrows;
+      const bool on = base + row < it.nrows;
       const int lim = on ? min(max(it.pos0 + i_row + 1, 0), it.len) : 0;
       const int lim_first = min(max(it.pos0 + i_first + 1, 0), it.len);
       RowRef rr{-INFINITY, -INFINITY, 0.f};
       bool ok = true;
       if constexpr (kWide) {
         wide_rows(it, ntiles, j0, lim, lim_first, x, kt, rr, ok);
-      } else if (busy) {
-        for (int j = 0; ok && j < ntiles; ++j) {
+      } else {
+        const int j1 = twice ? x : 0, by = twice ? 2 : 1;
+        for (int j = j1; ok && j < ntiles; j += by) {
           ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&c.s_full[x]), sph));
           if (!ok) break;
           sph ^= 1;
           tc_fence_after();
           const int key0 = (j0 + j) * kBN;
           const uint32_t there = c.there[(kt + j) & 3];
-          if (key0 + kBN > lim_first || there != 0xff || !rows_softmax<false, kHalf, D, kCodes>(tS, tO, j == 0, 0, 0, p.sl2, rr, [] {}))
-            rows_softmax<true, kHalf, D, kCodes>(tS, tO, j == 0, lim - key0, there, p.sl2, rr, [] {});
+          if (key0 + kBN > lim_first || there != 0xff || !rows_softmax<false, kHalf, D, kCodes>(tS, tO, j == j1, 0, 0, p.sl2, rr, [] {}))
+            rows_softmax<true, kHalf, D, kCodes>(tS, tO, j == j1, lim - key0, there, p.sl2, rr, [] {});
           tc_fence_before();
           mbar_arrive(smem_u32(&c.p_full[x]));
         }
-        if (ok) ok = mbar_wait(smem_u32(&c.o_full[x]), oph);
-        ok = __all_sync(0xffffffffu, ok);
-        oph ^= 1;
+        if (j1 < ntiles) {
+          if (ok) ok = mbar_wait(smem_u32(&c.o_full[x]), oph);
+          ok = __all_sync(0xffffffffu, ok);
+          oph ^= 1;
+        }
       }
       kt += ntiles;
-      if (busy && ok) {
+      if (!kWide && twice) {
+        // the row's two results joined; each tile's warps write every other 32 columns
+        c.pair_ml[x][row] = make_float2(rr.l != rr.l ? INFINITY : rr.ref, rr.l);
+        tc_fence_before();
+        rows_pair_barrier();
+        tc_fence_after();
+        const float2 ml0 = c.pair_ml[0][row], ml1 = c.pair_ml[1][row];
+        const float m = fmaxf(ml0.x, ml1.x);
+        const float f0 = ml0.x == -INFINITY ? 0.f : exp2f(ml0.x - m), f1 = ml1.x == -INFINITY ? 0.f : exp2f(ml1.x - m);
+        const float sum = (f0 == 0.f ? 0.f : f0 * ml0.y) + (f1 == 0.f ? 0.f : f1 * ml1.y);
+        const bool empty = m == -INFINITY;
+        if (ok) {
+          const float inv = it.slot >= 0 ? 1.f : empty ? 0.f : 1.f / sum;
+          const int64_t part_row = (int64_t)it.slot * kRows + row, off = c.ooff[n & 1][row];
+#pragma unroll 1
+          for (int ch = 32 * x; ch < kPart; ch += 64) {
+            uint32_t v[32], w[32];
+            tmem_ld32(tmem + lane_base + 256 + ch, v);
+            tmem_ld32(tmem + lane_base + 384 + ch, w);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float e0 = f0 == 0.f ? 0.f : f0 * __uint_as_float(v[i]), e1 = f1 == 0.f ? 0.f : f1 * __uint_as_float(w[i]);
+              v[i] = __float_as_uint((e0 + e1) * inv);
+            }
+            if (on && it.slot >= 0) {
+#pragma unroll
+              for (int u = 0; u < 32; u += 8) store32(a.part + part_row * D + ch + u, v + u);
+            } else if (on) {
+#pragma unroll
+              for (int u = 0; u < 32; u += 8) {
+                uint32_t y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = pack2_16<kHalf>(__uint_as_float(v[u + 2 * i]), __uint_as_float(v[u + 2 * i + 1]));
+                *reinterpret_cast<uint4*>(a.out + off + ch + u) = make_uint4(y[0], y[1], y[2], y[3]);
+              }
+            }
+            __syncwarp();
+          }
+          if (on && x == 0) {
+            if (it.slot >= 0) a.part_ml[part_row] = make_float2(m, sum);
+            else if (a.lse != nullptr) a.lse[(int64_t)(it.h * p.G + (at + row) - i_row * p.G) * p.T + it.row0 + i_row] = (m + log2f(sum)) * kLn2;
+          }
+          tc_fence_before();
+        } else {
+          atomicExch(&a.plan->status, RS_SOFTMAX);
+          c.abort = 1;
+        }
+        continue;
+      }
+      if (ok) {
         tc_fence_after();
         float m_ref = rr.ref;
         const float l = rr.l;
@@ -958,7 +1049,7 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
         if (l != l) m_ref = INFINITY;
         const int col0 = kWide ? x * kPart : 0;              // this warp's columns of O
         if (it.slot >= 0) {
-          const int64_t part_row = (int64_t)it.slot * kRows + (kWide ? 0 : x * kTileM) + row;
+          const int64_t part_row = (int64_t)it.slot * kRows + base + row;
           if (on && col0 == 0) a.part_ml[part_row] = make_float2(m_ref, l);
           float* dst = a.part + part_row * D + col0;
 #pragma unroll 1
@@ -976,7 +1067,7 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
           const float inv = kWide ? row_inv : empty ? 0.f : 1.f / l;
           // rows pass through this warp's 8 KB of the idle Q tile: 64 columns at a time, rows 144 bytes apart
           unsigned char* stage = smem + x * kTileBytes + (warp & 3) * 8192;
-          const int64_t* ooff = c.ooff[n & 1] + (kWide ? 0 : x * kTileM) + (warp & 3) * 32;
+          const int64_t* ooff = c.ooff[n & 1] + base + (warp & 3) * 32;
 #pragma unroll 1
           for (int ch = 0; ch < kPart; ch += 64) {
             const int cols = min(kPart - ch, 64);
@@ -1013,7 +1104,7 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
           }
         }
         tc_fence_before();
-      } else if (busy) {
+      } else {
         atomicExch(&a.plan->status, RS_SOFTMAX);
         c.abort = 1;
       }
