@@ -174,10 +174,25 @@ __device__ __forceinline__ FewItem few_item(const PagedParams& p, const FewPlan&
   return it;
 }
 
-// Units [first, last) of CTA c of n.
-__device__ __forceinline__ int64_t few_cut(int64_t units, int n, int c) { return units / n * c + units % n * c / n; }
-// CTAs that share the line: a piece is two units at least, so that short lines are joined from fewer pieces.
-__device__ __forceinline__ int few_ctas(int64_t units, int grid) { return (int)max(min((units + 1) / 2, (int64_t)grid), (int64_t)1); }
+// CTAs that share the line, and where the units of each begin: as many for all, one more for the first few.  A piece is two units at
+// least, so that short lines are joined from fewer pieces.
+struct FewCut {
+  int ctas, rest;
+  int64_t each;
+  __device__ __forceinline__ int64_t operator()(int c) const { return each * c + min(c, rest); }
+};
+__device__ __forceinline__ FewCut few_cut(int64_t units, int grid) {
+  FewCut f;
+  f.ctas = (int)max(min((units + 1) / 2, (int64_t)grid), (int64_t)1);
+  f.each = units / f.ctas;
+  f.rest = (int)(units - f.each * f.ctas);
+  return f;
+}
+
+// For the joining kernel, from each CTA: the item that it began and others end (pieces: theirs and its own; 0: there is none).
+struct FewShared {
+  int32_t pieces, row0, n, h, tile;
+};
 
 struct FewArgs {
   const void* q;
@@ -187,6 +202,7 @@ struct FewArgs {
   float* lse;
   float* part;                             // [2 * CTAs][kM][D]: outputs of shared items, by CTA: 0 one that others began, 1 one that others end
   float2* part_ml;                         // [2 * CTAs][kM]: {maximum, sum}
+  FewShared* shared;                       // [CTAs]
 };
 
 // Packed row (token, head) of row r of a tile, or -1.
@@ -228,9 +244,12 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
   pdl_wait();
   pdl_trigger();
   const int64_t units = few_plan<kM, S::kUnit, kFewThreads>(p, plan);
-  const int ctas = few_ctas(units, gridDim.x);
-  if ((int)blockIdx.x >= ctas) return;
-  const int64_t first = few_cut(units, ctas, blockIdx.x), last = few_cut(units, ctas, blockIdx.x + 1);
+  const FewCut cut = few_cut(units, gridDim.x);
+  const int64_t first = cut(blockIdx.x), last = cut(blockIdx.x + 1);
+  if ((int)blockIdx.x >= cut.ctas || first >= last) {
+    if (threadIdx.x == 0) a.shared[blockIdx.x].pieces = 0;
+    return;
+  }
   const uint32_t ring = smem_u32(smem) + warp * S::kWarpBytes;
   // addresses of ldmatrix within a sub-block: row of this lane, pieces in the order of the swizzle
   const int mrow = lane & 7, mi = lane >> 3;
@@ -561,6 +580,19 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
     }
     __syncthreads();
     const bool whole = it.u0 == 0 && it.u1 == it.units;
+    if (u >= last && threadIdx.x == 0) {                    // the CTA's last item
+      int pieces = 0;
+      if (it.u0 == 0 && !whole) {
+        const int64_t end_unit = last - it.u1 + it.units;
+        int lo = blockIdx.x + 1, hi = cut.ctas;             // the last CTA that begins before the item's end
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) / 2;
+          if (cut(mid) < end_unit) lo = mid; else hi = mid;
+        }
+        pieces = lo - (int)blockIdx.x + 1;
+      }
+      a.shared[blockIdx.x] = FewShared{pieces, s.row0, s.n, it.h, it.tile};
+    }
     const int64_t slot = 2 * (int64_t)blockIdx.x + (it.u0 == 0 ? 1 : 0);
     for (int n = threadIdx.x; n < kM * (D / 4); n += kFewThreads) {
       const int r = n / (D / 4), c = n % (D / 4) * 4;
@@ -600,32 +632,25 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
 // Joins the pieces of the items that several CTAs share.  Block c: the item that CTA c began and did not end.  A few long sequences
 // have a hundred pieces an item: threads in groups take every so many of them, their sums are added in the order of the groups.
 constexpr int kJoinThreads = 512;
-template <bool kHalf, int D, int kStore, int kM>
-__global__ void __launch_bounds__(kJoinThreads) paged_few_join_kernel(const PagedParams p, const FewArgs a, int grid) {
-  using S = FewShape<D, kStore>;
-  __shared__ FewPlan plan;
+template <bool kHalf, int D, int kM>
+__global__ void __launch_bounds__(kJoinThreads) paged_few_join_kernel(const PagedParams p, const FewArgs a) {
   __shared__ float weight[kFewMaxCtas][kM];
   __shared__ float most[kM], total[kM];
   __shared__ float4 sums[kJoinThreads];
   pdl_wait();
   pdl_trigger();
-  const int64_t units = few_plan<kM, S::kUnit, kJoinThreads>(p, plan);
-  const int ctas = few_ctas(units, grid);
   const int c0 = blockIdx.x;
-  if (c0 >= ctas) return;
-  const int64_t first = few_cut(units, ctas, c0), last = few_cut(units, ctas, c0 + 1);
-  if (last <= first || last >= units) return;
+  FewShared it;
+  it.pieces = __ldcg(&a.shared[c0].pieces);
+  it.row0 = __ldcg(&a.shared[c0].row0);
+  it.n = __ldcg(&a.shared[c0].n);
+  it.h = __ldcg(&a.shared[c0].h);
+  it.tile = __ldcg(&a.shared[c0].tile);
+  const int pieces = it.pieces;
+  if (pieces == 0) return;
   PagedSeq s;
-  const FewItem it = few_item<kM, S::kUnit>(p, plan, last - 1, last, s);
-  const int64_t begin = last - 1 - it.u0, end = begin + it.units;
-  if (begin < first || end <= last) return;                 // begun before, or ended here
-  // CTAs that begin before the item's end: [c0, c0 + pieces)
-  int lo = c0 + 1, hi = ctas;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (few_cut(units, ctas, mid) < end) lo = mid; else hi = mid;
-  }
-  const int pieces = lo - c0 + 1;
+  s.row0 = it.row0;
+  s.n = it.n;
   auto slot = [&](int k) { return 2 * (int64_t)(c0 + k) + (k == 0 ? 1 : 0); };
   const int rows = (int)min((int64_t)kM, (int64_t)s.n * p.G - (int64_t)it.tile * kM);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -686,7 +711,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_few_join_kernel(const Page
 
 struct FewKernels {
   void (*attend)(const PagedParams, const CUtensorMap, const CUtensorMap, const FewArgs);
-  void (*join)(const PagedParams, const FewArgs, int);
+  void (*join)(const PagedParams, const FewArgs);
   size_t smem;
   int per_sm;
   bool parts;                              // of the tensor maps
@@ -694,7 +719,7 @@ struct FewKernels {
 template <bool kHalf, int D, int kStore, int kM>
 FewKernels few_kernels() {
   using S = FewShape<D, kStore>;
-  return FewKernels{paged_few_kernel<kHalf, D, kStore, kM>, paged_few_join_kernel<kHalf, D, kStore, kM>, S::kSmem, S::kCtas, S::kParts};
+  return FewKernels{paged_few_kernel<kHalf, D, kStore, kM>, paged_few_join_kernel<kHalf, D, kM>, S::kSmem, S::kCtas, S::kParts};
 }
 template <bool kHalf, int D, int kM>
 FewKernels pick_few(int store) {
@@ -708,17 +733,20 @@ FewKernels pick_few_dim(int D, int store) {
 }
 
 
+constexpr size_t kSharedBytes = (kFewMaxCtas * sizeof(FewShared) + 255) / 256 * 256;
+
 }  // namespace
 
-size_t paged_few_workspace(const PagedParams& p) { return (size_t)2 * kFewMaxCtas * 16 * (p.D * sizeof(float) + sizeof(float2)); }
+size_t paged_few_workspace(const PagedParams& p) { return kSharedBytes + (size_t)2 * kFewMaxCtas * 16 * (p.D * sizeof(float) + sizeof(float2)); }
 
 cudaError_t launch_paged_few(const PagedParams& all, const void* q, const void* kp, const void* vp, const uint8_t* ks,
                              const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st) {
   const bool eight = (int64_t)all.max_new * all.G <= 8;
   const FewKernels k = all.fp16 ? (eight ? pick_few_dim<true, 8>(all.D, all.store) : pick_few_dim<true, 16>(all.D, all.store))
                                 : (eight ? pick_few_dim<false, 8>(all.D, all.store) : pick_few_dim<false, 16>(all.D, all.store));
-  FewArgs a{q, kp, vp, ks, vs, out, lse, nullptr, nullptr};
-  a.part_ml = static_cast<float2*>(workspace);
+  FewArgs a{q, kp, vp, ks, vs, out, lse, nullptr, nullptr, nullptr};
+  a.shared = static_cast<FewShared*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + kSharedBytes);
   a.part = reinterpret_cast<float*>(a.part_ml + 2 * kFewMaxCtas * 16);
   const int slots = 1 << all.page_shift, box = all.store == MOBA_STORE_SAME || slots < 32 ? 16 : 32;
   const int elem = all.store != MOBA_STORE_SAME ? 1 : all.fp16 ? 2 : 3;
@@ -740,7 +768,7 @@ cudaError_t launch_paged_few(const PagedParams& all, const void* q, const void* 
     p.lens += b;
     p.table += b * all.table_stride;
     if ((e = launch_pdl(k.attend, dim3(grid), kFewThreads, k.smem, st, p, mk, mv, a)) != cudaSuccess) return e;
-    if ((e = launch_pdl(k.join, dim3(grid), kJoinThreads, 0, st, p, a, grid)) != cudaSuccess) return e;
+    if ((e = launch_pdl(k.join, dim3(grid), kJoinThreads, 0, st, p, a)) != cudaSuccess) return e;
   }
   return cudaSuccess;
 }

@@ -77,7 +77,7 @@ __device__ __forceinline__ int even_piece(int tiles, int piece) {
 __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p, RowsPlan* plan, int sms) {
   __shared__ int rows_s[kPagedBatch], most_s[kPagedBatch], least_s[kPagedBatch];
   __shared__ float cost_s[32];
-  __shared__ int piece_s[32], best_s;
+  __shared__ int piece_s[32];
   __shared__ int scan_s[2][32];
   pdl_wait();
   pdl_trigger();
@@ -128,15 +128,11 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p, R
     piece_s[warp] = piece;
   }
   __syncthreads();
-  if (b == 0) {
-    int best = 0;
-    for (int i = 1; i < 32; ++i)
-      if (cost_s[i] < cost_s[best]) best = i;
-    best_s = piece_s[best];
-  }
-  __syncthreads();
+  // every warp for itself: the cheapest, of equal ones the first (costs are not negative: they compare as integers)
+  const uint32_t mine = __float_as_uint(cost_s[lane]);
+  const int best = piece_s[__ffs(__ballot_sync(0xffffffffu, mine == __reduce_min_sync(0xffffffffu, mine))) - 1];
   // first items and slots of the sequences
-  const int even = even_piece(most, best_s), cuts = (most + even - 1) / even;
+  const int even = even_piece(most, best), cuts = (most + even - 1) / even;
   const int n = rows * cuts, m = cuts > 1 ? n : 0;
   int x = n, y = m;
 #pragma unroll
@@ -146,8 +142,8 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p, R
   }
   if (lane == 31) { scan_s[0][warp] = x; scan_s[1][warp] = y; }
   __syncthreads();
-  int bx = 0, by = 0;
-  for (int i = 0; i < warp; ++i) { bx += scan_s[0][i]; by += scan_s[1][i]; }
+  const int bx = __reduce_add_sync(0xffffffffu, lane < warp ? scan_s[0][lane] : 0);
+  const int by = __reduce_add_sync(0xffffffffu, lane < warp ? scan_s[1][lane] : 0);
   if (b < p.B) {
     plan->begin[b] = bx + x - n;
     plan->slot0[b] = m > 0 ? by + y - m : -1;
