@@ -102,14 +102,18 @@ __device__ __forceinline__ void codes_to_half(uint32_t x, uint32_t& lo, uint32_t
 
 // ---- the line of units -------------------------------------------------------
 // Sequence b has tiles(b) row tiles of kM, each of units(b) units of keys, for every kv head: in the order
-// sequence, kv head, row tile, unit.  (Units behind the last key that a tile sees are empty: they differ by the few new tokens.)
+// sequence, kv head, row tile, unit.  (Units behind the last key that a tile sees are empty: they differ by the few new tokens.)  In
+// front of an item's units lie kItemUnits that stand for what it costs besides (its Q rows, the way of its first copies, its
+// output): without them a CTA that got two dozen short sequences came in last, 40 us behind the others of a decode step of 48 requests.
+constexpr int kItemUnits = 2;
 struct FewPlan {
   int64_t begin[kPagedBatch + 1];          // first unit of a sequence
   int64_t scan[16];
 };
 struct FewItem {
   int b, h, tile;
-  int u0, u1, units;                       // this piece's units of the item's
+  int u0, u1, units;                       // this piece's units of the item's (u1 <= u0: none)
+  int64_t end;                             // of the item on the line
 };
 
 template <int kM>
@@ -127,7 +131,7 @@ __device__ __forceinline__ int64_t few_plan(const PagedParams& p, FewPlan& plan)
       const PagedSeq s = paged_seq(p, b);
       // (rows without a key need an item too: they are written as zeros)
       const int units = max((s.len + kUnit - 1) / kUnit, 1);
-      w = (int64_t)few_tiles<kM>(p, s) * units * p.Hkv;
+      w = (int64_t)few_tiles<kM>(p, s) * (units + kItemUnits) * p.Hkv;
     }
     int64_t x = w;
 #pragma unroll
@@ -165,12 +169,15 @@ __device__ __forceinline__ FewItem few_item(const PagedParams& p, const FewPlan&
   FewItem it;
   it.b = lo;
   it.units = max((s.len + kUnit - 1) / kUnit, 1);
-  const int64_t at = u - plan.begin[lo], item = at / it.units;
+  const int line = it.units + kItemUnits;
+  const int64_t at = u - plan.begin[lo], item = at / line;
   const int tiles = few_tiles<kM>(p, s);
   it.h = (int)(item / tiles);
   it.tile = (int)(item - (int64_t)it.h * tiles);
-  it.u0 = (int)(at - item * it.units);
-  it.u1 = (int)min((int64_t)it.units, it.u0 + (end - u));
+  const int on = (int)(at - item * line) - kItemUnits;
+  it.u0 = max(on, 0);
+  it.u1 = (int)min((int64_t)it.units, on + (end - u));
+  it.end = u - on + it.units;
   return it;
 }
 
@@ -266,11 +273,13 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
   uint32_t phase = 0;                                       // of st_out
   uint32_t there = 0;                                       // groups in flight that have a page, the oldest block's lowest
   bool ok = true;
+  FewShared shared{0, 0, 0, 0, 0};
 
   for (int64_t u = first; u < last;) {
     PagedSeq s;
     const FewItem it = few_item<kM, S::kUnit>(p, plan, u, last, s);
-    u += it.u1 - it.u0;
+    u = it.end;
+    if (it.u1 <= it.u0) continue;
     // keys that some row of the tile sees: rows of the last new token see the most, the first row sees the least
     const int64_t tile_last = min((int64_t)s.n - 1, ((int64_t)(it.tile + 1) * kM - 1) / p.G);
     const int end = (int)min(max((int64_t)s.pos0 + tile_last + 1, (int64_t)0), (int64_t)s.len);
@@ -580,18 +589,13 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
     }
     __syncthreads();
     const bool whole = it.u0 == 0 && it.u1 == it.units;
-    if (u >= last && threadIdx.x == 0) {                    // the CTA's last item
-      int pieces = 0;
-      if (it.u0 == 0 && !whole) {
-        const int64_t end_unit = last - it.u1 + it.units;
-        int lo = blockIdx.x + 1, hi = cut.ctas;             // the last CTA that begins before the item's end
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) / 2;
-          if (cut(mid) < end_unit) lo = mid; else hi = mid;
-        }
-        pieces = lo - (int)blockIdx.x + 1;
+    if (it.u0 == 0 && !whole) {
+      int lo = blockIdx.x + 1, hi = cut.ctas;               // the last CTA that begins before the item's end
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (cut(mid) < it.end) lo = mid; else hi = mid;
       }
-      a.shared[blockIdx.x] = FewShared{pieces, s.row0, s.n, it.h, it.tile};
+      shared = FewShared{lo - (int)blockIdx.x + 1, s.row0, s.n, it.h, it.tile};
     }
     const int64_t slot = 2 * (int64_t)blockIdx.x + (it.u0 == 0 ? 1 : 0);
     for (int n = threadIdx.x; n < kM * (D / 4); n += kFewThreads) {
@@ -627,6 +631,7 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
     fence_proxy_async_smem();                               // the ring is copied to again
     __syncthreads();
   }
+  if (threadIdx.x == 0) a.shared[blockIdx.x] = shared;
 }
 
 // Joins the pieces of the items that several CTAs share.  Block c: the item that CTA c began and did not end.  A few long sequences
@@ -634,7 +639,9 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
 constexpr int kJoinThreads = 512;
 template <bool kHalf, int D, int kM>
 __global__ void __launch_bounds__(kJoinThreads) paged_few_join_kernel(const PagedParams p, const FewArgs a) {
-  __shared__ float weight[kFewMaxCtas][kM];
+  extern __shared__ float join_smem[];
+  float(*weight)[kM] = reinterpret_cast<float(*)[kM]>(join_smem);
+  float(*part_sum)[kM] = weight + kFewMaxCtas;
   __shared__ float most[kM], total[kM];
   __shared__ float4 sums[kJoinThreads];
   pdl_wait();
@@ -654,44 +661,67 @@ __global__ void __launch_bounds__(kJoinThreads) paged_few_join_kernel(const Page
   auto slot = [&](int k) { return 2 * (int64_t)(c0 + k) + (k == 0 ? 1 : 0); };
   const int rows = (int)min((int64_t)kM, (int64_t)s.n * p.G - (int64_t)it.tile * kM);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // ---- weights of the pieces, a warp a row
+  const int outputs = rows * (D / 4);
+  const int groups = outputs >= kJoinThreads ? 1 : kJoinThreads / outputs;
+  const int group = outputs >= kJoinThreads ? 0 : threadIdx.x / outputs;
+  const int n0 = outputs >= kJoinThreads ? threadIdx.x : threadIdx.x % outputs;
+  // the first pieces of this thread's first output are on their way while the weights are worked out
+  constexpr int kAhead = 8;
+  float4 ahead[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const int k = group + i * groups;
+    ahead[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (group < groups && k < pieces && n0 < outputs)
+      ahead[i] = __ldcg(reinterpret_cast<const float4*>(a.part + (slot(k) * kM + n0 / (D / 4)) * D + n0 % (D / 4) * 4));
+  }
+  // ---- weights of the pieces
+  for (int n = threadIdx.x; n < pieces * rows; n += kJoinThreads) {
+    const int k = n / rows, r = n - k * rows;
+    const float2 ml = __ldcg(a.part_ml + slot(k) * kM + r);
+    weight[k][r] = ml.x;
+    part_sum[k][r] = ml.y;
+  }
+  __syncthreads();
   for (int r = warp; r < rows; r += kJoinThreads / 32) {
     float mx = -INFINITY;
-    for (int k = lane; k < pieces; k += 32) mx = fmaxf(mx, __ldcg(a.part_ml + slot(k) * kM + r).x);
+    for (int k = lane; k < pieces; k += 32) mx = fmaxf(mx, weight[k][r]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     float sum = 0.f;
     for (int k = lane; k < pieces; k += 32) {
-      const float2 ml = __ldcg(a.part_ml + slot(k) * kM + r);
-      const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mx);
+      const float x = weight[k][r], f = x == -INFINITY ? 0.f : exp2f(x - mx);
       weight[k][r] = f;
-      if (f != 0.f) sum += f * ml.y;
+      if (f != 0.f) sum += f * part_sum[k][r];
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) { most[r] = mx; total[r] = sum; }
   }
   __syncthreads();
-  const int outputs = rows * (D / 4);
-  const int groups = outputs >= kJoinThreads ? 1 : kJoinThreads / outputs;
-  const int group = outputs >= kJoinThreads ? 0 : threadIdx.x / outputs;
-  for (int n = outputs >= kJoinThreads ? threadIdx.x : threadIdx.x % outputs; n < outputs; n += kJoinThreads) {
+  for (int n = n0; n < outputs; n += kJoinThreads) {
     const int r = n / (D / 4), c = n % (D / 4) * 4;
     float x[4] = {0.f, 0.f, 0.f, 0.f};
+    // (a piece that saw nothing has no weight; what it holds is no number that counts)
+    auto add = [&](float f, const float4& v) {
+      if (f == 0.f) return;
+      x[0] += f * v.x; x[1] += f * v.y; x[2] += f * v.z; x[3] += f * v.w;
+    };
     if (group < groups) {
-#pragma unroll 4
-      for (int k = group; k < pieces; k += groups) {
-        const float f = weight[k][r];
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part + (slot(k) * kM + r) * D + c));
-        // (a piece that saw nothing has no weight; what it holds is no number that counts)
-        x[0] += f == 0.f ? 0.f : f * v.x; x[1] += f == 0.f ? 0.f : f * v.y;
-        x[2] += f == 0.f ? 0.f : f * v.z; x[3] += f == 0.f ? 0.f : f * v.w;
+      int k = group;
+      if (n == n0) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i, k += groups) add(k < pieces ? weight[k][r] : 0.f, ahead[i]);
       }
+#pragma unroll 4
+      for (; k < pieces; k += groups) add(weight[k][r], __ldcg(reinterpret_cast<const float4*>(a.part + (slot(k) * kM + r) * D + c)));
     }
     if (groups > 1) {
       sums[threadIdx.x] = make_float4(x[0], x[1], x[2], x[3]);
       __syncthreads();
-      if (group != 0) break;
+    }
+    if (group != 0) break;
+    if (groups > 1) {
       for (int k = 1; k < groups; ++k) {
         const float4 v = sums[k * outputs + n];
         x[0] += v.x; x[1] += v.y; x[2] += v.z; x[3] += v.w;
@@ -759,6 +789,7 @@ cudaError_t launch_paged_few(const PagedParams& all, const void* q, const void* 
     return cudaErrorNotSupported;
   cudaError_t e = prepare_kernel(k.attend, k.smem, nullptr, true);
   if (e != cudaSuccess) return e;
+  if ((e = prepare_kernel(k.join, 2 * kFewMaxCtas * 16 * sizeof(float))) != cudaSuccess) return e;
   const int sms = device_info().sms;
   const int grid = k.per_sm * sms < kFewMaxCtas ? k.per_sm * sms : kFewMaxCtas;
   for (int b = 0; b < all.B; b += kPagedBatch) {
@@ -768,7 +799,7 @@ cudaError_t launch_paged_few(const PagedParams& all, const void* q, const void* 
     p.lens += b;
     p.table += b * all.table_stride;
     if ((e = launch_pdl(k.attend, dim3(grid), kFewThreads, k.smem, st, p, mk, mv, a)) != cudaSuccess) return e;
-    if ((e = launch_pdl(k.join, dim3(grid), kJoinThreads, 0, st, p, a)) != cudaSuccess) return e;
+    if ((e = launch_pdl(k.join, dim3(grid), kJoinThreads, 2 * kFewMaxCtas * (eight ? 8 : 16) * sizeof(float), st, p, a)) != cudaSuccess) return e;
   }
   return cudaSuccess;
 }

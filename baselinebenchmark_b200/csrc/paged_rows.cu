@@ -72,8 +72,8 @@ __device__ __forceinline__ int even_piece(int tiles, int piece) {
   return (tiles + cuts - 1) / cuts;
 }
 
-// Candidate k cuts the batch into about k pieces a CTA.  With equal pieces the time is that of the waves; longer ones than the average
-// may come last.
+// Candidate k cuts the batch into about k / 4 pieces a CTA, candidate 0 not at all.  With equal pieces the time is that of the waves;
+// longer ones than the average may come last.
 __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p, RowsPlan* plan, int sms) {
   __shared__ int rows_s[kPagedBatch], most_s[kPagedBatch], least_s[kPagedBatch];
   __shared__ float cost_s[32];
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p, R
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
   longest = __reduce_max_sync(0xffffffffu, longest);
-  const int piece = warp == 0 ? longest : max((int)ceilf(work / (float)(sms * warp)), 8);
+  const int piece = warp == 0 ? longest : max((int)ceilf(4.f * work / (float)(sms * warp)), 4);
   float items = 0.f;
   int slots = 0, top = 1;
   for (int i = lane; i < p.B; i += 32) {
