@@ -240,14 +240,18 @@ __global__ void __launch_bounds__(kRowThreads) paged_load_kernel(const PagedPara
 }
 
 typedef void (*RowKernel)(const PagedParams, const RowArgs);
+constexpr int kManyLoad = 4, kManyStore = 2;   // tokens of a warp, where there are many
 
 template <bool kHalf, int D, int kTokens>
 RowKernel pick_store(bool load, int store) {
-  if (load)
-    return store == MOBA_STORE_SAME ? paged_load_kernel<kHalf, D, MOBA_STORE_SAME, kTokens>
-         : store == MOBA_STORE_E4M3 ? paged_load_kernel<kHalf, D, MOBA_STORE_E4M3, kTokens>
-                                    : paged_load_kernel<kHalf, D, MOBA_STORE_INT8, kTokens>;
-  return store == MOBA_STORE_SAME ? paged_store_kernel<kHalf, D, MOBA_STORE_SAME, kTokens>
+  if constexpr (kTokens != kManyStore) {
+    if (load)
+      return store == MOBA_STORE_SAME ? paged_load_kernel<kHalf, D, MOBA_STORE_SAME, kTokens>
+           : store == MOBA_STORE_E4M3 ? paged_load_kernel<kHalf, D, MOBA_STORE_E4M3, kTokens>
+                                      : paged_load_kernel<kHalf, D, MOBA_STORE_INT8, kTokens>;
+  }
+  if constexpr (kTokens == kManyLoad) return nullptr;
+  else return store == MOBA_STORE_SAME ? paged_store_kernel<kHalf, D, MOBA_STORE_SAME, kTokens>
        : store == MOBA_STORE_E4M3 ? paged_store_kernel<kHalf, D, MOBA_STORE_E4M3, kTokens>
                                   : paged_store_kernel<kHalf, D, MOBA_STORE_INT8, kTokens>;
 }
@@ -264,15 +268,15 @@ RowKernel pick_row_kernel(bool load, const PagedParams& p) {
 
 cudaError_t launch_rows(bool load, const PagedParams& p, RowArgs a, cudaStream_t st) {
   const int rows = 32 * 8 / (p.D == 96 ? 128 : p.D);        // heads of one warp access
-  constexpr int kMany = 4;
-  // four tokens a warp where that still gives every SM its warps
-  const int passes = (p.Hkv + rows - 1) / rows;
-  const bool many = p.T * passes >= (int64_t)kMany * 148 * 64;
+  // A few tokens a warp where that still gives every SM its warps: more loads under way.  Four rows read back at a time, two written (131072 tokens
+  // of e4m3 read back, 8 heads of 128: 1 165, 2 165, 4 144, 8 148 us; 8191 written to int8 and read back, written by 4 30.5, by 2 28.1).
+  const int passes = (p.Hkv + rows - 1) / rows, several = load ? kManyLoad : kManyStore;
+  const bool many = p.T * passes >= (int64_t)several * 148 * 64;
   a.units = passes;
   a.heads = rows;
-  const int64_t warps = (p.T + (many ? kMany : 1) - 1) / (many ? kMany : 1) * a.units;
+  const int64_t warps = (p.T + (many ? several : 1) - 1) / (many ? several : 1) * a.units;
   const int64_t blocks = (warps + kRowThreads / 32 - 1) / (kRowThreads / 32);
-  return launch_pdl(many ? pick_row_kernel<kMany>(load, p) : pick_row_kernel<1>(load, p), dim3((unsigned)blocks), kRowThreads, 0, st, p, a);
+  return launch_pdl(!many ? pick_row_kernel<1>(load, p) : load ? pick_row_kernel<kManyLoad>(load, p) : pick_row_kernel<kManyStore>(load, p), dim3((unsigned)blocks), kRowThreads, 0, st, p, a);
 }
 
 }  // namespace

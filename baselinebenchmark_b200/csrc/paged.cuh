@@ -61,9 +61,18 @@ cudaError_t launch_paged_load(const PagedParams& p, const void* kp, const void* 
 // Sequences that one launch of an attention kernel takes: their work is added up in shared memory.
 constexpr int kPagedBatch = 1024;
 
-// Items of more rows run on tcgen05.
-constexpr int kPagedFewRows = 16;
-inline bool paged_few_rows(const PagedParams& p) { return (int64_t)p.max_new * p.G <= kPagedFewRows; }
+// Items of more rows run on tcgen05.  Two new launches (the plan, the join of many rows) cost a small call 8 us there; in a large one the tensor
+// memory kernel keeps up with the copies whatever the rows are, where the other's chain grows with them.  8-bit codes are turned once for each
+// tile of 16 rows here and once for each of 128 or 256 there, by fewer warps.  (rows: this kernel / tcgen05, us; 16 sequences of 8000 tokens
+// over 8 kv heads, the same over one, 2 of 500; 64-token pages)
+//   head dim 128          8:  93 / 94, 19 / 33, 12 / 20    16: 120 / 95, 39 / 33, 13 / 21     32: 207 / 96, 43 / 33, 16 / 21
+//   head dim 128, e4m3    8:  57 / 157, 17 / 41, 12 / 26   16:  59 / 157, 22 / 41, 13 / 26    32: 100 / 159, 24 / 41, 13 / 26
+//                         48 (8 sequences): 79 / 92        64: 100 / 92, 34 / 42
+//   head dim 256          8: 179 / 171, 51 / 50, 16 / 27    16: 186 / 171, 49 / 50, 17 / 27    32: 345 / 173, 58 / 51, 23 / 27
+inline bool paged_few_rows(const PagedParams& p) {
+  const int most = p.store != MOBA_STORE_SAME ? 48 : p.D == 256 ? 16 : 8;
+  return (int64_t)p.max_new * p.G <= most;
+}
 
 size_t paged_rows_workspace(const PagedParams& p);
 cudaError_t launch_paged_rows(const PagedParams& p, const void* q, const void* kp, const void* vp, const uint8_t* ks,

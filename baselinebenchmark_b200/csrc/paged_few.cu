@@ -36,7 +36,7 @@ constexpr int kFewWarps = 4, kFewThreads = kFewWarps * 32;
 constexpr int kFewMaxCtas = 148 * 3;
 constexpr float kLn2 = 0.6931471805599453f;
 
-template <int D, int kStore> struct FewShape {
+template <int D, int kStore, int kM> struct FewShape {
   static constexpr bool kCodes = kStore != MOBA_STORE_SAME;
   static constexpr int kKeys = kCodes ? 32 : 16;                     // of a warp's block
   static constexpr int kSpan = kCodes ? 128 : 64;                    // elements of 128 bytes
@@ -45,10 +45,11 @@ template <int D, int kStore> struct FewShape {
   static constexpr int kSideBytes = kSubs * kSubBytes;               // K; V behind it
   static constexpr int kStageBytes = 2 * kSideBytes;
   static constexpr bool kParts = !kCodes && kSubs > 1 && D % kSpan == 0;   // one box has all sub-blocks (not of head dim 96: a row's would end in the next)
-  // three CTAs, twelve warps, an SM with 16 KB of stages each (one CTA with 48 KB at head dim 256): what a warp waits for is its own chain of
-  // instructions, and there have to be others meanwhile
-  static constexpr int kCtas = kStageBytes == 16384 ? 1 : 3;
-  static constexpr int kStages = kStageBytes == 16384 ? 3 : kStageBytes == 8192 ? 2 : 4;
+  // Three CTAs, twelve warps, an SM with 16 KB of stages each: what a warp waits for is its own chain of instructions, and there have to be
+  // others meanwhile.  One CTA with 48 KB a warp at head dim 256; two with 24 KB for codes at head dim 128,
+  // which do not fit the registers of three (16 sequences of 8000 tokens, 32/8 heads, e4m3, tiles of 16 rows 97 us with three, 57 with two).
+  static constexpr int kCtas = kStageBytes == 16384 ? 1 : kCodes && D == 128 ? 2 : 3;
+  static constexpr int kStages = kStageBytes == 16384 || kCtas == 2 ? 3 : kStageBytes == 8192 ? 2 : 4;
   static constexpr int kWarpBytes = kStages * kStageBytes;
   static constexpr int kUnit = kKeys * kFewWarps;                    // keys of a CTA's unit
   static constexpr size_t kSmem = 1024 + (size_t)kFewWarps * kWarpBytes;
@@ -224,9 +225,9 @@ __device__ __forceinline__ bool few_row(const PagedParams& p, const PagedSeq& s,
 
 // kM: rows of a tile, 8 or 16 (the upper half of the MMA's rows is empty with 8, and its exponentials are left out)
 template <bool kHalf, int D, int kStore, int kM>
-__global__ void __launch_bounds__(kFewThreads, FewShape<D, kStore>::kCtas)
+__global__ void __launch_bounds__(kFewThreads, FewShape<D, kStore, kM>::kCtas)
 paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const FewArgs a) {
-  using S = FewShape<D, kStore>;
+  using S = FewShape<D, kStore, kM>;
   constexpr bool kCodes = S::kCodes;
   constexpr bool kF16 = kHalf || kCodes;                    // operands of the MMAs
   constexpr int kSteps = D / 16;                            // k-steps of Q.K^T
@@ -748,7 +749,7 @@ struct FewKernels {
 };
 template <bool kHalf, int D, int kStore, int kM>
 FewKernels few_kernels() {
-  using S = FewShape<D, kStore>;
+  using S = FewShape<D, kStore, kM>;
   return FewKernels{paged_few_kernel<kHalf, D, kStore, kM>, paged_few_join_kernel<kHalf, D, kM>, S::kSmem, S::kCtas, S::kParts};
 }
 template <bool kHalf, int D, int kM>

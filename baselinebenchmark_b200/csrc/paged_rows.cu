@@ -1215,27 +1215,38 @@ __global__ void __launch_bounds__(kJoinThreads) paged_rows_join_kernel(const Pag
     constexpr int kRows = item_rows(D);
     const int row = i * p.G + head - h * p.G, tile = row / kRows, r = row - tile * kRows;
     const int mine = (key_tiles(rows_end(p, s, tile)) + piece - 1) / piece;
-    for (int k = 0; k < mine; ++k) {
-      const int64_t at = ((int64_t)slot0 + ((int64_t)h * cuts + k) * tiles + tiles - 1 - tile) * kRows + r;
-      const float2 ml = __ldcg(a.part_ml + at);
-      float v[kPer];
-      const float* src = a.part + at * D + lane * kPer;
-      if constexpr (kPer % 4 == 0) {
+    // several pieces under way at a time
+    constexpr int kAhead = kPer > 4 ? 4 : 8;
+    for (int k0 = 0; k0 < mine; k0 += kAhead) {
+      float2 ml[kAhead];
+      float v[kAhead][kPer];
 #pragma unroll
-        for (int u = 0; u < kPer; u += 4) {
-          const float4 f = __ldcg(reinterpret_cast<const float4*>(src + u));
-          v[u] = f.x; v[u + 1] = f.y; v[u + 2] = f.z; v[u + 3] = f.w;
+      for (int k = 0; k < kAhead; ++k) {
+        ml[k] = make_float2(-INFINITY, 0.f);
+        if (k0 + k >= mine) continue;
+        const int64_t at = ((int64_t)slot0 + ((int64_t)h * cuts + k0 + k) * tiles + tiles - 1 - tile) * kRows + r;
+        ml[k] = __ldcg(a.part_ml + at);
+        const float* src = a.part + at * D + lane * kPer;
+        if constexpr (kPer % 4 == 0) {
+#pragma unroll
+          for (int u = 0; u < kPer; u += 4) {
+            const float4 f = __ldcg(reinterpret_cast<const float4*>(src + u));
+            v[k][u] = f.x; v[k][u + 1] = f.y; v[k][u + 2] = f.z; v[k][u + 3] = f.w;
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < kPer; ++u) v[k][u] = __ldcg(src + u);
         }
-      } else {
-#pragma unroll
-        for (int u = 0; u < kPer; ++u) v[u] = __ldcg(src + u);
       }
-      if (ml.x == -INFINITY) continue;
-      const float up = fmaxf(mx, ml.x), f0 = exp2f(mx - up), f1 = exp2f(ml.x - up);
-      mx = up;
-      sum = sum * f0 + ml.y * f1;
 #pragma unroll
-      for (int u = 0; u < kPer; ++u) x[u] = x[u] * f0 + v[u] * f1;
+      for (int k = 0; k < kAhead; ++k) {
+        if (ml[k].x == -INFINITY) continue;
+        const float up = fmaxf(mx, ml[k].x), f0 = exp2f(mx - up), f1 = exp2f(ml[k].x - up);
+        mx = up;
+        sum = sum * f0 + ml[k].y * f1;
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) x[u] = x[u] * f0 + v[k][u] * f1;
+      }
     }
   }
   const float inv = mx == -INFINITY ? 0.f : 1.f / sum;
