@@ -76,6 +76,11 @@ int check_pointers(const moba_paged_t* p, const void* a, const void* b, const in
 
 size_t workspace_of(const PagedParams& p) { return paged_few_rows(p) ? paged_few_workspace(p) : paged_rows_workspace(p); }
 
+// Rows that are written must not lie on one another (a single token or head is never stepped over).
+bool apart(const moba_paged_t* p, int64_t token, int64_t head, int heads) {
+  return (token > 0 || p->total_tokens == 1) && (head > 0 || heads == 1);
+}
+
 }  // namespace
 
 extern "C" {
@@ -95,6 +100,8 @@ int moba_paged_load(const moba_paged_t* p, const int32_t* cu, const int32_t* len
   int rc = check_paged(p);
   if (rc == MOBA_OK) rc = check_pointers(p, k, v, cu, lens, table, kp, vp, ks, vs);
   if (rc != MOBA_OK) return rc;
+  if (!apart(p, p->k_stride_token, p->k_stride_head, p->num_kv_heads) || !apart(p, p->v_stride_token, p->v_stride_head, p->num_kv_heads))
+    return MOBA_E_SHAPE;
   return (int)launch_paged_load(paged_params(p, cu, lens, table), kp, vp, ks, vs, k, v, (cudaStream_t)stream);
 }
 
@@ -112,6 +119,7 @@ int moba_paged_attention(const moba_paged_t* p, const void* q, const int32_t* cu
   int rc = check_paged(p);
   if (rc == MOBA_OK) rc = check_pointers(p, q, out, cu, lens, table, kp, vp, ks, vs);
   if (rc != MOBA_OK) return rc;
+  if (!apart(p, p->o_stride_token, p->o_stride_head, p->num_q_heads)) return MOBA_E_SHAPE;
   if ((uintptr_t)lse_out & 3) return MOBA_E_ALIGN;
   const PagedParams r = paged_params(p, cu, lens, table);
   if (workspace == nullptr || workspace_bytes < workspace_of(r)) return MOBA_E_WORKSPACE;

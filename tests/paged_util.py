@@ -15,12 +15,13 @@ def two(e):
 
 
 def quantise(x, store):
-    """(codes as float64, bytes) of rows x [..., D]: the rule of include/moba_b200.h, one comparison at a time."""
+    """(codes as float64, bytes) of rows x [..., D]: the rule of include/moba_b200.h."""
     y = x.double()
     amax = y.abs().amax(-1)
-    e = torch.full(amax.shape, -96, dtype=torch.int64, device=x.device)
-    for _ in range(230):                                     # the least power of two that is enough
-        e = torch.where(TOP[store] * two(e) < amax, e + 1, e)
+    # the least e with top * 2^e >= amax: amax / top is 2^(e - 1) < .. <= 2^e.  Both are numbers of at most 11 bits: in float64 the quotient is
+    # a power of two when it is one, and nowhere near one otherwise.
+    m, e = torch.frexp(torch.where(torch.isfinite(amax), amax, torch.zeros_like(amax)) / TOP[store])
+    e = torch.where(m == 0.5, e - 1, e).long().clamp(min=-96)
     e = torch.where(amax == 0, torch.zeros_like(e), e)
     bad = ~torch.isfinite(y).all(-1)
     e = torch.where(bad, torch.full_like(e, 128), e)

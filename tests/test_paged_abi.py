@@ -59,6 +59,8 @@ def test_pointers_are_checked_before_any_launch(lib):
     assert attend(p, off, ok) == -6 and attend(p, ok, ok, out=off) == -6 and attend(p, ok, ok, lse=0x10002) == -6
     assert attend(p, ok, ok, ws=None) == -3 and attend(p, ok, ok, size=need.value - 1) == -3
     assert attend(p, ok, ok, ws=0x10010) == -6
+    assert attend(C.byref(_paged(o_stride_token=0)), ok, ok) == -1 and attend(C.byref(_paged(o_stride_head=0)), ok, ok) == -1
+    assert load(C.byref(_paged(v_stride_token=0)), ok, ok, ok, ok, ok, None, None, ok, ok) == -1     # rows on one another
 
 
 def _tensors(**kw):
