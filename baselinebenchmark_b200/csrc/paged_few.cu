@@ -1,12 +1,12 @@
 // Attention over pages for sequences with few new tokens (decode steps, drafted tokens), with mma.sync.
 //
-// Rows of an item are the (new token, query head) pairs of one sequence and kv head, token by token, 16 at a time: the M of one
-// m16n8k16.  With so few rows the bytes of K and V bound the call (2 * 16 rows of products a key against 4 D bytes of it), so what
+// Rows of an item are the (new token, query head) pairs of one sequence and kv head, token by token, 8 or 16 at a time: the M of one
+// m16n8k16, or half of it.  With so few rows the bytes of K and V bound the call (2 * 16 rows of products a key against 4 D bytes of it), so what
 // counts is that many bytes are always on their way, and the tensor work only has to keep up: no tcgen05 here, whose 128
 // lanes would be mostly empty and whose tiles would have to be handed from warp to warp.
 //   - A warp is on its own: TMA brings it blocks of 16 keys (32 of 8-bit pages) of K and V into its own ring of swizzled shared memory, and it
 //     runs Q.K^T, the softmax step and P.V on them in registers.  Nothing is waited for but its copies.  (With a copy instruction
-//     and its addresses for every 16 bytes a block was 490 instructions, and a decode step of 48 requests 188 us.)
+//     and its addresses for every 16 bytes a block was 490 instructions; with boxes it is 300.)
 //   - The keys of all items are one line of units (a block for each warp of a CTA), cut into equal pieces, one for each CTA: whatever
 //     the lengths in the batch are, all SMs read the same number of bytes.  A CTA has at most two items that others share; their
 //     results (maximum, sum, unnormalised output, fp32) go through the workspace, and a second kernel joins them in the order of
@@ -18,6 +18,13 @@
 //     each row, the largest magnitude in [2^14, 2^15): fp16 then keeps three bits more of them than bf16 has.
 //   - P is rounded to the 16-bit type that V has (or fp16): 2^-9 (2^-12) relative at most, as in the dense stage of the prefill.
 // The maximum that weights refer to is only moved when it grows by more than 8 (a factor of 256).
+// Measured (replayed from a graph, us; head dim 128, 32/8 heads unless said otherwise; in brackets the bytes at the measured copy bandwidth):
+//   one token of 48 requests of 16 to 11001 tokens                        188 -> 172 (boxes) -> 151 (three CTAs an SM) -> 115 (what an item costs besides
+//                                                                         its keys counts on the line)                          [103]
+//   one token of 16 requests of 16385 to 40001, e4m3                      214 -> 153                                            [138]
+//   five tokens of 12 requests of 338 to 20016, int8, 16/4 heads, fp16    92 -> 49                                              [14]
+//   one token behind 20011, 16/4 heads, head dim 64, fp16                 64 -> 19 (pieces joined in parallel) -> 16            [3]
+// The last two are chains of latencies: the plan of the line, a page's number, its rows, four warps joined, the second kernel.
 #include "paged.cuh"
 #include "sm100_ptx.cuh"
 

@@ -6,9 +6,11 @@
 //   - 16-bit pages: TMA copies the pages of a tile straight into the swizzled operand tiles, one box for each page (or 128 slots of
 //     one).  Warp 0 brings K, warp 3 V.  What lies behind the sequence's end in its last page, or where a page is missing, may be
 //     anything: scores there are masked, and those rows of V are overwritten with zeros before the tensor core sees them (0 * NaN).
-//   - 8-bit pages: four more warps read the codes, multiply by the row's power of two (exact: see moba_b200.h) and store the operand
-//     tiles in the rows' 16-bit type; from there on nothing differs.  That is 2.5 instructions an element of bf16 (1 to 1.75 of fp16), 5
-//     of an SM's 8 thousand issue slots of a tile's MMAs with the softmax's, in place of a pass over the cache that would write it out in 16 bits.
+//   - 8-bit pages: eight warps (3, and 12-18) read the codes, multiply by the row's power of two (exact: see moba_b200.h) and store the operand
+//     tiles in the rows' 16-bit type; from there on nothing differs, and no pass over the cache writes it out in 16 bits.  They run through one
+//     stream of tiles, without a barrier at an item's end; warp 0 tells them where the codes are.  All 19 warps live with 96 registers,
+//     which is what bounds this form: the softmax reads its scores twice, 16 at a time (with 32 at a time some values were kept in
+//     local memory, in an L1 of the few KB that shared memory leaves, and each look at them went to L2).
 //   - An item of at most 128 rows (drafted tokens, a small group) has them in both row tiles: A takes every other key tile, B the ones between,
 //     each with its own output, and the two are joined at the end.  One softmax at a time left the copies waiting.
 //   - Pieces: a first kernel (one CTA) adds up the work of the batch and picks how many pieces an item is cut into, so that
@@ -19,6 +21,12 @@
 // Roles, tensor memory and the order of MMAs are those of the dense stage of the prefill (attend_tc5.cu): warps 4-7 and 8-11 the
 // softmax of tiles A and B, a thread a row; warp 1 issues QK_A(j+1) | PV_B(j) | QK_B(j+1) | PV_A(j+1) ...; warp 2 draws and resolves the
 // item after this one.  P is rounded to the rows' type before P.V; scores, sums and the output are fp32.
+// Measured (replayed from a graph; 32/8 heads, head dim 128 unless said otherwise; in brackets the products at the measured bf16 rate):
+//   700 tokens behind 50021                              527 us, 1095 TFLOP/s [351 us]: 3300 cycles a tile and SM against 2048 of its MMAs
+//   2048 behind 30720, e4m3                              7.1 ms (mma.sync) -> 3.1 (four warps for codes) -> 2.0 (eight) -> 1.66 (one stream of tiles)
+//                                                        -> 1.28 (no values in local memory), 830 TFLOP/s [648 us]: 4600 cycles a tile
+//   prompts of 1023, 4096 and 200, 16 heads, head dim 256   3.8 ms (mma.sync) -> 0.22 [89 us]
+//   4 tokens of 16 requests of 8000 over 8 kv heads      127 us (one row tile at work) -> 95 (both, key tiles by turns) [80 us of bytes]
 #include "attend_rows.cuh"
 #include "fast_div.cuh"
 #include "paged.cuh"
@@ -37,7 +45,9 @@ constexpr int kMostRows = 2 * kTileM;
 __host__ __device__ constexpr int item_rows(int D) { return D == 256 ? kTileM : kMostRows; }
 constexpr int kCodeWarps = 8;              // that turn codes into operand tiles: warp 3, which has no V to bring, and warps 12-18
 template <int kStore> constexpr int kRowsThreads = kStore == MOBA_STORE_SAME ? 384 : 384 + 32 * (kCodeWarps - 1);
-constexpr int kMostSlots = 8 * 148;        // results of pieces that the workspace has room for
+// Results of pieces that the workspace has room for (155 MB at head dim 128): with half of them 256 items could not be cut into the four
+// pieces each that fill the waves.
+constexpr int kMostSlots = 8 * 148;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // ---- the plan ------------------------------------------------------------------
@@ -204,6 +214,10 @@ struct RowsArgs {
   FastDiv by_group;
 };
 
+// Items that are not cut come longest first, all heads by turns, where the K and V of all heads stay in L2 together; otherwise head by head, so that
+// the last head's long items may come late (prompts of 1023, 4096 and 200 tokens, 16 heads of 256: 228 us head by head, 190 by turns).
+constexpr int64_t kAllHeadsBytes = (int64_t)80 << 20;
+
 // Both row tiles have the item's rows, and the key tiles by turns.
 __device__ __forceinline__ bool rows_twice(int D, const RowsItem& it) { return D != 256 && it.nrows <= kTileM; }
 
@@ -222,10 +236,16 @@ __device__ __forceinline__ void rows_prefetch(const PagedParams& p, const RowsAr
     const int tiles = rows_tiles(p, s.n), piece = __ldcg(a.plan->piece + it.b);
     const int most = key_tiles(rows_end(p, s, tiles - 1)), cuts = (most + piece - 1) / piece;
     const int i = idx - __ldcg(a.plan->begin + it.b);      // kv head, piece, row tile, the last one first
-    const int hc = i / tiles;
-    it.tile = tiles - 1 - (i - hc * tiles);
-    it.h = hc / cuts;
-    const int cut = hc - it.h * cuts;
+    int cut = 0;
+    if (cuts == 1 && (int64_t)s.len * p.Hkv * p.D * 4 <= kAllHeadsBytes) {
+      it.tile = tiles - 1 - i / p.Hkv;
+      it.h = i % p.Hkv;
+    } else {
+      const int hc = i / tiles;
+      it.tile = tiles - 1 - (i - hc * tiles);
+      it.h = hc / cuts;
+      cut = hc - it.h * cuts;
+    }
     it.end = rows_end(p, s, it.tile);
     it.j0 = cut * piece;
     it.ntiles = min(key_tiles(it.end) - it.j0, piece);

@@ -404,7 +404,7 @@ typedef struct moba_paged {
   int32_t batch, num_q_heads, num_kv_heads, head_dim;
   int32_t num_pages, page_size;            /* page_size: a power of two, at least 16               */
   int32_t pages_per_seq;    /* columns of page_table                                               */
-  int32_t max_new;          /* most rows of a sequence, which the kernel is chosen by (a wrong one costs time only) */
+  int32_t max_new;          /* most rows of a sequence, which the kernel of the attention is chosen by (a wrong one costs time only) */
   int32_t dtype, store;     /* MOBA_DTYPE_*, MOBA_STORE_*                                          */
   float softmax_scale;      /* factor of the scores; 0: head_dim^-0.5                              */
   int32_t reserved;         /* must be 0                                                           */
@@ -428,7 +428,8 @@ int moba_paged_load(const moba_paged_t* p, const int32_t* cu_seqlens, const int3
 /* Softmax attention of every packed row to the positions of its sequence up to its own, each kv head for its group of query
  * heads.  A row that sees nothing is zeros, its LSE -inf.  lse_out: optional fp32 [Hq, T], natural log.  Sums, maxima and the
  * accumulated output are fp32; probabilities are rounded to 16 bits before the product with V.
- * The workspace needs no clearing. */
+ * The workspace is 32-byte aligned and needs no clearing; its size follows from the structure alone.  An infinity or a NaN in a row of K
+ * or V that a token sees makes that token's output NaN; one in a token behind it, in the same tile of at most 128 positions, may too. */
 int moba_paged_workspace_size(const moba_paged_t* p, size_t* bytes);
 int moba_paged_attention(const moba_paged_t* p, const void* q, const int32_t* cu_seqlens, const int32_t* seq_lens,
                          const int32_t* page_table, const void* k_pages, const void* v_pages, const uint8_t* k_scales,
