@@ -262,7 +262,7 @@ def _attention(g: _Pages, q, kv, k_pages, page_table, cu_seqlens, seq_lens, max_
         os = _rows("out", out, g, heads, tokens, k_pages)
         _check_written(out)
     else:
-        out = torch.empty(q.shape, dtype=dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         os = (heads * g.shape[3], g.shape[3])
     if kv is not None:
         k, v = kv
@@ -270,7 +270,7 @@ def _attention(g: _Pages, q, kv, k_pages, page_table, cu_seqlens, seq_lens, max_
         vs = _rows("v", v, g, g.shape[2], tokens, k_pages)
         if k.dtype != dtype or v.dtype != dtype:
             raise TypeError("q, k, and v must have the same dtype")
-    lse = torch.empty((heads, tokens), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = q.new_empty((heads, tokens), dtype=torch.float32) if return_lse else None
     if tokens > 0:
         lib, need = _lib.lib(), C.c_size_t(0)
         prob = g.pack(tokens, heads, max_new, dtype, 0.0 if scale is None else float(scale), qs, os, ks, vs)
