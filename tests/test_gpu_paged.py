@@ -141,6 +141,22 @@ def test_append_and_rows_behind_the_batch(store, new):
     assert (out[b.rows:] == 3.0).all() and torch.equal(k[:b.rows], paged_load(ref.k, ref.v, *b.where, b.rows, **ref.scales)[0])
 
 
+@pytest.mark.parametrize("kernel", [FEW, MANY])
+@pytest.mark.parametrize("store", [None, E4M3])
+def test_pages_of_two_layouts(store, kernel):
+    """K head by head, V token by token within a page; pages longer than a key tile; one page, one kv head."""
+    k, v = (Batch(RAGGED, 8, 2, 128, 16, torch.bfloat16, store, seed=8, layout=x) for x in ("heads", "tokens"))
+    k.fill()
+    v.fill()
+    k.check(*paged_attention(k.q, k.k, v.v, *k.where, kernel, return_lse=True, **k.scales))
+    long = Batch([(40, 700), (1, 1500), (3, 3)], 8, 1, 64, 1024, torch.float16, store, seed=9)
+    long.fill()
+    long.check(*paged_attention(long.q, long.k, long.v, *long.where, kernel, return_lse=True, **long.scales))
+    one = Batch([(2, 60)], 4, 1, 96, 64, torch.float16, store, seed=10, spare=0)
+    one.fill()
+    one.check(*paged_attention(one.q, one.k, one.v, *one.where, kernel, return_lse=True, **one.scales))
+
+
 def test_strides_and_scale():
     """q, k and v side by side as a fused projection leaves them, an output inside a wider tensor, a table inside a wider one, a factor."""
     b = Batch(RAGGED, 8, 2, 128, 16, seed=9)
