@@ -643,8 +643,9 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
 }
 
 // Joins the pieces of the items that several CTAs share.  Block c: the item that CTA c began and did not end.  A few long sequences
-// have a hundred pieces an item: threads in groups take every so many of them, their sums are added in the order of the groups.
-constexpr int kJoinThreads = 512;
+// have a hundred pieces an item: blocks share its output, and threads in groups take every so many of the pieces, their sums are added in the
+// order of the groups.
+constexpr int kJoinThreads = 512, kJoinShare = 128;
 template <bool kHalf, int D, int kM>
 __global__ void __launch_bounds__(kJoinThreads) paged_few_join_kernel(const PagedParams p, const FewArgs a) {
   extern __shared__ float join_smem[];
@@ -669,10 +670,12 @@ __global__ void __launch_bounds__(kJoinThreads) paged_few_join_kernel(const Page
   auto slot = [&](int k) { return 2 * (int64_t)(c0 + k) + (k == 0 ? 1 : 0); };
   const int rows = (int)min((int64_t)kM, (int64_t)s.n * p.G - (int64_t)it.tile * kM);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int outputs = rows * (D / 4);
-  const int groups = outputs >= kJoinThreads ? 1 : kJoinThreads / outputs;
-  const int group = outputs >= kJoinThreads ? 0 : threadIdx.x / outputs;
-  const int n0 = outputs >= kJoinThreads ? threadIdx.x : threadIdx.x % outputs;
+  // this block's share of the item's output, four elements each: [from, from + outputs)
+  const int all = rows * (D / 4), share = (all + gridDim.y - 1) / gridDim.y, from = blockIdx.y * share;
+  const int outputs = min(share, all - from);
+  if (outputs <= 0) return;
+  const int groups = kJoinThreads / outputs;                // (a share has at most kJoinShare)
+  const int group = threadIdx.x / outputs, n = from + threadIdx.x % outputs;
   // the first pieces of this thread's first output are on their way while the weights are worked out
   constexpr int kAhead = 8;
   float4 ahead[kAhead];
@@ -680,12 +683,12 @@ __global__ void __launch_bounds__(kJoinThreads) paged_few_join_kernel(const Page
   for (int i = 0; i < kAhead; ++i) {
     const int k = group + i * groups;
     ahead[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (group < groups && k < pieces && n0 < outputs)
-      ahead[i] = __ldcg(reinterpret_cast<const float4*>(a.part + (slot(k) * kM + n0 / (D / 4)) * D + n0 % (D / 4) * 4));
+    if (group < groups && k < pieces)
+      ahead[i] = __ldcg(reinterpret_cast<const float4*>(a.part + (slot(k) * kM + n / (D / 4)) * D + n % (D / 4) * 4));
   }
   // ---- weights of the pieces
-  for (int n = threadIdx.x; n < pieces * rows; n += kJoinThreads) {
-    const int k = n / rows, r = n - k * rows;
+  for (int i = threadIdx.x; i < pieces * rows; i += kJoinThreads) {
+    const int k = i / rows, r = i - k * rows;
     const float2 ml = __ldcg(a.part_ml + slot(k) * kM + r);
     weight[k][r] = ml.x;
     part_sum[k][r] = ml.y;
@@ -707,44 +710,36 @@ __global__ void __launch_bounds__(kJoinThreads) paged_few_join_kernel(const Page
     if (lane == 0) { most[r] = mx; total[r] = sum; }
   }
   __syncthreads();
-  for (int n = n0; n < outputs; n += kJoinThreads) {
-    const int r = n / (D / 4), c = n % (D / 4) * 4;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    // (a piece that saw nothing has no weight; what it holds is no number that counts)
-    auto add = [&](float f, const float4& v) {
-      if (f == 0.f) return;
-      x[0] += f * v.x; x[1] += f * v.y; x[2] += f * v.z; x[3] += f * v.w;
-    };
-    if (group < groups) {
-      int k = group;
-      if (n == n0) {
+  const int r = n / (D / 4), c = n % (D / 4) * 4;
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  // (a piece that saw nothing has no weight; what it holds is no number that counts)
+  auto add = [&](float f, const float4& v) {
+    if (f == 0.f) return;
+    x[0] += f * v.x; x[1] += f * v.y; x[2] += f * v.z; x[3] += f * v.w;
+  };
+  if (group < groups) {
+    int k = group;
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i, k += groups) add(k < pieces ? weight[k][r] : 0.f, ahead[i]);
-      }
+    for (int i = 0; i < kAhead; ++i, k += groups) add(k < pieces ? weight[k][r] : 0.f, ahead[i]);
 #pragma unroll 4
-      for (; k < pieces; k += groups) add(weight[k][r], __ldcg(reinterpret_cast<const float4*>(a.part + (slot(k) * kM + r) * D + c)));
-    }
-    if (groups > 1) {
-      sums[threadIdx.x] = make_float4(x[0], x[1], x[2], x[3]);
-      __syncthreads();
-    }
-    if (group != 0) break;
-    if (groups > 1) {
-      for (int k = 1; k < groups; ++k) {
-        const float4 v = sums[k * outputs + n];
-        x[0] += v.x; x[1] += v.y; x[2] += v.z; x[3] += v.w;
-      }
-    }
-    int64_t token;
-    int head, i;
-    few_row<kM>(p, s, it.h, it.tile, r, token, head, i);
-    const float inv = most[r] == -INFINITY ? 0.f : 1.f / total[r];
-    uint2 y;
-    y.x = pack2_16<kHalf>(x[0] * inv, x[1] * inv);
-    y.y = pack2_16<kHalf>(x[2] * inv, x[3] * inv);
-    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + token * p.so_t + head * p.so_h + c) = y;
-    if (a.lse != nullptr && c == 0) a.lse[(int64_t)head * p.T + token] = (most[r] + log2f(total[r])) * kLn2;
+    for (; k < pieces; k += groups) add(weight[k][r], __ldcg(reinterpret_cast<const float4*>(a.part + (slot(k) * kM + r) * D + c)));
   }
+  sums[threadIdx.x] = make_float4(x[0], x[1], x[2], x[3]);
+  __syncthreads();
+  if (group != 0) return;
+  for (int k = 1; k < groups; ++k) {
+    const float4 v = sums[k * outputs + threadIdx.x];
+    x[0] += v.x; x[1] += v.y; x[2] += v.z; x[3] += v.w;
+  }
+  int64_t token;
+  int head, i;
+  few_row<kM>(p, s, it.h, it.tile, r, token, head, i);
+  const float inv = most[r] == -INFINITY ? 0.f : 1.f / total[r];
+  uint2 y;
+  y.x = pack2_16<kHalf>(x[0] * inv, x[1] * inv);
+  y.y = pack2_16<kHalf>(x[2] * inv, x[3] * inv);
+  *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + token * p.so_t + head * p.so_h + c) = y;
+  if (a.lse != nullptr && c == 0) a.lse[(int64_t)head * p.T + token] = (most[r] + log2f(total[r])) * kLn2;
 }
 
 struct FewKernels {
@@ -780,6 +775,7 @@ size_t paged_few_workspace(const PagedParams& p) { return kSharedBytes + (size_t
 cudaError_t launch_paged_few(const PagedParams& all, const void* q, const void* kp, const void* vp, const uint8_t* ks,
                              const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st) {
   const bool eight = (int64_t)all.max_new * all.G <= 8;
+  const int tile_rows = eight ? 8 : 16;
   const FewKernels k = all.fp16 ? (eight ? pick_few_dim<true, 8>(all.D, all.store) : pick_few_dim<true, 16>(all.D, all.store))
                                 : (eight ? pick_few_dim<false, 8>(all.D, all.store) : pick_few_dim<false, 16>(all.D, all.store));
   FewArgs a{q, kp, vp, ks, vs, out, lse, nullptr, nullptr, nullptr};
@@ -797,7 +793,7 @@ cudaError_t launch_paged_few(const PagedParams& all, const void* q, const void* 
     return cudaErrorNotSupported;
   cudaError_t e = prepare_kernel(k.attend, k.smem, nullptr, true);
   if (e != cudaSuccess) return e;
-  if ((e = prepare_kernel(k.join, 2 * kFewMaxCtas * 16 * sizeof(float))) != cudaSuccess) return e;
+  if ((e = prepare_kernel(k.join, 2 * kFewMaxCtas * tile_rows * sizeof(float))) != cudaSuccess) return e;
   const int sms = device_info().sms;
   const int grid = k.per_sm * sms < kFewMaxCtas ? k.per_sm * sms : kFewMaxCtas;
   for (int b = 0; b < all.B; b += kPagedBatch) {
@@ -807,7 +803,7 @@ cudaError_t launch_paged_few(const PagedParams& all, const void* q, const void* 
     p.lens += b;
     p.table += b * all.table_stride;
     if ((e = launch_pdl(k.attend, dim3(grid), kFewThreads, k.smem, st, p, mk, mv, a)) != cudaSuccess) return e;
-    if ((e = launch_pdl(k.join, dim3(grid), kJoinThreads, 2 * kFewMaxCtas * (eight ? 8 : 16) * sizeof(float), st, p, a)) != cudaSuccess) return e;
+    if ((e = launch_pdl(k.join, dim3(grid, (tile_rows * (all.D / 4) + kJoinShare - 1) / kJoinShare), kJoinThreads, 2 * kFewMaxCtas * tile_rows * sizeof(float), st, p, a)) != cudaSuccess) return e;
   }
   return cudaSuccess;
 }

@@ -172,7 +172,7 @@ struct RowsItem {
   int b, h, tile;                          // sequence, kv head, row tile
   int nrows;
   int j0, ntiles;                          // key tiles [j0, j0 + ntiles) of the sequence
-  int row0, n, pos0, len, end;             // the sequence's (PagedSeq); keys below `end` are seen by some row
+  int row0, pos0, len;                     // the sequence's (PagedSeq)
   int slot;                                // of its results; -1: not cut
 };
 
@@ -246,14 +246,12 @@ __device__ __forceinline__ void rows_prefetch(const PagedParams& p, const RowsAr
       it.h = hc / cuts;
       cut = hc - it.h * cuts;
     }
-    it.end = rows_end(p, s, it.tile);
     it.j0 = cut * piece;
-    it.ntiles = min(key_tiles(it.end) - it.j0, piece);
+    it.ntiles = min(key_tiles(rows_end(p, s, it.tile)) - it.j0, piece);
     if (it.ntiles <= 0) continue;
     const int rows = item_rows(p.D);
     it.nrows = (int)min((int64_t)s.n * p.G - (int64_t)it.tile * rows, (int64_t)rows);
     it.row0 = s.row0;
-    it.n = s.n;
     it.pos0 = s.pos0;
     it.len = s.len;
     it.slot = cuts > 1 ? __ldcg(a.plan->slot0 + it.b) + i : -1;

@@ -332,6 +332,10 @@ class PagedKV:
             raise TypeError(f"pages hold the rows' own dtype, float8_e4m3fn or int8, got {store}")
         if num_pages <= 0 or num_kv_heads <= 0:
             raise ValueError(f"num_pages and num_kv_heads must be positive, got {num_pages} and {num_kv_heads}")
+        if page_size < 16 or page_size & (page_size - 1):
+            raise NotImplementedError(f"page_size must be a power of two and at least 16, got {page_size}")
+        if head_dim not in HEAD_DIMS:
+            raise NotImplementedError(f"this build supports head_dim {HEAD_DIMS} only")
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self.dtype = dtype
         self.k, self.v = (torch.zeros(num_pages, num_kv_heads, page_size, head_dim, device=device, dtype=torch.int8 if store in _STORES else store)

@@ -169,7 +169,8 @@ def test_packed_structure_is_the_declared_one():
 
 def test_pool_arguments_are_checked():
     for error, args in ((TypeError, (4, 16, 2, 64, torch.float32)), (TypeError, (4, 16, 2, 64, torch.bfloat16, torch.float16)),
-                        (ValueError, (0, 16, 2, 64)), (ValueError, (4, 16, 0, 64))):
+                        (ValueError, (0, 16, 2, 64)), (ValueError, (4, 16, 0, 64)), (NotImplementedError, (4, 48, 2, 64)),
+                        (NotImplementedError, (4, 16, 2, 80))):
         with pytest.raises(error):
             moba.PagedKV(*args, device="cpu")
     pool = moba.PagedKV(4, 16, 2, 64, torch.float16, torch.float8_e4m3fn, device="cpu")
