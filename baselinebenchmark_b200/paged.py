@@ -103,56 +103,56 @@ _DTYPE_OF = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 class _Pages:
     """The tensors that describe a call, checked, with what the C structure needs of them; each attribute is read once, because this
     runs on every call of a decode step."""
-    __slots__ = ("index", "shape", "dtype", "store", "batch", "per_seq", "strides", "pointers", "scales")
+    __slots__ = ("index", "shape", "dtype", "store", "batch", "per_seq", "strides", "where")
 
     def __init__(self, k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales):
         shape, dtype, index = k_pages.shape, k_pages.dtype, k_pages.get_device()
-        store = _STORE_OF.get(dtype)
-        table, batch = page_table.shape, cu_seqlens.shape[0] - 1 if cu_seqlens.dim() == 1 else 0
-        sk, sv, i32 = k_pages.stride(), v_pages.stride(), torch.int32
-        good = (index >= 0 and store is not None and len(shape) == 4 and v_pages.shape == shape and v_pages.dtype == dtype
-                and v_pages.get_device() == index and shape[3] in HEAD_DIMS and sk[3] == 1 == sv[3] and batch > 0
-                and len(table) == 2 and table[0] == batch and page_table.dtype == i32 and page_table.get_device() == index
-                and cu_seqlens.dtype == i32 and cu_seqlens.get_device() == index and cu_seqlens.stride(0) == 1
-                and seq_lens.dtype == i32 and seq_lens.get_device() == index and seq_lens.shape == (batch,)
-                and shape[0] > 0 and shape[2] > 0 and shape[1] >= 16 and not shape[1] & (shape[1] - 1))
-        ts = page_table.stride() if good else (0, 0)
+        store, table, cu, i32 = _STORE_OF.get(dtype), page_table.shape, cu_seqlens.shape, torch.int32
+        good = (index >= 0 and store is not None and len(shape) == 4 == len(v_pages.shape) and len(table) == 2 and len(cu) == 1)
         if good:
-            good = table[1] > 0 and (ts[1] == 1 or table[1] == 1) and (batch == 1 or seq_lens.stride(0) == 1)
-        if good and store != _lib.STORE_SAME:
-            want = (shape[0], shape[2], shape[1])
-            good = (k_scales is not None and v_scales is not None and k_scales.shape == want and v_scales.shape == want
-                    and k_scales.dtype == torch.uint8 == v_scales.dtype and k_scales.get_device() == index
-                    and v_scales.get_device() == index and k_scales.is_contiguous() and v_scales.is_contiguous())
-        elif good:
-            good = k_scales is None and v_scales is None
+            (pages, size, heads, dim), batch = shape, cu[0] - 1
+            (kp, kt, kh, kd), (vp, vt, vh, vd), (ts, td) = k_pages.stride(), v_pages.stride(), page_table.stride()
+            per_seq = table[1]
+            good = (kd == 1 == vd and v_pages.shape == shape and v_pages.dtype == dtype and v_pages.get_device() == index
+                    and dim in HEAD_DIMS and size >= 16 and not size & (size - 1) and pages > 0 and heads > 0 and batch > 0
+                    and table[0] == batch and per_seq > 0 and (td == 1 or per_seq == 1) and seq_lens.shape == (batch,)
+                    and page_table.dtype == i32 and cu_seqlens.dtype == i32 and seq_lens.dtype == i32
+                    and page_table.get_device() == index and cu_seqlens.get_device() == index and seq_lens.get_device() == index
+                    and cu_seqlens.stride(0) == 1 and (batch == 1 or seq_lens.stride(0) == 1))
+            if store == _lib.STORE_SAME:
+                good = good and k_scales is None and v_scales is None
+            elif good:
+                want = (pages, heads, size)
+                good = (k_scales is not None and v_scales is not None and k_scales.shape == want and v_scales.shape == want
+                        and k_scales.dtype == torch.uint8 == v_scales.dtype and k_scales.get_device() == index
+                        and v_scales.get_device() == index and k_scales.is_contiguous() and v_scales.is_contiguous())
         if not good:
             _check_pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
-        pages, size, heads, dim = shape
-        (kp, kt, kh, _), (vp, vt, vh, _) = sk, sv
+            raise ValueError("k_pages, v_pages, page_table, cu_seqlens and seq_lens do not describe a paged cache")
         # a dimension of one page or head may have any stride: it is never stepped over
         if pages == 1:
             kp = vp = heads * size * dim
         if heads == 1:
             kh = vh = size * dim
-        self.index, self.shape, self.dtype, self.store, self.batch, self.per_seq = index, shape, dtype, store, batch, table[1]
-        self.strides = (kp, kt, kh, vp, vt, vh, ts[0] if batch > 1 else table[1])
-        self.pointers = (k_pages.data_ptr(), v_pages.data_ptr())
-        self.scales = (None, None) if k_scales is None else (k_scales.data_ptr(), v_scales.data_ptr())
+        self.index, self.shape, self.dtype, self.store, self.batch, self.per_seq = index, shape, dtype, store, batch, per_seq
+        self.strides = (kp, kt, kh, vp, vt, vh, ts if batch > 1 else per_seq)
+        # as the C calls take them
+        self.where = (cu_seqlens.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                      None if k_scales is None else k_scales.data_ptr(), None if v_scales is None else v_scales.data_ptr())
 
     def pack(self, tokens, q_heads, max_new, dtype, scale, q=(0, 0), o=(0, 0), k=(0, 0), v=(0, 0)) -> bytes:
         pages, size, heads, dim = self.shape
         return _PAGED.pack(tokens, self.batch, q_heads, heads, dim, pages, size, self.per_seq, max_new, _DTYPE_OF[dtype], self.store,
                            scale, 0, *q, *o, *k, *v, *self.strides)
 
-    def run(self, call) -> None:
-        """`call(stream)` with the pages' device current."""
+    def run(self, call, *args) -> None:
+        """`call(*args, stream)` with the pages' device current."""
         index = self.index
         if index != torch.cuda.current_device():
             with torch.cuda.device(index):
-                _lib.check(call(torch._C._cuda_getCurrentRawStream(index)))
+                _lib.check(call(*args, torch._C._cuda_getCurrentRawStream(index)))
         else:
-            _lib.check(call(torch._C._cuda_getCurrentRawStream(index)))
+            _lib.check(call(*args, torch._C._cuda_getCurrentRawStream(index)))
 
 
 def _rows(name, x, g: _Pages, heads: Optional[int], tokens: Optional[int], k_pages) -> Tuple[int, int]:
@@ -195,9 +195,7 @@ def paged_store(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages
     if tokens == 0:
         return
     prob = g.pack(tokens, heads, 1, k.dtype, 0.0, k=ks, v=vs)
-    g.run(lambda stream: _lib.lib().moba_paged_store(
-        prob, k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(), *g.pointers,
-        *g.scales, stream))
+    g.run(_lib.lib().moba_paged_store, prob, k.data_ptr(), v.data_ptr(), *g.where)
     _written(k_pages, v_pages, k_scales, v_scales)
 
 
@@ -220,7 +218,7 @@ def paged_load(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
             raise TypeError(f"only float16 and bfloat16 are supported, got {dtype}")
         if same and dtype != g.dtype:
             raise TypeError(f"rows of {g.dtype} pages are {g.dtype}, got {dtype}")
-        k = torch.empty((total_tokens, heads, dim), dtype=dtype, device=k_pages.device)
+        k = k_pages.new_empty((total_tokens, heads, dim), dtype=dtype)
         v = torch.empty_like(k)
         ks = vs = (heads * dim, dim)
     else:
@@ -233,9 +231,7 @@ def paged_load(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
     if total_tokens == 0:
         return k, v
     prob = g.pack(total_tokens, heads, 1, dtype, 0.0, k=ks, v=vs)
-    g.run(lambda stream: _lib.lib().moba_paged_load(
-        prob, cu_seqlens.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(), *g.pointers, *g.scales, k.data_ptr(),
-        v.data_ptr(), stream))
+    g.run(_lib.lib().moba_paged_load, prob, *g.where, k.data_ptr(), v.data_ptr())
     if out is not None:
         _written(*out)
     return k, v
@@ -252,7 +248,7 @@ def _check_attention(q, k_pages, max_new, scale, out) -> None:
         raise TypeError(f"out must be of {q.dtype}, got {out.dtype}")
 
 
-def _attention(g: _Pages, q, kv, k_pages, page_table, cu_seqlens, seq_lens, max_new, scale, return_lse, out):
+def _attention(g: _Pages, q, kv, k_pages, max_new, scale, return_lse, out):
     """Attention of q; with `kv` the rows of k and v are stored first."""
     qs = _rows("q", q, g, None, None, k_pages)
     tokens, heads, _ = q.shape
@@ -275,15 +271,11 @@ def _attention(g: _Pages, q, kv, k_pages, page_table, cu_seqlens, seq_lens, max_
         lib, need = _lib.lib(), C.c_size_t(0)
         prob = g.pack(tokens, heads, max_new, dtype, 0.0 if scale is None else float(scale), qs, os, ks, vs)
         _lib.check(lib.moba_paged_workspace_size(prob, C.byref(need)))
-        where = (cu_seqlens.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(), *g.pointers, *g.scales)
-
-        def call(stream):
-            ws = _workspace(q.device, need.value)
-            rc = 0 if kv is None else lib.moba_paged_store(prob, k.data_ptr(), v.data_ptr(), *where, stream)
-            return rc or lib.moba_paged_attention(prob, q.data_ptr(), *where, out.data_ptr(), None if lse is None else lse.data_ptr(),
-                                                  ws.data_ptr(), need.value, stream)
-
-        g.run(call)
+        if kv is not None:
+            g.run(lib.moba_paged_store, prob, k.data_ptr(), v.data_ptr(), *g.where)
+        ws = _workspace(q.device, need.value)                # (the caching allocator goes by the current stream of the device given)
+        g.run(lib.moba_paged_attention, prob, q.data_ptr(), *g.where, out.data_ptr(), None if lse is None else lse.data_ptr(),
+              ws.data_ptr(), need.value)
         if given:
             _written(out)
     return (out, lse) if return_lse else out
@@ -303,7 +295,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     they were (undefined without it).  8-bit pages are attended to as the rows that `paged_load` gives; they take float16 and
     bfloat16 queries whatever they were written from."""
     g = _Pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
-    return _attention(g, q, None, k_pages, page_table, cu_seqlens, seq_lens, max_new, scale, return_lse, out)
+    return _attention(g, q, None, k_pages, max_new, scale, return_lse, out)
 
 
 def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -313,7 +305,7 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
     """`paged_store` of the new tokens' k and v, then `paged_attention` of their q: a layer's step of a server."""
     g = _Pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
     _check_written(k_pages, v_pages, k_scales, v_scales)
-    got = _attention(g, q, (k, v), k_pages, page_table, cu_seqlens, seq_lens, max_new, scale, return_lse, out)
+    got = _attention(g, q, (k, v), k_pages, max_new, scale, return_lse, out)
     _written(k_pages, v_pages, k_scales, v_scales)
     return got
 
