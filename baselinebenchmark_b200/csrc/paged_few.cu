@@ -13,11 +13,15 @@
 //     the keys.  No atomics: a call gives the same bits every time.
 //   - 8-bit codes become fp16, which holds them exactly, on their way from shared memory to the tensor core.  Scales are applied to
 //     scores and probabilities, of which there are fewer than elements of K and V.  The power of two 2^e of a V row is part of its
-//     weight: with x = score * log2(e) and M the running maximum of x + e, a key weighs w = 2^(x + e - M) <= 1, so that w fits
-//     fp16 whatever the scales are; the output is sum(w * code) / sum(w * 2^-e).  bf16 queries become fp16 with a power of two for
-//     each row, the largest magnitude in [2^14, 2^15): fp16 then keeps three bits more of them than bf16 has.
-//   - P is rounded to the 16-bit type that V has (or fp16): 2^-9 (2^-12) relative at most, as in the dense stage of the prefill.
-// The maximum that weights refer to is only moved when it grows by more than 8 (a factor of 256).
+//     weight: with x = score * log2(e) and M a reference near the running maximum of x + e, a key weighs w = 2^(x + e - M), 2^8 at
+//     most; the output is sum(w * code) / sum(w * 2^-e).  Where all weights of a block are 2^-14 and more (or nothing at all) they go to P.V as
+//     fp16.  A row of zeros (e = 0) or one with a single large element may put M far above what the other channels are made of: a block with
+//     smaller weights takes them as two bf16 numbers each, which have fp32's range (2^-16 relative, in two products over codes turned to bf16).
+//     bf16 queries become fp16 with a power of two for each row, the largest magnitude in [2^14, 2^15): fp16 then keeps three bits more of them
+//     than bf16 has.
+//   - P is rounded to the 16-bit type that V has (or as said): 2^-8 (bf16), 2^-11 (fp16) relative at most, as in the dense stage of the prefill.
+// The reference that weights are taken to is only moved when the maximum exceeds it by more than 8 (a factor of 256); over codes it is set 4
+// below the maximum, so that fp16 holds weights down to 2^-18 of the largest at least.
 // Measured (replayed from a graph, us; head dim 128, 32/8 heads unless said otherwise; in brackets the bytes at the measured copy bandwidth):
 //   one token of 48 requests of 16 to 11001 tokens                        188 -> 172 (boxes) -> 151 (three CTAs an SM) -> 115 (what an item costs besides
 //                                                                         its keys counts on the line)                          [103]
@@ -108,6 +112,14 @@ __device__ __forceinline__ void codes_to_half(uint32_t x, uint32_t& lo, uint32_t
     hi = *reinterpret_cast<const uint32_t*>(&rb);
   }
 }
+
+// Two fp16 codes as bf16, which holds those of both types exactly.
+__device__ __forceinline__ uint32_t half_codes_to_bf16(uint32_t x) {
+  const float2 f = unpack2<true>(x);
+  return pack2_16<false>(f.x, f.y);
+}
+constexpr float kLift = 4.f;               // over codes: how far below the maximum the reference is set
+constexpr uint32_t kLeastHalf = 0x38800000;   // 2^-14, fp16's least normal number, as fp32
 
 // ---- the line of units -------------------------------------------------------
 // Sequence b has tiles(b) row tiles of kM, each of units(b) units of keys, for every kv head: in the order
@@ -518,8 +530,9 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         alpha[e] = 1.f;
         if (mx > m[e] + 8.f) {
-          alpha[e] = exp2f(m[e] - mx);                      // (0 the first time)
-          m[e] = mx;
+          const float ref = kCodes ? mx - kLift : mx;
+          alpha[e] = exp2f(m[e] - ref);                     // (0 the first time)
+          m[e] = ref;
           moved = true;
         }
       }
@@ -535,6 +548,7 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
         }
       }
       uint32_t pa[kGroups][4];
+      uint32_t least = 0xffffffffu;                         // the least weight that is not 0 (its bits, less one)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         if (e >= kE) {
@@ -549,25 +563,60 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
           const float w0 = ex2_approx(sc[n][2 * e] - ref), w1 = ex2_approx(sc[n][2 * e + 1] - ref);
           l[e] += kCodes ? w0 * vinv[n][0] + w1 * vinv[n][1] : w0 + w1;
           pa[n >> 1][(n & 1) * 2 + e] = pack2_16<kF16>(w0, w1);
+          if (kCodes) {
+            least = min(least, min(__float_as_uint(w0) - 1u, __float_as_uint(w1) - 1u));
+            sc[n][2 * e] = w0;
+            sc[n][2 * e + 1] = w1;
+          }
         }
       }
       // ---- O += P.V
+      if (kCodes && __any_sync(0xffffffffu, least < kLeastHalf - 1u)) {
+        // weights that fp16 has not: as bf16, and what that leaves of them as bf16
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) {
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        uint32_t b[4];
-        ldsm4_t(sv + v_at[i % kPer] + (i / kPer) * S::kSubBytes, b);
-        if (!kCodes) {                                      // matrices: keys 0-7, 8-15 of pieces 2i, the same of 2i + 1
-          mma_16816<kF16>(o[2 * i], pa[0], b[0], b[1]);
-          mma_16816<kF16>(o[2 * i + 1], pa[0], b[2], b[3]);
-        } else {
-          // matrices: keys 0-7, 8-15, 16-23, 24-31 of piece i; pairs of dims are their 16-bit elements: the even dims of 16, and the odd ones
+          for (int n = 0; n < kBlocksN; ++n)
 #pragma unroll
-          for (int gr = 0; gr < kGroups; ++gr) {
-            uint32_t e0, o0, e1, o1;
-            codes_to_half<kStore, 0x20, 0x31>(b[2 * gr], e0, o0);
-            codes_to_half<kStore, 0x20, 0x31>(b[2 * gr + 1], e1, o1);
-            mma_16816<kF16>(o[2 * i], pa[gr], e0, e1);
-            mma_16816<kF16>(o[2 * i + 1], pa[gr], o0, o1);
+            for (int e = 0; e < kE; ++e) {
+              const uint32_t y = pack2_16<false>(sc[n][2 * e], sc[n][2 * e + 1]);
+              const float2 f = unpack2<false>(y);
+              pa[n >> 1][(n & 1) * 2 + e] = y;
+              sc[n][2 * e] -= f.x;
+              sc[n][2 * e + 1] -= f.y;
+            }
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t b[4];
+            ldsm4_t(sv + v_at[i % kPer] + (i / kPer) * S::kSubBytes, b);
+#pragma unroll
+            for (int gr = 0; gr < kGroups; ++gr) {
+              uint32_t e0, o0, e1, o1;
+              codes_to_half<kStore, 0x20, 0x31>(b[2 * gr], e0, o0);
+              codes_to_half<kStore, 0x20, 0x31>(b[2 * gr + 1], e1, o1);
+              mma_16816<false>(o[2 * i], pa[gr], half_codes_to_bf16(e0), half_codes_to_bf16(e1));
+              mma_16816<false>(o[2 * i + 1], pa[gr], half_codes_to_bf16(o0), half_codes_to_bf16(o1));
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t b[4];
+          ldsm4_t(sv + v_at[i % kPer] + (i / kPer) * S::kSubBytes, b);
+          if (!kCodes) {                                    // matrices: keys 0-7, 8-15 of pieces 2i, the same of 2i + 1
+            mma_16816<kF16>(o[2 * i], pa[0], b[0], b[1]);
+            mma_16816<kF16>(o[2 * i + 1], pa[0], b[2], b[3]);
+          } else {
+            // matrices: keys 0-7, 8-15, 16-23, 24-31 of piece i; pairs of dims are their 16-bit elements: the even dims of 16, and the odd ones
+#pragma unroll
+            for (int gr = 0; gr < kGroups; ++gr) {
+              uint32_t e0, o0, e1, o1;
+              codes_to_half<kStore, 0x20, 0x31>(b[2 * gr], e0, o0);
+              codes_to_half<kStore, 0x20, 0x31>(b[2 * gr + 1], e1, o1);
+              mma_16816<kF16>(o[2 * i], pa[gr], e0, e1);
+              mma_16816<kF16>(o[2 * i + 1], pa[gr], o0, o1);
+            }
           }
         }
       }

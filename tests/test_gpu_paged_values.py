@@ -1,0 +1,119 @@
+"""GPU: the paged cache over values of unusual sizes, for the kernel for few rows (tiles of 8 and of 16) and the one for many."""
+import math
+
+import pytest
+import torch
+
+from baselinebenchmark_b200 import PagedKV, paged_attention
+from tests.paged_util import Batch
+
+pytestmark = pytest.mark.gpu
+
+E4M3, INT8 = torch.float8_e4m3fn, torch.int8
+BF16, FP16 = torch.bfloat16, torch.float16
+#: `max_new` for tiles of 8 rows, of 16, and for the kernel for many rows, with groups of four query heads
+KERNELS = [1, 4, 4096]
+#: rows, pages
+STORES = [(BF16, E4M3), (BF16, INT8), (FP16, E4M3), (FP16, INT8)]
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _attend(b, kernel):
+    b.fill()
+    b.check(*paged_attention(b.q, b.k, b.v, *b.where, kernel, return_lse=True, **b.scales))
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype,store", STORES)
+def test_two_keys_with_a_channel_each(dtype, store, kernel):
+    """Equal scores, V rows [2^15, 0, ..] and [0, 2^-10, ..]: the second channel is 2^-11, however much larger the other row is."""
+    cache = PagedKV(1, 16, 1, 64, dtype, store)
+    k, v = torch.zeros(2, 1, 64), torch.zeros(2, 1, 64)
+    k[:, 0, 0] = 1
+    v[0, 0, 0], v[1, 0, 1] = 2.0 ** 15, 2.0 ** -10
+    where = (_i32([[0]]), _i32([0, 2]), _i32([2]))
+    cache.store(k.to(dtype).cuda(), v.to(dtype).cuda(), *where)
+    out = cache.attend(torch.ones(1, 4, 64, dtype=dtype, device="cuda"), where[0], _i32([0, 1]), where[2], kernel).double()
+    want = torch.zeros(64, dtype=torch.float64, device="cuda")
+    want[0], want[1] = 2.0 ** 14, 2.0 ** -11
+    # the weights are halves; a cubic's 1e-4 in numerator and denominator, a rounding of P and one of the output
+    assert ((out - want).abs() <= want * (2e-4 + torch.finfo(dtype).eps)).all()
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype,store", STORES)
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -10])
+def test_v_rows_of_zeros(dtype, store, size, kernel):
+    """Rows of V that are zeros take their share of the weights and nothing else, also the one with most of it (a first token that is attended
+    to and adds nothing): 2^10 and 2^24 times the others', the former where weights are fp16, which holds the others' then."""
+    b = Batch([(1, 500), (3, 777), (2, 40)], 8, 2, 128, 16, dtype, store, seed=70, q_scale=0.25)
+    gap = 7.0 if dtype == FP16 else 17.0
+    for i, (k, v) in enumerate(b.hist):
+        v *= size
+        v[5::9] = 0
+        v[0] = 0
+        # the first key: the sum of a kv head's queries, stretched until each of them scores `gap` or more above its average
+        rows = b.q[b.cu_list[i]:b.cu_list[i + 1]].cpu().float().unflatten(1, (2, 4))
+        mean = rows.mean((0, 2))
+        least = (rows * mean[None, :, None]).sum(-1).amin((0, 2)) / 128 ** 0.5
+        good = least > 0.05
+        k[0] = torch.where(good[:, None], mean * (gap / least.clamp(min=0.05))[:, None], k[0].float()).to(dtype)
+    _attend(b, kernel)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype,store", STORES)
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+def test_v_rows_with_one_large_channel(dtype, store, dim, kernel):
+    """Every seventh row of V has one element, which no other row has: its power of two is far above the others', and they alone make
+    all other channels."""
+    b = Batch([(1, 400), (4, 300), (2, 33)], 8, 2, dim, 32, dtype, store, seed=71 + dim, q_scale=0.5)
+    for _, v in b.hist:
+        big = v[::7]
+        v[:, :, 5] = 0
+        big[:] = 0
+        big[:, :, 5] = 2.0 ** 15 if dtype == FP16 else 2.0 ** 30
+        v[1::7] *= 2.0 ** -9 if dtype == FP16 else 2.0 ** -20
+    _attend(b, kernel)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("store", [E4M3, INT8])
+def test_scores_far_apart_and_a_channel_each(store, kernel):
+    """bfloat16 weights have the range of fp32: keys 2^-30 and 2^-60 of the largest weight still make the channels that they alone have."""
+    cache = PagedKV(8, 16, 1, 128, BF16, store)
+    n = 100
+    k, v = torch.zeros(n, 1, 128), torch.zeros(n, 1, 128)
+    score = torch.zeros(n)
+    score[10:40], score[40:90], score[90:] = -20.0, -41.0, -60.0     # natural log
+    k[:, 0, 0] = score
+    v[:10, 0, :32], v[10:40, 0, 32:64], v[40:90, 0, 64:96], v[90:, 0, 96:] = 1.0, 1.0, 2.0 ** 20, 2.0 ** -20
+    where = (_i32([[3, 1, 0, 7, 2, 6, 5]]), _i32([0, n]), _i32([n]))
+    cache.store(k.to(BF16).cuda(), v.to(BF16).cuda(), *where)
+    q = torch.zeros(1, 4, 128, dtype=BF16, device="cuda")
+    q[..., 0] = 1.0
+    k64 = cache.load(*where, n)[0].double()[:, 0, 0]
+    p = torch.softmax(k64, 0)
+    v64 = cache.load(*where, n)[1].double()[:, 0]
+    want = p @ v64
+    out = cache.attend(q, where[0], _i32([0, 1]), where[2], kernel, scale=1.0).double()
+    # a score's exponential is off by 2^-24 of the score (60 at most) and by 1e-4; one rounding of P, one of the output
+    tol = want * (2 * (1e-4 + 60 * 2.0 ** -23) + 2.0 ** -8 + 2.0 ** -8)
+    assert (want > 0).all() and ((out - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype,store", STORES)
+def test_zeros_alone(dtype, store, kernel):
+    """Nothing but zeros in V, and a pool that nothing was ever written to."""
+    b = Batch([(1, 100), (2, 50)], 8, 2, 64, 16, dtype, store, seed=72)
+    for _, v in b.hist:
+        v.zero_()
+    _attend(b, kernel)
+    cache = PagedKV(4, 16, 2, 64, dtype, store)
+    q = torch.ones(1, 8, 64, dtype=dtype, device="cuda")
+    out, lse = cache.attend(q, _i32([[0, 1, 2, 3]]), _i32([0, 1]), _i32([60]), kernel, return_lse=True)
+    assert (out == 0).all() and (lse - math.log(60)).abs().max() < 1e-3
