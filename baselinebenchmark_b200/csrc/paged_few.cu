@@ -17,8 +17,8 @@
 //     most; the output is sum(w * code) / sum(w * 2^-e).  Where all weights of a block are 2^-14 and more (or nothing at all) they go to P.V as
 //     fp16.  A row of zeros (e = 0) or one with a single large element may put M far above what the other channels are made of: a block with
 //     smaller weights takes them as two bf16 numbers each, which have fp32's range (2^-16 relative, in two products over codes turned to bf16).
-//     bf16 queries become fp16 with a power of two for each row, the largest magnitude in [2^14, 2^15): fp16 then keeps three bits more of them
-//     than bf16 has.
+//     bf16 queries become fp16, which holds them exactly where they lie within 2^-23 to 2^10 (or are zeros); a tile with others stays bf16
+//     and has the codes turned to bf16 for its Q.K^T.
 //   - P is rounded to the 16-bit type that V has (or as said): 2^-8 (bf16), 2^-11 (fp16) relative at most, as in the dense stage of the prefill.
 // The reference that weights are taken to is only moved when the maximum exceeds it by more than 8 (a factor of 256); over codes it is set 4
 // below the maximum, so that fp16 holds weights down to 2^-18 of the largest at least.
@@ -118,6 +118,25 @@ __device__ __forceinline__ uint32_t half_codes_to_bf16(uint32_t x) {
   const float2 f = unpack2<true>(x);
   return pack2_16<false>(f.x, f.y);
 }
+// bf16 queries over codes are taken 2^6-fold to fp16, where that changes none of a tile's (they are zeros, or 2^-23 to 2^10 in magnitude).
+constexpr float kQueryScale = 64.f;
+template <bool kHalf>
+__device__ __forceinline__ uint32_t scaled_query(uint32_t x, float f) {
+  const float2 y = unpack2<false>(x);
+  return pack2_16<kHalf>(y.x * f, y.y * f);
+}
+// Magnitudes of a tile's elements, as pairs of bf16: the least that is not 0 (its bits, less one) and the largest.
+struct QueryRange {
+  uint32_t least = 0xffffffffu, most = 0;
+  __device__ __forceinline__ void add(uint32_t x) {
+    const uint32_t y = x & 0x7fff7fffu;
+    least = __viaddmin_u16x2(y, 0xffffffffu, least);
+    most = __vmaxu2(y, most);
+  }
+  // the largest is 2^e or more; all that are not 0 are
+  __device__ __forceinline__ bool reaches(int e) const { return max(most & 0xffffu, most >> 16) >= (uint32_t)(127 + e) << 7; }
+  __device__ __forceinline__ bool all_reach(int e) const { return min(least & 0xffffu, least >> 16) >= ((uint32_t)(127 + e) << 7) - 1; }
+};
 constexpr float kLift = 4.f;               // over codes: how far below the maximum the reference is set
 constexpr uint32_t kLeastHalf = 0x38800000;   // 2^-14, fp16's least normal number, as fp32
 
@@ -371,7 +390,8 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
 
     // ---- rows of this thread
     int lim[kE];                                            // keys below are visible
-    float rs[kE];                                           // factor of the scores
+    bool wide = false;                                      // over codes: bf16 rows that fp16 does not hold
+    QueryRange range;
     uint32_t qa[kSteps][4];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -385,7 +405,6 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
       const bool on = few_row<kM>(p, s, it.h, it.tile, g + 8 * e, token, head, i);
       lim[e] = on ? (int)min(max((int64_t)s.pos0 + i + 1, (int64_t)0), (int64_t)s.len) : 0;
       const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + token * p.sq_t + head * p.sq_h;
-      rs[e] = p.sl2;
       if (!kCodes) {
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
@@ -397,31 +416,34 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
         uint2 x[kSteps];
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) x[k] = on ? __ldg(reinterpret_cast<const uint2*>(q + 16 * k + 4 * t4)) : make_uint2(0, 0);
-        float f = 1.f;
-        if (!kHalf) {
-          float amax = 0.f;
-#pragma unroll
-          for (int k = 0; k < kSteps; ++k) {
-            const float2 u0 = unpack2<false>(x[k].x), u1 = unpack2<false>(x[k].y);
-            amax = fmaxf(fmaxf(fmaxf(amax, fabsf(u0.x)), fabsf(u0.y)), fmaxf(fabsf(u1.x), fabsf(u1.y)));
-          }
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-          // 2^(14 - k), between 2^-113 and 2^100 (rows of next to nothing score next to nothing)
-          const int k14 = min(max(14 - ((int)(__float_as_uint(amax) >> 23) - 127), -113), 100);
-          f = __uint_as_float((uint32_t)(127 + k14) << 23);
-          rs[e] = p.sl2 * __uint_as_float((uint32_t)(127 - k14) << 23);
-        }
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
-          if (kHalf) {
-            qa[k][e] = x[k].x;
-            qa[k][2 + e] = x[k].y;
-          } else {
-            const float2 u0 = unpack2<false>(x[k].x), u1 = unpack2<false>(x[k].y);
-            qa[k][e] = pack2_half(u0.x * f, u0.y * f);
-            qa[k][2 + e] = pack2_half(u1.x * f, u1.y * f);
-          }
+          qa[k][e] = x[k].x;
+          qa[k][2 + e] = x[k].y;
+          if (!kHalf) { range.add(x[k].x); range.add(x[k].y); }
+        }
+      }
+    }
+    float rs = p.sl2;                                       // factor of the scores
+    if (kCodes && !kHalf) {
+      wide = __any_sync(0xffffffffu, range.reaches(10) || !range.all_reach(-23));
+      if (!wide) {
+        rs *= 1.f / kQueryScale;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if ((i & 1) < kE) qa[k][i] = scaled_query<true>(qa[k][i], kQueryScale);
+      } else {
+        // as they are, unless sums of their products with codes might leave fp32
+        const bool large = __any_sync(0xffffffffu, range.reaches(100)), small = !__any_sync(0xffffffffu, range.reaches(-60));
+        if (large || small) {
+          rs *= large ? 0x1p64f : 0x1p-64f;
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if ((i & 1) < kE) qa[k][i] = scaled_query<false>(qa[k][i], large ? 0x1p-64f : 0x1p64f);
         }
       }
     }
@@ -467,6 +489,19 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
       for (int n = 0; n < kBlocksN; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
+      if (kCodes && !kHalf && wide) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          uint32_t b[4];
+          ldsm4(sk + k_at[k % kPer] + (k / kPer) * S::kSubBytes, b);
+#pragma unroll
+          for (int n = 0; n < kBlocksN; ++n) {
+            uint32_t b0, b1;
+            codes_to_half<kStore, 0x10, 0x32>(b[n], b0, b1);
+            mma_16816<false>(sc[n], qa[k], half_codes_to_bf16(b0), half_codes_to_bf16(b1));
+          }
+        }
+      } else
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) {
         uint32_t b[4];
@@ -496,7 +531,7 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
             const float kf = paged_scale(ke), vf = (float)((int)ve - 127);
             vinv[n][c] = ve == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((254u - ve) << 23);
 #pragma unroll
-            for (int e = 0; e < kE; ++e) sc[n][2 * e + c] = fmaf(sc[n][2 * e + c], rs[e] * kf, vf);
+            for (int e = 0; e < kE; ++e) sc[n][2 * e + c] = fmaf(sc[n][2 * e + c], rs * kf, vf);
           }
         }
       } else {

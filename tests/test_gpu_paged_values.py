@@ -117,3 +117,17 @@ def test_zeros_alone(dtype, store, kernel):
     q = torch.ones(1, 8, 64, dtype=dtype, device="cuda")
     out, lse = cache.attend(q, _i32([[0, 1, 2, 3]]), _i32([0, 1]), _i32([60]), kernel, return_lse=True)
     assert (out == 0).all() and (lse - math.log(60)).abs().max() < 1e-3
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("store", [E4M3, INT8])
+@pytest.mark.parametrize("big,small", [(2.0 ** 14, 2.0 ** -20), (2.0 ** 40, 2.0 ** -1), (2.0 ** 110, 2.0 ** -10), (2.0 ** -70, 2.0 ** -100)])
+def test_queries_with_a_channel_for_some_keys(store, big, small, kernel):
+    """A query's largest element meets zeros in every key: what the others, however much smaller, make of the keys decides."""
+    b = Batch([(1, 300), (4, 200)], 8, 2, 128, 16, BF16, store, seed=73)
+    for k, _ in b.hist:
+        k[:, :, 9] = 0
+        k /= small
+    b.q *= small
+    b.q[:, :, 9] = big
+    _attend(b, kernel)
