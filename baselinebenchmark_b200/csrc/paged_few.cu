@@ -137,6 +137,12 @@ struct QueryRange {
   __device__ __forceinline__ bool reaches(int e) const { return max(most & 0xffffu, most >> 16) >= (uint32_t)(127 + e) << 7; }
   __device__ __forceinline__ bool all_reach(int e) const { return min(least & 0xffffu, least >> 16) >= ((uint32_t)(127 + e) << 7) - 1; }
 };
+// fp16 rows: two codes, and what they become where a value is beyond fp16 (pages that were written from bf16 rows).
+template <int kStore> constexpr uint32_t kMostHalfByte = kStore == MOBA_STORE_E4M3 ? 134 : 135;   // 448 * 2^7 and -128 * 2^8 are fp16's
+__device__ __forceinline__ uint32_t codes_within_half(uint32_t x, float s0, float s1) {
+  const float2 c = unpack2<true>(x);
+  return pack2_half(fabsf(c.x * s0) >= 65520.f ? copysignf(INFINITY, c.x) : c.x, fabsf(c.y * s1) >= 65520.f ? copysignf(INFINITY, c.y) : c.y);
+}
 constexpr float kLift = 4.f;               // over codes: how far below the maximum the reference is set
 constexpr uint32_t kLeastHalf = 0x38800000;   // 2^-14, fp16's least normal number, as fp32
 
@@ -484,12 +490,31 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
         __syncwarp();
       }
       // ---- S = Q.K^T
+      bool beyond = false;                                  // fp16 rows: values of the block may be beyond fp16
       float sc[kBlocksN][4];
 #pragma unroll
       for (int n = 0; n < kBlocksN; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
-      if (kCodes && !kHalf && wide) {
+      if (kCodes && kHalf) {
+        const bool seen = key0 + lane < end && ((mine >> (lane >> 4)) & 1);
+        const uint32_t most = max(scales[warp][st_out][0][lane], scales[warp][st_out][1][lane]);
+        beyond = __any_sync(0xffffffffu, seen && most > kMostHalfByte<kStore>);
+      }
+      if (kCodes && kHalf && beyond) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          uint32_t b[4];
+          ldsm4(sk + k_at[k % kPer] + (k / kPer) * S::kSubBytes, b);
+#pragma unroll
+          for (int n = 0; n < kBlocksN; ++n) {
+            const float s = paged_scale(scales[warp][st_out][0][8 * n + g]);
+            uint32_t b0, b1;
+            codes_to_half<kStore, 0x10, 0x32>(b[n], b0, b1);
+            mma_16816<true>(sc[n], qa[k], codes_within_half(b0, s, s), codes_within_half(b1, s, s));
+          }
+        }
+      } else if (kCodes && !kHalf && wide) {
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
           uint32_t b[4];
@@ -527,9 +552,10 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
           const uint32_t kb = *reinterpret_cast<const uint16_t*>(sb[0] + 8 * n + 2 * t4), vb = *reinterpret_cast<const uint16_t*>(sb[1] + 8 * n + 2 * t4);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const uint32_t ke = (kb >> (8 * c)) & 255, ve = (vb >> (8 * c)) & 255;
+            // (fp16 rows: from 2^25 all that is not 0 is beyond fp16; how far does not count for the other channels' weights)
+            const uint32_t ke = (kb >> (8 * c)) & 255, vs = (vb >> (8 * c)) & 255, ve = kHalf ? min(vs, 127u + 25u) : vs;
             const float kf = paged_scale(ke), vf = (float)((int)ve - 127);
-            vinv[n][c] = ve == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((254u - ve) << 23);
+            vinv[n][c] = vs == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((254u - ve) << 23);
 #pragma unroll
             for (int e = 0; e < kE; ++e) sc[n][2 * e + c] = fmaf(sc[n][2 * e + c], rs * kf, vf);
           }
@@ -606,7 +632,7 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
         }
       }
       // ---- O += P.V
-      if (kCodes && __any_sync(0xffffffffu, least < kLeastHalf - 1u)) {
+      if (kCodes && (__any_sync(0xffffffffu, least < kLeastHalf - 1u) || beyond)) {
         // weights that fp16 has not: as bf16, and what that leaves of them as bf16
 #pragma unroll 1
         for (int part = 0; part < 2; ++part) {
@@ -629,6 +655,18 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
               uint32_t e0, o0, e1, o1;
               codes_to_half<kStore, 0x20, 0x31>(b[2 * gr], e0, o0);
               codes_to_half<kStore, 0x20, 0x31>(b[2 * gr + 1], e1, o1);
+              if (kHalf && beyond) {
+                float s[4];                                 // (rows that nobody sees are zeros: their bytes are anything)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                  const int n = 16 * gr + 8 * (c >> 1) + 2 * t4 + (c & 1);
+                  s[c] = paged_scale(min((uint32_t)scales[warp][st_out][1][n], 254u));
+                }
+                e0 = codes_within_half(e0, s[0], s[1]);
+                o0 = codes_within_half(o0, s[0], s[1]);
+                e1 = codes_within_half(e1, s[2], s[3]);
+                o1 = codes_within_half(o1, s[2], s[3]);
+              }
               mma_16816<false>(o[2 * i], pa[gr], half_codes_to_bf16(e0), half_codes_to_bf16(e1));
               mma_16816<false>(o[2 * i + 1], pa[gr], half_codes_to_bf16(o0), half_codes_to_bf16(o1));
             }

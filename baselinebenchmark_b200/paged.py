@@ -292,8 +292,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     `max_new`: the most new tokens that a sequence has (the kernel is chosen by it; another number costs time only).  `scale`:
     factor of the scores, head_dim ** -0.5 unless given.  Returns out [T, Hq, D], with `return_lse` (out, lse [Hq, T] fp32, natural
     log).  A token that sees nothing is zeros and -inf.  `out`: a tensor to write to; rows behind the last sequence are left as
-    they were (undefined without it).  8-bit pages are attended to as the rows that `paged_load` gives; they take float16 and
-    bfloat16 queries whatever they were written from."""
+    they were (undefined without it).  8-bit pages are attended to as the rows that `paged_load` gives in the queries' dtype,
+    whichever they were written from: a value beyond float16 is an infinity to float16 queries."""
     g = _Pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
     return _attention(g, q, None, k_pages, max_new, scale, return_lse, out)
 

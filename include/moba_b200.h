@@ -387,11 +387,13 @@ int moba_problem_attend_kernel(const moba_problem_t* p);
  *               page_table[b][x / page_size].  An entry outside 0 .. num_pages-1 is a page that is not there: rows for it are
  *               not stored, load as zeros, and take no part in attention; so do positions behind the table, and below 0.
  * Neither is read back to the host.  Pages hold rows of the 16-bit type `dtype` (MOBA_STORE_SAME), or 8-bit codes
- * (MOBA_STORE_E4M3, MOBA_STORE_INT8) and one byte per row and head: code c with byte s stands for c * 2^(s - 127), which both 16-bit types
- * hold exactly (a power of two costs e4m3 next to nothing and int8 half a bit on average; nothing is rounded twice, and
- * codes do not depend on how a division is rounded).  The byte is that of the least power of two, from 2^-96, whose product with the
+ * (MOBA_STORE_E4M3, MOBA_STORE_INT8) and one byte per row and head: code c with byte s stands for c * 2^(s - 127), which the 16-bit type that
+ * was stored holds exactly (a power of two costs e4m3 next to nothing and int8 half a bit on average; nothing is rounded twice, and
+ * codes do not depend on how a division is rounded).  Pages may be read and attended to in the other 16-bit type: every value is
+ * rounded to it, one above fp16's range is an infinity (the attention may keep more digits of values below 2^-14).  The byte is that of the least power of two, from 2^-96, whose product with the
  * largest code (448, 127) reaches the row's largest magnitude; a row of zeros has 127; a row with an infinity or a NaN has
  * 255 and reads back as NaN.  A value whose code would stand for an infinity of `dtype` is stored as the largest finite one.
+ * Bytes are as the store writes them, 31 to 249 and 255.
  * A pool's element (page, slot, head, dim) is at page * page_stride + slot * token_stride + head * head_stride + dim, in
  * elements; the bytes of the codes are [num_pages, num_kv_heads, page_size]. */
 enum {

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from baselinebenchmark_b200 import PagedKV, paged_attention
+from baselinebenchmark_b200 import PagedKV, paged_attention, paged_load
 from tests.paged_util import Batch
 
 pytestmark = pytest.mark.gpu
@@ -130,4 +130,58 @@ def test_queries_with_a_channel_for_some_keys(store, big, small, kernel):
         k /= small
     b.q *= small
     b.q[:, :, 9] = big
+    _attend(b, kernel)
+
+
+@pytest.mark.parametrize("store", [E4M3, INT8])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_float16_queries_over_rows_written_from_bfloat16(store, kernel):
+    """The rows count as `paged_load` gives them in the queries' type: rounded to it, infinities above its range, whichever kernel runs."""
+    seqs = [(1, 300), (4, 200), (2, 100)]
+    b = Batch(seqs, 8, 2, 64, 16, BF16, store, seed=74)
+    for k, v in b.hist:
+        k[:, :, 3:] *= 2.0 ** -3
+        k[::5] *= 2.0 ** -12
+        v[1::4] *= 2.0 ** -11
+        v[2::4, :, 10:20] *= 2.0 ** 12                       # up to 2^14 or so: within fp16
+    b.fill()
+    k, v = b.hist[1]
+    k[30, 0, 7], v[77, 1, 5], v[78, 1, 6], v[79, 1, 6] = 2.0 ** 20, 1e5, -3e5, 3.0e38
+    b.fill()
+    half = Batch(seqs, 8, 2, 64, 16, FP16, store, seed=74)
+    got, lse = paged_attention(half.q, b.k, b.v, *b.where, kernel, return_lse=True, **b.scales)
+    # what the rows are in fp16
+    whole = torch.cat([torch.tensor([0]), torch.tensor([n for _, n in seqs]).cumsum(0)]).tolist()
+    rows = [x.cpu() for x in paged_load(b.k, b.v, b.table, _i32(whole), b.lens, whole[-1], dtype=FP16, **b.scales)]
+    assert torch.isinf(rows[0]).sum() == 1 and torch.isinf(rows[1]).sum() == 3
+    bad = torch.isinf(rows[1]).flatten().nonzero()
+    half.hist = [tuple(x[whole[i]:whole[i + 1]] for x in rows) for i in range(3)]
+    half.store = FP16
+    # an infinite key element: -inf or +inf, as the query's element has it; +inf makes NaN.  An infinite value makes its channel infinite or NaN.
+    own = slice(1, 5)
+    hit = half.q[own, :4, 7] > 0
+    assert torch.equal(torch.isnan(got[own, :4]).all(-1), hit) and torch.equal(torch.isnan(lse[:4, own].t()), hit)
+    assert (~torch.isfinite(got[own, 4:, 5])).all() and (~torch.isfinite(got[own, 4:, 6])).all()
+    # everything else as the formula has it, with the key that scored -inf out of it
+    half.hist[1][0][torch.isinf(half.hist[1][0])] = 0
+    half.hist[1][1][torch.isinf(half.hist[1][1])] = 0
+    out, ref, mass, size = half.attention()
+    fine = torch.ones(half.rows, 8, 64, dtype=torch.bool, device="cuda")
+    fine[own, :4] = False
+    fine[own, 4:, 5:7] = False
+    got = torch.where(fine, got, out.to(FP16))
+    half.check(got, None, (out, ref, mass, size))
+    assert len(bad) == 3
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("store", [E4M3, INT8])
+def test_float16_rows_up_to_the_largest(store, kernel):
+    """fp16 rows up to 65504, whose codes come near the border of the type."""
+    b = Batch([(1, 300), (3, 100)], 8, 2, 128, 32, FP16, store, seed=75)
+    for k, v in b.hist:
+        k[::3, :, 4] = 60000.0
+        k[1::3, :, 4] = -65504.0
+        v[::4] = (v[::4].float() * 3e4).clamp(-65504, 65504).to(FP16)
+    b.q[:, :, 4] *= 2.0 ** -14
     _attend(b, kernel)
