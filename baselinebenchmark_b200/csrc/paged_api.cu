@@ -15,7 +15,7 @@ int check_paged(const moba_paged_t* p) {
   if (p->page_size < 16 || (p->page_size & (p->page_size - 1)) != 0) return MOBA_E_UNSUPPORTED;
   if ((p->dtype != MOBA_DTYPE_BF16 && p->dtype != MOBA_DTYPE_FP16) || p->reserved != 0) return MOBA_E_UNSUPPORTED;
   if (p->store != MOBA_STORE_SAME && p->store != MOBA_STORE_E4M3 && p->store != MOBA_STORE_INT8) return MOBA_E_UNSUPPORTED;
-  if (!(p->softmax_scale >= 0.f) || p->softmax_scale > 3e38f) return MOBA_E_SHAPE;
+  if (!(p->softmax_scale >= 0.f) || p->softmax_scale > 2.3e38f) return MOBA_E_SHAPE;   // (times log2 e it is still finite)
   // rows and grids are counted in 32 bits, positions too
   if (p->total_tokens >= ((int64_t)1 << 31) / p->num_q_heads) return MOBA_E_UNSUPPORTED;
   if ((int64_t)p->pages_per_seq * p->page_size >= ((int64_t)1 << 30)) return MOBA_E_UNSUPPORTED;

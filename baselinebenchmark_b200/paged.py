@@ -242,8 +242,9 @@ def _check_attention(q, k_pages, max_new, scale, out) -> None:
         raise ValueError(f"q heads ({q.shape[1]}) must be divisible by kv heads ({k_pages.shape[2]})")
     if not isinstance(max_new, int) or max_new <= 0:
         raise ValueError(f"max_new must be a positive int, got {max_new}")
-    if scale is not None and not 0.0 < float(scale) < 3e38:
-        raise ValueError(f"scale must be a positive number, got {scale}")
+    # (in the structure 0 stands for none given; times log2(e) it has to be finite)
+    if scale is not None and not (0.0 < C.c_float(float(scale)).value and float(scale) <= 2.3e38):
+        raise ValueError(f"scale must be a positive number of 32 bits, at most 2.3e38, got {scale}")
     if out is not None and out.dtype != q.dtype:
         raise TypeError(f"out must be of {q.dtype}, got {out.dtype}")
 

@@ -408,7 +408,7 @@ typedef struct moba_paged {
   int32_t pages_per_seq;    /* columns of page_table                                               */
   int32_t max_new;          /* most rows of a sequence, which the kernel of the attention is chosen by (a wrong one costs time only) */
   int32_t dtype, store;     /* MOBA_DTYPE_*, MOBA_STORE_*                                          */
-  float softmax_scale;      /* factor of the scores; 0: head_dim^-0.5                              */
+  float softmax_scale;      /* factor of the scores, at most 2.3e38; 0: head_dim^-0.5             */
   int32_t reserved;         /* must be 0                                                           */
   int64_t q_stride_token, q_stride_head;   /* elements; of the packed q ...                        */
   int64_t o_stride_token, o_stride_head;   /* ... and out                                          */

@@ -1,0 +1,27 @@
+"""CPU: arguments of the paged cache's operators at the ends of their ranges.  No kernel is launched."""
+import ctypes as C
+
+import pytest
+import torch
+
+from baselinebenchmark_b200 import _lib, build, paged
+from tests.test_paged_abi import _dev, _paged
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build.build()
+    return _lib.lib()
+
+
+def test_factor_of_the_scores_is_a_number_of_32_bits(lib):
+    """A factor that becomes 0 in 32 bits would stand for head_dim^-0.5, and one whose product with log2(e) is infinite for NaN rows."""
+    pages, q = _dev(torch.zeros(5, 16, 2, 64, dtype=torch.bfloat16)), _dev(torch.zeros(7, 4, 64, dtype=torch.bfloat16))
+    for scale in (1e-46, 7e-46, 2.5e38, 3.0e38, 1e300, float("inf"), -1e-46):
+        with pytest.raises(ValueError, match="scale"):
+            paged._check_attention(q, pages, 3, scale, None)
+    for scale in (2e-45, 1e-38, 0.3, 2.2e38):
+        paged._check_attention(q, pages, 3, scale, None)
+    check = lambda x: lib.moba_paged_check(C.byref(_paged(softmax_scale=x)))  # noqa: E731
+    assert [check(x) for x in (2.5e38, 3.0e38, 3.3e38)] == [-1] * 3
+    assert [check(x) for x in (0.0, 2e-45, 2.2e38)] == [0] * 3
