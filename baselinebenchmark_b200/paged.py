@@ -22,6 +22,7 @@ import struct
 from typing import Optional, Tuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _lib
 from .parallel import HEAD_DIMS, _workspace
@@ -165,6 +166,18 @@ def _rows(name, x, g: _Pages, heads: Optional[int], tokens: Optional[int], k_pag
     return t if shape[0] > 1 else 0, h if shape[1] > 1 else 0
 
 
+def _check_not_followed(**tensors) -> None:
+    """Nothing here has a backward or a forward derivative: what autograd follows is refused, not dropped."""
+    if torch.is_grad_enabled():
+        for name, x in tensors.items():
+            if x is not None and x.requires_grad:
+                raise NotImplementedError(f"{name} requires grad: a paged cache is state of a server, its operators have no backward")
+    if getattr(forward_ad, "_current_level", 0) >= 0:        # (-1: outside of forward mode, where a look at each tensor is saved)
+        for name, x in tensors.items():
+            if x is not None and forward_ad.unpack_dual(x).tangent is not None:
+                raise NotImplementedError(f"{name} has a tangent: the operators of a paged cache have no derivatives")
+
+
 def _check_written(*tensors) -> None:
     inference = torch.is_inference_mode_enabled()
     for x in tensors:
@@ -192,6 +205,7 @@ def paged_store(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages
     if k.dtype != v.dtype:
         raise TypeError("k and v must have the same dtype")
     _check_written(k_pages, v_pages, k_scales, v_scales)
+    _check_not_followed(k=k, v=v, k_pages=k_pages, v_pages=v_pages)
     if tokens == 0:
         return
     prob = g.pack(tokens, heads, 1, k.dtype, 0.0, k=ks, v=vs)
@@ -228,6 +242,7 @@ def paged_load(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
         if k.dtype != dtype or v.dtype != dtype:
             raise TypeError(f"out must be of {dtype}, got {k.dtype} and {v.dtype}")
         _check_written(k, v)
+    _check_not_followed(k_pages=k_pages, v_pages=v_pages, **{"out[0]": k, "out[1]": v})
     if total_tokens == 0:
         return k, v
     prob = g.pack(total_tokens, heads, 1, dtype, 0.0, k=ks, v=vs)
@@ -249,8 +264,9 @@ def _check_attention(q, k_pages, max_new, scale, out) -> None:
         raise TypeError(f"out must be of {q.dtype}, got {out.dtype}")
 
 
-def _attention(g: _Pages, q, kv, k_pages, max_new, scale, return_lse, out):
+def _attention(g: _Pages, q, kv, k_pages, v_pages, max_new, scale, return_lse, out):
     """Attention of q; with `kv` the rows of k and v are stored first."""
+    _check_not_followed(q=q, k=kv and kv[0], v=kv and kv[1], k_pages=k_pages, v_pages=v_pages, out=out)
     qs = _rows("q", q, g, None, None, k_pages)
     tokens, heads, _ = q.shape
     _check_attention(q, k_pages, max_new, scale, out)
@@ -296,7 +312,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     they were (undefined without it).  8-bit pages are attended to as the rows that `paged_load` gives in the queries' dtype,
     whichever they were written from: a value beyond float16 is an infinity to float16 queries."""
     g = _Pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
-    return _attention(g, q, None, k_pages, max_new, scale, return_lse, out)
+    return _attention(g, q, None, k_pages, v_pages, max_new, scale, return_lse, out)
 
 
 def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -306,7 +322,7 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
     """`paged_store` of the new tokens' k and v, then `paged_attention` of their q: a layer's step of a server."""
     g = _Pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
     _check_written(k_pages, v_pages, k_scales, v_scales)
-    got = _attention(g, q, (k, v), k_pages, max_new, scale, return_lse, out)
+    got = _attention(g, q, (k, v), k_pages, v_pages, max_new, scale, return_lse, out)
     _written(k_pages, v_pages, k_scales, v_scales)
     return got
 

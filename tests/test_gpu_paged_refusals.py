@@ -1,0 +1,51 @@
+"""GPU: calls of the paged cache that are refused, and what they leave behind."""
+import pytest
+import torch
+
+from baselinebenchmark_b200 import PagedKV, paged_attention, paged_load, paged_store
+
+pytestmark = pytest.mark.gpu
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _call():
+    cache = PagedKV(4, 16, 2, 64)
+    where = (_i32([[0]]), _i32([0, 2]), _i32([2]))
+    k, q = (torch.ones(2, h, 64, dtype=torch.bfloat16, device="cuda") for h in (2, 4))
+    return cache, where, q, k
+
+
+def test_pages_that_require_grad():
+    cache, where, q, k = _call()
+    for name in ("k", "v"):
+        pages = [x.clone().requires_grad_(name == n) for n, x in (("k", cache.k), ("v", cache.v))]
+        with pytest.raises(NotImplementedError, match="backward"):
+            paged_load(*pages, *where, 2)
+        with pytest.raises(NotImplementedError, match="backward"):
+            paged_attention(q, *pages, *where, 2)
+        with torch.no_grad():
+            assert paged_attention(q, *pages, *where, 2).shape == q.shape and paged_load(*pages, *where, 2)[0].shape == k.shape
+
+
+def test_tangents():
+    cache, where, q, k = _call()
+    forward = torch.autograd.forward_ad
+    with forward.dual_level():
+        dual = lambda x: forward.make_dual(x, torch.ones_like(x))  # noqa: E731
+        with pytest.raises(NotImplementedError, match="tangent"):
+            cache.attend(dual(q), *where, 2)
+        with pytest.raises(NotImplementedError, match="tangent"):
+            paged_attention(q, dual(cache.k), cache.v, *where, 2)
+        with pytest.raises(NotImplementedError, match="tangent"):
+            paged_load(cache.k, dual(cache.v), *where, 2)
+        with pytest.raises(NotImplementedError, match="tangent"):
+            cache.store(k, dual(k), *where)
+        with pytest.raises(NotImplementedError, match="tangent"):
+            paged_store(k, k, cache.k, dual(cache.v), *where)
+        with pytest.raises(NotImplementedError, match="tangent"):
+            cache.append(q, dual(k), k, *where, 2)
+        assert (cache.k == 0).all() and (cache.v == 0).all()
+        assert cache.append(q, k, k, *where, 2).shape == q.shape

@@ -25,3 +25,20 @@ def test_factor_of_the_scores_is_a_number_of_32_bits(lib):
     check = lambda x: lib.moba_paged_check(C.byref(_paged(softmax_scale=x)))  # noqa: E731
     assert [check(x) for x in (2.5e38, 3.0e38, 3.3e38)] == [-1] * 3
     assert [check(x) for x in (0.0, 2e-45, 2.2e38)] == [0] * 3
+
+
+def test_tensors_that_autograd_follows_are_refused():
+    """Pages, too, and tangents of forward mode (a dual tensor does not require grad)."""
+    x, y = torch.zeros(3), torch.zeros(3, requires_grad=True)
+    with pytest.raises(NotImplementedError, match="v_pages.*backward"):
+        paged._check_not_followed(k_pages=x, v_pages=y)
+    with torch.no_grad():
+        paged._check_not_followed(k_pages=x, v_pages=y)
+    paged._check_not_followed(k_pages=x, v_pages=x, out=None)
+    with torch.autograd.forward_ad.dual_level():
+        paged._check_not_followed(k_pages=x)
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones(3))
+        with pytest.raises(NotImplementedError, match="q has a tangent"):
+            paged._check_not_followed(q=dual, k_pages=x)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="tangent"):
+            paged._check_not_followed(q=dual)
