@@ -33,6 +33,8 @@ SYMBOLS = (
 #: MOBA_DTYPE_*, MOBA_STORE_*
 DTYPE_BF16, DTYPE_FP16 = 0, 1
 STORE_SAME, STORE_E4M3, STORE_INT8 = range(3)
+#: MOBA_E_*
+E_SHAPE, E_ALIGN = -1, -6
 
 
 class Problem(C.Structure):

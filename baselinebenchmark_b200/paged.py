@@ -264,8 +264,8 @@ def _check_attention(q, k_pages, max_new, scale, out) -> None:
         raise TypeError(f"out must be of {q.dtype}, got {out.dtype}")
 
 
-def _attention(g: _Pages, q, kv, k_pages, v_pages, max_new, scale, return_lse, out):
-    """Attention of q; with `kv` the rows of k and v are stored first."""
+def _attention(g: _Pages, q, kv, k_pages, v_pages, max_new, scale, return_lse, out, written=()):
+    """Attention of q; with `kv` the rows of k and v are stored first, in the tensors of `written`."""
     _check_not_followed(q=q, k=kv and kv[0], v=kv and kv[1], k_pages=k_pages, v_pages=v_pages, out=out)
     qs = _rows("q", q, g, None, None, k_pages)
     tokens, heads, _ = q.shape
@@ -288,9 +288,15 @@ def _attention(g: _Pages, q, kv, k_pages, v_pages, max_new, scale, return_lse, o
         lib, need = _lib.lib(), C.c_size_t(0)
         prob = g.pack(tokens, heads, max_new, dtype, 0.0 if scale is None else float(scale), qs, os, ks, vs)
         _lib.check(lib.moba_paged_workspace_size(prob, C.byref(need)))
-        if kv is not None:
-            g.run(lib.moba_paged_store, prob, k.data_ptr(), v.data_ptr(), *g.where)
         ws = _workspace(q.device, need.value)                # (the caching allocator goes by the current stream of the device given)
+        if kv is not None:
+            # what only the attention would refuse comes before anything is written
+            if (q.data_ptr() | out.data_ptr()) & 15:
+                _lib.check(_lib.E_ALIGN)
+            if (os[0] == 0 and tokens > 1) or (os[1] == 0 and heads > 1):
+                _lib.check(_lib.E_SHAPE)
+            g.run(lib.moba_paged_store, prob, k.data_ptr(), v.data_ptr(), *g.where)
+            _written(*written)
         g.run(lib.moba_paged_attention, prob, q.data_ptr(), *g.where, out.data_ptr(), None if lse is None else lse.data_ptr(),
               ws.data_ptr(), need.value)
         if given:
@@ -322,9 +328,7 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
     """`paged_store` of the new tokens' k and v, then `paged_attention` of their q: a layer's step of a server."""
     g = _Pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
     _check_written(k_pages, v_pages, k_scales, v_scales)
-    got = _attention(g, q, (k, v), k_pages, v_pages, max_new, scale, return_lse, out)
-    _written(k_pages, v_pages, k_scales, v_scales)
-    return got
+    return _attention(g, q, (k, v), k_pages, v_pages, max_new, scale, return_lse, out, (k_pages, v_pages, k_scales, v_scales))
 
 
 class PagedKV:

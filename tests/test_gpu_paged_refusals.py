@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from baselinebenchmark_b200 import PagedKV, paged_attention, paged_load, paged_store
+from baselinebenchmark_b200 import PagedKV, _lib, paged, paged_attention, paged_load, paged_store
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,31 @@ def test_tangents():
             cache.append(q, dual(k), k, *where, 2)
         assert (cache.k == 0).all() and (cache.v == 0).all()
         assert cache.append(q, k, k, *where, 2).shape == q.shape
+
+
+@pytest.mark.parametrize("tokens", [2, 40])
+def test_a_refused_append_writes_nothing(tokens, monkeypatch):
+    """What only the attention refuses is found before the new rows are stored: an output whose rows lie on one another, addresses, no
+    memory for scratch.  A call that goes through tells autograd of its writes."""
+    cache = PagedKV(4, 16, 2, 64)
+    where = (_i32([[0, 1, 2]]), _i32([0, tokens]), _i32([tokens]))
+    k, q = (torch.ones(tokens, h, 64, dtype=torch.bfloat16, device="cuda") for h in (2, 4))
+    shifted = torch.ones(tokens * 4 * 64 + 4, dtype=torch.bfloat16, device="cuda")[4:].view(tokens, 4, 64)
+    version = cache.k._version
+
+    def refused(error, query=q, **options):
+        with pytest.raises(error):
+            cache.append(query, k, k, *where, tokens, **options)
+        torch.cuda.synchronize()
+        assert (cache.k == 0).all() and (cache.v == 0).all() and cache.k._version == version
+
+    refused(_lib.MobaError, out=torch.zeros(1, 4, 64, dtype=torch.bfloat16, device="cuda").expand(tokens, 4, 64))
+    refused(_lib.MobaError, out=torch.zeros(tokens, 1, 64, dtype=torch.bfloat16, device="cuda").expand(tokens, 4, 64))
+    refused(_lib.MobaError, out=shifted)
+    refused(_lib.MobaError, query=shifted)
+    with monkeypatch.context() as m:
+        def none(*_):
+            raise torch.cuda.OutOfMemoryError("no memory")
+        m.setattr(paged, "_workspace", none)
+        refused(torch.cuda.OutOfMemoryError)
+    assert cache.append(q, k, k, *where, tokens).shape == q.shape and cache.k._version > version and (cache.k[0, 0] == 1).all()
