@@ -143,8 +143,11 @@ class _Pages:
 
     def pack(self, tokens, q_heads, max_new, dtype, scale, q=(0, 0), o=(0, 0), k=(0, 0), v=(0, 0)) -> bytes:
         pages, size, heads, dim = self.shape
-        return _PAGED.pack(tokens, self.batch, q_heads, heads, dim, pages, size, self.per_seq, max_new, _DTYPE_OF[dtype], self.store,
-                           scale, 0, *q, *o, *k, *v, *self.strides)
+        try:
+            return _PAGED.pack(tokens, self.batch, q_heads, heads, dim, pages, size, self.per_seq, min(max_new, 0x7fffffff), _DTYPE_OF[dtype],
+                               self.store, scale, 0, *q, *o, *k, *v, *self.strides)
+        except struct.error as e:
+            raise NotImplementedError("pages, columns of the table and sequences are counted in 32 bits") from e
 
     def run(self, call, *args) -> None:
         """`call(*args, stream)` with the pages' device current."""

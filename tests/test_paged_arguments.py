@@ -42,3 +42,17 @@ def test_tensors_that_autograd_follows_are_refused():
             paged._check_not_followed(q=dual, k_pages=x)
         with torch.no_grad(), pytest.raises(NotImplementedError, match="tangent"):
             paged._check_not_followed(q=dual)
+
+
+def test_sizes_beyond_32_bits():
+    """`max_new` is a hint: any positive number is one.  Sizes that the structure has no room for are refused with a word of it."""
+    g = paged._Pages.__new__(paged._Pages)
+    g.shape, g.batch, g.per_seq, g.store, g.strides = (11, 16, 2, 64), 3, 9, 0, (8,) * 7
+    field = lambda n: _lib.Paged.from_buffer_copy(g.pack(21, 4, n, torch.float16, 0.0)).max_new  # noqa: E731
+    assert [field(n) for n in (1, 2 ** 31 - 1, 2 ** 31, 2 ** 70)] == [1] + [2 ** 31 - 1] * 3
+    for name, x in (("shape", (2 ** 31, 16, 2, 64)), ("per_seq", 2 ** 31), ("batch", 2 ** 32)):
+        kept = getattr(g, name)
+        setattr(g, name, x)
+        with pytest.raises(NotImplementedError, match="32 bits"):
+            g.pack(21, 4, 1, torch.float16, 0.0)
+        setattr(g, name, kept)
