@@ -45,9 +45,18 @@ constexpr int kMostRows = 2 * kTileM;
 __host__ __device__ constexpr int item_rows(int D) { return D == 256 ? kTileM : kMostRows; }
 constexpr int kCodeWarps = 8;              // that turn codes into operand tiles: warp 3, which has no V to bring, and warps 12-18
 template <int kStore> constexpr int kRowsThreads = kStore == MOBA_STORE_SAME ? 384 : 384 + 32 * (kCodeWarps - 1);
-// Results of pieces that the workspace has room for (155 MB at head dim 128): with half of them 256 items could not be cut into the four
+// Results of pieces that the workspace has room for at most (158 MB at head dim 128): with half of them 256 items could not be cut into the four
 // pieces each that fill the waves.
 constexpr int kMostSlots = 8 * 148;
+constexpr int kLeastPiece = 4;             // key tiles
+// ... and those that a launch can come to: its row tiles, each in as many pieces as the table has room for.  (Sequences that overlap, which no
+// call has, might ask for more: the plan does not go beyond it.)
+int rows_slots(const PagedParams& p) {
+  const int64_t keys = ((int64_t)p.per_seq << p.page_shift), cuts = ((keys + kBN - 1) / kBN + kLeastPiece - 1) / kLeastPiece;
+  if (cuts < 2) return 0;
+  const int64_t tiles = p.T * p.G / item_rows(p.D) + (p.T < p.B ? p.T : p.B);
+  return (int)(tiles * p.Hkv >= kMostSlots ? kMostSlots : tiles * p.Hkv * cuts < kMostSlots ? tiles * p.Hkv * cuts : kMostSlots);
+}
 constexpr float kLn2 = 0.6931471805599453f;
 
 // ---- the plan ------------------------------------------------------------------
@@ -84,7 +93,7 @@ __device__ __forceinline__ int even_piece(int tiles, int piece) {
 
 // Candidate k cuts the batch into about k / 4 pieces a CTA, candidate 0 not at all.  With equal pieces the time is that of the waves;
 // longer ones than the average may come last.
-__global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p, RowsPlan* plan, int sms) {
+__global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p, RowsPlan* plan, int sms, int most_slots) {
   __shared__ int rows_s[kPagedBatch], most_s[kPagedBatch], least_s[kPagedBatch];
   __shared__ float cost_s[32];
   __shared__ int piece_s[32];
@@ -117,7 +126,7 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p, R
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
   longest = __reduce_max_sync(0xffffffffu, longest);
-  const int piece = warp == 0 ? longest : max((int)ceilf(4.f * work / (float)(sms * warp)), 4);
+  const int piece = warp == 0 ? longest : max((int)ceilf(4.f * work / (float)(sms * warp)), kLeastPiece);
   float items = 0.f;
   int slots = 0, top = 1;
   for (int i = lane; i < p.B; i += 32) {
@@ -134,7 +143,7 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p, R
   if (lane == 0) {
     const float average = work / fmaxf(items, 1.f);
     const float cost = ceilf(items / (float)sms) * (average + kItemCost) + 0.5f * fmaxf((float)top - average, 0.f);
-    cost_s[warp] = slots > kMostSlots ? INFINITY : cost;
+    cost_s[warp] = slots > most_slots ? INFINITY : cost;
     piece_s[warp] = piece;
   }
   __syncthreads();
@@ -935,7 +944,7 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
     const uint32_t tS = tmem + lane_base + x * kBN, tO = tmem + lane_base + 256 + (kWide ? 0 : x * 128);
     uint32_t sph = 0, oph = 0, kt = 0;     // kt: key tiles of this CTA before the item's
     // head dim 256: the softmax of an item, by warps 4-7; all eight leave when its last P.V has executed
-    auto wide_rows = [&](const RowsItem& it, int ntiles, int j0, int lim, int lim_first, int x, uint32_t kt, RowRef& rr, bool& ok) {
+    auto wide_rows = [&](int ntiles, int j0, int lim, int lim_first, int x, uint32_t kt, RowRef& rr, bool& ok) {
       uint32_t g = kt;                                      // the CTA's tiles before this one
       if (x == 0) {
         for (int j = 0; ok && j < ntiles; ++j, ++g) {
@@ -966,7 +975,6 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
       ok = __all_sync(0xffffffffu, ok);
       if (x == 0) c.row_inv[row] = rr.ref == -INFINITY && rr.l == 0.f ? 0.f : 1.f / rr.l;
       rows_pair_barrier();                                  // the rows' factors are visible to warps 8-11
-      (void)it;
     };
     for (int n = 0; rows_next<true, D, kCodes>(a, c, smem, n & 1); ++n) {
       const RowsItem& it = c.item[n & 1];
@@ -981,7 +989,7 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
       RowRef rr{-INFINITY, -INFINITY, 0.f};
       bool ok = true;
       if constexpr (kWide) {
-        wide_rows(it, ntiles, j0, lim, lim_first, x, kt, rr, ok);
+        wide_rows(ntiles, j0, lim, lim_first, x, kt, rr, ok);
       } else {
         const int j1 = twice ? x : 0, by = twice ? 2 : 1;
         for (int j = j1; ok && j < ntiles; j += by) {
@@ -1284,13 +1292,13 @@ __global__ void __launch_bounds__(kJoinThreads) paged_rows_join_kernel(const Pag
 }
 
 template <bool kHalf, int D>
-cudaError_t launch_rows_dim(const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, const RowsArgs& a, int sms, cudaStream_t st) {
+cudaError_t launch_rows_dim(const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, const RowsArgs& a, int sms, int slots, cudaStream_t st) {
   auto kernel = p.store == MOBA_STORE_SAME ? paged_rows_kernel<kHalf, D, MOBA_STORE_SAME>
               : p.store == MOBA_STORE_E4M3 ? paged_rows_kernel<kHalf, D, MOBA_STORE_E4M3> : paged_rows_kernel<kHalf, D, MOBA_STORE_INT8>;
   const int threads = p.store == MOBA_STORE_SAME ? kRowsThreads<MOBA_STORE_SAME> : kRowsThreads<MOBA_STORE_E4M3>;
   cudaError_t e = prepare_kernel(kernel, kRowsSmem);
   if (e != cudaSuccess) return e;
-  if ((e = launch_pdl(paged_plan_kernel, dim3(1), kPagedBatch, 0, st, p, a.plan, sms)) != cudaSuccess) return e;
+  if ((e = launch_pdl(paged_plan_kernel, dim3(1), kPagedBatch, 0, st, p, a.plan, sms, slots)) != cudaSuccess) return e;
   if ((e = launch_pdl(kernel, dim3(sms), threads, kRowsSmem, st, p, mk, mv, a)) != cudaSuccess) return e;
   const int64_t warps = p.T * p.Hq, per = kJoinThreads / 32;
   return launch_pdl(paged_rows_join_kernel<kHalf, D>, dim3((unsigned)((warps + per - 1) / per)), kJoinThreads, 0, st, p, a);
@@ -1302,7 +1310,7 @@ constexpr size_t kPlanBytes = (sizeof(RowsPlan) + 255) / 256 * 256;
 }  // namespace
 
 size_t paged_rows_workspace(const PagedParams& p) {
-  return kPlanBytes + (size_t)kMostSlots * item_rows(p.D) * (sizeof(float2) + p.D * sizeof(float));
+  return kPlanBytes + (size_t)rows_slots(p) * item_rows(p.D) * (sizeof(float2) + p.D * sizeof(float));
 }
 
 cudaError_t launch_paged_rows(const PagedParams& all, const void* q, const void* kp, const void* vp, const uint8_t* ks,
@@ -1317,7 +1325,8 @@ cudaError_t launch_paged_rows(const PagedParams& all, const void* q, const void*
   a.lse = lse;
   a.plan = static_cast<RowsPlan*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + kPlanBytes);
-  a.part = reinterpret_cast<float*>(a.part_ml + (size_t)kMostSlots * item_rows(all.D));
+  const int slots_of_results = rows_slots(all);
+  a.part = reinterpret_cast<float*>(a.part_ml + (size_t)slots_of_results * item_rows(all.D));
   a.by_group = fast_div(all.G);
   CUtensorMap mk{}, mv{};
   if (all.store == MOBA_STORE_SAME) {
@@ -1333,10 +1342,10 @@ cudaError_t launch_paged_rows(const PagedParams& all, const void* q, const void*
     p.cu += b;
     p.lens += b;
     p.table += b * all.table_stride;
-    const cudaError_t e = p.D == 64 ? (p.fp16 ? launch_rows_dim<true, 64>(p, mk, mv, a, sms, st) : launch_rows_dim<false, 64>(p, mk, mv, a, sms, st))
-                        : p.D == 96 ? (p.fp16 ? launch_rows_dim<true, 96>(p, mk, mv, a, sms, st) : launch_rows_dim<false, 96>(p, mk, mv, a, sms, st))
-                        : p.D == 128 ? (p.fp16 ? launch_rows_dim<true, 128>(p, mk, mv, a, sms, st) : launch_rows_dim<false, 128>(p, mk, mv, a, sms, st))
-                                     : (p.fp16 ? launch_rows_dim<true, 256>(p, mk, mv, a, sms, st) : launch_rows_dim<false, 256>(p, mk, mv, a, sms, st));
+    const cudaError_t e = p.D == 64 ? (p.fp16 ? launch_rows_dim<true, 64>(p, mk, mv, a, sms, slots_of_results, st) : launch_rows_dim<false, 64>(p, mk, mv, a, sms, slots_of_results, st))
+                        : p.D == 96 ? (p.fp16 ? launch_rows_dim<true, 96>(p, mk, mv, a, sms, slots_of_results, st) : launch_rows_dim<false, 96>(p, mk, mv, a, sms, slots_of_results, st))
+                        : p.D == 128 ? (p.fp16 ? launch_rows_dim<true, 128>(p, mk, mv, a, sms, slots_of_results, st) : launch_rows_dim<false, 128>(p, mk, mv, a, sms, slots_of_results, st))
+                                     : (p.fp16 ? launch_rows_dim<true, 256>(p, mk, mv, a, sms, slots_of_results, st) : launch_rows_dim<false, 256>(p, mk, mv, a, sms, slots_of_results, st));
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;

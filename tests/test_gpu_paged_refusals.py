@@ -1,4 +1,6 @@
 """GPU: calls of the paged cache that are refused, and what they leave behind."""
+import ctypes
+
 import pytest
 import torch
 
@@ -77,3 +79,25 @@ def test_a_refused_append_writes_nothing(tokens, monkeypatch):
         m.setattr(paged, "_workspace", none)
         refused(torch.cuda.OutOfMemoryError)
     assert cache.append(q, k, k, *where, tokens).shape == q.shape and cache.k._version > version and (cache.k[0, 0] == 1).all()
+
+
+@pytest.mark.parametrize("dim,store", [(128, None), (256, torch.int8), (64, torch.float8_e4m3fn)])
+def test_scratch_is_not_exceeded(dim, store):
+    """Bytes behind the workspace that a call asks for are not touched, also where sequences that overlap make more items than it counts."""
+    hq, hkv, tokens, pages = 8, 2, 60, 130
+    cache = PagedKV(pages, 64, hkv, dim, torch.bfloat16, store)
+    for batch, cu in ((1, [0, tokens]), (40, [0, tokens] * 20 + [0]), (3, [0, 20, 21, tokens])):
+        table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(batch, 1)
+        lens, cu = _i32([8000 - 64 * i for i in range(batch)]), _i32(cu)
+        q = torch.randn(tokens, hq, dim, device="cuda").bfloat16()
+        out = torch.empty_like(q)
+        g = paged._Pages(cache.k, cache.v, table, cu, lens, cache.k_scales, cache.v_scales)
+        rows = (hq * dim, dim)
+        prob = g.pack(tokens, hq, tokens, q.dtype, 0.0, rows, rows)
+        need = ctypes.c_size_t(0)
+        _lib.check(_lib.lib().moba_paged_workspace_size(prob, ctypes.byref(need)))
+        scratch = torch.full((need.value + 65536,), 0x5a, dtype=torch.uint8, device="cuda")
+        g.run(_lib.lib().moba_paged_attention, prob, q.data_ptr(), *g.where, out.data_ptr(), None, scratch.data_ptr(), need.value)
+        assert (scratch[need.value:] == 0x5a).all()
+        # (sequences that overlap are owed nothing: rows behind the last entry, 0, are behind the batch)
+        assert (out == 0).all() or batch == 40

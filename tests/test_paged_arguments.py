@@ -56,3 +56,20 @@ def test_sizes_beyond_32_bits():
         with pytest.raises(NotImplementedError, match="32 bits"):
             g.pack(21, 4, 1, torch.float16, 0.0)
         setattr(g, name, kept)
+
+
+def test_scratch_follows_the_call(lib):
+    """No more results of pieces than a call's row tiles, heads and table can come to: a few rows of one request do not take what a prompt does."""
+    def size(**kw):
+        need = C.c_size_t(0)
+        assert lib.moba_paged_workspace_size(C.byref(_paged(**kw)), C.byref(need)) == 0
+        return need.value
+    one = dict(batch=1, num_kv_heads=1, num_q_heads=8, max_new=16)
+    plan = size(total_tokens=16, pages_per_seq=8, **one)     # 512 keys are one piece: nothing to join
+    assert plan < 1 << 16
+    slot = 256 * (128 + 2) * 4                               # head dim 128: 256 rows of output, maximum and sum
+    assert size(total_tokens=16, pages_per_seq=9, table_stride=9, **one) == plan + 2 * slot
+    assert size(total_tokens=16, pages_per_seq=640, table_stride=640, **one) == plan + 80 * slot
+    many = size(total_tokens=65536, pages_per_seq=2048, table_stride=2048, batch=3, max_new=30000)
+    assert many == plan + 8 * 148 * slot
+    assert size(total_tokens=2 ** 27, num_q_heads=8, batch=2000, max_new=2 ** 17, pages_per_seq=2 ** 14, table_stride=2 ** 14) == many
