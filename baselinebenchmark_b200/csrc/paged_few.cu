@@ -29,6 +29,8 @@
 //   five tokens of 12 requests of 338 to 20016, int8, 16/4 heads, fp16    92 -> 49                                              [14]
 //   one token behind 20011, 16/4 heads, head dim 64, fp16                 64 -> 19 (pieces joined in parallel) -> 16            [3]
 // The last two are chains of latencies: the plan of the line, a page's number, its rows, four warps joined, the second kernel.
+#include <type_traits>
+
 #include "paged.cuh"
 #include "sm100_ptx.cuh"
 
@@ -65,6 +67,10 @@ template <int D, int kStore, int kM> struct FewShape {
   static constexpr int kWarpBytes = kStages * kStageBytes;
   static constexpr int kUnit = kKeys * kFewWarps;                    // keys of a CTA's unit
   static constexpr size_t kSmem = 1024 + (size_t)kFewWarps * kWarpBytes;
+  // bf16 queries over codes: turned to fp16 as they come, and read again by a tile that cannot have them so; or kept until that is known, where
+  // registers are short (8 rows at head dim 128 and 256; 8 rows of 16 sequences of 8000 tokens, e4m3, 16/4 heads of 256: 86 us at once, 77 kept;
+  // 16 rows, 32/8 heads of 128: 65 at once, 68 kept).
+  static constexpr bool kAtOnce = kM == 16 || D == 64;
   static_assert(kWarpBytes >= 16 * D * 4, "the output of a warp fits its ring");
 };
 
@@ -424,32 +430,50 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
         for (int k = 0; k < kSteps; ++k) x[k] = on ? __ldg(reinterpret_cast<const uint2*>(q + 16 * k + 4 * t4)) : make_uint2(0, 0);
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
-          qa[k][e] = x[k].x;
-          qa[k][2 + e] = x[k].y;
           if (!kHalf) { range.add(x[k].x); range.add(x[k].y); }
+          qa[k][e] = S::kAtOnce && !kHalf ? scaled_query<true>(x[k].x, kQueryScale) : x[k].x;
+          qa[k][2 + e] = S::kAtOnce && !kHalf ? scaled_query<true>(x[k].y, kQueryScale) : x[k].y;
         }
       }
     }
-    float rs = p.sl2;                                       // factor of the scores
-    if (kCodes && !kHalf) {
-      wide = __any_sync(0xffffffffu, range.reaches(10) || !range.all_reach(-23));
-      if (!wide) {
-        rs *= 1.f / kQueryScale;
+    float rs = kCodes && !kHalf && S::kAtOnce ? p.sl2 * (1.f / kQueryScale) : p.sl2;   // factor of the scores
+    if (kCodes && !kHalf) wide = __any_sync(0xffffffffu, range.reaches(10) || !range.all_reach(-23));
+    // (a wide tile's rows are taken as they are, unless sums of their products with codes might leave fp32)
+    if constexpr (kCodes && !kHalf && S::kAtOnce) {
+      if (wide) {
+        const bool large = __any_sync(0xffffffffu, range.reaches(100)), small = !__any_sync(0xffffffffu, range.reaches(-60));
+        const float f = large ? 0x1p-64f : small ? 0x1p64f : 1.f;
+        rs = p.sl2 * (large ? 0x1p64f : small ? 0x1p-64f : 1.f);
+#pragma unroll
+        for (int e = 0; e < kE; ++e) {
+          int64_t token;
+          int head, i;
+          if (!few_row<kM>(p, s, it.h, it.tile, g + 8 * e, token, head, i)) continue;
+          const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + token * p.sq_t + head * p.sq_h;
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k) {
+            const uint2 x = __ldg(reinterpret_cast<const uint2*>(q + 16 * k + 4 * t4));
+            qa[k][e] = scaled_query<false>(x.x, f);
+            qa[k][2 + e] = scaled_query<false>(x.y, f);
+          }
+        }
+      }
+    } else if constexpr (kCodes && !kHalf) {
+      auto scale_rows = [&](auto half, float f) {
 #pragma unroll
         for (int k = 0; k < kSteps; ++k)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if ((i & 1) < kE) qa[k][i] = scaled_query<true>(qa[k][i], kQueryScale);
+            if ((i & 1) < kE) qa[k][i] = scaled_query<decltype(half)::value>(qa[k][i], f);
+      };
+      if (!wide) {
+        rs *= 1.f / kQueryScale;
+        scale_rows(std::true_type(), kQueryScale);
       } else {
-        // as they are, unless sums of their products with codes might leave fp32
         const bool large = __any_sync(0xffffffffu, range.reaches(100)), small = !__any_sync(0xffffffffu, range.reaches(-60));
         if (large || small) {
           rs *= large ? 0x1p64f : 0x1p-64f;
-#pragma unroll
-          for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if ((i & 1) < kE) qa[k][i] = scaled_query<false>(qa[k][i], large ? 0x1p-64f : 0x1p64f);
+          scale_rows(std::false_type(), large ? 0x1p-64f : 0x1p64f);
         }
       }
     }
