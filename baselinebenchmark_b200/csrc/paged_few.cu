@@ -16,7 +16,8 @@
 //     weight: with x = score * log2(e) and M a reference near the running maximum of x + e, a key weighs w = 2^(x + e - M), 2^8 at
 //     most; the output is sum(w * code) / sum(w * 2^-e).  Where all weights of a block are 2^-14 and more (or nothing at all) they go to P.V as
 //     fp16.  A row of zeros (e = 0) or one with a single large element may put M far above what the other channels are made of: a block with
-//     smaller weights takes them as two bf16 numbers each, which have fp32's range (2^-16 relative, in two products over codes turned to bf16).
+//     smaller weights takes them as bf16, which has fp32's range, over codes turned to bf16; fp16 rows, which are owed three bits more, as the
+//     sum of two bf16 numbers, in two products.
 //     bf16 queries become fp16, which holds them exactly where they lie within 2^-23 to 2^10 (or are zeros); a tile with others stays bf16
 //     and has the codes turned to bf16 for its Q.K^T.
 //   - P is rounded to the 16-bit type that V has (or as said): 2^-8 (bf16), 2^-11 (fp16) relative at most, as in the dense stage of the prefill.
@@ -657,9 +658,9 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
       }
       // ---- O += P.V
       if (kCodes && (__any_sync(0xffffffffu, least < kLeastHalf - 1u) || beyond)) {
-        // weights that fp16 has not: as bf16, and what that leaves of them as bf16
+        // weights that fp16 has not: as bf16, and for fp16 rows what that leaves of them, as bf16 again
 #pragma unroll 1
-        for (int part = 0; part < 2; ++part) {
+        for (int part = 0; part < (kHalf ? 2 : 1); ++part) {
 #pragma unroll
           for (int n = 0; n < kBlocksN; ++n)
 #pragma unroll
