@@ -64,13 +64,19 @@ constexpr int kPagedBatch = 1024;
 // Items of more rows run on tcgen05.  Two new launches (the plan, the join of many rows) cost a small call 8 us there; in a large one the tensor
 // memory kernel keeps up with the copies whatever the rows are, where the other's chain grows with them.  8-bit codes are turned once for each
 // tile of 16 rows here and once for each of 128 or 256 there, by fewer warps.  (rows: this kernel / tcgen05, us; 16 sequences of 8000 tokens
-// over 8 kv heads, the same over one, 2 of 500; 64-token pages)
-//   head dim 128          8:  93 / 94, 19 / 33, 12 / 20    16: 120 / 95, 39 / 33, 13 / 21     32: 207 / 96, 43 / 33, 16 / 21
-//   head dim 128, e4m3    8:  57 / 157, 17 / 41, 12 / 26   16:  59 / 157, 22 / 41, 13 / 26    32: 100 / 159, 24 / 41, 13 / 26
-//                         48 (8 sequences): 79 / 92        64: 100 / 92, 34 / 42
-//   head dim 256          8: 179 / 171, 51 / 50, 16 / 27    16: 186 / 171, 49 / 50, 17 / 27    32: 345 / 173, 58 / 51, 23 / 27
+// over 8 kv heads, the same over one, 2 of 500 over 8, one of 40000 over 8; 64-token pages; 16-bit rows are bf16)
+//   head dim 64           8: 53 / 71, 14 / 25, 9 / 18, 21 / 39        16: 56 / 72, 17 / 25, 10 / 18, 24 / 39      32: 95 / 73, 20 / 25, 12 / 18, 30 / 40
+//   head dim 128          8: 93 / 93, 18 / 33, 11 / 20, 39 / 56       16: 100 / 94, 25 / 31, 14 / 20, 43 / 56     32: 183 / 96, 30 / 31, 16 / 20, 60 / 57
+//   head dim 256          8: 182 / 170, 40 / 50, 13 / 25, 65 / 91     16: 187 / 171, 43 / 48, 17 / 26, 70 / 93    32: 331 / 174, 57 / 48, 19 / 26, 119 / 95
+//   e4m3, head dim 64    16: 45 / 112, 17 / 30, 12 / 21, 25 / 49      48: 110 / 114, 24 / 30, 14 / 21, 40 / 49    64: 140 / 115, 29 / 31, 15 / 22, 49 / 50
+//   e4m3, head dim 96    16: 56 / 147, 19 / 36, 13 / 24, 29 / 61      48: 133 / 149, 29 / 36, 16 / 24, 48 / 62    64: 171 / 150, 34 / 36, 17 / 25, 59 / 62
+//   e4m3, head dim 128   16: 65 / 157, 20 / 37, 14 / 26, 29 / 64      48: 161 / 160, 32 / 37, 16 / 26, 55 / 65    64: 206 / 162, 38 / 37, 17 / 25, 69 / 67
+//   e4m3, head dim 256   16: 164 / 342, 37 / 57, 21 / 37, 65 / 123    32: 298 / 343, 56 / 59, 22 / 37, 103 / 125  48: 428 / 345, 74 / 60, 23 / 38, 141 / 126
+//   int8, fp16, 128      16: 73 / 153, 20 / 36, 14 / 25, 31 / 63      48: 188 / 157, 35 / 37, 16 / 26, 63 / 65    64: 244 / 159, 42 / 37, 17 / 25, 80 / 66
+// The limits are those of large calls, where most is at stake.  Calls of one sequence or of short ones would be served better here up to 32 rows
+// and more of 16-bit pages; the rule does not look at that.
 inline bool paged_few_rows(const PagedParams& p) {
-  const int most = p.store != MOBA_STORE_SAME ? 48 : p.D == 256 ? 16 : 8;
+  const int most = p.store != MOBA_STORE_SAME ? (p.D == 256 ? 32 : 48) : p.D == 256 ? 16 : 8;
   return (int64_t)p.max_new * p.G <= most;
 }
 
