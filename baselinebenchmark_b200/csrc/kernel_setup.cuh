@@ -66,7 +66,7 @@ class KernelSetup {
   }
 
  private:
-  static constexpr int kDevices = 64, kContexts = 16, kKernels = 256;   // (some 100 kernels of the library ask)
+  static constexpr int kDevices = 64, kContexts = 16, kKernels = 256;   // (some 200 kernels of the library ask)
   struct Device {
     bool known;
     DeviceInfo info;

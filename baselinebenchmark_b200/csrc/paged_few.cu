@@ -26,8 +26,10 @@
 // Measured (replayed from a graph, us; head dim 128, 32/8 heads unless said otherwise; in brackets the bytes at the measured copy bandwidth):
 //   one token of 48 requests of 16 to 11001 tokens                        188 -> 172 (boxes) -> 151 (three CTAs an SM) -> 115 (what an item costs besides
 //                                                                         its keys counts on the line)                          [103]
-//   one token of 16 requests of 16385 to 40001, e4m3                      214 -> 153 (169 where no page is left in L2)          [138]
-//   five tokens of 12 requests of 338 to 20016, int8, 16/4 heads, fp16    92 -> 49                                              [14]
+//   one token of 16 requests of 16385 to 40001, e4m3                      214 -> 147 (172 where no page is left in L2)          [138]
+//     the same where no block's weights fit fp16: bf16 172, fp16 263; where no tile's queries do: 168; fp16 with every block near or beyond 65504: 739
+//   five tokens of 12 requests of 338 to 20016, int8, 16/4 heads, fp16    92 -> 52                                              [14]
+//   one token of 16 requests of 8000, 16/4 heads, head dim 256, e4m3      77; int8, fp16 88                                     [40]
 //   one token behind 20011, 16/4 heads, head dim 64, fp16                 64 -> 19 (pieces joined in parallel) -> 16            [3]
 // The last two are chains of latencies: the plan of the line, a page's number, its rows, four warps joined, the second kernel.
 #include <type_traits>
@@ -60,9 +62,9 @@ template <int D, int kStore, int kM> struct FewShape {
   static constexpr int kStageBytes = 2 * kSideBytes;
   static constexpr bool kParts = !kCodes && kSubs > 1 && D % kSpan == 0;   // one box has all sub-blocks (not of head dim 96: a row's would end in the next)
   // Three CTAs, twelve warps, an SM with 16 KB of stages each: what a warp waits for is its own chain of instructions, and there have to be
-  // others meanwhile.  One CTA with 48 KB a warp at head dim 256; two with 24 KB for 16 rows over codes at
-  // head dim 128, which do not fit the registers of three (16 sequences of 8000 tokens, 32/8 heads, e4m3 97 us with three, 57 with two; 8 rows of 16
-  // longer ones 169 with three, 175 with two).
+  // others meanwhile.  One CTA with 48 KB a warp at head dim 256, where output and queries alone are 192 registers (over codes 255 with
+  // 100 to 290 bytes spilled); two with 24 KB for 16 rows over codes at head dim 128, which do not fit the registers of three (16 sequences of 8000
+  // tokens, 32/8 heads, e4m3 97 us with three, 57 with two; 8 rows of 16 longer ones 169 with three, 175 with two; both before weights were looked at).
   static constexpr int kCtas = kStageBytes == 16384 ? 1 : kCodes && kM == 16 && D == 128 ? 2 : 3;
   static constexpr int kStages = kStageBytes == 16384 || kCtas == 2 ? 3 : kStageBytes == 8192 ? 2 : 4;
   static constexpr int kWarpBytes = kStages * kStageBytes;

@@ -9,8 +9,9 @@
 //   - 8-bit pages: eight warps (3, and 12-18) read the codes, multiply by the row's power of two (exact: see moba_b200.h) and store the operand
 //     tiles in the rows' 16-bit type; from there on nothing differs, and no pass over the cache writes it out in 16 bits.  They run through one
 //     stream of tiles, without a barrier at an item's end; warp 0 tells them where the codes are.  All 19 warps live with 96 registers,
-//     which is what bounds this form: the softmax reads its scores twice, 16 at a time (with 32 at a time some values were kept in
-//     local memory, in an L1 of the few KB that shared memory leaves, and each look at them went to L2).
+//     which is what bounds this form: the softmax reads its scores twice, 16 at a time (with 32 at a time its loop kept values in
+//     local memory, in an L1 of the few KB that shared memory leaves, and each look at them went to L2; 4 to 8 bytes are spilled now, 48 at
+//     head dim 96, and 16 bytes by the form for 16-bit pages).
 //   - An item of at most 128 rows (drafted tokens, a small group) has them in both row tiles: A takes every other key tile, B the ones between,
 //     each with its own output, and the two are joined at the end.  One softmax at a time left the copies waiting.
 //   - Pieces: a first kernel (one CTA) adds up the work of the batch and picks how many pieces an item is cut into, so that
@@ -24,7 +25,7 @@
 // Measured (replayed from a graph; 32/8 heads, head dim 128 unless said otherwise; in brackets the products at the measured bf16 rate):
 //   700 tokens behind 50021                              527 us, 1095 TFLOP/s [351 us]: 3300 cycles a tile and SM against 2048 of its MMAs
 //   2048 behind 30720, e4m3                              7.1 ms (mma.sync) -> 3.1 (four warps for codes) -> 2.0 (eight) -> 1.66 (one stream of tiles)
-//                                                        -> 1.28 (no values in local memory), 830 TFLOP/s [648 us]: 4600 cycles a tile
+//                                                        -> 1.28 (next to nothing in local memory), 830 TFLOP/s [648 us]: 4600 cycles a tile
 //   prompts of 1023, 4096 and 200, 16 heads, head dim 256   3.8 ms (mma.sync) -> 0.22 [89 us]
 //   4 tokens of 16 requests of 8000 over 8 kv heads      127 us (one row tile at work) -> 95 (both, key tiles by turns) [80 us of bytes]
 #include "attend_rows.cuh"

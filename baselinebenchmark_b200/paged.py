@@ -200,7 +200,8 @@ def paged_store(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages
                 cu_seqlens: torch.Tensor, seq_lens: torch.Tensor, *, k_scales: Optional[torch.Tensor] = None,
                 v_scales: Optional[torch.Tensor] = None) -> None:
     """Writes the packed rows k, v [T, Hkv, D] into the pages of their sequences; 8-bit pages are quantised to, each row
-    and head with a power of two of its own.  Rows behind the last sequence, and rows whose page is not there, are not written."""
+    and head with a power of two of its own.  Rows behind the last sequence, and rows whose page is not there, are not written.
+    A slot that two rows of a call are for (a page in two sequences' tables) is undefined."""
     g = _Pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
     heads, tokens = g.shape[2], k.shape[0] if k.dim() else None
     ks = _rows("k", k, g, heads, None, k_pages)

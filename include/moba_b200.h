@@ -420,7 +420,7 @@ typedef struct moba_paged {
 } moba_paged_t;
 
 int moba_paged_check(const moba_paged_t* p);
-/* k, v -> pages.  A slot that two rows of a call are for (pages shared by sequences) holds one of them. */
+/* k, v -> pages.  A slot that two rows of a call are for (a page in two sequences' tables) is undefined: it may hold parts of both. */
 int moba_paged_store(const moba_paged_t* p, const void* k, const void* v, const int32_t* cu_seqlens, const int32_t* seq_lens,
                      const int32_t* page_table, void* k_pages, void* v_pages, uint8_t* k_scales, uint8_t* v_scales, void* stream);
 /* pages -> k, v: the same rows back, in `dtype`. */
@@ -430,8 +430,11 @@ int moba_paged_load(const moba_paged_t* p, const int32_t* cu_seqlens, const int3
 /* Softmax attention of every packed row to the positions of its sequence up to its own, each kv head for its group of query
  * heads.  A row that sees nothing is zeros, its LSE -inf.  lse_out: optional fp32 [Hq, T], natural log.  Sums, maxima and the
  * accumulated output are fp32; probabilities are rounded to 16 bits before the product with V.
- * The workspace is 32-byte aligned and needs no clearing; its size follows from the structure alone.  An infinity or a NaN in a row of K
- * or V that a token sees makes that token's output NaN; one in a token behind it, in the same tile of at most 128 positions, may too. */
+ * The workspace is 32-byte aligned and needs no clearing; its size follows from the structure alone.  A NaN in a row of K or V that a
+ * token sees makes that token's output NaN, one in V of 16-bit pages in its own channel at least; so does an infinity in 8-bit pages, which
+ * reads back as NaN.  In 16-bit pages a score of +infinity makes the output NaN, one of -infinity is a weight of 0, and an infinity in V
+ * makes its channel infinite or NaN.  Any of them in a token behind, in the same tile of at most 128 positions, may do the same.
+ * Over 8-bit pages a key whose weight times its V row's power of two is less than 2^-126 of the largest such product may count for nothing. */
 int moba_paged_workspace_size(const moba_paged_t* p, size_t* bytes);
 int moba_paged_attention(const moba_paged_t* p, const void* q, const int32_t* cu_seqlens, const int32_t* seq_lens,
                          const int32_t* page_table, const void* k_pages, const void* v_pages, const uint8_t* k_scales,
