@@ -28,10 +28,10 @@
 //                                                                         its keys counts on the line)                          [103]
 //   one token of 16 requests of 16385 to 40001, e4m3                      214 -> 147 (172 where no page is left in L2)          [138]
 //     the same where no block's weights fit fp16: bf16 172, fp16 263; where no tile's queries do: 168; fp16 with every block near or beyond 65504: 739
-//   five tokens of 12 requests of 338 to 20016, int8, 16/4 heads, fp16    92 -> 52                                              [14]
 //   one token of 16 requests of 8000, 16/4 heads, head dim 256, e4m3      77; int8, fp16 88                                     [40]
+//   five tokens of 12 requests of 338 to 20016, int8, 16/4 heads, fp16    92 -> 52                                              [14]
 //   one token behind 20011, 16/4 heads, head dim 64, fp16                 64 -> 19 (pieces joined in parallel) -> 16            [3]
-// The last two are chains of latencies: the plan of the line, a page's number, its rows, four warps joined, the second kernel.
+// The last is a chain of latencies, and much of the one before it: the plan of the line, a page's number, its rows, four warps joined, the second kernel.
 #include <type_traits>
 
 #include "paged.cuh"
