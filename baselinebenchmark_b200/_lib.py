@@ -27,11 +27,13 @@ SYMBOLS = (
     "moba_attend", "moba_merge", "moba_attend_tile_rows", "moba_attend_tile_rows_for", "moba_problem_tile_rows", "moba_problem_attend_kernel", "moba_route_static",
     "moba_backward_workspace_size", "moba_backward",
     "moba_cp_workspace_size", "moba_cp_forward", "moba_cp_poll", "moba_cp_abort", "moba_selftest_bounded_wait",
-    "moba_paged_check", "moba_paged_store", "moba_paged_load", "moba_paged_workspace_size", "moba_paged_attention",
+    "moba_paged_check", "moba_paged_store", "moba_paged_load", "moba_paged_workspace_size", "moba_paged_attention", "moba_paged_tree_attention", "moba_paged_keep",
+    "moba_page_pool_check", "moba_paged_reserve", "moba_paged_release",
+    "moba_rotary_check", "moba_rotary", "moba_drafts_check", "moba_verify_drafts",
 )
 
 #: MOBA_DTYPE_*, MOBA_STORE_*
-DTYPE_BF16, DTYPE_FP16 = 0, 1
+DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = range(3)
 STORE_SAME, STORE_E4M3, STORE_INT8 = range(3)
 #: MOBA_E_*
 E_SHAPE, E_ALIGN = -1, -6
@@ -64,6 +66,35 @@ class Paged(C.Structure):
         ("k_page_stride", C.c_int64), ("k_page_token", C.c_int64), ("k_page_head", C.c_int64),
         ("v_page_stride", C.c_int64), ("v_page_token", C.c_int64), ("v_page_head", C.c_int64),
         ("table_stride", C.c_int64),
+    ]
+
+
+class PagePool(C.Structure):
+    """struct moba_page_pool"""
+    _fields_ = [
+        ("total_tokens", C.c_int64), ("batch", C.c_int32), ("pages_per_seq", C.c_int32), ("num_pages", C.c_int32),
+        ("page_size", C.c_int32), ("table_stride", C.c_int64), ("reserved", C.c_int64),
+    ]
+
+
+class Rotary(C.Structure):
+    """struct moba_rotary"""
+    _fields_ = [
+        ("total_tokens", C.c_int64),
+        ("num_q_heads", C.c_int32), ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("rotary_dim", C.c_int32),
+        ("interleaved", C.c_int32), ("inverse", C.c_int32), ("dtype", C.c_int32), ("reserved", C.c_int32),
+        ("magnitude", C.c_float), ("reserved2", C.c_int32),
+        ("q_stride_token", C.c_int64), ("q_stride_head", C.c_int64), ("k_stride_token", C.c_int64), ("k_stride_head", C.c_int64),
+        ("qo_stride_token", C.c_int64), ("qo_stride_head", C.c_int64), ("ko_stride_token", C.c_int64), ("ko_stride_head", C.c_int64),
+    ]
+
+
+class Drafts(C.Structure):
+    """struct moba_drafts"""
+    _fields_ = [
+        ("total_tokens", C.c_int64), ("vocabulary", C.c_int64), ("batch", C.c_int32), ("max_new", C.c_int32),
+        ("dtype", C.c_int32), ("token_bits", C.c_int32), ("target_stride", C.c_int64), ("draft_stride", C.c_int64),
+        ("reserved", C.c_int64),
     ]
 
 
@@ -133,7 +164,16 @@ def lib() -> C.CDLL:
         handle.moba_paged_store.argtypes = [pg, vp, vp, i32p, i32p, i32p, vp, vp, vp, vp, vp]
         handle.moba_paged_load.argtypes = [pg, i32p, i32p, i32p, vp, vp, vp, vp, vp, vp, vp]
         handle.moba_paged_workspace_size.argtypes = [pg, C.POINTER(sz)]
+        handle.moba_paged_tree_attention.argtypes = [pg, vp, i32p, i32p, i32p, i32p, vp, vp, vp, vp, vp, vp, vp, sz, vp]
         handle.moba_paged_attention.argtypes = [pg, vp, i32p, i32p, i32p, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+        handle.moba_paged_keep.argtypes = [pg, i32p, i32p, i32p, i32p, C.c_int64, C.c_int32, i32p, vp, vp, vp, vp, i32p, vp]
+        handle.moba_page_pool_check.argtypes = [vp]
+        handle.moba_paged_reserve.argtypes = [vp, i32p, i32p, i32p, i32p, i32p, i32p, vp, i32p, i32p, vp]
+        handle.moba_paged_release.argtypes = [vp, i32p, i32p, i32p, i32p, vp]
+        handle.moba_rotary_check.argtypes = [vp]
+        handle.moba_rotary.argtypes = [vp, vp, vp, i32p, vp, vp, vp, vp]
+        handle.moba_drafts_check.argtypes = [vp]
+        handle.moba_verify_drafts.argtypes = [vp, vp, vp, vp, i32p, i32p, vp, vp, i32p, i32p, vp, vp]
         _lib = handle
     return _lib
 

@@ -1,0 +1,298 @@
+// Page tables, slots and positions from the lengths of requests, and pages given back, without the host.
+//
+// Free pages lie on a stack of numbers.  The entries of the tables that a call may change are one line, sequence by sequence: of a sequence
+// with new tokens those that the tokens lie in, of one that is cut those behind its kept tokens.  An entry that lacks a page (or has one to
+// give back) is number r of them, a prefix sum, and takes the r-th page from the top (or its place there, in the same order: what a call took, the
+// same cut puts back as it was).  A warp has a stretch of the line, its count goes to all blocks of the cluster, and every entry then knows its
+// number: no atomics, the same pages every time.
+// Slots and positions follow row by row; the depth of a row in a tree of drafted tokens by doubling, d(i) += d(up(i)), up(i) <- up(up(i)), which takes
+// as many rounds as the depth has bits.
+// All of it is a few KB: what bounds it is the chain of dependent loads and barriers, and the launches.  Small calls are one block, one launch.
+#include "page_pool.cuh"
+
+#include "cluster.cuh"
+#include "common.cuh"
+
+namespace moba {
+namespace {
+
+constexpr int kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kBlocks = 8;                 // of the cluster, where there is much to do
+constexpr int kSmallRows = 2048, kSmallEntries = 4096;
+
+struct Range {                             // entries of a sequence
+  int first, count;
+};
+__device__ __forceinline__ Range entries_of(const PoolParams& p, int b) {
+  const int64_t room = (int64_t)p.per_seq << p.page_shift, mask = ((int64_t)1 << p.page_shift) - 1;
+  const int64_t len = min(max((int64_t)__ldg(p.lens + b), (int64_t)0), room);
+  const int up = (int)((len + mask) >> p.page_shift);
+  if (p.cu == nullptr) return Range{up, p.per_seq - up};    // behind the kept tokens
+  const int64_t n = (int64_t)__ldg(p.cu + b + 1) - __ldg(p.cu + b);
+  if (n <= 0) return Range{0, 0};
+  const int from = (int)(min(max((int64_t)__ldg(p.lens + b) - n, (int64_t)0), room) >> p.page_shift);
+  return Range{from, max(up - from, 0)};
+}
+
+// Last b with start[b] <= x.
+template <typename F>
+__device__ __forceinline__ int search(int n, int64_t x, F&& start) {
+  int lo = 0;
+  while (n > 1) {
+    const int half = n >> 1;
+    const bool up = start(lo + half) <= x;
+    lo = up ? lo + half : lo;
+    n = up ? n - half : half;
+  }
+  return lo;
+}
+
+struct Row {                               // a packed row: its sequence, index in it, first row and position of index 0
+  int b, i;
+  int64_t row0, pos0;
+};
+__device__ __forceinline__ bool row_of(const PoolParams& p, int64_t row, Row& r) {
+  if (row >= p.rows) return false;
+  r.b = search(p.batch, row, [&](int b) { return (int64_t)__ldg(p.cu + b); });
+  r.row0 = __ldg(p.cu + r.b);
+  const int64_t n = __ldg(p.cu + r.b + 1) - r.row0;
+  r.i = (int)(row - r.row0);
+  r.pos0 = __ldg(p.lens + r.b) - n;
+  return row >= r.row0 && r.i < n;
+}
+// (the table was written by this launch, or by the one before it: past the read-only path)
+__device__ __forceinline__ long long slot_of(const PoolParams& p, const Row& r) {
+  const int64_t pos = r.pos0 + r.i;
+  if (pos < 0 || (pos >> p.page_shift) >= p.per_seq) return -1;
+  const int id = __ldcg(p.table + r.b * p.table_stride + (pos >> p.page_shift));
+  if ((unsigned)id >= (unsigned)p.pages) return -1;
+  return ((long long)id << p.page_shift) + (pos & (((int64_t)1 << p.page_shift) - 1));
+}
+__device__ __forceinline__ int clamp_position(int64_t x) { return (int)min(max(x, -((int64_t)1 << 31)), (((int64_t)1 << 31) - 1)); }
+
+// Depths of `rows` rows (a thread has rows tid, tid + kThreads ..; a parent in the block is its place there, depth known so far in `depth`).
+template <int kPer>
+__device__ __forceinline__ void double_depths(int* up, int* depth) {
+  for (;;) {
+    int u[kPer], d[kPer];
+    bool more = false;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int i = threadIdx.x + k * kThreads;
+      u[k] = up[i];
+      d[k] = depth[i];
+      if (u[k] >= 0) {
+        d[k] += depth[u[k]];
+        u[k] = up[u[k]];
+        more |= u[k] >= 0;
+      }
+    }
+    more = __syncthreads_or(more);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      up[threadIdx.x + k * kThreads] = u[k];
+      depth[threadIdx.x + k * kThreads] = d[k];
+    }
+    __syncthreads();
+    if (!more) return;
+  }
+}
+
+// kCut: pages are given back.  kRows: one block, which also does the rows.
+template <bool kCut, bool kRows>
+__global__ void __launch_bounds__(kThreads) pool_kernel(const PoolParams p) {
+  extern __shared__ int32_t smem[];
+  int32_t* begin = smem;                                    // [batch + 1]: first entry of a sequence on the line
+  int32_t* first = begin + p.batch + 1;                     // [batch]: its first entry in the table
+  __shared__ int32_t scan[kWarps], counts[kWarps], block_total[kBlocks];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = kRows ? 0 : cluster_rank(), blocks = kRows ? 1 : cluster_size();
+  pdl_wait();
+  pdl_trigger();
+  const int have = min(max(__ldcg(p.count), 0), p.pages);
+  // ---- the line (every block for itself)
+  int carry = 0;
+  for (int base = 0; base < p.batch; base += kThreads) {
+    const int b = base + tid;
+    Range r{0, 0};
+    if (b < p.batch) r = entries_of(p, b);
+    int x = r.count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) scan[warp] = x;
+    __syncthreads();
+    const int s = scan[lane], before = __reduce_add_sync(0xffffffffu, lane < warp ? s : 0), all = __reduce_add_sync(0xffffffffu, s);
+    if (b < p.batch) {
+      begin[b] = carry + before + x - r.count;
+      first[b] = r.first;
+    }
+    carry += all;
+    __syncthreads();
+  }
+  if (tid == 0) begin[p.batch] = carry;
+  __syncthreads();
+  // ---- how many of each warp's entries count
+  const int warps = (int)blocks * kWarps, me = (int)rank * kWarps + warp;
+  const int per = ((carry + warps - 1) / warps + 31) / 32 * 32;
+  const int lo = (int)min((int64_t)per * me, (int64_t)carry), hi = (int)min((int64_t)lo + per, (int64_t)carry);
+  auto entry = [&](int at, int32_t*& place) {               // the entry's number, and whether it counts
+    const int b = search(p.batch, at, [&](int k) { return (int64_t)begin[k]; });
+    place = p.table + b * p.table_stride + first[b] + (at - begin[b]);
+    const int id = *place;
+    return kCut ? ((unsigned)id < (unsigned)p.pages ? id : -1) : (unsigned)id < (unsigned)p.pages ? -1 : 0;
+  };
+  int mine = 0, id0 = -1;
+  int32_t* place0 = nullptr;                                // (of the first round, which is the only one as a rule)
+  for (int at = lo; at < hi; at += 32) {
+    int32_t* place = nullptr;
+    const int id = at + lane < hi ? entry(at + lane, place) : -1;
+    mine += __popc(__ballot_sync(0xffffffffu, id >= 0));
+    if (at == lo) { id0 = id; place0 = place; }
+  }
+  if (lane == 0) counts[warp] = mine;
+  __syncthreads();
+  const int c = counts[lane], block_sum = __reduce_add_sync(0xffffffffu, c);
+  int before = __reduce_add_sync(0xffffffffu, lane < warp ? c : 0), total = block_sum;
+  if (!kRows) {
+    if (warp == 0 && lane < (int)blocks) cluster_store(cluster_place(&block_total[rank], lane), (uint32_t)block_sum);
+    cluster_sync();
+    total = 0;
+    for (int i = 0; i < (int)blocks; ++i) {
+      if (i < (int)rank) before += block_total[i];
+      total += block_total[i];
+    }
+  }
+  // ---- pages taken, or put back
+  for (int at = lo; at < hi; at += 32) {
+    int32_t* place = place0;
+    const int id = at == lo ? id0 : at + lane < hi ? entry(at + lane, place) : -1;
+    const uint32_t votes = __ballot_sync(0xffffffffu, id >= 0);
+    const int r = before + __popc(votes & ((1u << lane) - 1));
+    before += __popc(votes);
+    if (id < 0) continue;
+    if (kCut) {
+      const int64_t to = (int64_t)have + total - 1 - r;
+      if (to < p.pages) p.free[to] = id;
+      *place = -1;
+    } else if (r < have) {
+      *place = p.free[have - 1 - r];
+    }
+  }
+  if (rank == 0 && tid == 0) {
+    *p.count = kCut ? (int)min((int64_t)have + total, (int64_t)p.pages) : max(have - total, 0);
+    if (!kCut) *p.missing = max(total - have, 0);
+  }
+  if constexpr (kRows && !kCut) {
+    // ---- the rows
+    __shared__ int32_t up[kSmallRows], depth[kSmallRows];
+    constexpr int kPer = kSmallRows / kThreads;
+    __threadfence_block();
+    __syncthreads();
+    Row r[kPer];
+    bool on[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int64_t row = tid + k * kThreads;
+      on[k] = row_of(p, row, r[k]);
+      if (p.parents != nullptr) {
+        const int parent = on[k] ? __ldg(p.parents + row) : -1;
+        const bool has = parent >= 0 && parent < r[k].i;
+        up[row] = has ? (int)r[k].row0 + parent : -1;
+        depth[row] = has ? 1 : 0;
+      }
+    }
+    if (p.parents != nullptr) {
+      __syncthreads();
+      double_depths<kPer>(up, depth);
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int64_t row = tid + k * kThreads;
+      if (row >= p.rows) continue;
+      p.slots[row] = on[k] ? slot_of(p, r[k]) : -1;
+      p.positions[row] = on[k] ? clamp_position(r[k].pos0 + (p.parents != nullptr ? depth[row] : r[k].i)) : -1;
+  }
+  }
+}
+
+// A row a thread, where no trees are.
+constexpr int kRowThreads = 256;
+__global__ void __launch_bounds__(kRowThreads) pool_rows_kernel(const PoolParams p) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t row = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
+  if (row >= p.rows) return;
+  Row r;
+  const bool on = row_of(p, row, r);
+  p.slots[row] = on ? slot_of(p, r) : -1;
+  p.positions[row] = on ? clamp_position(r.pos0 + r.i) : -1;
+}
+
+// A sequence a block; its rows in order, kThreads at a time: a parent lies among them, or its depth is known from its position.
+__global__ void __launch_bounds__(kThreads) pool_tree_kernel(const PoolParams p) {
+  __shared__ int32_t up[kThreads], depth[kThreads];
+  pdl_wait();
+  pdl_trigger();
+  const int b = blockIdx.x, tid = threadIdx.x;
+  if (b == p.batch) {                                       // rows of no sequence
+    const int64_t lead = min((int64_t)__ldg(p.cu), p.rows), tail = max((int64_t)__ldg(p.cu + p.batch), (int64_t)0);
+    for (int64_t row = tid; row < lead; row += kThreads) { p.slots[row] = -1; p.positions[row] = -1; }
+    for (int64_t row = tail + tid; row < p.rows; row += kThreads) { p.slots[row] = -1; p.positions[row] = -1; }
+    return;
+  }
+  Row r;
+  r.b = b;
+  r.row0 = __ldg(p.cu + b);
+  const int64_t n = __ldg(p.cu + b + 1) - r.row0;
+  r.pos0 = __ldg(p.lens + b) - n;
+  if (r.row0 < 0) return;
+  const int64_t rows = min(n, p.rows - r.row0);
+  for (int64_t base = 0; base < rows; base += kThreads) {
+    const int64_t i = base + tid;
+    const bool on = i < rows;
+    int parent = on ? __ldg(p.parents + r.row0 + i) : -1;
+    if (parent >= i) parent = -1;
+    int d = parent >= 0 ? 1 : 0;
+    if (parent >= 0 && parent < base) d += p.positions[r.row0 + parent] - clamp_position(r.pos0);
+    up[tid] = parent >= base ? (int)(parent - base) : -1;
+    depth[tid] = d;
+    __syncthreads();
+    double_depths<1>(up, depth);
+    if (on) {
+      r.i = (int)i;
+      p.slots[r.row0 + i] = slot_of(p, r);
+      p.positions[r.row0 + i] = clamp_position(r.pos0 + depth[tid]);
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_pool(const PoolParams& p, cudaStream_t st) {
+  const size_t smem = (2 * (size_t)p.batch + 1) * sizeof(int32_t);
+  cudaError_t e;
+  if (p.cu == nullptr) {
+    // one block where a round of its threads has all entries there can be
+    const bool small = (int64_t)p.batch * p.per_seq <= kSmallEntries;
+    if (small) {
+      if ((e = prepare_kernel(pool_kernel<true, true>, smem)) != cudaSuccess) return e;
+      return launch_pdl(pool_kernel<true, true>, dim3(1), kThreads, smem, st, p);
+    }
+    if ((e = prepare_kernel(pool_kernel<true, false>, smem)) != cudaSuccess) return e;
+    return launch_clusters(pool_kernel<true, false>, kBlocks, dim3(kBlocks), kThreads, smem, st, p);
+  }
+  if (p.rows <= kSmallRows) {
+    if ((e = prepare_kernel(pool_kernel<false, true>, smem)) != cudaSuccess) return e;
+    return launch_pdl(pool_kernel<false, true>, dim3(1), kThreads, smem, st, p);
+  }
+  if ((e = prepare_kernel(pool_kernel<false, false>, smem)) != cudaSuccess) return e;
+  if ((e = launch_clusters(pool_kernel<false, false>, kBlocks, dim3(kBlocks), kThreads, smem, st, p)) != cudaSuccess) return e;
+  if (p.parents != nullptr) return launch_pdl(pool_tree_kernel, dim3((unsigned)p.batch + 1), kThreads, 0, st, p);
+  return launch_pdl(pool_rows_kernel, dim3((unsigned)((p.rows + kRowThreads - 1) / kRowThreads)), kRowThreads, 0, st, p);
+}
+
+}  // namespace moba

@@ -279,7 +279,73 @@ cudaError_t launch_rows(bool load, const PagedParams& p, RowArgs a, cudaStream_t
   return launch_pdl(!many ? pick_row_kernel<1>(load, p) : load ? pick_row_kernel<kManyLoad>(load, p) : pick_row_kernel<kManyStore>(load, p), dim3((unsigned)blocks), kRowThreads, 0, st, p, a);
 }
 
+// Rows path[0] < path[1] < .. of a sequence's packed ones go to its places 0, 1, ...  A thread has 16 bytes of a head's rows (or their bytes of scale), from
+// the first row of the path to the last, several loads ahead of the stores: row j is written when path[0 .. j], which may lie there, have been read,
+// and no thread touches another's bytes.  Bound by the chain path -> page -> row -> store.
+constexpr int kKeepThreads = 128, kKeepAhead = 8;
+template <bool kCodes>
+__global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedParams p, const KeepArgs a, int pieces) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t at = (int64_t)blockIdx.x * kKeepThreads + threadIdx.x;
+  const int piece = (int)(at % pieces);
+  int64_t rest = at / pieces;
+  const int h = (int)(rest % p.Hkv);
+  rest /= p.Hkv;
+  const bool is_v = rest & 1;
+  const int64_t b = rest >> 1;
+  if (b >= p.B) return;
+  const int64_t n = max((int64_t)__ldg(p.cu + b + 1) - __ldg(p.cu + b), (int64_t)0), base = (int64_t)__ldg(p.lens + b) - n;
+  const int most = (int)min((int64_t)min(max(__ldg(a.count + b), 0), a.columns), n);
+  const int32_t* path = a.path + b * a.path_stride;
+  const bool is_scale = kCodes && piece == pieces - 1;
+  uint8_t* pool = is_scale ? (is_v ? a.vs : a.ks) : static_cast<uint8_t*>(is_v ? a.vp : a.kp);
+  constexpr int kSize = kCodes ? 1 : 2;
+  auto place = [&](int64_t pos) -> int64_t {                // offset of this thread's bytes of a position, -1: it has no page
+    if (pos < 0 || pos > 0x7fffffff) return -1;
+    const int page = paged_page(p, (int)b, (int)pos), slot = (int)pos & ((1 << p.page_shift) - 1);
+    if (page < 0) return -1;
+    if (is_scale) return (((int64_t)page * p.Hkv + h) << p.page_shift) + slot;
+    return (is_v ? page * p.vp_p + slot * p.vp_t + h * p.vp_h : page * p.kp_p + slot * p.kp_t + h * p.kp_h) * kSize + 16 * piece;
+  };
+  int kept = 0, before = -1;
+  bool good = true;
+  while (good && kept < most) {
+    uint4 x[kKeepAhead];
+    int64_t to[kKeepAhead];
+    int got = 0;
+#pragma unroll
+    for (int i = 0; i < kKeepAhead; ++i) {
+      to[i] = -1;
+      if (!good || kept + i >= most) continue;
+      const int row = __ldg(path + kept + i);
+      if (row <= before || row >= n) { good = false; continue; }   // (no branch: the rows up to here are one)
+      before = row;
+      ++got;
+      if (row == kept + i) continue;
+      const int64_t from = place(base + row);
+      to[i] = from < 0 ? -1 : place(base + kept + i);
+      if (to[i] < 0) continue;
+      if (is_scale) x[i].x = pool[from]; else x[i] = *reinterpret_cast<const uint4*>(pool + from);
+    }
+#pragma unroll
+    for (int i = 0; i < kKeepAhead; ++i) {
+      if (to[i] < 0) continue;
+      if (is_scale) pool[to[i]] = (uint8_t)x[i].x; else *reinterpret_cast<uint4*>(pool + to[i]) = x[i];
+    }
+    kept += got;
+  }
+  if (piece == 0 && h == 0 && !is_v) a.lens_out[b] = (int32_t)min(max(base + kept, -((int64_t)1 << 31)), ((int64_t)1 << 31) - 1);
+}
+
 }  // namespace
+
+cudaError_t launch_paged_keep(const PagedParams& p, const KeepArgs& a, cudaStream_t st) {
+  const bool codes = p.store != MOBA_STORE_SAME;
+  const int pieces = p.D * (codes ? 1 : 2) / 16 + (codes ? 1 : 0);
+  const int64_t threads = (int64_t)p.B * 2 * p.Hkv * pieces, blocks = (threads + kKeepThreads - 1) / kKeepThreads;
+  return launch_pdl(codes ? paged_keep_kernel<true> : paged_keep_kernel<false>, dim3((unsigned)blocks), kKeepThreads, 0, st, p, a, pieces);
+}
 
 cudaError_t launch_paged_store(const PagedParams& p, const void* k, const void* v, void* kp, void* vp, uint8_t* ks, uint8_t* vs,
                                cudaStream_t st) {

@@ -22,6 +22,7 @@ struct PagedParams {
   const int32_t* cu;
   const int32_t* lens;
   const int32_t* table;
+  const int32_t* parents;                  // of the packed rows, within their sequences; null: each row sees all before it
 };
 
 // A sequence of the batch: its packed rows [row0, row0 + n), of which row i is at position pos0 + i.  Numbers that make no
@@ -49,6 +50,19 @@ __device__ __forceinline__ int paged_page(const PagedParams& p, int b, int pos) 
   return (unsigned)id < (unsigned)p.pages ? id : -1;
 }
 
+// Which of the 32 keys from `key0` on row i of a sequence sees, of which `up` are the parents of its rows: those in front of the packed rows, the
+// row's own and its ancestors'.  A parent is an earlier row (anything else is none), so that the walk ends; it stops below the keys in question.
+__device__ __forceinline__ uint32_t tree_keys(const int32_t* up, int i, int pos0, int key0) {
+  const int64_t front = (int64_t)pos0 - key0;
+  uint32_t see = front <= 0 ? 0u : front >= 32 ? 0xffffffffu : (1u << (int)front) - 1u;
+  for (int j = i; j >= 0 && front + j >= 0;) {
+    if (front + j < 32) see |= 1u << (int)(front + j);
+    const int parent = __ldg(up + j);
+    j = parent < j ? parent : -1;
+  }
+  return see;
+}
+
 // The least power of two of a row: 2^-96, so that the inverses of a million rows' add up within fp32.
 constexpr int kPagedLeastByte = 127 - 96;
 __device__ __forceinline__ float paged_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
@@ -57,6 +71,17 @@ cudaError_t launch_paged_store(const PagedParams& p, const void* k, const void* 
                                cudaStream_t st);
 cudaError_t launch_paged_load(const PagedParams& p, const void* kp, const void* vp, const uint8_t* ks, const uint8_t* vs, void* k,
                               void* v, cudaStream_t st);
+
+// Rows of an accepted branch moved together.
+struct KeepArgs {
+  void *kp, *vp;
+  uint8_t *ks, *vs;
+  const int32_t *path, *count;             // [batch][columns], rows `path_stride` apart; [batch]
+  int64_t path_stride;
+  int columns;
+  int32_t* lens_out;
+};
+cudaError_t launch_paged_keep(const PagedParams& p, const KeepArgs& a, cudaStream_t st);
 
 // Sequences that one launch of an attention kernel takes: their work is added up in shared memory.
 constexpr int kPagedBatch = 1024;
@@ -80,11 +105,16 @@ inline bool paged_few_rows(const PagedParams& p) {
   return (int64_t)p.max_new * p.G <= most;
 }
 
+// Both kernels have a form for trees of drafted tokens (PagedParams::parents), each in a source file of its own.
 size_t paged_rows_workspace(const PagedParams& p);
 cudaError_t launch_paged_rows(const PagedParams& p, const void* q, const void* kp, const void* vp, const uint8_t* ks,
                               const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st);
 size_t paged_few_workspace(const PagedParams& p);
 cudaError_t launch_paged_few(const PagedParams& p, const void* q, const void* kp, const void* vp, const uint8_t* ks,
                              const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st);
+cudaError_t launch_paged_rows_tree(const PagedParams& p, const void* q, const void* kp, const void* vp, const uint8_t* ks,
+                                   const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st);
+cudaError_t launch_paged_few_tree(const PagedParams& p, const void* q, const void* kp, const void* vp, const uint8_t* ks,
+                                  const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st);
 
 }  // namespace moba

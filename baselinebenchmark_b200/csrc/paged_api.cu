@@ -1,4 +1,5 @@
 // C ABI of the paged keys and values (declared in include/moba_b200.h): argument checks and launches.  Host-side only.
+#include "page_pool.cuh"
 #include "paged.cuh"
 
 using namespace moba;
@@ -60,6 +61,7 @@ PagedParams paged_params(const moba_paged_t* p, const int32_t* cu, const int32_t
   r.cu = cu;
   r.lens = lens;
   r.table = table;
+  r.parents = nullptr;
   return r;
 }
 
@@ -116,15 +118,92 @@ int moba_paged_workspace_size(const moba_paged_t* p, size_t* bytes) {
 int moba_paged_attention(const moba_paged_t* p, const void* q, const int32_t* cu, const int32_t* lens, const int32_t* table,
                          const void* kp, const void* vp, const uint8_t* ks, const uint8_t* vs, void* out, float* lse_out,
                          void* workspace, size_t workspace_bytes, void* stream) {
+  return moba_paged_tree_attention(p, q, nullptr, cu, lens, table, kp, vp, ks, vs, out, lse_out, workspace, workspace_bytes, stream);
+}
+
+int moba_paged_tree_attention(const moba_paged_t* p, const void* q, const int32_t* parents, const int32_t* cu, const int32_t* lens,
+                              const int32_t* table, const void* kp, const void* vp, const uint8_t* ks, const uint8_t* vs, void* out,
+                              float* lse_out, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_paged(p);
   if (rc == MOBA_OK) rc = check_pointers(p, q, out, cu, lens, table, kp, vp, ks, vs);
   if (rc != MOBA_OK) return rc;
   if (!apart(p, p->o_stride_token, p->o_stride_head, p->num_q_heads)) return MOBA_E_SHAPE;
-  if ((uintptr_t)lse_out & 3) return MOBA_E_ALIGN;
-  const PagedParams r = paged_params(p, cu, lens, table);
+  if (((uintptr_t)lse_out | (uintptr_t)parents) & 3) return MOBA_E_ALIGN;
+  PagedParams r = paged_params(p, cu, lens, table);
+  r.parents = parents;
   if (workspace == nullptr || workspace_bytes < workspace_of(r)) return MOBA_E_WORKSPACE;
   if ((uintptr_t)workspace & 31) return MOBA_E_ALIGN;
-  return (int)(paged_few_rows(r) ? launch_paged_few : launch_paged_rows)(r, q, kp, vp, ks, vs, out, lse_out, workspace, (cudaStream_t)stream);
+  const auto launch = paged_few_rows(r) ? (parents ? launch_paged_few_tree : launch_paged_few) : parents ? launch_paged_rows_tree : launch_paged_rows;
+  return (int)launch(r, q, kp, vp, ks, vs, out, lse_out, workspace, (cudaStream_t)stream);
+}
+
+int moba_paged_keep(const moba_paged_t* p, const int32_t* cu, const int32_t* lens, const int32_t* table, const int32_t* path,
+                    int64_t path_stride, int32_t path_columns, const int32_t* count, void* kp, void* vp, uint8_t* ks, uint8_t* vs,
+                    int32_t* lens_out, void* stream) {
+  int rc = check_paged(p);
+  if (rc == MOBA_OK) rc = check_pointers(p, kp, vp, cu, lens, table, kp, vp, ks, vs);
+  if (rc != MOBA_OK) return rc;
+  if (!path || !count || !lens_out) return MOBA_E_NULL;
+  if (((uintptr_t)path | (uintptr_t)count | (uintptr_t)lens_out) & 3) return MOBA_E_ALIGN;
+  if (path_columns <= 0 || path_stride < (p->batch > 1 ? path_columns : 0)) return MOBA_E_SHAPE;
+  if ((int64_t)p->batch * p->num_kv_heads >= ((int64_t)1 << 31)) return MOBA_E_UNSUPPORTED;
+  const KeepArgs a{kp, vp, ks, vs, path, count, path_stride, path_columns, lens_out};
+  return (int)launch_paged_keep(paged_params(p, cu, lens, table), a, (cudaStream_t)stream);
+}
+
+static int check_pool(const moba_page_pool_t* p) {
+  if (p == nullptr) return MOBA_E_NULL;
+  if (p->batch <= 0 || p->pages_per_seq <= 0 || p->num_pages <= 0 || p->page_size <= 0 || p->total_tokens < 0) return MOBA_E_SHAPE;
+  if (p->page_size < 16 || (p->page_size & (p->page_size - 1)) != 0 || p->reserved != 0) return MOBA_E_UNSUPPORTED;
+  if (p->batch > kPoolMostBatch || p->total_tokens >= ((int64_t)1 << 31)) return MOBA_E_UNSUPPORTED;
+  if ((int64_t)p->batch * p->pages_per_seq >= ((int64_t)1 << 31) || (int64_t)p->pages_per_seq * p->page_size >= ((int64_t)1 << 30))
+    return MOBA_E_UNSUPPORTED;
+  if (p->table_stride < (p->batch > 1 ? p->pages_per_seq : 0)) return MOBA_E_SHAPE;
+  return MOBA_OK;
+}
+static PoolParams pool_params(const moba_page_pool_t* p, const int32_t* lens, int32_t* table, int32_t* free_pages, int32_t* free_count) {
+  PoolParams r{};
+  r.rows = p->total_tokens;
+  r.table_stride = p->table_stride;
+  r.batch = p->batch;
+  r.per_seq = p->pages_per_seq;
+  while ((1 << r.page_shift) < p->page_size) ++r.page_shift;
+  r.pages = p->num_pages;
+  r.lens = lens;
+  r.table = table;
+  r.free = free_pages;
+  r.count = free_count;
+  return r;
+}
+
+int moba_page_pool_check(const moba_page_pool_t* p) { return check_pool(p); }
+
+int moba_paged_reserve(const moba_page_pool_t* p, const int32_t* cu, const int32_t* lens, const int32_t* parents, int32_t* table,
+                       int32_t* free_pages, int32_t* free_count, int64_t* slots, int32_t* positions, int32_t* missing, void* stream) {
+  const int rc = check_pool(p);
+  if (rc != MOBA_OK) return rc;
+  if (!cu || !lens || !table || !free_pages || !free_count || !missing) return MOBA_E_NULL;
+  if (p->total_tokens > 0 && (!slots || !positions)) return MOBA_E_NULL;
+  if (((uintptr_t)cu | (uintptr_t)lens | (uintptr_t)parents | (uintptr_t)table | (uintptr_t)free_pages | (uintptr_t)free_count |
+       (uintptr_t)positions | (uintptr_t)missing) & 3)
+    return MOBA_E_ALIGN;
+  if ((uintptr_t)slots & 7) return MOBA_E_ALIGN;
+  PoolParams r = pool_params(p, lens, table, free_pages, free_count);
+  r.cu = cu;
+  r.parents = parents;
+  r.slots = reinterpret_cast<long long*>(slots);
+  r.positions = positions;
+  r.missing = missing;
+  return (int)launch_pool(r, (cudaStream_t)stream);
+}
+
+int moba_paged_release(const moba_page_pool_t* p, const int32_t* keep_lens, int32_t* table, int32_t* free_pages, int32_t* free_count,
+                       void* stream) {
+  const int rc = check_pool(p);
+  if (rc != MOBA_OK) return rc;
+  if (!keep_lens || !table || !free_pages || !free_count) return MOBA_E_NULL;
+  if (((uintptr_t)keep_lens | (uintptr_t)table | (uintptr_t)free_pages | (uintptr_t)free_count) & 3) return MOBA_E_ALIGN;
+  return (int)launch_pool(pool_params(p, keep_lens, table, free_pages, free_count), (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,95 @@
+"""Drafted tokens checked against the target's probabilities.
+
+A server that drafts tokens attends to a tree of them in one call (`paged_attention` with `parents`), has the target's probabilities behind each of its rows
+from that, and keeps a branch of it such that the tokens are distributed as the target's own.  No counterpart in the reference, which
+samples nothing.  include/moba_b200.h has the rules in full.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .paged import _check_not_followed, _check_parents, _i32_rows, _run_on
+
+__all__ = ["verify_drafts"]
+
+_DTYPES = {torch.float32: _lib.DTYPE_FP32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
+
+
+def _check_drafts(target, draft, tokens, cu_seqlens, accept, sample, max_new) -> None:
+    if target.ndim != 2 or target.shape[1] == 0:
+        raise ValueError(f"target must have shape [tokens, vocabulary], got {tuple(target.shape)}")
+    if target.dtype not in _DTYPES:
+        raise TypeError(f"probabilities are float32, bfloat16 or float16, got {target.dtype}")
+    index = target.get_device()
+    if index < 0:
+        raise ValueError("target must be an accelerator tensor")
+    rows = target.shape[0]
+    for name, x in (("target", target), ("draft", draft)):
+        if x is None:
+            continue
+        if x.shape != target.shape:
+            raise ValueError(f"draft must have the shape of target, {tuple(target.shape)}, got {tuple(x.shape)}")
+        if x.dtype != target.dtype or x.get_device() != index:
+            raise TypeError("draft must have target's dtype and device")
+        if x.stride(1) != 1 and x.shape[1] > 1:
+            raise NotImplementedError(f"{name} must be contiguous in its last dimension")
+    if tokens.shape != (rows,):
+        raise ValueError(f"tokens must have shape [{rows}], got {tuple(tokens.shape)}")
+    if tokens.dtype not in (torch.int32, torch.int64) or tokens.get_device() != index:
+        raise TypeError("tokens must be an int32 or int64 tensor on target's device")
+    if cu_seqlens.ndim != 1 or cu_seqlens.numel() < 2:
+        raise ValueError("cu_seqlens must be a one-dimensional tensor of length >= 2")
+    _i32_rows("cu_seqlens", cu_seqlens, cu_seqlens.shape, index)
+    for name, x, shape in (("accept", accept, (rows,)), ("sample", sample, (cu_seqlens.numel() - 1,))):
+        if x.shape != shape:
+            raise ValueError(f"{name} must have shape {list(shape)}, got {list(x.shape)}")
+        if x.dtype != torch.float32 or x.get_device() != index:
+            raise TypeError(f"{name} must be a float32 tensor on target's device")
+    for name, x in (("tokens", tokens), ("accept", accept), ("sample", sample)):
+        if x.shape[0] > 1 and x.stride(0) != 1:
+            raise NotImplementedError(f"{name} must be contiguous")
+    if not isinstance(max_new, int) or max_new <= 0:
+        raise ValueError(f"max_new must be a positive int, got {max_new}")
+    if max_new > 1024:
+        raise NotImplementedError(f"at most 1024 packed tokens of a sequence, got max_new = {max_new}")
+    if target.shape[1] > 2 ** 22:
+        raise NotImplementedError(f"vocabularies of at most 2**22 tokens, got {target.shape[1]}")
+
+
+def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: torch.Tensor, cu_seqlens: torch.Tensor,
+                  accept: torch.Tensor, sample: torch.Tensor, max_new: int, *,
+                  parents: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Which drafted tokens stand, and the token behind them.  The packed rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 are a tree (`parents` as
+    in `paged_attention`; without it each row follows the one before): row 0 is the last accepted token, the others are drafted ones.
+
+    `target`, `draft` [T, V] (float32, bfloat16 or float16): the target's and the draft's probabilities of the token behind each row; a row's children
+    were drawn from its `draft` one by one.  draft = None: children are given tokens, such as the draft's likeliest.  `tokens` [T] int32 or int64,
+    `accept` [T] and `sample` [batch] float32: random numbers from [0, 1), for each drafted row and each sequence.  `max_new`: the most rows of a
+    sequence, at most 1024; rows beyond are not looked at.
+
+    A child with token x of row r is accepted where accept * draft[r, x] < target[r, x]; after one that is not, its siblings are tried against what is
+    left, max(target[r] - draft[r], 0) over its sum (draft = None: target[r] without x over its sum), and so on; the walk goes on from an accepted one.
+    The next token is drawn from what is left of the last row's target by `sample`.
+
+    Returns (path, count, next): path int32 [batch, max_new], the accepted rows counted from the sequence's first (row 0 among them), -1 behind
+    them; count int32 [batch]; next [batch] of tokens' dtype.  A sequence without rows has 0 and -1; a next token of -1 else means that the row's
+    probabilities are all zeros.  Computed in 64 bits; values that are not above 0 and finite count as 0."""
+    _check_drafts(target, draft, tokens, cu_seqlens, accept, sample, max_new)
+    index, rows, batch = target.get_device(), target.shape[0], cu_seqlens.numel() - 1
+    if parents is not None:
+        _check_parents(parents, rows, index)
+    _check_not_followed(target=target, draft=draft, accept=accept, sample=sample)
+    path = cu_seqlens.new_empty((batch, max_new))
+    count, token = cu_seqlens.new_empty(batch), tokens.new_empty(batch)
+    if rows == 0:
+        return path.fill_(-1), count.zero_(), token.fill_(-1)
+    call = _lib.Drafts(rows, target.shape[1], batch, max_new, _DTYPES[target.dtype], 64 if tokens.dtype == torch.int64 else 32,
+                       target.stride(0) if rows > 1 else 0, draft.stride(0) if draft is not None and rows > 1 else 0, 0)
+    _run_on(index, _lib.lib().moba_verify_drafts, C.byref(call), target.data_ptr(), draft.data_ptr() if draft is not None else None,
+            tokens.data_ptr(), cu_seqlens.data_ptr(), parents.data_ptr() if parents is not None else None, accept.data_ptr(),
+            sample.data_ptr(), path.data_ptr(), count.data_ptr(), token.data_ptr())
+    return path, count, token

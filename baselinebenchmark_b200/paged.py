@@ -27,7 +27,7 @@ import torch.autograd.forward_ad as forward_ad
 from . import _lib
 from .parallel import HEAD_DIMS, _workspace
 
-__all__ = ["PagedKV", "paged_store", "paged_load", "paged_attention", "paged_append"]
+__all__ = ["PagedKV", "PagePool", "paged_store", "paged_load", "paged_attention", "paged_append", "paged_keep", "paged_reserve", "paged_release"]
 
 _STORES = {torch.float8_e4m3fn: _lib.STORE_E4M3, torch.int8: _lib.STORE_INT8}
 _ROWS = (torch.float16, torch.bfloat16)
@@ -268,12 +268,24 @@ def _check_attention(q, k_pages, max_new, scale, out) -> None:
         raise TypeError(f"out must be of {q.dtype}, got {out.dtype}")
 
 
-def _attention(g: _Pages, q, kv, k_pages, v_pages, max_new, scale, return_lse, out, written=()):
+def _check_parents(parents, tokens: int, index: int) -> None:
+    """`parents` of the packed rows, on device number `index`."""
+    if parents.ndim != 1 or parents.shape[0] != tokens:
+        raise ValueError(f"parents must have shape [{tokens}], got {tuple(parents.shape)}")
+    if parents.dtype != torch.int32 or parents.get_device() != index:
+        raise TypeError("parents must be an int32 tensor on the device of the call's other tensors")
+    if tokens > 1 and parents.stride(0) != 1:
+        raise NotImplementedError("parents must be contiguous")
+
+
+def _attention(g: _Pages, q, kv, k_pages, v_pages, max_new, scale, return_lse, out, parents, written=()):
     """Attention of q; with `kv` the rows of k and v are stored first, in the tensors of `written`."""
     _check_not_followed(q=q, k=kv and kv[0], v=kv and kv[1], k_pages=k_pages, v_pages=v_pages, out=out)
     qs = _rows("q", q, g, None, None, k_pages)
     tokens, heads, _ = q.shape
     _check_attention(q, k_pages, max_new, scale, out)
+    if parents is not None:
+        _check_parents(parents, tokens, g.index)
     dtype, given, ks, vs = q.dtype, out is not None, (0, 0), (0, 0)
     if given:
         os = _rows("out", out, g, heads, tokens, k_pages)
@@ -301,7 +313,7 @@ def _attention(g: _Pages, q, kv, k_pages, v_pages, max_new, scale, return_lse, o
                 _lib.check(_lib.E_SHAPE)
             g.run(lib.moba_paged_store, prob, k.data_ptr(), v.data_ptr(), *g.where)
             _written(*written)
-        g.run(lib.moba_paged_attention, prob, q.data_ptr(), *g.where, out.data_ptr(), None if lse is None else lse.data_ptr(),
+        g.run(lib.moba_paged_tree_attention, prob, q.data_ptr(), None if parents is None else parents.data_ptr(), *g.where, out.data_ptr(), None if lse is None else lse.data_ptr(),
               ws.data_ptr(), need.value)
         if given:
             _written(out)
@@ -311,7 +323,7 @@ def _attention(g: _Pages, q, kv, k_pages, v_pages, max_new, scale, return_lse, o
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                     cu_seqlens: torch.Tensor, seq_lens: torch.Tensor, max_new: int, *, scale: Optional[float] = None,
                     k_scales: Optional[torch.Tensor] = None, v_scales: Optional[torch.Tensor] = None,
-                    return_lse: bool = False, out: Optional[torch.Tensor] = None):
+                    return_lse: bool = False, out: Optional[torch.Tensor] = None, parents: Optional[torch.Tensor] = None):
     """Causal softmax attention of the packed new tokens q [T, Hq, D] over the pages of their sequences: every token sees the
     positions of its sequence up to its own, which the pages hold already (`paged_append` writes them first).  One token a sequence
     is a decode step, a few are drafted tokens, many a block of a prompt; a batch may mix them.
@@ -320,19 +332,152 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     factor of the scores, head_dim ** -0.5 unless given.  Returns out [T, Hq, D], with `return_lse` (out, lse [Hq, T] fp32, natural
     log).  A token that sees nothing is zeros and -inf.  `out`: a tensor to write to; rows behind the last sequence are left as
     they were (undefined without it).  8-bit pages are attended to as the rows that `paged_load` gives in the queries' dtype,
-    whichever they were written from: a value beyond float16 is an infinity to float16 queries."""
+    whichever they were written from: a value beyond float16 is an infinity to float16 queries.
+
+    `parents` [T] int32: the packed tokens are trees of drafted ones.  parents[row] is the row of the same sequence, counted from its
+    first packed one, that the token follows; what is not an earlier row (-1) is none.  A token then sees the tokens in front of
+    the packed ones, its ancestors and itself.  Rows keep their places in the pages, whatever branch they are of."""
     g = _Pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
-    return _attention(g, q, None, k_pages, v_pages, max_new, scale, return_lse, out)
+    return _attention(g, q, None, k_pages, v_pages, max_new, scale, return_lse, out, parents)
 
 
 def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                  page_table: torch.Tensor, cu_seqlens: torch.Tensor, seq_lens: torch.Tensor, max_new: int, *,
                  scale: Optional[float] = None, k_scales: Optional[torch.Tensor] = None,
-                 v_scales: Optional[torch.Tensor] = None, return_lse: bool = False, out: Optional[torch.Tensor] = None):
+                 v_scales: Optional[torch.Tensor] = None, return_lse: bool = False, out: Optional[torch.Tensor] = None,
+                 parents: Optional[torch.Tensor] = None):
     """`paged_store` of the new tokens' k and v, then `paged_attention` of their q: a layer's step of a server."""
     g = _Pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
     _check_written(k_pages, v_pages, k_scales, v_scales)
-    return _attention(g, q, (k, v), k_pages, v_pages, max_new, scale, return_lse, out, (k_pages, v_pages, k_scales, v_scales))
+    return _attention(g, q, (k, v), k_pages, v_pages, max_new, scale, return_lse, out, parents, (k_pages, v_pages, k_scales, v_scales))
+
+
+def _i32_rows(name, x, shape, index) -> None:
+    """An int32 tensor of this shape, contiguous in its last dimension, on device number `index`."""
+    if x.shape != shape:
+        raise ValueError(f"{name} must have shape {list(shape)}, got {list(x.shape)}")
+    if x.dtype != torch.int32 or x.get_device() != index:
+        raise TypeError(f"{name} must be an int32 tensor on the device of the call's other tensors")
+    if x.stride(-1) != 1 and shape[-1] > 1:
+        raise NotImplementedError(f"{name} must be contiguous in its last dimension")
+
+
+def paged_keep(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor, seq_lens: torch.Tensor,
+               path: torch.Tensor, count: torch.Tensor, *, k_scales: Optional[torch.Tensor] = None,
+               v_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Moves the rows of an accepted branch together: of the packed tokens of sequence b, which the pages hold, rows path[b, 0] < path[b, 1]
+    < .. (count[b] of them; `verify_drafts` gives both) go to the places of rows 0, 1, ..  Returns the sequences' lengths then, int32 [batch]: the tokens in
+    front of the packed ones and the kept ones; what is behind them is no longer the sequence's.  8-bit rows are moved as they are, with
+    their powers of two.  A path ends in front of an entry that is no later row of the sequence than the one before it.  Each layer's pages are
+    moved with the same seq_lens, those with the drafted tokens."""
+    g = _Pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
+    if path.ndim != 2 or path.shape[1] == 0:
+        raise ValueError(f"path must have shape [{g.batch}, rows], got {tuple(path.shape)}")
+    _i32_rows("path", path, (g.batch, path.shape[1]), g.index)
+    _i32_rows("count", count, (g.batch,), g.index)
+    _check_written(k_pages, v_pages, k_scales, v_scales)
+    _check_not_followed(k_pages=k_pages, v_pages=v_pages)
+    lens = torch.empty_like(seq_lens, memory_format=torch.contiguous_format)
+    dtype = g.dtype if g.store == _lib.STORE_SAME else torch.bfloat16
+    cu, old, table, k, v, ks, vs = g.where
+    columns = path.shape[1]
+    g.run(_lib.lib().moba_paged_keep, g.pack(1, g.shape[2], 1, dtype, 0.0), cu, old, table, path.data_ptr(),
+          path.stride(0) if g.batch > 1 else columns, columns, count.data_ptr(), k, v, ks, vs, lens.data_ptr())
+    _written(k_pages, v_pages, k_scales, v_scales)
+    return lens
+
+
+def _pool_call(page_table, free_pages, free_count, page_size, total_tokens, lens_name, lens) -> Tuple[_lib.PagePool, int]:
+    """The structure of a call on a pool, with its tensors checked, and their device's number."""
+    index = page_table.get_device()
+    if index < 0:
+        raise ValueError("page_table must be an accelerator tensor")
+    if page_table.ndim != 2 or 0 in page_table.shape:
+        raise ValueError(f"page_table must have shape [batch, pages of a sequence], got {tuple(page_table.shape)}")
+    if free_pages.ndim != 1 or free_pages.shape[0] == 0:
+        raise ValueError(f"free_pages must have shape [pages], got {tuple(free_pages.shape)}")
+    if not isinstance(page_size, int) or page_size <= 0:
+        raise ValueError(f"page_size must be a positive int, got {page_size}")
+    if page_size < 16 or page_size & (page_size - 1):
+        raise NotImplementedError(f"page_size must be a power of two and at least 16, got {page_size}")
+    batch, per_seq = page_table.shape
+    _i32_rows("page_table", page_table, page_table.shape, index)
+    _i32_rows("free_pages", free_pages, free_pages.shape, index)
+    _i32_rows("free_count", free_count, (1,), index)
+    _i32_rows(lens_name, lens, (batch,), index)
+    if batch > 1 and page_table.stride(0) < per_seq:
+        raise ValueError("rows of page_table must not lie on one another")
+    if not isinstance(total_tokens, int) or total_tokens < 0:
+        raise ValueError(f"total_tokens must be an int that is not negative, got {total_tokens}")
+    if max(free_pages.shape[0], per_seq, page_size, batch) >= 2 ** 31:
+        raise NotImplementedError("pages, columns of the table and sequences are counted in 32 bits")
+    _check_written(page_table, free_pages, free_count)
+    return _lib.PagePool(total_tokens, batch, per_seq, free_pages.shape[0], page_size, page_table.stride(0) if batch > 1 else per_seq, 0), index
+
+
+def _run_on(index: int, call, *args) -> None:
+    """`call(*args, stream)` with device number `index` current."""
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            _lib.check(call(*args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        _lib.check(call(*args, torch._C._cuda_getCurrentRawStream(index)))
+
+
+def paged_reserve(page_table: torch.Tensor, cu_seqlens: torch.Tensor, seq_lens: torch.Tensor, free_pages: torch.Tensor,
+                  free_count: torch.Tensor, page_size: int, total_tokens: int, *,
+                  parents: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Pages for the packed tokens of a call, and where they lie.  Every entry of the tables that a packed token's position is in and that is no
+    page's number gets one from the stack of free pages (free_pages int32 [pages], of which the first free_count, int32 [1], are free ones; the last
+    is taken first), in the order of the sequences and entries.  The table, the stack and its count are written.
+
+    Returns (slots, positions, missing): slots int64 [total_tokens], page * page_size + place of each packed row, -1 where it has no page;
+    positions int32 [total_tokens], as `rotary` takes them, with `parents` (see `paged_attention`) those of a row's depth in its tree; missing int32
+    [1], the entries for which no page was left.  Rows of no sequence have -1 in both.  Calls on one pool are ordered by the caller's
+    streams.  At most 16384 sequences."""
+    call, index = _pool_call(page_table, free_pages, free_count, page_size, total_tokens, "seq_lens", seq_lens)
+    _i32_rows("cu_seqlens", cu_seqlens, (call.batch + 1,), index)
+    if parents is not None:
+        _check_parents(parents, total_tokens, index)
+    slots = page_table.new_empty(total_tokens, dtype=torch.int64)
+    positions, missing = page_table.new_empty(total_tokens), page_table.new_empty(1)
+    _run_on(index, _lib.lib().moba_paged_reserve, C.byref(call), cu_seqlens.data_ptr(), seq_lens.data_ptr(),
+            parents.data_ptr() if parents is not None else None, page_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
+            slots.data_ptr(), positions.data_ptr(), missing.data_ptr())
+    _written(page_table, free_pages, free_count)
+    return slots, positions, missing
+
+
+def paged_release(page_table: torch.Tensor, keep_lens: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
+                  page_size: int) -> None:
+    """Gives pages back: those behind the first keep_lens[b] (int32) tokens of sequence b, all of them for 0, go to the stack of free pages and
+    their entries become -1.  The other way round of `paged_reserve`: what one call took, a release leaves as it was.  Pages that other
+    sequences share must not be given back."""
+    call, index = _pool_call(page_table, free_pages, free_count, page_size, 0, "keep_lens", keep_lens)
+    _run_on(index, _lib.lib().moba_paged_release, C.byref(call), keep_lens.data_ptr(), page_table.data_ptr(), free_pages.data_ptr(),
+            free_count.data_ptr())
+    _written(page_table, free_pages, free_count)
+
+
+class PagePool:
+    """The free pages of a `PagedKV` (of all layers' caches, which share one page table): `free_pages` int32 [num_pages], the stack of their
+    numbers, and `free_count` int32 [1].  All are free at first."""
+
+    def __init__(self, num_pages: int, page_size: int, device: Optional[torch.device] = None):
+        if num_pages <= 0:
+            raise ValueError(f"num_pages must be positive, got {num_pages}")
+        if page_size < 16 or page_size & (page_size - 1):
+            raise NotImplementedError(f"page_size must be a power of two and at least 16, got {page_size}")
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        self.page_size = page_size
+        self.free_pages = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device)
+        self.free_count = torch.full((1,), num_pages, dtype=torch.int32, device=device)
+
+    def reserve(self, page_table, cu_seqlens, seq_lens, total_tokens: int, parents=None):
+        return paged_reserve(page_table, cu_seqlens, seq_lens, self.free_pages, self.free_count, self.page_size, total_tokens, parents=parents)
+
+    def release(self, page_table, keep_lens) -> None:
+        paged_release(page_table, keep_lens, self.free_pages, self.free_count, self.page_size)
 
 
 class PagedKV:
@@ -376,3 +521,6 @@ class PagedKV:
 
     def append(self, q, k, v, page_table, cu_seqlens, seq_lens, max_new: int, **options):
         return paged_append(q, k, v, self.k, self.v, page_table, cu_seqlens, seq_lens, max_new, **self._scales(), **options)
+
+    def keep(self, page_table, cu_seqlens, seq_lens, path, count):
+        return paged_keep(self.k, self.v, page_table, cu_seqlens, seq_lens, path, count, **self._scales())

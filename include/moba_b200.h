@@ -57,7 +57,8 @@ enum {
  * reference's suite runs bf16 and fp16, moba_compare.py:56, :69-71). */
 enum {
   MOBA_DTYPE_BF16 = 0,
-  MOBA_DTYPE_FP16 = 1
+  MOBA_DTYPE_FP16 = 1,
+  MOBA_DTYPE_FP32 = 2       /* of probabilities only: moba_verify_drafts */
 };
 
 /* Problem description.  Mirrors the arguments of parallel_moba
@@ -440,6 +441,91 @@ int moba_paged_attention(const moba_paged_t* p, const void* q, const int32_t* cu
                          const int32_t* page_table, const void* k_pages, const void* v_pages, const uint8_t* k_scales,
                          const uint8_t* v_scales, void* out, float* lse_out, void* workspace, size_t workspace_bytes,
                          void* stream);
+/* The same for packed rows that are trees of drafted tokens.  parents: int32[total_tokens] on the device; parents[cu[b] + i] is the row of
+ * sequence b, counted from cu[b], that row i follows.  A row sees the positions in front of the sequence's packed rows, its own and those of its
+ * ancestors; a parent that is not in 0 .. i-1 is none.  Positions of the table are by row, as in every call: the branches lie one behind
+ * another in the pages.  parents == NULL: moba_paged_attention. */
+int moba_paged_tree_attention(const moba_paged_t* p, const void* q, const int32_t* parents, const int32_t* cu_seqlens,
+                              const int32_t* seq_lens, const int32_t* page_table, const void* k_pages, const void* v_pages,
+                              const uint8_t* k_scales, const uint8_t* v_scales, void* out, float* lse_out, void* workspace,
+                              size_t workspace_bytes, void* stream);
+/* The rows of an accepted branch moved together.  path: int32[batch][path_columns], rows `path_stride` apart, and count: int32[batch], on
+ * the device: of sequence b's packed rows, path[b][0] < path[b][1] < .. < its number are kept, count[b] of them; row path[b][j] of K and V
+ * (bytes of 8-bit rows included) goes to the place of row j.  A path ends in front of an entry that is no later row of the sequence than the one before it.
+ * lens_out: int32[batch] (not seq_lens itself), the sequence's tokens then: those in front of the packed rows and the kept ones.  Rows behind are left as they are; a row whose page, or whose new place's, is not there is not moved.  total_tokens, q_strides,
+ * k_strides and v_strides of the structure are not looked at beyond their checks. */
+int moba_paged_keep(const moba_paged_t* p, const int32_t* cu_seqlens, const int32_t* seq_lens, const int32_t* page_table,
+                    const int32_t* path, int64_t path_stride, int32_t path_columns, const int32_t* count, void* k_pages, void* v_pages,
+                    uint8_t* k_scales, uint8_t* v_scales, int32_t* lens_out, void* stream);
+
+/* ---- pages taken from a pool and given back -----------------------------------------------------
+ *
+ * free_pages int32[num_pages] and free_count int32[1], on the device: a stack of the numbers of free pages, free_pages[free_count - 1] on its top.
+ * page_table as above, written here; an entry outside 0 .. num_pages-1 is no page. */
+typedef struct moba_page_pool {
+  int64_t total_tokens;     /* packed rows (reserve)                                               */
+  int32_t batch, pages_per_seq, num_pages, page_size;   /* at most 16384 sequences; page_size: a power of two, at least 16 */
+  int64_t table_stride;
+  int64_t reserved;         /* must be 0                                                           */
+} moba_page_pool_t;
+int moba_page_pool_check(const moba_page_pool_t* p);
+/* Every entry of the tables that a packed row's position lies in and that has no page gets one, in the order of the sequences and
+ * entries, from the top of the stack; missing (int32[1]): those for which none was left.  slots int64[total_tokens]: page * page_size + slot of each packed row, -1
+ * without a page; positions int32[total_tokens]: the row's position, with `parents` (see moba_paged_tree_attention) the position of its depth: that of
+ * the sequence's first packed row and one for each ancestor.  Rows of no sequence have -1 in both. */
+int moba_paged_reserve(const moba_page_pool_t* p, const int32_t* cu_seqlens, const int32_t* seq_lens, const int32_t* parents,
+                       int32_t* page_table, int32_t* free_pages, int32_t* free_count, int64_t* slots, int32_t* positions,
+                       int32_t* missing, void* stream);
+/* The pages behind the first keep_lens[b] tokens of sequence b (0: all) go back to the stack, and their entries become -1.  They lie there in the
+ * order in which a reserve would take them again: a release of what a reserve took leaves the stack as it was. */
+int moba_paged_release(const moba_page_pool_t* p, const int32_t* keep_lens, int32_t* page_table, int32_t* free_pages, int32_t* free_count,
+                       void* stream);
+
+/* ---- rotary positions -------------------------------------------------------------------------
+ *
+ * Pair j of the first rotary_dim dims of each head, (x, y), becomes magnitude * (x cos a - y sin a, x sin a + y cos a); a is positions[row] times
+ * turns[j] / 2^64 whole turns.  A pair is dims j and j + rotary_dim / 2, interleaved dims 2 j and 2 j + 1.  inverse: the turn by -a, the
+ * operator's gradient.  Other dims, and rows with a position below 0, are copied.  q_out and k_out may be q and k themselves (the same
+ * address and strides).  num_kv_heads may be 0: q alone. */
+typedef struct moba_rotary {
+  int64_t total_tokens;
+  int32_t num_q_heads, num_kv_heads, head_dim, rotary_dim;
+  int32_t interleaved, inverse, dtype, reserved;
+  float magnitude;
+  int32_t reserved2;
+  int64_t q_stride_token, q_stride_head, k_stride_token, k_stride_head;
+  int64_t qo_stride_token, qo_stride_head, ko_stride_token, ko_stride_head;
+} moba_rotary_t;
+int moba_rotary_check(const moba_rotary_t* p);
+int moba_rotary(const moba_rotary_t* p, const void* q, const void* k, const int32_t* positions, const int64_t* turns, void* q_out,
+                void* k_out, void* stream);
+
+/* ---- drafted tokens checked against the target's probabilities --------------------------------
+ *
+ * The packed rows of a sequence are a tree as for moba_paged_tree_attention (parents == NULL: each row follows the one before it); row 0 is the
+ * sequence's last accepted token, the others are drafted ones.  target[row], draft[row]: the target's and the draft's probabilities
+ * of the token behind a row, [total_tokens][vocabulary], rows `target_stride` and `draft_stride` elements apart.  From row 0 on, a row's
+ * children are tried in their order; t is what is left of the row's target probabilities and S its sum, at first the probabilities and 1:
+ *     a child with token x is accepted, and the walk goes on from it, where t[x] > 0 and accept[child] * draft[row][x] * S < t[x];
+ *     otherwise t becomes max(t / S - draft[row], 0) and S its sum.
+ * draft == NULL: children are given tokens; one is accepted where t[x] > 0 and accept[child] * S < t[x], otherwise t[x] becomes 0 and S
+ * loses what it was.  Where no child is accepted the next token is the first with sum(t[0 .. token]) > sample[b] * sum(t); where that
+ * exceeds the sum, the last with t > 0; where nothing is left of t, the same of target[row]; -1 where that is all zeros.  Values that are not above 0 and finite
+ * are 0; a token outside the vocabulary has probability 0; rows from max_new on are not looked at.  Everything is computed in 64 bits.
+ *   path  int32[batch][max_new]  the accepted rows, counted from the sequence's first, row 0 the first of them; -1 behind them
+ *   count int32[batch]           how many (0 and next -1: the sequence has no row)
+ *   next  int32 or int64[batch], as tokens */
+typedef struct moba_drafts {
+  int64_t total_tokens, vocabulary;        /* vocabulary: at most 2^22                             */
+  int32_t batch, max_new;                  /* max_new: at most 1024                                */
+  int32_t dtype, token_bits;               /* MOBA_DTYPE_* of target and draft; 32 or 64           */
+  int64_t target_stride, draft_stride;
+  int64_t reserved;
+} moba_drafts_t;
+int moba_drafts_check(const moba_drafts_t* p);
+int moba_verify_drafts(const moba_drafts_t* p, const void* target, const void* draft, const void* tokens, const int32_t* cu_seqlens,
+                       const int32_t* parents, const float* accept, const float* sample, int32_t* path, int32_t* count, void* next,
+                       void* stream);
 
 #ifdef __cplusplus
 }
