@@ -137,6 +137,7 @@ __global__ void __launch_bounds__(kThreads) pool_kernel(const PoolParams p) {
   // ---- how many of each warp's entries count
   const int warps = (int)blocks * kWarps, me = (int)rank * kWarps + warp;
   const int per = ((carry + warps - 1) / warps + 31) / 32 * 32;
+  constexpr int kRound = 4, kStep = 32 * kRound;            // entries under way: of a lane, of a warp
   const int lo = (int)min((int64_t)per * me, (int64_t)carry), hi = (int)min((int64_t)lo + per, (int64_t)carry);
   auto entry = [&](int at, int32_t*& place) {               // the entry's number, and whether it counts
     const int b = search(p.batch, at, [&](int k) { return (int64_t)begin[k]; });
@@ -144,13 +145,20 @@ __global__ void __launch_bounds__(kThreads) pool_kernel(const PoolParams p) {
     const int id = *place;
     return kCut ? ((unsigned)id < (unsigned)p.pages ? id : -1) : (unsigned)id < (unsigned)p.pages ? -1 : 0;
   };
-  int mine = 0, id0 = -1;
-  int32_t* place0 = nullptr;                                // (of the first round, which is the only one as a rule)
-  for (int at = lo; at < hi; at += 32) {
-    int32_t* place = nullptr;
-    const int id = at + lane < hi ? entry(at + lane, place) : -1;
-    mine += __popc(__ballot_sync(0xffffffffu, id >= 0));
-    if (at == lo) { id0 = id; place0 = place; }
+  int mine = 0, ids[kRound];
+  int32_t* places[kRound];
+  auto load_round = [&](int at) {
+#pragma unroll
+    for (int k = 0; k < kRound; ++k) {
+      ids[k] = -1;
+      if (at + 32 * k + lane < hi) ids[k] = entry(at + 32 * k + lane, places[k]);
+    }
+  };
+  // (the last round first: where there is one, as a rule, it is kept for what follows)
+  for (int at = lo + (hi - lo - 1) / kStep * kStep; at >= lo && lo < hi; at -= kStep) {
+    load_round(at);
+#pragma unroll
+    for (int k = 0; k < kRound; ++k) mine += __popc(__ballot_sync(0xffffffffu, ids[k] >= 0));
   }
   if (lane == 0) counts[warp] = mine;
   __syncthreads();
@@ -166,19 +174,21 @@ __global__ void __launch_bounds__(kThreads) pool_kernel(const PoolParams p) {
     }
   }
   // ---- pages taken, or put back
-  for (int at = lo; at < hi; at += 32) {
-    int32_t* place = place0;
-    const int id = at == lo ? id0 : at + lane < hi ? entry(at + lane, place) : -1;
-    const uint32_t votes = __ballot_sync(0xffffffffu, id >= 0);
-    const int r = before + __popc(votes & ((1u << lane) - 1));
-    before += __popc(votes);
-    if (id < 0) continue;
-    if (kCut) {
-      const int64_t to = (int64_t)have + total - 1 - r;
-      if (to < p.pages) p.free[to] = id;
-      *place = -1;
-    } else if (r < have) {
-      *place = p.free[have - 1 - r];
+  for (int at = lo; at < hi; at += kStep) {
+    if (at > lo) load_round(at);
+#pragma unroll
+    for (int k = 0; k < kRound; ++k) {
+      const uint32_t votes = __ballot_sync(0xffffffffu, ids[k] >= 0);
+      const int r = before + __popc(votes & ((1u << lane) - 1));
+      before += __popc(votes);
+      if (ids[k] < 0) continue;
+      if (kCut) {
+        const int64_t to = (int64_t)have + total - 1 - r;
+        if (to < p.pages) p.free[to] = ids[k];
+        *places[k] = -1;
+      } else if (r < have) {
+        *places[k] = p.free[have - 1 - r];
+      }
     }
   }
   if (rank == 0 && tid == 0) {
@@ -218,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) pool_kernel(const PoolParams p) {
   }
 }
 
-// A row a thread, where no trees are.
+// A row a thread.  With parents the position is there already.
 constexpr int kRowThreads = 256;
 __global__ void __launch_bounds__(kRowThreads) pool_rows_kernel(const PoolParams p) {
   pdl_wait();
@@ -228,46 +238,72 @@ __global__ void __launch_bounds__(kRowThreads) pool_rows_kernel(const PoolParams
   Row r;
   const bool on = row_of(p, row, r);
   p.slots[row] = on ? slot_of(p, r) : -1;
-  p.positions[row] = on ? clamp_position(r.pos0 + r.i) : -1;
+  if (p.parents == nullptr) p.positions[row] = on ? clamp_position(r.pos0 + r.i) : -1;
 }
 
-// A sequence a block; its rows in order, kThreads at a time: a parent lies among them, or its depth is known from its position.
-__global__ void __launch_bounds__(kThreads) pool_tree_kernel(const PoolParams p) {
-  __shared__ int32_t up[kThreads], depth[kThreads];
+// Depths of many rows, in two steps.  First blocks of kWayRows rows for themselves: by doubling each row gets the way to the first ancestor in front
+// of the block's rows (or its root) and how long it is, kept in the row's slot until that is written.  Then every row goes from block to block; a
+// prompt without branches has a step for each kWayRows rows.
+constexpr int kWayPer = 4, kWayRows = kWayPer * kThreads;
+__device__ __forceinline__ long long pack_way(int exit, int length) { return ((long long)exit << 32) | (unsigned)length; }
+__global__ void __launch_bounds__(kThreads) pool_ways_kernel(const PoolParams p) {
+  extern __shared__ int32_t smem[];
+  int32_t *up = smem, *depth = up + kWayRows, *out = depth + kWayRows;
   pdl_wait();
   pdl_trigger();
-  const int b = blockIdx.x, tid = threadIdx.x;
-  if (b == p.batch) {                                       // rows of no sequence
-    const int64_t lead = min((int64_t)__ldg(p.cu), p.rows), tail = max((int64_t)__ldg(p.cu + p.batch), (int64_t)0);
-    for (int64_t row = tid; row < lead; row += kThreads) { p.slots[row] = -1; p.positions[row] = -1; }
-    for (int64_t row = tail + tid; row < p.rows; row += kThreads) { p.slots[row] = -1; p.positions[row] = -1; }
-    return;
+  const int64_t base = (int64_t)blockIdx.x * kWayRows;
+  int u[kWayPer], d[kWayPer], e[kWayPer];
+#pragma unroll
+  for (int k = 0; k < kWayPer; ++k) {
+    const int64_t row = base + threadIdx.x + k * kThreads;
+    Row r;
+    const bool on = row_of(p, row, r);
+    const int parent = on ? __ldg(p.parents + row) : -1;
+    const bool has = parent >= 0 && parent < r.i;
+    const int64_t to = has ? r.row0 + parent : -1;
+    u[k] = to >= base ? (int)(to - base) : -1;
+    d[k] = has ? 1 : 0;
+    e[k] = has && u[k] < 0 ? (int)to : -1;
   }
-  Row r;
-  r.b = b;
-  r.row0 = __ldg(p.cu + b);
-  const int64_t n = __ldg(p.cu + b + 1) - r.row0;
-  r.pos0 = __ldg(p.lens + b) - n;
-  if (r.row0 < 0) return;
-  const int64_t rows = min(n, p.rows - r.row0);
-  for (int64_t base = 0; base < rows; base += kThreads) {
-    const int64_t i = base + tid;
-    const bool on = i < rows;
-    int parent = on ? __ldg(p.parents + r.row0 + i) : -1;
-    if (parent >= i) parent = -1;
-    int d = parent >= 0 ? 1 : 0;
-    if (parent >= 0 && parent < base) d += p.positions[r.row0 + parent] - clamp_position(r.pos0);
-    up[tid] = parent >= base ? (int)(parent - base) : -1;
-    depth[tid] = d;
-    __syncthreads();
-    double_depths<1>(up, depth);
-    if (on) {
-      r.i = (int)i;
-      p.slots[r.row0 + i] = slot_of(p, r);
-      p.positions[r.row0 + i] = clamp_position(r.pos0 + depth[tid]);
+  for (;;) {
+    bool more = false;
+#pragma unroll
+    for (int k = 0; k < kWayPer; ++k) {
+      const int i = threadIdx.x + k * kThreads;
+      up[i] = u[k];
+      depth[i] = d[k];
+      out[i] = e[k];
+      more |= u[k] >= 0;
+    }
+    if (!__syncthreads_or(more)) break;
+#pragma unroll
+    for (int k = 0; k < kWayPer; ++k) {
+      const int at = u[k];
+      if (at >= 0) { d[k] += depth[at]; e[k] = out[at]; u[k] = up[at]; }
     }
     __syncthreads();
   }
+#pragma unroll
+  for (int k = 0; k < kWayPer; ++k) {
+    const int64_t row = base + threadIdx.x + k * kThreads;
+    if (row < p.rows) p.slots[row] = pack_way(e[k], d[k]);
+  }
+}
+__global__ void __launch_bounds__(kRowThreads) pool_depths_kernel(const PoolParams p) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t row = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
+  if (row >= p.rows) return;
+  Row r;
+  const bool on = row_of(p, row, r);
+  int64_t depth = 0;
+  for (int64_t at = row; on && at >= 0;) {                  // (an exit lies in front of its row)
+    const long long way = __ldcg(p.slots + at);
+    depth += (int)way;
+    const int exit = (int)(way >> 32);
+    at = exit < at ? exit : -1;
+  }
+  p.positions[row] = on ? clamp_position(r.pos0 + depth) : -1;
 }
 
 }  // namespace
@@ -291,8 +327,14 @@ cudaError_t launch_pool(const PoolParams& p, cudaStream_t st) {
   }
   if ((e = prepare_kernel(pool_kernel<false, false>, smem)) != cudaSuccess) return e;
   if ((e = launch_clusters(pool_kernel<false, false>, kBlocks, dim3(kBlocks), kThreads, smem, st, p)) != cudaSuccess) return e;
-  if (p.parents != nullptr) return launch_pdl(pool_tree_kernel, dim3((unsigned)p.batch + 1), kThreads, 0, st, p);
-  return launch_pdl(pool_rows_kernel, dim3((unsigned)((p.rows + kRowThreads - 1) / kRowThreads)), kRowThreads, 0, st, p);
+  const dim3 grid((unsigned)((p.rows + kRowThreads - 1) / kRowThreads));
+  if (p.parents != nullptr) {
+    constexpr size_t way_smem = 3 * kWayRows * sizeof(int32_t);
+    if ((e = prepare_kernel(pool_ways_kernel, way_smem)) != cudaSuccess) return e;
+    if ((e = launch_pdl(pool_ways_kernel, dim3((unsigned)((p.rows + kWayRows - 1) / kWayRows)), kThreads, way_smem, st, p)) != cudaSuccess) return e;
+    if ((e = launch_pdl(pool_depths_kernel, grid, kRowThreads, 0, st, p)) != cudaSuccess) return e;
+  }
+  return launch_pdl(pool_rows_kernel, grid, kRowThreads, 0, st, p);
 }
 
 }  // namespace moba

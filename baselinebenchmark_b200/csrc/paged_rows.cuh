@@ -71,6 +71,7 @@ struct RowsPlan {
   int32_t begin[kPagedBatch + 1];          // first item of a sequence
   int32_t slot0[kPagedBatch];              // first result slot of a sequence whose items are cut
   int32_t piece[kPagedBatch];              // key tiles of a piece
+  int32_t order[kPagedBatch];              // of trees: the sequences, those with the longest pieces first; `begin` is in this order
 };
 
 __device__ __forceinline__ int rows_tiles(const PagedParams& p, int n) {
@@ -179,6 +180,120 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p, R
   }
 }
 
+// Trees: few rows behind keys of any number, so that a batch is a few hundred items of all lengths, and what counts is that no CTA is left with a long
+// one at the end.  Items are drawn longest first, and a candidate's time is the largest of what no order can beat: the work of all, evenly; the
+// longest item; and k items of the length of number (k - 1) * SMs + 1, of which some CTA has k.  Candidates go down from the longest
+// sequence in even steps of a ratio.
+// (24 trees of 64 rows behind 1K to 16K tokens, 8 kv heads: 22 key tiles a piece in the order of the sequences, 274 us; 63, longest first, 246.)
+constexpr int kTreeSorted = 128;           // sequences up to which it is worth looking at their order
+constexpr int kTreeItem = 4, kTreePiece = 2;   // what an item costs besides its key tiles, in tiles, and what more when it is cut
+__global__ void __launch_bounds__(1024) paged_tree_plan_kernel(const PagedParams p, RowsPlan* plan, int sms, int most_slots) {
+  __shared__ int rows_s[kPagedBatch], most_s[kPagedBatch], least_s[kPagedBatch];
+  __shared__ float cost_s[32];
+  __shared__ int piece_s[32], scan_s[2][32];
+  pdl_wait();
+  pdl_trigger();
+  const int b = threadIdx.x, warp = b >> 5, lane = b & 31;
+  int rows = 0, most = 1, least = 1;
+  if (b < p.B) {
+    const PagedSeq s = paged_seq(p, b);
+    const int tiles = rows_tiles(p, s.n);
+    rows = tiles * p.Hkv;
+    if (tiles > 0) {
+      most = key_tiles(rows_end(p, s, tiles - 1));
+      least = key_tiles(rows_end(p, s, 0));
+    }
+  }
+  rows_s[b] = rows;
+  most_s[b] = most;
+  least_s[b] = least;
+  __syncthreads();
+  int longest = 1;
+  for (int i = lane; i < p.B; i += 32)
+    if (rows_s[i] > 0) longest = max(longest, most_s[i]);
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  const int piece = warp == 0 ? longest : max((int)ceilf((float)longest * exp2f(log2f((float)kLeastPiece / (float)max(longest, kLeastPiece)) * (float)warp / 31.f)), kLeastPiece);
+  float work = 0.f;
+  int slots = 0, top = 1, items = 0;
+  int size[2] = {0, 0}, count[2] = {0, 0};                  // of this lane's sequences, where there are up to 64
+  for (int i = lane, k = 0; i < p.B; i += 32, ++k) {
+    if (rows_s[i] == 0) continue;
+    const int even = even_piece(most_s[i], piece), cuts = (most_s[i] + even - 1) / even, mine = min(rows_s[i], 1 << 15) * min(cuts, 1 << 10);
+    const int cost = even + kTreeItem + (cuts > 1 ? kTreePiece : 0);
+    work += (float)rows_s[i] * (0.5f * (float)(most_s[i] + least_s[i]) + (float)cuts * (float)(cost - even));
+    if (cuts > 1) slots += (int)min((int64_t)rows_s[i] * cuts, (int64_t)(1 << 20));
+    top = max(top, cost);
+    items += min(mine, 1 << 20);
+    if (k < 2) {
+      if (k == 0) { size[0] = cost; count[0] = mine; } else { size[1] = cost; count[1] = mine; }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
+  slots = __reduce_add_sync(0xffffffffu, min(slots, 1 << 25));
+  items = __reduce_add_sync(0xffffffffu, min(items, 1 << 25));
+  top = __reduce_max_sync(0xffffffffu, top);
+  float cost = fmaxf(work / (float)sms, (float)top);
+  if (p.B <= 64) {
+    for (int k = 2; k <= 4 && items > (k - 1) * sms; ++k) {
+      int lo = 1, hi = top;                                 // the largest size that as many items have
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        const int n = __reduce_add_sync(0xffffffffu, (size[0] >= mid ? count[0] : 0) + (size[1] >= mid ? count[1] : 0));
+        if (n > (k - 1) * sms) lo = mid; else hi = mid - 1;
+      }
+      cost = fmaxf(cost, (float)(k * lo));
+    }
+  }
+  if (lane == 0) {
+    cost_s[warp] = slots > most_slots ? INFINITY : cost;
+    piece_s[warp] = piece;
+  }
+  __syncthreads();
+  // every warp for itself: the cheapest, of equal ones the first (costs are not negative: they compare as integers)
+  const uint32_t mine = __float_as_uint(cost_s[lane]);
+  const int best = piece_s[__ffs(__ballot_sync(0xffffffffu, mine == __reduce_min_sync(0xffffffffu, mine))) - 1];
+  const int even = even_piece(most, best), cuts = (most + even - 1) / even;
+  // the sequences' places in the order
+  int place = b;
+  if (p.B <= kTreeSorted) {
+    least_s[b] = rows > 0 ? even : 0;
+    __syncthreads();
+    if (b < p.B) {
+      place = 0;
+      for (int i = 0; i < p.B; ++i) place += least_s[i] > least_s[b] || (least_s[i] == least_s[b] && i < b);
+    }
+    __syncthreads();
+  }
+  most_s[place] = rows * cuts;                              // (a thread without a sequence has its own place)
+  rows_s[place] = b;
+  __syncthreads();
+  // first items of the places, first slots of the sequences
+  const int n = b < p.B ? most_s[b] : 0, m = cuts > 1 && b < p.B ? rows * cuts : 0;
+  int x = n, y = m;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) { x += u; y += v; }
+  }
+  if (lane == 31) { scan_s[0][warp] = x; scan_s[1][warp] = y; }
+  __syncthreads();
+  const int bx = __reduce_add_sync(0xffffffffu, lane < warp ? scan_s[0][lane] : 0);
+  const int by = __reduce_add_sync(0xffffffffu, lane < warp ? scan_s[1][lane] : 0);
+  if (b < p.B) {
+    plan->begin[b] = bx + x - n;
+    plan->order[b] = rows_s[b];
+    plan->slot0[b] = m > 0 ? by + y - m : -1;
+    plan->piece[b] = even;
+    if (b == p.B - 1) {
+      plan->begin[p.B] = bx + x;
+      plan->items = bx + x;
+      plan->counter = 0;
+      plan->status = 0;
+    }
+  }
+}
+
 // ---- items ---------------------------------------------------------------------
 struct RowsItem {
   int b, h, tile;                          // sequence, kv head, row tile
@@ -234,6 +349,7 @@ constexpr int64_t kAllHeadsBytes = (int64_t)80 << 20;
 __device__ __forceinline__ bool rows_twice(int D, const RowsItem& it) { return D != 256 && it.nrows <= kTileM; }
 
 // Warp 2, one item ahead of the others.
+template <bool kTree>
 __device__ __forceinline__ void rows_prefetch(const PagedParams& p, const RowsArgs& a, RowsCtrl& c, int at) {
   const int lane = threadIdx.x & 31;
   RowsItem it;
@@ -243,11 +359,12 @@ __device__ __forceinline__ void rows_prefetch(const PagedParams& p, const RowsAr
     if (lane == 0) idx = c.abort ? 0x7fffffff : atomicAdd(&a.plan->counter, 1);
     idx = __shfl_sync(0xffffffffu, idx, 0);
     if (idx >= c.items) { done = true; break; }
-    it.b = search_warp(p.B, idx, [&](int k) { return __ldcg(a.plan->begin + k); });
+    const int place = search_warp(p.B, idx, [&](int k) { return __ldcg(a.plan->begin + k); });
+    it.b = kTree ? __ldcg(a.plan->order + place) : place;
     const PagedSeq s = paged_seq(p, it.b);
     const int tiles = rows_tiles(p, s.n), piece = __ldcg(a.plan->piece + it.b);
     const int most = key_tiles(rows_end(p, s, tiles - 1)), cuts = (most + piece - 1) / piece;
-    const int i = idx - __ldcg(a.plan->begin + it.b);      // kv head, piece, row tile, the last one first
+    const int i = idx - __ldcg(a.plan->begin + place);      // kv head, piece, row tile, the last one first
     int cut = 0;
     if (cuts == 1 && (int64_t)s.len * p.Hkv * p.D * 4 <= kAllHeadsBytes) {
       it.tile = tiles - 1 - i / p.Hkv;
@@ -719,7 +836,7 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
       ended = true;
     };
     for (int n = 0;; ++n) {
-      if (warp == 2) rows_prefetch(p, a, c, n & 1);
+      if (warp == 2) rows_prefetch<kTree>(p, a, c, n & 1);
       if (!rows_next<false, D, kCodes>(a, c, smem, n & 1)) break;
       const RowsItem& it = c.item[n & 1];
       if (kCodes && warp == 0) {
@@ -1332,7 +1449,7 @@ cudaError_t launch_rows_dim(const PagedParams& p, const CUtensorMap& mk, const C
   const int threads = p.store == MOBA_STORE_SAME ? kRowsThreads<MOBA_STORE_SAME> : kRowsThreads<MOBA_STORE_E4M3>;
   cudaError_t e = prepare_kernel(kernel, kRowsSmem);
   if (e != cudaSuccess) return e;
-  if ((e = launch_pdl(paged_plan_kernel, dim3(1), kPagedBatch, 0, st, p, a.plan, sms, slots)) != cudaSuccess) return e;
+  if ((e = launch_pdl(kTree ? paged_tree_plan_kernel : paged_plan_kernel, dim3(1), kPagedBatch, 0, st, p, a.plan, sms, slots)) != cudaSuccess) return e;
   if ((e = launch_pdl(kernel, dim3(sms), threads, kRowsSmem, st, p, mk, mv, a)) != cudaSuccess) return e;
   const int64_t warps = p.T * p.Hq, per = kJoinThreads / 32;
   return launch_pdl(paged_rows_join_kernel<kHalf, D>, dim3((unsigned)((warps + per - 1) / per)), kJoinThreads, 0, st, p, a);

@@ -28,7 +28,8 @@
 namespace moba {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kAbreast = 2;               // vectors of p, and of q, that a lane has under way
 constexpr int kMostBlocks = 8;             // of a cluster
 
 struct Node {                              // a row: what its test needs
@@ -49,8 +50,7 @@ __device__ __forceinline__ float probability(float x) { return x > 0.f && x < IN
 
 template <typename T> constexpr int kVector = 16 / sizeof(T);
 template <typename T>
-__device__ __forceinline__ void load_vector(const T* at, float (&x)[kVector<T>]) {
-  const uint4 w = __ldg(reinterpret_cast<const uint4*>(at));
+__device__ __forceinline__ void widen(const uint4& w, float (&x)[kVector<T>]) {
   if constexpr (std::is_same<T, float>::value) {
     x[0] = __uint_as_float(w.x); x[1] = __uint_as_float(w.y); x[2] = __uint_as_float(w.z); x[3] = __uint_as_float(w.w);
   } else {
@@ -60,7 +60,7 @@ __device__ __forceinline__ void load_vector(const T* at, float (&x)[kVector<T>])
 
 // What is left of an element after the rejections of a row's children.
 struct Residual {
-  const double* sums;                      // S after each rejection, from the first on; the last one may not be known yet
+  const double* inverse;                   // 1 / S after each rejection, from the first on (0: nothing is left); the last one may not be known yet
   int rejected;
   const uint32_t* taken;                   // without a draft: tokens that were rejected, bits from `taken0` on; null: none
   int64_t taken0;
@@ -71,7 +71,8 @@ struct Residual {
       if (rejected > 0) {
         const double d = (double)probability(q);
         t = fmax(t - d, 0.0);
-        for (int j = 0; j + 1 < rejected; ++j) t = fmax((sums[j] > 0.0 ? t / sums[j] : 0.0) - d, 0.0);
+#pragma unroll 1
+        for (int j = 0; j + 1 < rejected; ++j) t = fmax(__dsub_rn(__dmul_rn(t, inverse[j]), d), 0.0);
       }
     } else if (taken != nullptr) {
       const int64_t i = at - taken0;
@@ -94,7 +95,7 @@ struct Walk {
   double mass;
 };
 template <bool kDraft>
-__device__ __forceinline__ Command walk_on(const Node* nodes, int n, Walk& w, double* sums, int16_t* path) {
+__device__ __forceinline__ Command walk_on(const Node* nodes, int n, Walk& w, const double* inverse, int16_t* path) {
   const int lane = threadIdx.x & 31;
   for (;;) {
     // the next child of row `at`, behind row `before`
@@ -112,7 +113,7 @@ __device__ __forceinline__ Command walk_on(const Node* nodes, int n, Walk& w, do
       if (w.rejected > 0 && w.mass < 0.0) return Command{w.at, w.rejected, 0};
       if (w.rejected > 0) {
         have = fmax(have - drawn, 0.0);
-        for (int j = 0; j + 1 < w.rejected; ++j) have = fmax((sums[j] > 0.0 ? have / sums[j] : 0.0) - drawn, 0.0);
+        for (int j = 0; j + 1 < w.rejected; ++j) have = fmax(__dsub_rn(__dmul_rn(have, inverse[j]), drawn), 0.0);
       }
     } else if (w.rejected > 0) {
       bool twice = false;                                   // a sibling had the token
@@ -131,15 +132,16 @@ __device__ __forceinline__ Command walk_on(const Node* nodes, int n, Walk& w, do
   }
 }
 
+// (four blocks an SM: a batch of 74 sequences is resident at once)
 template <typename T, bool kDraft>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyParams a) {
+__global__ void __launch_bounds__(kThreads, 4) verify_kernel(const VerifyParams a) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ double totals[kMostBlocks], warp_total[kWarps];
   __shared__ Command told;
   __shared__ int first_at, last_at;
   const int most = a.max_new;
-  double* sums = reinterpret_cast<double*>(smem);           // [max_new]
-  Node* nodes = reinterpret_cast<Node*>(sums + most);       // [max_new]
+  double* inverse = reinterpret_cast<double*>(smem);        // [max_new]
+  Node* nodes = reinterpret_cast<Node*>(inverse + most);    // [max_new]
   int16_t* path = reinterpret_cast<int16_t*>(nodes + most);   // [max_new, even]
   uint32_t* taken = reinterpret_cast<uint32_t*>(path + ((most + 1) & ~1));   // a bit for each token of this block's part
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -153,9 +155,8 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyParams a) 
   const T* draft = kDraft ? static_cast<const T*>(a.draft) + row0 * a.draft_stride : nullptr;
   auto token_of = [&](int64_t i) { return a.tokens64 ? (int64_t)__ldg(static_cast<const long long*>(a.tokens) + i) : (int64_t)__ldg(static_cast<const int*>(a.tokens) + i); };
   // this block's part of the vocabulary, and each warp's of it
-  const int64_t part = a.part, lo = min((int64_t)rank * part, a.vocabulary), hi = min(lo + part, a.vocabulary);
-  const int64_t share = part / kWarps, wlo = min(lo + warp * share, hi), whi = min(wlo + share, hi);
-
+  const int64_t part = a.part, share = part / kWarps;
+  constexpr int kV = kVector<T>;
   Walk walk{0, 0, 0, 1, 1.0};
   if (rank == 0) {
     for (int i = tid; i < n; i += kThreads) {
@@ -179,10 +180,11 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyParams a) 
     __syncthreads();
   }
   bool raw = false;                                         // nothing was left of the row: the token is drawn from all of it
+  bool infinite = false, again = false;                     // the sum was: there are infinities, which the quick way does not look for
   for (;;) {
     // ---- what is needed next: the first block tells all
     if (rank == 0 && warp == 0) {
-      Command c = n == 0 ? Command{-1, 0, 1} : raw ? Command{walk.at, 0, 1} : walk_on<kDraft>(nodes, n, walk, sums, path);
+      Command c = n == 0 ? Command{-1, 0, 1} : again ? told : raw ? Command{walk.at, 0, 1} : walk_on<kDraft>(nodes, n, walk, inverse, path);
       __syncwarp();
       for (uint32_t i = lane; i < blocks * 3; i += 32) {
         const uint32_t to = i / 3, word = i - to * 3;
@@ -191,13 +193,23 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyParams a) 
       // the sums of the rejections (the other blocks need them, the newest one excepted)
       if (kDraft && c.rejected > 1)
         for (uint32_t to = 1 + lane; to < blocks; to += 32)
-          cluster_store(cluster_place(&sums[c.rejected - 2], to), (uint64_t)__double_as_longlong(sums[c.rejected - 2]));
+          cluster_store(cluster_place(&inverse[c.rejected - 2], to), (uint64_t)__double_as_longlong(inverse[c.rejected - 2]));
     }
     // without a draft the rejected tokens do not count any more
-    if (!kDraft) for (int i = tid; i < (int)((part + 31) / 32); i += kThreads) taken[i] = 0;
+    if (!kDraft) for (int i = tid; i < (int)((part + kV + 31) / 32); i += kThreads) taken[i] = 0;
     cluster_sync();
     const Command c = told;
     if (c.row < 0) break;
+    const T* p = target + c.row * a.target_stride;
+    const T* q = kDraft ? draft + c.row * a.draft_stride : nullptr;
+    const bool with_draft = kDraft && c.rejected > 0;
+    // parts begin where p is aligned for vectors, `head` elements behind a multiple of their size; the first part has those too
+    const int head = (int)(((16 - ((uintptr_t)p & 15)) & 15) / sizeof(T));
+    const bool vectors = !with_draft || (((uintptr_t)p ^ (uintptr_t)q) & 15) == 0;
+    const int64_t lo = rank == 0 ? 0 : min((int64_t)rank * part + head, a.vocabulary), hi = min(((int64_t)rank + 1) * part + head, a.vocabulary);
+    auto first_of = [&](int w) { return w == 0 ? lo : min((int64_t)rank * part + head + w * share, hi); };
+    auto end_of = [&](int w) { return min((int64_t)rank * part + head + (w + 1) * share, hi); };
+    const int64_t wlo = first_of(warp), whi = end_of(warp);
     if (!kDraft && c.rejected > 0) {
       // (of the children of a row all were rejected)
       for (int i = c.row + 1 + tid; i < n; i += kThreads) {
@@ -208,25 +220,49 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyParams a) 
       __syncthreads();
     }
     // ---- the sum of what is left, warp by warp
-    const Residual left{sums, c.rejected, !kDraft && c.rejected > 0 ? taken : nullptr, lo};
-    const T* p = target + c.row * a.target_stride;
-    const T* q = kDraft ? draft + c.row * a.draft_stride : nullptr;
-    const bool with_draft = kDraft && c.rejected > 0;
-    constexpr int kV = kVector<T>;
+    const Residual left{inverse, c.rejected, !kDraft && c.rejected > 0 ? taken : nullptr, lo};
+    // quick: t is p, or max(p - q, 0) = max(p, q) - q with p and q no less than 0 (which drops what is not a number)
+    const bool quick = !infinite && (c.rejected == 0 || (kDraft && c.rejected == 1));
     double s0 = 0.0, s1 = 0.0;
-    const bool aligned = (((uintptr_t)p | (with_draft ? (uintptr_t)q : 0)) & 15) == 0;
+    auto one = [&](float x, float y, int64_t e, int i) {
+      double t;
+      if (quick) {
+        const float d = fmaxf(y, 0.f);
+        t = kDraft ? (double)fmaxf(fmaxf(x, 0.f), d) - (double)d : (double)fmaxf(x, 0.f);
+      } else {
+        t = left.template operator()<kDraft>(x, y, e);
+      }
+      if (i & 1) s1 += t; else s0 += t;
+    };
     int64_t at = wlo;
-    if (aligned) {
-      for (; at + 32 * kV <= whi; at += 32 * kV) {
-        float x[kV], y[kV];
-        const int64_t e = at + lane * kV;
-        load_vector<T>(p + e, x);
-        if (with_draft) load_vector<T>(q + e, y);
+    if (vectors) {
+      if (rank == 0 && warp == 0 && lane < head && lane < whi) one(element(p + lane), with_draft ? element(q + lane) : 0.f, lane, 0);
+      if (rank == 0 && warp == 0) at = min((int64_t)head, whi);
+      for (; at + 32 * kV * kAbreast <= whi; at += 32 * kV * kAbreast) {
+        uint4 x[kAbreast], y[kAbreast];
 #pragma unroll
-        for (int i = 0; i < kV; ++i) {
-          const double t = left.template operator()<kDraft>(x[i], with_draft ? y[i] : 0.f, e + i);
-          if (i & 1) s1 += t; else s0 += t;
+        for (int k = 0; k < kAbreast; ++k) {
+          const int64_t e = at + (k * 32 + lane) * kV;
+          x[k] = __ldg(reinterpret_cast<const uint4*>(p + e));
+          y[k] = with_draft ? __ldg(reinterpret_cast<const uint4*>(q + e)) : make_uint4(0, 0, 0, 0);
         }
+#pragma unroll
+        for (int k = 0; k < kAbreast; ++k) {
+          float f[kV], g[kV];
+          widen<T>(x[k], f);
+          widen<T>(y[k], g);
+#pragma unroll
+          for (int i = 0; i < kV; ++i) one(f[i], g[i], at + (k * 32 + lane) * kV + i, i);
+        }
+      }
+#pragma unroll 1
+      for (; at + 32 * kV <= whi; at += 32 * kV) {
+        const int64_t e = at + lane * kV;
+        float f[kV], g[kV];
+        widen<T>(__ldg(reinterpret_cast<const uint4*>(p + e)), f);
+        widen<T>(with_draft ? __ldg(reinterpret_cast<const uint4*>(q + e)) : make_uint4(0, 0, 0, 0), g);
+#pragma unroll
+        for (int i = 0; i < kV; ++i) one(f[i], g[i], e + i, i);
       }
     }
     for (; at < whi; at += 32 * kV) {
@@ -240,8 +276,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyParams a) 
 #pragma unroll
       for (int i = 0; i < kV; ++i) {
         const int64_t e = at + lane + 32 * i;
-        const double t = e < whi ? left.template operator()<kDraft>(x[i], y[i], e) : 0.0;
-        if (i & 1) s1 += t; else s0 += t;
+        if (e < whi) one(x[i], y[i], e, i);
       }
     }
     const double mine = warp_sum(s0 + s1);
@@ -256,10 +291,12 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyParams a) 
     cluster_sync();
     double total = 0.0;
     for (uint32_t i = 0; i < blocks; ++i) total += totals[i];
+    again = quick && !(total <= 1e300);
+    if (again) { infinite = true; continue; }
     if (!c.last) {
       if (rank == 0 && warp == 0) {
         walk.mass = total;
-        if (lane == 0) sums[c.rejected - 1] = total;
+        if (lane == 0) inverse[c.rejected - 1] = total > 0.0 ? 1.0 / total : 0.0;
         __syncwarp();
       }
       continue;
@@ -287,8 +324,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyParams a) 
       if (in_block != (int)rank) break;                     // (no barrier of the cluster comes behind this)
       const int in_warp = before == INFINITY ? -1 : pick(warp_total, kWarps, before);
       int64_t flo, fhi;
-      if (in_warp < 0) { flo = lo; fhi = hi; } else { flo = min(lo + in_warp * share, hi); fhi = min(flo + share, hi); }
-      if (before == INFINITY && in_warp >= 0) { flo = lo; fhi = hi; }
+      if (before == INFINITY) { flo = lo; fhi = hi; } else { flo = first_of(in_warp); fhi = end_of(in_warp); }
       // each thread has a few elements that lie together
       const int64_t per = (fhi - flo + kThreads - 1) / kThreads, from = min(flo + tid * per, fhi), to = min(from + per, fhi);
       auto value = [&](int64_t e) { return left.template operator()<kDraft>(element(p + e), with_draft ? element(q + e) : 0.f, e); };
@@ -353,10 +389,19 @@ cudaError_t launch_verify(VerifyParams a, int dtype, cudaStream_t st) {
   const VerifyKernel kernel = dtype == MOBA_DTYPE_FP32 ? pick_kernel<float>(a.draft != nullptr)
                             : dtype == MOBA_DTYPE_FP16 ? pick_kernel<__half>(a.draft != nullptr) : pick_kernel<__nv_bfloat16>(a.draft != nullptr);
   const int64_t step = (int64_t)kWarps * 32 * (dtype == MOBA_DTYPE_FP32 ? 4 : 8);   // whole vectors of all warps
-  const int blocks = kMostBlocks;
+  // Blocks of a cluster: a round of them (four an SM) takes 8 us and 0.5 us for each 1000 tokens of a part.  (sequences x tokens, us with 8 / 4 / 2 / 1 blocks:
+  // 1 x 32000 10 / 12 / 16 / 23, 100 x 32000 19 / 14 / 18 / 25, 300 x 32000 44 / 32 / 29 / 31, 64 x 128000 21 / 29 / 51 / 93, 300 x 128000 86 / 83 / 107 / 124,
+  // 600 x 1000 65 / 37 / 23 / 16)
+  const int64_t round = 4 * (int64_t)device_info().sms;
+  int blocks = 0;
+  int64_t least = 0;
+  for (int n = kMostBlocks; n >= 1; n /= 2) {
+    const int64_t cost = (a.batch * (int64_t)n + round - 1) / round * (16000 + a.vocabulary / n);
+    if (blocks == 0 || cost < least) { blocks = n; least = cost; }
+  }
   a.part = (a.vocabulary + blocks * step - 1) / (blocks * step) * step;
   const size_t smem = (size_t)a.max_new * (sizeof(double) + sizeof(Node)) + (size_t)((a.max_new + 1) & ~1) * sizeof(int16_t) +
-                      (a.draft == nullptr ? (size_t)((a.part + 31) / 32) * 4 : 0);
+                      (a.draft == nullptr ? (size_t)((a.part + 8 + 31) / 32) * 4 : 0);
   cudaError_t e = prepare_kernel(kernel, smem);
   if (e != cudaSuccess) return e;
   return launch_clusters(kernel, blocks, dim3((unsigned)(a.batch * blocks)), kThreads, smem, st, a);

@@ -7,6 +7,7 @@ samples nothing.  include/moba_b200.h has the rules in full.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -17,6 +18,10 @@ from .paged import _check_not_followed, _check_parents, _i32_rows, _run_on
 __all__ = ["verify_drafts"]
 
 _DTYPES = {torch.float32: _lib.DTYPE_FP32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
+_TOKEN_BITS = {torch.int32: 32, torch.int64: 64}
+#: struct moba_drafts, field by field
+_CALL = struct.Struct("@2q4i3q")
+assert _CALL.size == C.sizeof(_lib.Drafts)
 
 
 def _check_drafts(target, draft, tokens, cu_seqlens, accept, sample, max_new) -> None:
@@ -78,18 +83,31 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: t
     Returns (path, count, next): path int32 [batch, max_new], the accepted rows counted from the sequence's first (row 0 among them), -1 behind
     them; count int32 [batch]; next [batch] of tokens' dtype.  A sequence without rows has 0 and -1; a next token of -1 else means that the row's
     probabilities are all zeros.  Computed in 64 bits; values that are not above 0 and finite count as 0."""
-    _check_drafts(target, draft, tokens, cu_seqlens, accept, sample, max_new)
-    index, rows, batch = target.get_device(), target.shape[0], cu_seqlens.numel() - 1
+    # each attribute is read once: this runs in every step of a server
+    shape, dtype, index, token = target.shape, target.dtype, target.get_device(), tokens.dtype
+    good = len(shape) == 2 and index >= 0 and dtype in _DTYPES and token in _TOKEN_BITS and isinstance(max_new, int) and 0 < max_new <= 1024
+    if good:
+        (rows, vocabulary), (ts, t1), i32, f32, ds = shape, target.stride(), torch.int32, torch.float32, 0
+        batch = cu_seqlens.shape[0] - 1 if cu_seqlens.dim() == 1 else 0
+        good = (0 < vocabulary <= 2 ** 22 and (t1 == 1 or vocabulary == 1) and batch > 0 and cu_seqlens.dtype == i32 and cu_seqlens.get_device() == index
+                and cu_seqlens.stride(0) == 1 and tokens.shape == (rows,) and tokens.get_device() == index and tokens.is_contiguous()
+                and accept.shape == (rows,) and accept.dtype == f32 and accept.get_device() == index and accept.is_contiguous()
+                and sample.shape == (batch,) and sample.dtype == f32 and sample.get_device() == index and sample.is_contiguous())
+        if good and draft is not None:
+            ds, d1 = draft.stride() if draft.dim() == 2 else (0, 0)
+            good = draft.shape == shape and draft.dtype == dtype and draft.get_device() == index and (d1 == 1 or vocabulary == 1)
+    if not good:
+        _check_drafts(target, draft, tokens, cu_seqlens, accept, sample, max_new)
+        raise ValueError("target, draft, tokens, cu_seqlens, accept and sample do not describe a call")
     if parents is not None:
         _check_parents(parents, rows, index)
     _check_not_followed(target=target, draft=draft, accept=accept, sample=sample)
-    path = cu_seqlens.new_empty((batch, max_new))
-    count, token = cu_seqlens.new_empty(batch), tokens.new_empty(batch)
+    path = torch.empty((batch, max_new), dtype=i32, device=target.device)
+    count, following = torch.empty(batch, dtype=i32, device=target.device), torch.empty(batch, dtype=token, device=target.device)
     if rows == 0:
-        return path.fill_(-1), count.zero_(), token.fill_(-1)
-    call = _lib.Drafts(rows, target.shape[1], batch, max_new, _DTYPES[target.dtype], 64 if tokens.dtype == torch.int64 else 32,
-                       target.stride(0) if rows > 1 else 0, draft.stride(0) if draft is not None and rows > 1 else 0, 0)
-    _run_on(index, _lib.lib().moba_verify_drafts, C.byref(call), target.data_ptr(), draft.data_ptr() if draft is not None else None,
-            tokens.data_ptr(), cu_seqlens.data_ptr(), parents.data_ptr() if parents is not None else None, accept.data_ptr(),
-            sample.data_ptr(), path.data_ptr(), count.data_ptr(), token.data_ptr())
-    return path, count, token
+        return path.fill_(-1), count.zero_(), following.fill_(-1)
+    call = _CALL.pack(rows, vocabulary, batch, max_new, _DTYPES[dtype], _TOKEN_BITS[token], ts if rows > 1 else 0, ds if rows > 1 else 0, 0)
+    _run_on(index, _lib.lib().moba_verify_drafts, call, target.data_ptr(), None if draft is None else draft.data_ptr(), tokens.data_ptr(),
+            cu_seqlens.data_ptr(), None if parents is None else parents.data_ptr(), accept.data_ptr(), sample.data_ptr(), path.data_ptr(),
+            count.data_ptr(), following.data_ptr())
+    return path, count, following

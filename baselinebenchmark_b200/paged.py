@@ -377,7 +377,7 @@ def paged_keep(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
     _i32_rows("count", count, (g.batch,), g.index)
     _check_written(k_pages, v_pages, k_scales, v_scales)
     _check_not_followed(k_pages=k_pages, v_pages=v_pages)
-    lens = torch.empty_like(seq_lens, memory_format=torch.contiguous_format)
+    lens = torch.empty(g.batch, dtype=torch.int32, device=k_pages.device)
     dtype = g.dtype if g.store == _lib.STORE_SAME else torch.bfloat16
     cu, old, table, k, v, ks, vs = g.where
     columns = path.shape[1]
@@ -387,8 +387,12 @@ def paged_keep(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
     return lens
 
 
-def _pool_call(page_table, free_pages, free_count, page_size, total_tokens, lens_name, lens) -> Tuple[_lib.PagePool, int]:
-    """The structure of a call on a pool, with its tensors checked, and their device's number."""
+#: struct moba_page_pool, field by field
+_POOL = struct.Struct("@q4i2q")
+assert _POOL.size == C.sizeof(_lib.PagePool)
+
+
+def _check_pool(page_table, free_pages, free_count, page_size, total_tokens, lens_name, lens) -> None:
     index = page_table.get_device()
     if index < 0:
         raise ValueError("page_table must be an accelerator tensor")
@@ -409,10 +413,27 @@ def _pool_call(page_table, free_pages, free_count, page_size, total_tokens, lens
         raise ValueError("rows of page_table must not lie on one another")
     if not isinstance(total_tokens, int) or total_tokens < 0:
         raise ValueError(f"total_tokens must be an int that is not negative, got {total_tokens}")
-    if max(free_pages.shape[0], per_seq, page_size, batch) >= 2 ** 31:
-        raise NotImplementedError("pages, columns of the table and sequences are counted in 32 bits")
+
+
+def _pool_call(page_table, free_pages, free_count, page_size, total_tokens, lens_name, lens) -> Tuple[bytes, int, int]:
+    """The structure of a call on a pool, with its tensors checked, their device's number and the sequences."""
+    table, pages, index, i32 = page_table.shape, free_pages.shape, page_table.get_device(), torch.int32
+    good = len(table) == 2 and index >= 0 and len(pages) == 1 and isinstance(page_size, int) and isinstance(total_tokens, int)
+    if good:
+        (batch, per_seq), (ts, td) = table, page_table.stride()
+        good = (batch > 0 and per_seq > 0 and pages[0] > 0 and page_size >= 16 and not page_size & (page_size - 1) and total_tokens >= 0
+                and (td == 1 or per_seq == 1) and (batch == 1 or ts >= per_seq) and page_table.dtype == i32
+                and free_pages.dtype == i32 and free_pages.get_device() == index and (pages[0] == 1 or free_pages.stride(0) == 1)
+                and free_count.shape == (1,) and free_count.dtype == i32 and free_count.get_device() == index
+                and lens.shape == (batch,) and lens.dtype == i32 and lens.get_device() == index and (batch == 1 or lens.stride(0) == 1))
+    if not good:
+        _check_pool(page_table, free_pages, free_count, page_size, total_tokens, lens_name, lens)
+        raise ValueError("page_table, free_pages, free_count and the lengths do not describe a call")
     _check_written(page_table, free_pages, free_count)
-    return _lib.PagePool(total_tokens, batch, per_seq, free_pages.shape[0], page_size, page_table.stride(0) if batch > 1 else per_seq, 0), index
+    try:
+        return _POOL.pack(total_tokens, batch, per_seq, pages[0], page_size, ts if batch > 1 else per_seq, 0), index, batch
+    except struct.error as e:
+        raise NotImplementedError("pages, columns of the table, tokens and sequences are counted in 32 bits") from e
 
 
 def _run_on(index: int, call, *args) -> None:
@@ -435,13 +456,14 @@ def paged_reserve(page_table: torch.Tensor, cu_seqlens: torch.Tensor, seq_lens: 
     positions int32 [total_tokens], as `rotary` takes them, with `parents` (see `paged_attention`) those of a row's depth in its tree; missing int32
     [1], the entries for which no page was left.  Rows of no sequence have -1 in both.  Calls on one pool are ordered by the caller's
     streams.  At most 16384 sequences."""
-    call, index = _pool_call(page_table, free_pages, free_count, page_size, total_tokens, "seq_lens", seq_lens)
-    _i32_rows("cu_seqlens", cu_seqlens, (call.batch + 1,), index)
+    call, index, batch = _pool_call(page_table, free_pages, free_count, page_size, total_tokens, "seq_lens", seq_lens)
+    _i32_rows("cu_seqlens", cu_seqlens, (batch + 1,), index)
     if parents is not None:
         _check_parents(parents, total_tokens, index)
-    slots = page_table.new_empty(total_tokens, dtype=torch.int64)
-    positions, missing = page_table.new_empty(total_tokens), page_table.new_empty(1)
-    _run_on(index, _lib.lib().moba_paged_reserve, C.byref(call), cu_seqlens.data_ptr(), seq_lens.data_ptr(),
+    device, i32 = page_table.device, torch.int32
+    slots = torch.empty(total_tokens, dtype=torch.int64, device=device)
+    positions, missing = torch.empty(total_tokens, dtype=i32, device=device), torch.empty(1, dtype=i32, device=device)
+    _run_on(index, _lib.lib().moba_paged_reserve, call, cu_seqlens.data_ptr(), seq_lens.data_ptr(),
             parents.data_ptr() if parents is not None else None, page_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
             slots.data_ptr(), positions.data_ptr(), missing.data_ptr())
     _written(page_table, free_pages, free_count)
@@ -453,8 +475,8 @@ def paged_release(page_table: torch.Tensor, keep_lens: torch.Tensor, free_pages:
     """Gives pages back: those behind the first keep_lens[b] (int32) tokens of sequence b, all of them for 0, go to the stack of free pages and
     their entries become -1.  The other way round of `paged_reserve`: what one call took, a release leaves as it was.  Pages that other
     sequences share must not be given back."""
-    call, index = _pool_call(page_table, free_pages, free_count, page_size, 0, "keep_lens", keep_lens)
-    _run_on(index, _lib.lib().moba_paged_release, C.byref(call), keep_lens.data_ptr(), page_table.data_ptr(), free_pages.data_ptr(),
+    call, index, _ = _pool_call(page_table, free_pages, free_count, page_size, 0, "keep_lens", keep_lens)
+    _run_on(index, _lib.lib().moba_paged_release, call, keep_lens.data_ptr(), page_table.data_ptr(), free_pages.data_ptr(),
             free_count.data_ptr())
     _written(page_table, free_pages, free_count)
 

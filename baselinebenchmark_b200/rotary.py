@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from fractions import Fraction
 from typing import Optional, Tuple
 
@@ -22,6 +23,9 @@ __all__ = ["RotaryTable", "rotary", "rotary_frequencies"]
 
 _TURN = 2 * Fraction(314159265358979323846264338327950288419716939937510, 10 ** 50)
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
+#: struct moba_rotary, field by field (filling a ctypes structure by name takes ten times as long)
+_CALL = struct.Struct("@q8ifi8q")
+assert _CALL.size == C.sizeof(_lib.Rotary)
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str = "none", factor: float = 1.0,
@@ -73,6 +77,7 @@ class RotaryTable:
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self.rotary_dim, self.interleaved, self.magnitude = 2 * f.numel(), bool(interleaved), float(magnitude)
         self.turns = torch.tensor(turns, dtype=torch.int64).to(device)
+        self.index = self.turns.get_device()
 
 
 def _check_rotary(q, k, positions, table) -> None:
@@ -97,7 +102,7 @@ def _check_rotary(q, k, positions, table) -> None:
         raise ValueError(f"the table turns {table.rotary_dim} dims, head_dim is {q.shape[2]}")
     if positions.shape != (q.shape[0],):
         raise ValueError(f"positions must have shape [{q.shape[0]}], got {tuple(positions.shape)}")
-    if positions.dtype != torch.int32 or positions.get_device() != q.get_device() or table.turns.get_device() != q.get_device():
+    if positions.dtype != torch.int32 or positions.get_device() != q.get_device() or table.index != q.get_device():
         raise TypeError("positions must be an int32 tensor, and the table, on the device of q")
     if q.shape[0] > 1 and positions.stride(0) != 1:
         raise NotImplementedError("positions must be contiguous")
@@ -105,24 +110,60 @@ def _check_rotary(q, k, positions, table) -> None:
 
 def _strides(x) -> Tuple[int, int]:
     """Of tokens and heads (one token or head may have any: it is never stepped over)."""
-    if x is None:
-        return 0, 0
-    return x.stride(0) if x.shape[0] > 1 else 0, x.stride(1) if x.shape[1] > 1 else 0
+    (tokens, heads, _), (t, h, _) = x.shape, x.stride()
+    return t if tokens > 1 else 0, h if heads > 1 else 0
+
+
+def _launch(q, k, positions, table, inverse, qo, ko, shape, index, dtype, q_heads_k) -> None:
+    """The call itself; everything has been looked at."""
+    (tokens, heads, dim), (heads_k, qs, ks) = shape, q_heads_k
+    call = _CALL.pack(tokens, heads, heads_k, dim, table.rotary_dim, table.interleaved, inverse, _DTYPES[dtype], 0, table.magnitude, 0, *qs, *ks,
+                      *_strides(qo), *((0, 0) if ko is None else _strides(ko)))
+    _run_on(index, _lib.lib().moba_rotary, call, q.data_ptr(), None if k is None else k.data_ptr(), positions.data_ptr(), table.turns.data_ptr(),
+            qo.data_ptr(), None if k is None else ko.data_ptr())
 
 
 def _turn(q, k, positions, table, inverse, out=None):
-    """(q, k) turned, in `out` or in new tensors."""
-    tokens, heads, dim = q.shape
+    """(q, k) turned, in `out` or in new tensors; looks at q, k, positions and the table first, each attribute once."""
+    shape, index, dtype = q.shape, q.get_device(), q.dtype
+    good = len(shape) == 3 and index >= 0 and dtype in _DTYPES
+    if good:
+        tokens, heads, dim = shape
+        qt, qh, qd = q.stride()
+        good = (qd == 1 and heads > 0 and dim in HEAD_DIMS and table.rotary_dim <= dim and positions.shape == (tokens,)
+                and positions.dtype == torch.int32 and positions.get_device() == index and table.index == index
+                and (tokens < 2 or positions.stride(0) == 1))
+        ks, heads_k = (0, 0), 0
+        if good and k is not None:
+            other = k.shape
+            good = len(other) == 3 and other[0] == tokens and other[2] == dim and other[1] > 0 and k.dtype == dtype and k.get_device() == index
+            if good:
+                heads_k, (kt, kh, kd) = other[1], k.stride()
+                good, ks = kd == 1, (kt if tokens > 1 else 0, kh if heads_k > 1 else 0)
+    if not good:
+        _check_rotary(q, k, positions, table)
+        raise ValueError("q, k, positions and the table do not describe a call")
     if out is None:
-        out = (torch.empty_like(q, memory_format=torch.contiguous_format), None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format))
-    if tokens == 0 or heads == 0:
-        return out
-    qo, ko = out
-    call = _lib.Rotary(tokens, heads, 0 if k is None else k.shape[1], dim, table.rotary_dim, table.interleaved, inverse, _DTYPES[q.dtype], 0,
-                       table.magnitude, 0, *_strides(q), *_strides(k), *_strides(qo), *_strides(ko))
-    _run_on(q.get_device(), _lib.lib().moba_rotary, C.byref(call), q.data_ptr(), None if k is None else k.data_ptr(), positions.data_ptr(),
-            table.turns.data_ptr(), qo.data_ptr(), None if k is None else ko.data_ptr())
+        out = (torch.empty(shape, dtype=dtype, device=q.device), None if k is None else torch.empty(other, dtype=dtype, device=q.device))
+    else:
+        _check_out(q, k, out)
+    if tokens > 0:
+        _launch(q, k, positions, table, inverse, *out, shape, index, dtype, (heads_k, (qt if tokens > 1 else 0, qh if heads > 1 else 0), ks))
     return out
+
+
+def _check_out(q, k, out) -> None:
+    qo, ko = out
+    if (k is None) != (ko is None):
+        raise ValueError("out must have a tensor for each of q and k")
+    for name, x, y in (("out[0]", q, qo), ("out[1]", k, ko)):
+        if x is None or x is y:
+            continue
+        if y.shape != x.shape or y.dtype != x.dtype or y.get_device() != x.get_device():
+            raise ValueError(f"{name} must have the shape, dtype and device of what is turned")
+        if y.stride(2) != 1:
+            raise NotImplementedError(f"{name} must be contiguous in its last dimension")
+    _check_written(qo, ko)
 
 
 def _kernel_rows(x):
@@ -135,18 +176,14 @@ class _Rotary(torch.autograd.Function):
     """The operator is linear: its gradient is the turn back, its tangent the turn itself, and both may be differentiated again."""
 
     @staticmethod
-    def forward(q, k, positions, table, inverse):
+    def forward(ctx, q, k, positions, table, inverse):
         qo, ko = _turn(q, k, positions, table, inverse)
-        return qo if k is None else (qo, ko)
-
-    @staticmethod
-    def setup_context(ctx, inputs, output):
-        q, k, positions, ctx.table, ctx.inverse = inputs
         ctx.save_for_backward(positions)
         ctx.save_for_forward(positions)
-        ctx.alone = k is None
+        ctx.table, ctx.inverse, ctx.alone = table, inverse, k is None
         ctx.set_materialize_grads(False)
         ctx.like = tuple((x.shape, x.dtype, x.device) for x in (q, k) if x is not None)
+        return qo if k is None else (qo, ko)
 
     @staticmethod
     def _each(ctx, tensors, inverse):
@@ -155,7 +192,11 @@ class _Rotary(torch.autograd.Function):
         given = [None if x is None else _kernel_rows(x) for x in tensors]
         if all(x is None for x in given):
             return given
-        if len(given) == 2 and all(x is not None for x in given):
+        if not torch.is_grad_enabled() and getattr(forward_ad, "_current_level", 0) < 0:
+            if len(given) == 2 and given[0] is not None and given[1] is not None:
+                return list(_turn(*given, positions, ctx.table, inverse))
+            return [None if x is None else _turn(x, None, positions, ctx.table, inverse)[0] for x in given]
+        if len(given) == 2 and given[0] is not None and given[1] is not None:
             return list(_Rotary.apply(given[0], given[1], positions, ctx.table, inverse))
         return [None if x is None else _Rotary.apply(x, None, positions, ctx.table, inverse) for x in given]
 
@@ -179,7 +220,6 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
 
     Returns (q, k) turned, as new tensors, or written to `out`, which may be (q, k) themselves; tensors that lie on them otherwise are not
     allowed.  Gradients of both orders, and forward derivatives, are followed (not with `out`)."""
-    _check_rotary(q, k, positions, table)
     followed = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
     if not followed and getattr(forward_ad, "_current_level", 0) >= 0:
         followed = any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in (q, k))
@@ -190,17 +230,6 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         return (got, None) if k is None else got
     if followed:
         raise NotImplementedError("out is for rows that autograd does not follow")
-    qo, ko = out
-    if (k is None) != (ko is None):
-        raise ValueError("out must have a tensor for each of q and k")
-    for name, x, y in (("out[0]", q, qo), ("out[1]", k, ko)):
-        if x is None:
-            continue
-        if y.shape != x.shape or y.dtype != x.dtype or y.get_device() != x.get_device():
-            raise ValueError(f"{name} must have the shape, dtype and device of what is turned")
-        if y.stride(2) != 1:
-            raise NotImplementedError(f"{name} must be contiguous in its last dimension")
-    _check_written(qo, ko)
-    _turn(q, k, positions, table, False, (qo, ko))
-    _written(qo, ko)
+    _turn(q, k, positions, table, False, out)
+    _written(*out)
     return out
