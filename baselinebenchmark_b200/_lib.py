@@ -27,7 +27,8 @@ SYMBOLS = (
     "moba_attend", "moba_merge", "moba_attend_tile_rows", "moba_attend_tile_rows_for", "moba_problem_tile_rows", "moba_problem_attend_kernel", "moba_route_static",
     "moba_backward_workspace_size", "moba_backward",
     "moba_cp_workspace_size", "moba_cp_forward", "moba_cp_poll", "moba_cp_abort", "moba_selftest_bounded_wait",
-    "moba_paged_check", "moba_paged_store", "moba_paged_load", "moba_paged_workspace_size", "moba_paged_attention", "moba_paged_tree_attention", "moba_paged_keep",
+    "moba_paged_check", "moba_paged_store", "moba_paged_load", "moba_paged_workspace_size", "moba_paged_attention",
+    "moba_paged_tree_workspace_size", "moba_paged_tree_attention", "moba_paged_keep",
     "moba_page_pool_check", "moba_paged_reserve", "moba_paged_release",
     "moba_rotary_check", "moba_rotary", "moba_drafts_check", "moba_verify_drafts",
 )
@@ -164,6 +165,7 @@ def lib() -> C.CDLL:
         handle.moba_paged_store.argtypes = [pg, vp, vp, i32p, i32p, i32p, vp, vp, vp, vp, vp]
         handle.moba_paged_load.argtypes = [pg, i32p, i32p, i32p, vp, vp, vp, vp, vp, vp, vp]
         handle.moba_paged_workspace_size.argtypes = [pg, C.POINTER(sz)]
+        handle.moba_paged_tree_workspace_size.argtypes = [pg, C.POINTER(sz)]
         handle.moba_paged_tree_attention.argtypes = [pg, vp, i32p, i32p, i32p, i32p, vp, vp, vp, vp, vp, vp, vp, sz, vp]
         handle.moba_paged_attention.argtypes = [pg, vp, i32p, i32p, i32p, vp, vp, vp, vp, vp, vp, vp, sz, vp]
         handle.moba_paged_keep.argtypes = [pg, i32p, i32p, i32p, i32p, C.c_int64, C.c_int32, i32p, vp, vp, vp, vp, i32p, vp]

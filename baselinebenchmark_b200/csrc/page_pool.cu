@@ -1,10 +1,9 @@
 // Page tables, slots and positions from the lengths of requests, and pages given back, without the host.
 //
-// Free pages lie on a stack of numbers.  The entries of the tables that a call may change are one line, sequence by sequence: of a sequence
-// with new tokens those that the tokens lie in, of one that is cut those behind its kept tokens.  An entry that lacks a page (or has one to
-// give back) is number r of them, a prefix sum, and takes the r-th page from the top (or its place there, in the same order: what a call took, the
-// same cut puts back as it was).  A warp has a stretch of the line, its count goes to all blocks of the cluster, and every entry then knows its
-// number: no atomics, the same pages every time.
+// Free pages lie on a stack of numbers.  The entries that a call's new tokens lie in are one line, sequence by sequence.  One that lacks a page is
+// number r of those, a prefix sum, and takes the r-th page from the top; pages given back are numbered the same way, and the stack is left as the reserve that took
+// them found it.  A warp has a stretch of the line, its count goes to all blocks of the cluster, and every entry then knows its number: no
+// atomics, the same pages every time.
 // Slots and positions follow row by row; the depth of a row in a tree of drafted tokens by doubling, d(i) += d(up(i)), up(i) <- up(up(i)), which takes
 // as many rounds as the depth has bits.
 // All of it is a few KB: what bounds it is the chain of dependent loads and barriers, and the launches.  Small calls are one block, one launch.
@@ -18,16 +17,19 @@ namespace {
 
 constexpr int kThreads = 1024, kWarps = kThreads / 32;
 constexpr int kBlocks = 8;                 // of the cluster, where there is much to do
-constexpr int kSmallRows = 2048, kSmallEntries = 4096;
+constexpr int kSmallRows = 2048;            // that one block does
 
-struct Range {                             // entries of a sequence
+// Pages of a sequence's tokens, as many as its row of the table has room for.
+__device__ __forceinline__ int pages_of(const PoolParams& p, int b) {
+  const int64_t room = (int64_t)p.per_seq << p.page_shift, mask = ((int64_t)1 << p.page_shift) - 1;
+  return (int)((min(max((int64_t)__ldg(p.lens + b), (int64_t)0), room) + mask) >> p.page_shift);
+}
+struct Range {                             // entries of a sequence's packed tokens
   int first, count;
 };
 __device__ __forceinline__ Range entries_of(const PoolParams& p, int b) {
-  const int64_t room = (int64_t)p.per_seq << p.page_shift, mask = ((int64_t)1 << p.page_shift) - 1;
-  const int64_t len = min(max((int64_t)__ldg(p.lens + b), (int64_t)0), room);
-  const int up = (int)((len + mask) >> p.page_shift);
-  if (p.cu == nullptr) return Range{up, p.per_seq - up};    // behind the kept tokens
+  const int64_t room = (int64_t)p.per_seq << p.page_shift;
+  const int up = pages_of(p, b);
   const int64_t n = (int64_t)__ldg(p.cu + b + 1) - __ldg(p.cu + b);
   if (n <= 0) return Range{0, 0};
   const int from = (int)(min(max((int64_t)__ldg(p.lens + b) - n, (int64_t)0), room) >> p.page_shift);
@@ -98,8 +100,8 @@ __device__ __forceinline__ void double_depths(int* up, int* depth) {
   }
 }
 
-// kCut: pages are given back.  kRows: one block, which also does the rows.
-template <bool kCut, bool kRows>
+// Pages taken.  kRows: one block, which also does the rows.
+template <bool kRows>
 __global__ void __launch_bounds__(kThreads) pool_kernel(const PoolParams p) {
   extern __shared__ int32_t smem[];
   int32_t* begin = smem;                                    // [batch + 1]: first entry of a sequence on the line
@@ -139,11 +141,11 @@ __global__ void __launch_bounds__(kThreads) pool_kernel(const PoolParams p) {
   const int per = ((carry + warps - 1) / warps + 31) / 32 * 32;
   constexpr int kRound = 4, kStep = 32 * kRound;            // entries under way: of a lane, of a warp
   const int lo = (int)min((int64_t)per * me, (int64_t)carry), hi = (int)min((int64_t)lo + per, (int64_t)carry);
-  auto entry = [&](int at, int32_t*& place) {               // the entry's number, and whether it counts
+  auto entry = [&](int at, int32_t*& place) {               // not below 0: it lacks a page
     const int b = search(p.batch, at, [&](int k) { return (int64_t)begin[k]; });
     place = p.table + b * p.table_stride + first[b] + (at - begin[b]);
     const int id = *place;
-    return kCut ? ((unsigned)id < (unsigned)p.pages ? id : -1) : (unsigned)id < (unsigned)p.pages ? -1 : 0;
+    return (unsigned)id < (unsigned)p.pages ? -1 : 0;
   };
   int mine = 0, ids[kRound];
   int32_t* places[kRound];
@@ -173,7 +175,7 @@ __global__ void __launch_bounds__(kThreads) pool_kernel(const PoolParams p) {
       total += block_total[i];
     }
   }
-  // ---- pages taken, or put back
+  // ---- pages taken
   for (int at = lo; at < hi; at += kStep) {
     if (at > lo) load_round(at);
 #pragma unroll
@@ -181,21 +183,14 @@ __global__ void __launch_bounds__(kThreads) pool_kernel(const PoolParams p) {
       const uint32_t votes = __ballot_sync(0xffffffffu, ids[k] >= 0);
       const int r = before + __popc(votes & ((1u << lane) - 1));
       before += __popc(votes);
-      if (ids[k] < 0) continue;
-      if (kCut) {
-        const int64_t to = (int64_t)have + total - 1 - r;
-        if (to < p.pages) p.free[to] = ids[k];
-        *places[k] = -1;
-      } else if (r < have) {
-        *places[k] = p.free[have - 1 - r];
-      }
+      if (ids[k] >= 0 && r < have) *places[k] = p.free[have - 1 - r];
     }
   }
   if (rank == 0 && tid == 0) {
-    *p.count = kCut ? (int)min((int64_t)have + total, (int64_t)p.pages) : max(have - total, 0);
-    if (!kCut) *p.missing = max(total - have, 0);
+    *p.count = max(have - total, 0);
+    *p.missing = max(total - have, 0);
   }
-  if constexpr (kRows && !kCut) {
+  if constexpr (kRows) {
     // ---- the rows
     __shared__ int32_t up[kSmallRows], depth[kSmallRows];
     constexpr int kPer = kSmallRows / kThreads;
@@ -226,6 +221,76 @@ __global__ void __launch_bounds__(kThreads) pool_kernel(const PoolParams p) {
       p.positions[row] = on[k] ? clamp_position(r[k].pos0 + (p.parents != nullptr ? depth[row] : r[k].i)) : -1;
   }
   }
+}
+
+// Pages given back.  The tables are looked through in units of kSegment entries of a row, an even share of them a warp: counted, then (units that
+// have some) numbered and moved.
+constexpr int kSegment = 1024, kAbreast = 8;   // entries that a lane has under way
+template <bool kOne>
+__global__ void __launch_bounds__(kThreads) pool_cut_kernel(const PoolParams p) {
+  __shared__ int32_t counts[kWarps], block_total[kBlocks];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = kOne ? 0 : cluster_rank(), blocks = kOne ? 1 : cluster_size();
+  pdl_wait();
+  pdl_trigger();
+  const int have = min(max(__ldcg(p.count), 0), p.pages);
+  const int segments = (p.per_seq + kSegment - 1) / kSegment, warps = (int)blocks * kWarps, me = (int)rank * kWarps + warp;
+  const int64_t units = (int64_t)p.batch * segments, lo = units * me / warps, hi = units * (me + 1) / warps;
+  // runs `step(entries, first column, end)` over a unit, 32 * kAbreast entries at a time
+  auto over = [&](int64_t unit, auto&& step) {
+    const int b = (int)(unit / segments), from = (int)(unit - (int64_t)b * segments) * kSegment;
+    const int end = min(from + kSegment, p.per_seq);
+    int32_t* row = p.table + b * p.table_stride;
+    for (int at = max(from, pages_of(p, b)); at < end; at += 32 * kAbreast) {
+      int ids[kAbreast];
+#pragma unroll
+      for (int k = 0; k < kAbreast; ++k) {
+        const int column = at + 32 * k + lane;
+        ids[k] = column < end ? __ldcg(row + column) : -1;
+        if ((unsigned)ids[k] >= (unsigned)p.pages) ids[k] = -1;
+      }
+      step(ids, row + at);
+    }
+  };
+  int mine = 0;
+  uint32_t some = 0;                                        // units with pages; those from the 32nd on as one
+  for (int64_t unit = lo; unit < hi; ++unit) {
+    int n = 0;
+    over(unit, [&](const int (&ids)[kAbreast], int32_t*) {
+#pragma unroll
+      for (int k = 0; k < kAbreast; ++k) n += __popc(__ballot_sync(0xffffffffu, ids[k] >= 0));
+    });
+    mine += n;
+    if (n > 0) some |= 1u << (int)min(unit - lo, (int64_t)31);
+  }
+  if (lane == 0) counts[warp] = mine;
+  __syncthreads();
+  const int c = counts[lane], block_sum = __reduce_add_sync(0xffffffffu, c);
+  int before = __reduce_add_sync(0xffffffffu, lane < warp ? c : 0), total = block_sum;
+  if (!kOne) {
+    if (warp == 0 && lane < (int)blocks) cluster_store(cluster_place(&block_total[rank], lane), (uint32_t)block_sum);
+    cluster_sync();
+    total = 0;
+    for (int i = 0; i < (int)blocks; ++i) {
+      if (i < (int)rank) before += block_total[i];
+      total += block_total[i];
+    }
+  }
+  for (int64_t unit = lo; unit < hi; ++unit) {
+    if (!((some >> (int)min(unit - lo, (int64_t)31)) & 1)) continue;
+    over(unit, [&](const int (&ids)[kAbreast], int32_t* row) {
+#pragma unroll
+      for (int k = 0; k < kAbreast; ++k) {
+        const uint32_t votes = __ballot_sync(0xffffffffu, ids[k] >= 0);
+        const int64_t to = (int64_t)have + total - 1 - before - __popc(votes & ((1u << lane) - 1));
+        before += __popc(votes);
+        if (ids[k] < 0) continue;
+        if (to >= 0 && to < p.pages) p.free[to] = ids[k];
+        row[32 * k + lane] = -1;
+      }
+    });
+  }
+  if (rank == 0 && threadIdx.x == 0) *p.count = (int)min((int64_t)have + total, (int64_t)p.pages);
 }
 
 // A row a thread.  With parents the position is there already.
@@ -312,21 +377,17 @@ cudaError_t launch_pool(const PoolParams& p, cudaStream_t st) {
   const size_t smem = (2 * (size_t)p.batch + 1) * sizeof(int32_t);
   cudaError_t e;
   if (p.cu == nullptr) {
-    // one block where a round of its threads has all entries there can be
-    const bool small = (int64_t)p.batch * p.per_seq <= kSmallEntries;
-    if (small) {
-      if ((e = prepare_kernel(pool_kernel<true, true>, smem)) != cudaSuccess) return e;
-      return launch_pdl(pool_kernel<true, true>, dim3(1), kThreads, smem, st, p);
-    }
-    if ((e = prepare_kernel(pool_kernel<true, false>, smem)) != cudaSuccess) return e;
-    return launch_clusters(pool_kernel<true, false>, kBlocks, dim3(kBlocks), kThreads, smem, st, p);
+    // (units: two for each warp of a block)
+    const int64_t units = (int64_t)p.batch * ((p.per_seq + kSegment - 1) / kSegment);
+    return units <= 2 * kWarps ? launch_pdl(pool_cut_kernel<true>, dim3(1), kThreads, 0, st, p)
+                               : launch_clusters(pool_cut_kernel<false>, kBlocks, dim3(kBlocks), kThreads, 0, st, p);
   }
   if (p.rows <= kSmallRows) {
-    if ((e = prepare_kernel(pool_kernel<false, true>, smem)) != cudaSuccess) return e;
-    return launch_pdl(pool_kernel<false, true>, dim3(1), kThreads, smem, st, p);
+    if ((e = prepare_kernel(pool_kernel<true>, smem)) != cudaSuccess) return e;
+    return launch_pdl(pool_kernel<true>, dim3(1), kThreads, smem, st, p);
   }
-  if ((e = prepare_kernel(pool_kernel<false, false>, smem)) != cudaSuccess) return e;
-  if ((e = launch_clusters(pool_kernel<false, false>, kBlocks, dim3(kBlocks), kThreads, smem, st, p)) != cudaSuccess) return e;
+  if ((e = prepare_kernel(pool_kernel<false>, smem)) != cudaSuccess) return e;
+  if ((e = launch_clusters(pool_kernel<false>, kBlocks, dim3(kBlocks), kThreads, smem, st, p)) != cudaSuccess) return e;
   const dim3 grid((unsigned)((p.rows + kRowThreads - 1) / kRowThreads));
   if (p.parents != nullptr) {
     constexpr size_t way_smem = 3 * kWayRows * sizeof(int32_t);

@@ -106,7 +106,22 @@ inline bool paged_few_rows(const PagedParams& p) {
 }
 
 // Both kernels have a form for trees of drafted tokens (PagedParams::parents), each in a source file of its own.
+// Of trees over 16-bit pages up to 64 rows also where they are so few, before keys so few, that the other kernel's launches and items cost more than reading
+// the keys again for each 16 rows.  The lengths are on the device: what the tables have room for stands for them.  (rows: this kernel / tcgen05, us)
+//   head dim 64           1 sequence of 4000, 4 kv heads  32: 15 / 27, 64: 17 / 27     8 of 8000, 8  32: 56 / 60, 48: 72 / 61     48 of 500, 8  64: 51 / 62
+//   head dim 128          1 sequence of 4000, 8 kv heads  32: 22 / 31, 64: 25 / 31     4 of 8000, 8  32: 45 / 60, 48: 65 / 60     8 of 8000, 8  32: 103 / 78
+//                         2 of 8000, 8                    48: 38 / 43, 64: 43 / 43     1 of 40000, 8  48: 69 / 71
+//   head dim 256          1 sequence of 4000, 8 kv heads  32: 31 / 39, 64: 42 / 41     2 of 8000, 8  32: 62 / 58
+inline bool paged_few_tree(const PagedParams& p) {
+  if (paged_few_rows(p)) return true;
+  const int64_t rows = (int64_t)p.max_new * p.G, again = (rows + 15) / 16 - 1;
+  if (p.store != MOBA_STORE_SAME || rows > 64) return false;
+  const double elements = (double)p.B * p.Hkv * ((int64_t)p.per_seq << p.page_shift) * p.D;
+  return elements * again <= (p.D == 256 ? 24e6 : 48e6);
+}
+
 size_t paged_rows_workspace(const PagedParams& p);
+size_t paged_rows_tree_workspace(const PagedParams& p);
 cudaError_t launch_paged_rows(const PagedParams& p, const void* q, const void* kp, const void* vp, const uint8_t* ks,
                               const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st);
 size_t paged_few_workspace(const PagedParams& p);

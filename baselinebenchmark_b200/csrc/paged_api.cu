@@ -76,7 +76,10 @@ int check_pointers(const moba_paged_t* p, const void* a, const void* b, const in
   return MOBA_OK;
 }
 
-size_t workspace_of(const PagedParams& p) { return paged_few_rows(p) ? paged_few_workspace(p) : paged_rows_workspace(p); }
+size_t workspace_of(const PagedParams& p, bool tree) {
+  if (tree) return paged_few_tree(p) ? paged_few_workspace(p) : paged_rows_tree_workspace(p);
+  return paged_few_rows(p) ? paged_few_workspace(p) : paged_rows_workspace(p);
+}
 
 // Rows that are written must not lie on one another (a single token or head is never stepped over).
 bool apart(const moba_paged_t* p, int64_t token, int64_t head, int heads) {
@@ -107,13 +110,15 @@ int moba_paged_load(const moba_paged_t* p, const int32_t* cu, const int32_t* len
   return (int)launch_paged_load(paged_params(p, cu, lens, table), kp, vp, ks, vs, k, v, (cudaStream_t)stream);
 }
 
-int moba_paged_workspace_size(const moba_paged_t* p, size_t* bytes) {
+static int workspace_size(const moba_paged_t* p, bool tree, size_t* bytes) {
   const int rc = check_paged(p);
   if (rc != MOBA_OK) return rc;
   if (bytes == nullptr) return MOBA_E_NULL;
-  *bytes = workspace_of(paged_params(p, nullptr, nullptr, nullptr));
+  *bytes = workspace_of(paged_params(p, nullptr, nullptr, nullptr), tree);
   return MOBA_OK;
 }
+int moba_paged_workspace_size(const moba_paged_t* p, size_t* bytes) { return workspace_size(p, false, bytes); }
+int moba_paged_tree_workspace_size(const moba_paged_t* p, size_t* bytes) { return workspace_size(p, true, bytes); }
 
 int moba_paged_attention(const moba_paged_t* p, const void* q, const int32_t* cu, const int32_t* lens, const int32_t* table,
                          const void* kp, const void* vp, const uint8_t* ks, const uint8_t* vs, void* out, float* lse_out,
@@ -131,9 +136,9 @@ int moba_paged_tree_attention(const moba_paged_t* p, const void* q, const int32_
   if (((uintptr_t)lse_out | (uintptr_t)parents) & 3) return MOBA_E_ALIGN;
   PagedParams r = paged_params(p, cu, lens, table);
   r.parents = parents;
-  if (workspace == nullptr || workspace_bytes < workspace_of(r)) return MOBA_E_WORKSPACE;
+  if (workspace == nullptr || workspace_bytes < workspace_of(r, parents != nullptr)) return MOBA_E_WORKSPACE;
   if ((uintptr_t)workspace & 31) return MOBA_E_ALIGN;
-  const auto launch = paged_few_rows(r) ? (parents ? launch_paged_few_tree : launch_paged_few) : parents ? launch_paged_rows_tree : launch_paged_rows;
+  const auto launch = parents ? (paged_few_tree(r) ? launch_paged_few_tree : launch_paged_rows_tree) : paged_few_rows(r) ? launch_paged_few : launch_paged_rows;
   return (int)launch(r, q, kp, vp, ks, vs, out, lse_out, workspace, (cudaStream_t)stream);
 }
 

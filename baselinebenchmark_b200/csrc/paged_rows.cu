@@ -3,7 +3,7 @@
 
 namespace moba {
 
-size_t paged_rows_workspace(const PagedParams& p) { return rows_workspace(p); }
+size_t paged_rows_workspace(const PagedParams& p) { return rows_workspace(p, false); }
 
 cudaError_t launch_paged_rows(const PagedParams& p, const void* q, const void* kp, const void* vp, const uint8_t* ks,
                               const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st) {

@@ -60,6 +60,16 @@ int rows_slots(const PagedParams& p) {
   const int64_t tiles = p.T * p.G / item_rows(p.D) + (p.T < p.B ? p.T : p.B);
   return (int)(tiles * p.Hkv >= kMostSlots ? kMostSlots : tiles * p.Hkv * cuts < kMostSlots ? tiles * p.Hkv * cuts : kMostSlots);
 }
+// Trees on a line (see paged_tree_plan_kernel): two slots for each CTA that has a stretch of it.
+constexpr int kTreeLeast = 8;              // units of a stretch, at least
+constexpr int kTreeItem = 4, kTreePiece = 2;   // what an item costs besides its key tiles, in tiles, and what more when it is cut
+int tree_slots(const PagedParams& p) {
+  const int64_t keys = ((int64_t)p.per_seq << p.page_shift), units = (keys + kBN - 1) / kBN + kTreeItem;
+  const int64_t items = (p.T < p.B ? p.T : p.B) * (int64_t)p.Hkv;
+  const int64_t ctas = items >= 148 * kTreeLeast || items * units >= 148 * kTreeLeast ? 148 : items * units / kTreeLeast;
+  const int slots = rows_slots(p);
+  return slots > 2 * ctas ? slots : (int)(2 * ctas);
+}
 constexpr float kLn2 = 0.6931471805599453f;
 
 // ---- the plan ------------------------------------------------------------------
@@ -67,7 +77,8 @@ constexpr float kLn2 = 0.6931471805599453f;
 struct RowsPlan {
   int32_t counter, status;                 // items drawn; a bounded wait gave up
   int32_t items;
-  int32_t pad;
+  int32_t ctas;                            // of trees that lie on a line (see paged_tree_plan_kernel): CTAs that share it; else 0
+  int32_t each, rest;                      // its units of each of them, of the first `rest` one more
   int32_t begin[kPagedBatch + 1];          // first item of a sequence
   int32_t slot0[kPagedBatch];              // first result slot of a sequence whose items are cut
   int32_t piece[kPagedBatch];              // key tiles of a piece
@@ -180,19 +191,75 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p, R
   }
 }
 
+// What packed row t sees of the kTreeGroup packed rows of its group (those with the same t / kTreeGroup), and the nearest ancestor in front of it (-1:
+// none).  A row's branch is a walk along its ancestors, a load from L2 each where shared memory leaves no L1: with the walk in the softmax of
+// the last key tile 24 trees of 64 rows took 267 us where they take 229 without it.  Here the walk is one through shared memory.
+constexpr int kTreeGroup = 128;
+struct alignas(32) TreeMask {
+  uint32_t bits[4];
+  int32_t exit;
+  int32_t pad[3];
+};
+// Of 1024 packed rows from `base` on; all threads of a block.
+__device__ __forceinline__ void tree_masks(const PagedParams& p, TreeMask* masks, int64_t base, int* up) {
+  const int64_t t = base + threadIdx.x;
+  int parent = -1;
+  bool on = false;
+  if (t < p.T) {
+    int b = 0, n = p.B;
+    while (n > 1) {
+      const int half = n >> 1;
+      const bool more = __ldg(p.cu + b + half) <= t;
+      b = more ? b + half : b;
+      n = more ? n - half : half;
+    }
+    const PagedSeq s = paged_seq(p, b);
+    const int64_t i = t - s.row0;
+    on = i >= 0 && i < s.n;
+    if (on) {
+      const int of = __ldg(p.parents + t);
+      if (of >= 0 && of < i) parent = s.row0 + of;          // (rows are counted in 32 bits)
+    }
+  }
+  up[threadIdx.x] = parent;
+  __syncthreads();
+  if (t >= p.T) return;
+  const int group = (int)threadIdx.x & ~(kTreeGroup - 1);   // its first row, from `base`
+  uint64_t lo = 0, hi = 0;
+  int64_t at = t;
+  do {
+    const int bit = (int)at & (kTreeGroup - 1);
+    if (bit < 64) lo |= 1ull << bit; else hi |= 1ull << (bit - 64);
+    at = up[at - base];
+  } while (at >= base + group);
+  TreeMask m{};
+  m.bits[0] = (uint32_t)lo; m.bits[1] = (uint32_t)(lo >> 32); m.bits[2] = (uint32_t)hi; m.bits[3] = (uint32_t)(hi >> 32);
+  m.exit = (int)at;
+  if (!on) m = TreeMask{{0, 0, 0, 0}, -1, {0, 0, 0}};
+  masks[t] = m;
+}
+static_assert(1024 % kTreeGroup == 0, "groups do not lie in two blocks");
+
 // Trees: few rows behind keys of any number, so that a batch is a few hundred items of all lengths, and what counts is that no CTA is left with a long
-// one at the end.  Items are drawn longest first, and a candidate's time is the largest of what no order can beat: the work of all, evenly; the
+// one at the end.
+// Where no sequence has more than one row tile, the items are a line of units, kTreeItem in front of each for what it costs besides its key
+// tiles, and every CTA has an equal stretch of it: the end of an item, whole ones, the beginning of one.  Its two parts of items
+// go to two slots of results of its own, and the join finds an item's parts by where it lies on the line.
+// Otherwise row tiles see different numbers of keys, and those of one head read the same ones: items are drawn longest first, and a candidate's time is the largest of what no order can beat: the work of all, evenly; the
 // longest item; and k items of the length of number (k - 1) * SMs + 1, of which some CTA has k.  Candidates go down from the longest
 // sequence in even steps of a ratio.
-// (24 trees of 64 rows behind 1K to 16K tokens, 8 kv heads: 22 key tiles a piece in the order of the sequences, 274 us; 63, longest first, 246.)
+// Behind the plan's block, others write down what each packed row sees of the rows around it (see TreeMask).
 constexpr int kTreeSorted = 128;           // sequences up to which it is worth looking at their order
-constexpr int kTreeItem = 4, kTreePiece = 2;   // what an item costs besides its key tiles, in tiles, and what more when it is cut
-__global__ void __launch_bounds__(1024) paged_tree_plan_kernel(const PagedParams p, RowsPlan* plan, int sms, int most_slots) {
+__global__ void __launch_bounds__(1024) paged_tree_plan_kernel(const PagedParams p, RowsPlan* plan, TreeMask* masks, int sms, int most_slots) {
   __shared__ int rows_s[kPagedBatch], most_s[kPagedBatch], least_s[kPagedBatch];
   __shared__ float cost_s[32];
   __shared__ int piece_s[32], scan_s[2][32];
   pdl_wait();
   pdl_trigger();
+  if (blockIdx.x > 0) {
+    tree_masks(p, masks, (int64_t)(blockIdx.x - 1) * 1024, rows_s);
+    return;
+  }
   const int b = threadIdx.x, warp = b >> 5, lane = b & 31;
   int rows = 0, most = 1, least = 1;
   if (b < p.B) {
@@ -207,7 +274,37 @@ __global__ void __launch_bounds__(1024) paged_tree_plan_kernel(const PagedParams
   rows_s[b] = rows;
   most_s[b] = most;
   least_s[b] = least;
-  __syncthreads();
+  // ---- a line?
+  {
+    const int units = rows > 0 ? most + kTreeItem : 0;
+    // (rows: kv heads of the one row tile)
+    const bool good = rows <= p.Hkv && (int64_t)units * p.Hkv < ((int64_t)1 << 20);
+    const int mine = rows > 0 ? units * p.Hkv : 0;
+    if (__syncthreads_and(good)) {
+      int x = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += u;
+      }
+      if (lane == 31) scan_s[0][warp] = x;
+      __syncthreads();
+      const int all = __reduce_add_sync(0xffffffffu, scan_s[0][lane]), before = __reduce_add_sync(0xffffffffu, lane < warp ? scan_s[0][lane] : 0);
+      const int ctas = max(min(min(sms, most_slots / 2), all / kTreeLeast), 1);
+      if (b < p.B) {
+        plan->begin[b] = before + x - mine;
+        if (b == p.B - 1) {
+          plan->begin[p.B] = all;
+          plan->ctas = ctas;
+          plan->each = all / ctas;
+          plan->rest = all % ctas;
+          plan->status = 0;
+          plan->items = 0;
+        }
+      }
+      return;
+    }
+  }
   int longest = 1;
   for (int i = lane; i < p.B; i += 32)
     if (rows_s[i] > 0) longest = max(longest, most_s[i]);
@@ -290,8 +387,15 @@ __global__ void __launch_bounds__(1024) paged_tree_plan_kernel(const PagedParams
       plan->items = bx + x;
       plan->counter = 0;
       plan->status = 0;
+      plan->ctas = 0;
     }
   }
+}
+// Where the stretch of CTA c begins, and whose a unit is.
+__device__ __forceinline__ int line_first(int each, int rest, int c) { return each * c + min(c, rest); }
+__device__ __forceinline__ int line_cta(int each, int rest, int u) {
+  const int more = (each + 1) * rest;                       // units of those that have one more
+  return u < more ? u / (each + 1) : rest + (u - more) / max(each, 1);
 }
 
 // ---- items ---------------------------------------------------------------------
@@ -339,6 +443,7 @@ struct RowsArgs {
   float* part;                             // [slots][rows of an item][D]
   float2* part_ml;                         // the same rows: {maximum, sum}
   FastDiv by_group;
+  const TreeMask* masks;                   // of trees: a packed row each
 };
 
 // Items that are not cut come longest first, all heads by turns, where the K and V of all heads stay in L2 together; otherwise head by head, so that
@@ -348,13 +453,46 @@ constexpr int64_t kAllHeadsBytes = (int64_t)80 << 20;
 // Both row tiles have the item's rows, and the key tiles by turns.
 __device__ __forceinline__ bool rows_twice(int D, const RowsItem& it) { return D != 256 && it.nrows <= kTileM; }
 
+// A CTA's stretch of the line, from `u` on; `ctas` 0: items are drawn.
+struct RowsLine {
+  int ctas, u, last;
+};
+__device__ __forceinline__ RowsLine rows_line(const RowsArgs& a) {
+  RowsLine line{__ldcg(&a.plan->ctas), 0, 0};
+  if (line.ctas > 0) {
+    const int each = __ldcg(&a.plan->each), rest = __ldcg(&a.plan->rest), c = (int)blockIdx.x;
+    line.u = line_first(each, rest, min(c, line.ctas));
+    line.last = c < line.ctas ? line_first(each, rest, c + 1) : line.u;
+  }
+  return line;
+}
+
 // Warp 2, one item ahead of the others.
 template <bool kTree>
-__device__ __forceinline__ void rows_prefetch(const PagedParams& p, const RowsArgs& a, RowsCtrl& c, int at) {
+__device__ __forceinline__ void rows_prefetch(const PagedParams& p, const RowsArgs& a, RowsCtrl& c, int at, RowsLine& line) {
   const int lane = threadIdx.x & 31;
   RowsItem it;
   bool done = false;
   for (;;) {
+    if (kTree && line.ctas > 0) {
+      if (line.u >= line.last || c.abort) { done = true; break; }
+      it.b = search_warp(p.B, line.u, [&](int k) { return __ldcg(a.plan->begin + k); });
+      const PagedSeq s = paged_seq(p, it.b);
+      const int begin = __ldcg(a.plan->begin + it.b), tiles = key_tiles(rows_end(p, s, 0)), length = tiles + kTreeItem;
+      it.h = (line.u - begin) / length;
+      const int on = line.u - begin - it.h * length - kTreeItem;
+      it.j0 = max(on, 0);
+      it.ntiles = min(tiles, on + (line.last - line.u)) - it.j0;
+      line.u += tiles - on;
+      if (it.ntiles <= 0) continue;                         // (what is left of the stretch is not a key tile: the next CTA's item)
+      it.tile = 0;
+      it.nrows = (int)min((int64_t)s.n * p.G, (int64_t)item_rows(p.D));
+      it.row0 = s.row0;
+      it.pos0 = s.pos0;
+      it.len = s.len;
+      it.slot = it.ntiles == tiles ? -1 : 2 * (int)blockIdx.x + (it.j0 == 0 ? 1 : 0);
+      break;
+    }
     int idx = 0;
     if (lane == 0) idx = c.abort ? 0x7fffffff : atomicAdd(&a.plan->counter, 1);
     idx = __shfl_sync(0xffffffffu, idx, 0);
@@ -743,9 +881,38 @@ __device__ __forceinline__ void zero_rows(unsigned char* tile, const RowsItem& i
   }
 }
 
-// What row i of an item's sequence sees of the key tile from key0 on; `lim`: the keys below that it might see (0: it is no row).
+// The branch of a row in the key tile from key0 on, whatever pages there are: the keys in front of the packed rows, and of those the ones that
+// packed row t's masks say.  The tile's packed rows lie in two groups; farther groups are passed by their exits.
+__device__ __forceinline__ RowSees<true> branch_keys(const TreeMask* masks, const RowsItem& it, int i, int key0) {
+  const int64_t front = (int64_t)it.pos0 - key0;            // keys of the tile in front of the packed rows
+  const int64_t first = it.row0 - front;                    // packed row of the tile's first key (below row0 in front)
+  const int64_t group = first >> 7;
+  const int off = (int)(first & 127);
+  static_assert(kTreeGroup == 128, "a key tile");
+  auto load = [&](int64_t t, uint64_t& lo, uint64_t& hi) {
+    const uint4 w = __ldcg(reinterpret_cast<const uint4*>(masks[t].bits));
+    lo = w.x | (uint64_t)w.y << 32;
+    hi = w.z | (uint64_t)w.w << 32;
+    return (int64_t)__ldcg(&masks[t].exit);
+  };
+  uint64_t a0 = 0, a1 = 0, b0 = 0, b1 = 0;
+  int64_t at = (int64_t)it.row0 + i;
+  while ((at >> 7) > group + 1) at = __ldcg(&masks[at].exit);   // (each in front of the last; -1 ends it)
+  if (at >= 0 && (at >> 7) == group + 1) at = load(at, b0, b1);
+  if (at >= 0 && (at >> 7) == group) load(at, a0, a1);
+  // 128 bits from bit `off` of the two groups' 256 on
+  const uint64_t x0 = off & 64 ? a1 : a0, x1 = off & 64 ? b0 : a1, x2 = off & 64 ? b1 : b0;
+  const int s = off & 63;
+  uint64_t lo = s ? x0 >> s | x1 << (64 - s) : x0, hi = s ? x1 >> s | x2 << (64 - s) : x1;
+  if (front > 0) {
+    lo |= front >= 64 ? ~0ull : (1ull << front) - 1;
+    if (front > 64) hi |= front >= 128 ? ~0ull : (1ull << (front - 64)) - 1;
+  }
+  return RowSees<true>{{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)}};
+}
+// What a row sees of the key tile from key0 on; `lim`: the keys below that it might see (0: it is no row), `branch`: of those (trees).
 template <bool kTree>
-__device__ __forceinline__ RowSees<kTree> row_sees(const PagedParams& p, const RowsItem& it, int i, int lim, int key0, uint32_t there) {
+__device__ __forceinline__ RowSees<kTree> row_sees(const RowSees<kTree>& branch, int lim, int key0, uint32_t there) {
   if constexpr (!kTree) {
     return RowSees<false>{lim - key0, there};
   } else {
@@ -754,7 +921,7 @@ __device__ __forceinline__ RowSees<kTree> row_sees(const PagedParams& p, const R
     for (int w = 0; w < 4; ++w) {
       const int rem = lim - key0 - 32 * w;
       const uint32_t pages = ((there >> (2 * w)) & 1 ? 0xffffu : 0u) | ((there >> (2 * w + 1)) & 1 ? 0xffff0000u : 0u);
-      s.keys[w] = rem <= 0 ? 0u : tree_keys(p.parents + it.row0, i, it.pos0, key0 + 32 * w) & pages & (rem >= 32 ? 0xffffffffu : (1u << rem) - 1u);
+      s.keys[w] = rem <= 0 ? 0u : branch.keys[w] & pages & (rem >= 32 ? 0xffffffffu : (1u << rem) - 1u);
     }
     return s;
   }
@@ -826,6 +993,8 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
     const uint32_t dv = __shfl_sync(0xffffffffu, desc_lo(sV, kHalfBytes), 0);
     const uint32_t el = elect_one();
     bool ended = false;
+    RowsLine line{0, 0, 0};
+    if (kTree && warp == 2) line = rows_line(a);
     auto end_tiles = [&] {                                  // warp 0: there are no more tiles of codes
       const uint32_t s = kc % kInfoSlots;
       if (lane == 0 && mbar_wait(smem_u32(&c.info_empty[s]), ((kc / kInfoSlots) & 1) ^ 1)) {
@@ -836,7 +1005,7 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
       ended = true;
     };
     for (int n = 0;; ++n) {
-      if (warp == 2) rows_prefetch<kTree>(p, a, c, n & 1);
+      if (warp == 2) rows_prefetch<kTree>(p, a, c, n & 1, line);
       if (!rows_next<false, D, kCodes>(a, c, smem, n & 1)) break;
       const RowsItem& it = c.item[n & 1];
       if (kCodes && warp == 0) {
@@ -1099,11 +1268,13 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
       uint32_t g = kt;                                      // the CTA's tiles before this one
       if (x == 0) {
         for (int j = 0; ok && j < ntiles; ++j, ++g) {
+          const int key0 = (j0 + j) * kBN;
+          RowSees<kTree> branch{};
+          if constexpr (kTree) { if (lim > 0 && key0 + kBN > lim_first) branch = branch_keys(a.masks, it, i_row, key0); }
           ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&c.s_full[g & 1]), (g >> 1) & 1));
           if (!ok) break;
           tc_fence_after();
           const uint32_t tSg = tmem + lane_base + (g & 1) * kBN;
-          const int key0 = (j0 + j) * kBN;
           const uint32_t there = c.there[g & 3];
           // the P.V of tile g - 1 must have executed before O is touched (that of tile g - 2 has)
           auto quiet = [&] {
@@ -1111,7 +1282,7 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
             tc_fence_after();
           };
           if (key0 + kBN > lim_first || there != 0xff || !rows_softmax<false, kHalf, D, kCodes, kTree>(tSg, tO, j == 0, {}, p.sl2, rr, quiet))
-            rows_softmax<true, kHalf, D, kCodes, kTree>(tSg, tO, j == 0, row_sees<kTree>(p, it, i_row, lim, key0, there), p.sl2, rr, quiet);
+            rows_softmax<true, kHalf, D, kCodes, kTree>(tSg, tO, j == 0, row_sees<kTree>(branch, lim, key0, there), p.sl2, rr, quiet);
           // completions of o_full stay at most one behind: the parity of a tile never answers for an older one
           if (j > 0 && !mbar_wait(smem_u32(&c.o_full[0]), (g - 1) & 1)) ok = false;
           ok = __all_sync(0xffffffffu, ok);
@@ -1144,14 +1315,16 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
       } else {
         const int j1 = twice ? x : 0, by = twice ? 2 : 1;
         for (int j = j1; ok && j < ntiles; j += by) {
+          const int key0 = (j0 + j) * kBN;
+          RowSees<kTree> branch{};                          // (asked for before the scores are waited for)
+          if constexpr (kTree) { if (lim > 0 && key0 + kBN > lim_first) branch = branch_keys(a.masks, it, i_row, key0); }
           ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&c.s_full[x]), sph));
           if (!ok) break;
           sph ^= 1;
           tc_fence_after();
-          const int key0 = (j0 + j) * kBN;
           const uint32_t there = c.there[(kt + j) & 3];
           if (key0 + kBN > lim_first || there != 0xff || !rows_softmax<false, kHalf, D, kCodes, kTree>(tS, tO, j == j1, {}, p.sl2, rr, [] {}))
-            rows_softmax<true, kHalf, D, kCodes, kTree>(tS, tO, j == j1, row_sees<kTree>(p, it, i_row, lim, key0, there), p.sl2, rr, [] {});
+            rows_softmax<true, kHalf, D, kCodes, kTree>(tS, tO, j == j1, row_sees<kTree>(branch, lim, key0, there), p.sl2, rr, [] {});
           tc_fence_before();
           mbar_arrive(smem_u32(&c.p_full[x]));
         }
@@ -1359,49 +1532,39 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
 }
 
 // ---- the pieces' results, joined -------------------------------------------------
-// A warp for each packed row (token, head).  Rows whose items were not cut are there already.
+// A warp for each packed row (token, head) whose item was cut.  The others are there already.
 constexpr int kJoinThreads = 256;
+// Piece k of a row's item is in slot `first` for k = 0, else base + k * step.
+struct RowsPieces {
+  int64_t first, base;
+  int step, count;
+};
+// Row r of its item.  `failed`: a bounded wait gave up.
 template <bool kHalf, int D>
-__global__ void __launch_bounds__(kJoinThreads) paged_rows_join_kernel(const PagedParams p, const RowsArgs a) {
-  pdl_wait();
-  pdl_trigger();
-  const int64_t g = (int64_t)blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
+__device__ __forceinline__ void join_row(const PagedParams& p, const RowsArgs& a, const RowsPieces& pieces, int r, int64_t token, int head,
+                                         bool failed) {
   const int lane = threadIdx.x & 31;
-  const int64_t token = g / p.Hq;
-  const int head = (int)(g - token * p.Hq);
-  if (token >= p.T || token < __ldg(p.cu) || token >= __ldg(p.cu + p.B)) return;
-  const int b = search_warp(p.B, (int)token, [&](int k) { return __ldg(p.cu + k); });
-  const PagedSeq s = paged_seq(p, b);
-  const int i = (int)(token - s.row0);
-  if (i < 0 || i >= s.n) return;
+  constexpr int kRows = item_rows(D);
   constexpr int kPer = D / 32;                              // elements of a lane
   __nv_bfloat16* dst = a.out + token * p.so_t + (int64_t)head * p.so_h + lane * kPer;
   float x[kPer];
 #pragma unroll
   for (int u = 0; u < kPer; ++u) x[u] = 0.f;
   float mx = -INFINITY, sum = 0.f;
-  if (__ldcg(&a.plan->status) != 0) {
-    sum = __uint_as_float(0x7fc00000u);                     // a bounded wait gave up: NaN in place of half a result
+  if (failed) {
+    sum = __uint_as_float(0x7fc00000u);                     // NaN in place of half a result
     mx = 0.f;
   } else {
-    const int slot0 = __ldcg(a.plan->slot0 + b);
-    if (slot0 < 0) return;
-    const int tiles = rows_tiles(p, s.n), piece = __ldcg(a.plan->piece + b);
-    const int cuts = (key_tiles(rows_end(p, s, tiles - 1)) + piece - 1) / piece;
-    const int h = head / p.G;
-    constexpr int kRows = item_rows(D);
-    const int row = i * p.G + head - h * p.G, tile = row / kRows, r = row - tile * kRows;
-    const int mine = (key_tiles(rows_end(p, s, tile)) + piece - 1) / piece;
     // several pieces under way at a time
     constexpr int kAhead = kPer > 4 ? 4 : 8;
-    for (int k0 = 0; k0 < mine; k0 += kAhead) {
+    for (int k0 = 0; k0 < pieces.count; k0 += kAhead) {
       float2 ml[kAhead];
       float v[kAhead][kPer];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         ml[k] = make_float2(-INFINITY, 0.f);
-        if (k0 + k >= mine) continue;
-        const int64_t at = ((int64_t)slot0 + ((int64_t)h * cuts + k0 + k) * tiles + tiles - 1 - tile) * kRows + r;
+        if (k0 + k >= pieces.count) continue;
+        const int64_t at = (k0 + k == 0 ? pieces.first : pieces.base + (int64_t)(k0 + k) * pieces.step) * kRows + r;
         ml[k] = __ldcg(a.part_ml + at);
         const float* src = a.part + at * D + lane * kPer;
         if constexpr (kPer % 4 == 0) {
@@ -1442,6 +1605,66 @@ __global__ void __launch_bounds__(kJoinThreads) paged_rows_join_kernel(const Pag
   if (a.lse != nullptr && lane == 0) a.lse[(int64_t)head * p.T + token] = (mx + log2f(sum)) * kLn2;
 }
 
+// Items on a line: jobs of kLineRows rows of the item that CTA c began and others end, if it is there.  (With a look at every packed row 148 uncut
+// items of 256 rows cost 15 us.)
+constexpr int kLineRows = 32;
+template <bool kHalf, int D>
+__device__ __forceinline__ void join_line(const PagedParams& p, const RowsArgs& a, int ctas) {
+  constexpr int kJobs = item_rows(D) / kLineRows;
+  const int warp = threadIdx.x >> 5;
+  const int each = __ldcg(&a.plan->each), rest = __ldcg(&a.plan->rest);
+  for (int job = blockIdx.x; job < (ctas - 1) * kJobs; job += gridDim.x) {
+    const int c = job / kJobs, end = line_first(each, rest, c + 1);
+    const int b = search_warp(p.B, end, [&](int k) { return __ldcg(a.plan->begin + k); });
+    const PagedSeq s = paged_seq(p, b);
+    const int keys = key_tiles(rows_end(p, s, 0)), begin = __ldcg(a.plan->begin + b), length = keys + kTreeItem;
+    const int h = (end - begin) / length, from = begin + h * length + kTreeItem;
+    if (end <= from || line_cta(each, rest, from) != c) continue;
+    const RowsPieces pieces{2 * (int64_t)c + 1, 2 * (int64_t)c, 2, line_cta(each, rest, from + keys - 1) - c + 1};
+    const int rows = (int)min((int64_t)s.n * p.G, (int64_t)item_rows(D));
+    const int r0 = (job - c * kJobs) * kLineRows;
+    for (int r = r0 + warp; r < min(r0 + kLineRows, rows); r += kJoinThreads / 32) {
+      const int i = r / a.by_group;
+      join_row<kHalf, D>(p, a, pieces, r, (int64_t)s.row0 + i, h * p.G + r - i * p.G, false);
+    }
+  }
+}
+
+template <bool kHalf, int D, bool kTree>
+__global__ void __launch_bounds__(kJoinThreads) paged_rows_join_kernel(const PagedParams p, const RowsArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  const bool failed = __ldcg(&a.plan->status) != 0;
+  if (kTree) {
+    const int ctas = __ldcg(&a.plan->ctas);
+    if (ctas > 0 && !failed) {
+      join_line<kHalf, D>(p, a, ctas);
+      return;
+    }
+  }
+  const int64_t g = (int64_t)blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
+  const int64_t token = g / p.Hq;
+  const int head = (int)(g - token * p.Hq);
+  if (token >= p.T || token < __ldg(p.cu) || token >= __ldg(p.cu + p.B)) return;
+  const int b = search_warp(p.B, (int)token, [&](int k) { return __ldg(p.cu + k); });
+  const PagedSeq s = paged_seq(p, b);
+  const int i = (int)(token - s.row0);
+  if (i < 0 || i >= s.n) return;
+  constexpr int kRows = item_rows(D);
+  const int h = head / p.G, row = i * p.G + head - h * p.G, tile = row / kRows, r = row - tile * kRows;
+  RowsPieces pieces{0, 0, 0, 0};
+  if (!failed) {
+    const int slot0 = __ldcg(a.plan->slot0 + b);
+    if (slot0 < 0) return;
+    const int tiles = rows_tiles(p, s.n), piece = __ldcg(a.plan->piece + b);
+    const int cuts = (key_tiles(rows_end(p, s, tiles - 1)) + piece - 1) / piece;
+    pieces.count = (key_tiles(rows_end(p, s, tile)) + piece - 1) / piece;
+    pieces.first = pieces.base = (int64_t)slot0 + (int64_t)h * cuts * tiles + tiles - 1 - tile;
+    pieces.step = tiles;
+  }
+  join_row<kHalf, D>(p, a, pieces, r, token, head, failed);
+}
+
 template <bool kTree, bool kHalf, int D>
 cudaError_t launch_rows_dim(const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, const RowsArgs& a, int sms, int slots, cudaStream_t st) {
   auto kernel = p.store == MOBA_STORE_SAME ? paged_rows_kernel<kHalf, D, MOBA_STORE_SAME, kTree>
@@ -1449,17 +1672,24 @@ cudaError_t launch_rows_dim(const PagedParams& p, const CUtensorMap& mk, const C
   const int threads = p.store == MOBA_STORE_SAME ? kRowsThreads<MOBA_STORE_SAME> : kRowsThreads<MOBA_STORE_E4M3>;
   cudaError_t e = prepare_kernel(kernel, kRowsSmem);
   if (e != cudaSuccess) return e;
-  if ((e = launch_pdl(kTree ? paged_tree_plan_kernel : paged_plan_kernel, dim3(1), kPagedBatch, 0, st, p, a.plan, sms, slots)) != cudaSuccess) return e;
+  if constexpr (kTree) {
+    e = launch_pdl(paged_tree_plan_kernel, dim3((unsigned)(1 + (p.T + 1023) / 1024)), kPagedBatch, 0, st, p, a.plan, const_cast<TreeMask*>(a.masks), sms, slots);
+  } else {
+    e = launch_pdl(paged_plan_kernel, dim3(1), kPagedBatch, 0, st, p, a.plan, sms, slots);
+  }
+  if (e != cudaSuccess) return e;
   if ((e = launch_pdl(kernel, dim3(sms), threads, kRowsSmem, st, p, mk, mv, a)) != cudaSuccess) return e;
-  const int64_t warps = p.T * p.Hq, per = kJoinThreads / 32;
-  return launch_pdl(paged_rows_join_kernel<kHalf, D>, dim3((unsigned)((warps + per - 1) / per)), kJoinThreads, 0, st, p, a);
+  const int64_t warps = p.T * p.Hq, per = kJoinThreads / 32, lines = kTree ? (int64_t)sms * (item_rows(D) / kLineRows) : 0;
+  const int64_t blocks = (warps + per - 1) / per > lines ? (warps + per - 1) / per : lines;
+  return launch_pdl(paged_rows_join_kernel<kHalf, D, kTree>, dim3((unsigned)blocks), kJoinThreads, 0, st, p, a);
 }
 static_assert(kPagedBatch == 1024, "a thread of the plan kernel for each sequence");
 
 constexpr size_t kPlanBytes = (sizeof(RowsPlan) + 255) / 256 * 256;
 
-size_t rows_workspace(const PagedParams& p) {
-  return kPlanBytes + (size_t)rows_slots(p) * item_rows(p.D) * (sizeof(float2) + p.D * sizeof(float));
+size_t rows_results(const PagedParams& p, int slots) { return kPlanBytes + (size_t)slots * item_rows(p.D) * (sizeof(float2) + p.D * sizeof(float)); }
+size_t rows_workspace(const PagedParams& p, bool tree) {
+  return tree ? rows_results(p, tree_slots(p)) + (size_t)p.T * sizeof(TreeMask) : rows_results(p, rows_slots(p));
 }
 
 template <bool kTree>
@@ -1475,9 +1705,10 @@ cudaError_t launch_rows(const PagedParams& all, const void* q, const void* kp, c
   a.lse = lse;
   a.plan = static_cast<RowsPlan*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + kPlanBytes);
-  const int slots_of_results = rows_slots(all);
+  const int slots_of_results = kTree ? tree_slots(all) : rows_slots(all);
   a.part = reinterpret_cast<float*>(a.part_ml + (size_t)slots_of_results * item_rows(all.D));
   a.by_group = fast_div(all.G);
+  a.masks = reinterpret_cast<const TreeMask*>(static_cast<const char*>(workspace) + rows_results(all, slots_of_results));
   CUtensorMap mk{}, mv{};
   if (all.store == MOBA_STORE_SAME) {
     const int slots = 1 << all.page_shift, box = slots < kBN ? slots : kBN;

@@ -303,7 +303,7 @@ def _attention(g: _Pages, q, kv, k_pages, v_pages, max_new, scale, return_lse, o
     if tokens > 0:
         lib, need = _lib.lib(), C.c_size_t(0)
         prob = g.pack(tokens, heads, max_new, dtype, 0.0 if scale is None else float(scale), qs, os, ks, vs)
-        _lib.check(lib.moba_paged_workspace_size(prob, C.byref(need)))
+        _lib.check((lib.moba_paged_workspace_size if parents is None else lib.moba_paged_tree_workspace_size)(prob, C.byref(need)))
         ws = _workspace(q.device, need.value)                # (the caching allocator goes by the current stream of the device given)
         if kv is not None:
             # what only the attention would refuse comes before anything is written

@@ -95,7 +95,9 @@ def test_pointers_are_checked_before_any_launch(lib):
     assert keep(path=None) == -4 and keep(count=None) == -4 and keep(lens=None) == -4 and keep(k=None) == -4
     assert keep(path=odd) == -6 and keep(stride=3) == -1 and keep(columns=0) == -1
     need = C.c_size_t(0)
-    assert lib.moba_paged_workspace_size(p, C.byref(need)) == 0
+    assert lib.moba_paged_tree_workspace_size(p, C.byref(need)) == 0 and lib.moba_paged_tree_workspace_size(p, None) == -4
+    tree = lambda size: lib.moba_paged_tree_attention(p, ok, ok, ok, ok, ok, ok, ok, None, None, ok, None, ok, size, None)  # noqa: E731
+    assert tree(need.value - 1) == -3
     assert lib.moba_paged_tree_attention(p, ok, odd, ok, ok, ok, ok, ok, None, None, ok, None, ok, need.value, None) == -6
 
 

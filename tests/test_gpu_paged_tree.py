@@ -158,3 +158,24 @@ def test_parents_are_checked():
             cache.attend(q, *where, 2, parents=parents)
     assert cache.attend(q, *where, 2, parents=i32([-1, 0])).shape == q.shape
     assert cache.attend(q[:0], *where, 2, parents=i32([])).shape == (0, 4, 64)
+
+
+# The same calls in both kernels: a table with room for many pages, of which the batch has a few, puts trees of 9 to 64 rows on tcgen05.
+@pytest.mark.parametrize("new,g,dim", [(3, 4, 64), (12, 4, 128), (16, 4, 256), (64, 1, 96), (9, 1, 128), (17, 3, 64)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_both_kernels(new, g, dim, wide):
+    b = TreeBatch([(new, 300), (new, new), (0, 40), (1, 130), (new, 1500)], 2 * g, 2, dim, 16, seed=10, spread=3)
+    b.fill()
+    table = torch.full((5, 200000), -1, dtype=torch.int32, device="cuda") if wide else b.table
+    table[:, :b.table.shape[1]] = b.table
+    b.check(*paged_attention(b.q, b.k, b.v, table, b.cu, b.lens, new, parents=b.parents, return_lse=True))
+
+
+def test_even_and_uneven_batches_of_one_row_tile():
+    """Items on a line of units: one key tile, many, more items than CTAs, fewer; sequences without rows between them."""
+    for seqs in ([(40, 40)], [(33, 5000)], [(40, 200 + 37 * i) if i % 3 else (0, 50) for i in range(70)], [(64, 64)] * 90, [(50, 3000), (64, 100)] * 3):
+        b = TreeBatch(seqs, 8, 2, 64, 64, seed=13, spread=6)
+        b.fill()
+        table = torch.full((len(seqs), 8000), -1, dtype=torch.int32, device="cuda")
+        table[:, :b.table.shape[1]] = b.table
+        b.check(*paged_attention(b.q, b.k, b.v, table, b.cu, b.lens, 64, parents=b.parents, return_lse=True))
