@@ -15,7 +15,9 @@
 namespace moba {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+// (16384 tokens of 32/8 heads of 128, us: one head of a lane under way 64, two 57.5, four 58; 256 threads a block 57.5, at head dim 96 47.7 for 47.2)
+constexpr int kThreads = 128, kWarps = kThreads / 32;
+constexpr int kHeads = 2;                  // of a lane under way
 
 // kPairs: of a lane.  Untouched dims are copied, as many as two halves of a lane's at a time.
 template <int kPairs> struct Piece;
@@ -74,33 +76,46 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
         s[i] *= p.inverse ? -p.magnitude : p.magnitude;
       }
     }
-    for (int h = unit * p.per_unit + sub; h < last; h += abreast) {
-      const bool of_q = h < p.heads_q;
-      const int hh = of_q ? h : h - p.heads_q;
-      const uint16_t* src = static_cast<const uint16_t*>(of_q ? p.q : p.k) + (of_q ? row * p.q_t + hh * p.q_h : row * p.k_t + hh * p.k_h);
-      uint16_t* dst = static_cast<uint16_t*>(of_q ? p.q_out : p.k_out) + (of_q ? row * p.qo_t + hh * p.qo_h : row * p.ko_t + hh * p.ko_h);
-      Word w0 = *reinterpret_cast<const Word*>(src + at0), w1 = *reinterpret_cast<const Word*>(src + at1);
-      if (turn) {
-        float f0[kPairs], f1[kPairs];
-        widen<kHalf, kPairs>(w0, f0);
-        widen<kHalf, kPairs>(w1, f1);
-        float x[2 * kPairs];                                // both pieces: x of pair i, y of it
+    // (loads of kHeads heads before their stores: rows may be turned where they are, so that the compiler does not bring loads forward)
+    for (int h0 = unit * p.per_unit + sub; h0 < last; h0 += kHeads * abreast) {
+      Word w[kHeads][2];
+      uint16_t* to[kHeads];
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) { x[i] = f0[i]; x[kPairs + i] = f1[i]; }
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-          const int a = kInterleaved ? 2 * i : i, b = kInterleaved ? 2 * i + 1 : kPairs + i;
-          const float u = x[a], v = x[b];
-          x[a] = u * c[i] - v * s[i];
-          x[b] = u * s[i] + v * c[i];
-        }
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) { f0[i] = x[i]; f1[i] = x[kPairs + i]; }
-        w0 = narrow<kHalf, kPairs>(f0);
-        w1 = narrow<kHalf, kPairs>(f1);
+      for (int k = 0; k < kHeads; ++k) {
+        const int h = h0 + k * abreast, hh = h < p.heads_q ? h : h - p.heads_q;
+        to[k] = nullptr;
+        if (h >= last) continue;
+        const bool of_q = h < p.heads_q;
+        const uint16_t* src = static_cast<const uint16_t*>(of_q ? p.q : p.k) + (of_q ? row * p.q_t + hh * p.q_h : row * p.k_t + hh * p.k_h);
+        to[k] = static_cast<uint16_t*>(of_q ? p.q_out : p.k_out) + (of_q ? row * p.qo_t + hh * p.qo_h : row * p.ko_t + hh * p.ko_h);
+        w[k][0] = *reinterpret_cast<const Word*>(src + at0);
+        w[k][1] = *reinterpret_cast<const Word*>(src + at1);
       }
-      *reinterpret_cast<Word*>(dst + at0) = w0;
-      *reinterpret_cast<Word*>(dst + at1) = w1;
+#pragma unroll
+      for (int k = 0; k < kHeads; ++k) {
+        if (to[k] == nullptr) continue;
+        if (turn) {
+          float f0[kPairs], f1[kPairs];
+          widen<kHalf, kPairs>(w[k][0], f0);
+          widen<kHalf, kPairs>(w[k][1], f1);
+          float x[2 * kPairs];                              // both pieces
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) { x[i] = f0[i]; x[kPairs + i] = f1[i]; }
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) {
+            const int a = kInterleaved ? 2 * i : i, b = kInterleaved ? 2 * i + 1 : kPairs + i;
+            const float u = x[a], v = x[b];
+            x[a] = u * c[i] - v * s[i];
+            x[b] = u * s[i] + v * c[i];
+          }
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) { f0[i] = x[i]; f1[i] = x[kPairs + i]; }
+          w[k][0] = narrow<kHalf, kPairs>(f0);
+          w[k][1] = narrow<kHalf, kPairs>(f1);
+        }
+        *reinterpret_cast<Word*>(to[k] + at0) = w[k][0];
+        *reinterpret_cast<Word*>(to[k] + at1) = w[k][1];
+      }
     }
   }
 }

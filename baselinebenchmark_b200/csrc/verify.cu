@@ -64,6 +64,8 @@ struct Residual {
   int rejected;
   const uint32_t* taken;                   // without a draft: tokens that were rejected, bits from `taken0` on; null: none
   int64_t taken0;
+  // bit of element `at`, and those behind it in its word
+  __device__ __forceinline__ uint32_t gone(int64_t at) const { return taken == nullptr ? 0u : taken[(at - taken0) >> 5] >> ((at - taken0) & 31); }
   template <bool kDraft>
   __device__ __forceinline__ double operator()(float p, float q, int64_t at) const {
     double t = (double)probability(p);
@@ -74,9 +76,8 @@ struct Residual {
 #pragma unroll 1
         for (int j = 0; j + 1 < rejected; ++j) t = fmax(__dsub_rn(__dmul_rn(t, inverse[j]), d), 0.0);
       }
-    } else if (taken != nullptr) {
-      const int64_t i = at - taken0;
-      if ((taken[i >> 5] >> (i & 31)) & 1) t = 0.0;
+    } else if (gone(at) & 1) {
+      t = 0.0;
     }
     return t;
   }
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const VerifyParams 
           cluster_store(cluster_place(&inverse[c.rejected - 2], to), (uint64_t)__double_as_longlong(inverse[c.rejected - 2]));
     }
     // without a draft the rejected tokens do not count any more
-    if (!kDraft) for (int i = tid; i < (int)((part + kV + 31) / 32); i += kThreads) taken[i] = 0;
+    if (!kDraft) for (int i = tid; i < (int)((part + 2 * kV + 31) / 32); i += kThreads) taken[i] = 0;
     cluster_sync();
     const Command c = told;
     if (c.row < 0) break;
@@ -207,6 +208,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const VerifyParams 
     const int head = (int)(((16 - ((uintptr_t)p & 15)) & 15) / sizeof(T));
     const bool vectors = !with_draft || (((uintptr_t)p ^ (uintptr_t)q) & 15) == 0;
     const int64_t lo = rank == 0 ? 0 : min((int64_t)rank * part + head, a.vocabulary), hi = min(((int64_t)rank + 1) * part + head, a.vocabulary);
+    const int64_t taken0 = (int64_t)rank * part + head - kV;   // a vector's bits lie in one word
     auto first_of = [&](int w) { return w == 0 ? lo : min((int64_t)rank * part + head + w * share, hi); };
     auto end_of = [&](int w) { return min((int64_t)rank * part + head + (w + 1) * share, hi); };
     const int64_t wlo = first_of(warp), whi = end_of(warp);
@@ -215,20 +217,20 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const VerifyParams 
       for (int i = c.row + 1 + tid; i < n; i += kThreads) {
         const int parent = a.parents != nullptr ? __ldg(a.parents + row0 + i) : i - 1;
         const int64_t x = token_of(row0 + i);
-        if (parent == c.row && x >= lo && x < hi) atomicOr(&taken[(x - lo) >> 5], 1u << ((x - lo) & 31));
+        if (parent == c.row && x >= lo && x < hi) atomicOr(&taken[(x - taken0) >> 5], 1u << ((x - taken0) & 31));
       }
       __syncthreads();
     }
     // ---- the sum of what is left, warp by warp
-    const Residual left{inverse, c.rejected, !kDraft && c.rejected > 0 ? taken : nullptr, lo};
+    const Residual left{inverse, c.rejected, !kDraft && c.rejected > 0 ? taken : nullptr, taken0};
     // quick: t is p, or max(p - q, 0) = max(p, q) - q with p and q no less than 0 (which drops what is not a number)
-    const bool quick = !infinite && (c.rejected == 0 || (kDraft && c.rejected == 1));
+    const bool quick = !infinite && (!kDraft || c.rejected <= 1);
     double s0 = 0.0, s1 = 0.0;
-    auto one = [&](float x, float y, int64_t e, int i) {
+    auto one = [&](float x, float y, int64_t e, int i, uint32_t gone) {
       double t;
       if (quick) {
         const float d = fmaxf(y, 0.f);
-        t = kDraft ? (double)fmaxf(fmaxf(x, 0.f), d) - (double)d : (double)fmaxf(x, 0.f);
+        t = kDraft ? (double)fmaxf(fmaxf(x, 0.f), d) - (double)d : (double)(gone & 1 ? 0.f : fmaxf(x, 0.f));
       } else {
         t = left.template operator()<kDraft>(x, y, e);
       }
@@ -236,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const VerifyParams 
     };
     int64_t at = wlo;
     if (vectors) {
-      if (rank == 0 && warp == 0 && lane < head && lane < whi) one(element(p + lane), with_draft ? element(q + lane) : 0.f, lane, 0);
+      if (rank == 0 && warp == 0 && lane < head && lane < whi) one(element(p + lane), with_draft ? element(q + lane) : 0.f, lane, 0, left.gone(lane));
       if (rank == 0 && warp == 0) at = min((int64_t)head, whi);
       for (; at + 32 * kV * kAbreast <= whi; at += 32 * kV * kAbreast) {
         uint4 x[kAbreast], y[kAbreast];
@@ -251,18 +253,21 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const VerifyParams 
           float f[kV], g[kV];
           widen<T>(x[k], f);
           widen<T>(y[k], g);
+          const int64_t e = at + (k * 32 + lane) * kV;
+          const uint32_t gone = kDraft ? 0u : left.gone(e);
 #pragma unroll
-          for (int i = 0; i < kV; ++i) one(f[i], g[i], at + (k * 32 + lane) * kV + i, i);
+          for (int i = 0; i < kV; ++i) one(f[i], g[i], e + i, i, gone >> i);
         }
       }
 #pragma unroll 1
       for (; at + 32 * kV <= whi; at += 32 * kV) {
         const int64_t e = at + lane * kV;
         float f[kV], g[kV];
+        const uint32_t gone = kDraft ? 0u : left.gone(e);
         widen<T>(__ldg(reinterpret_cast<const uint4*>(p + e)), f);
         widen<T>(with_draft ? __ldg(reinterpret_cast<const uint4*>(q + e)) : make_uint4(0, 0, 0, 0), g);
 #pragma unroll
-        for (int i = 0; i < kV; ++i) one(f[i], g[i], e + i, i);
+        for (int i = 0; i < kV; ++i) one(f[i], g[i], e + i, i, gone >> i);
       }
     }
     for (; at < whi; at += 32 * kV) {
@@ -276,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const VerifyParams 
 #pragma unroll
       for (int i = 0; i < kV; ++i) {
         const int64_t e = at + lane + 32 * i;
-        if (e < whi) one(x[i], y[i], e, i);
+        if (e < whi) one(x[i], y[i], e, i, kDraft ? 0u : left.gone(e));
       }
     }
     const double mine = warp_sum(s0 + s1);
@@ -401,7 +406,7 @@ cudaError_t launch_verify(VerifyParams a, int dtype, cudaStream_t st) {
   }
   a.part = (a.vocabulary + blocks * step - 1) / (blocks * step) * step;
   const size_t smem = (size_t)a.max_new * (sizeof(double) + sizeof(Node)) + (size_t)((a.max_new + 1) & ~1) * sizeof(int16_t) +
-                      (a.draft == nullptr ? (size_t)((a.part + 8 + 31) / 32) * 4 : 0);
+                      (a.draft == nullptr ? (size_t)((a.part + 16 + 31) / 32) * 4 : 0);
   cudaError_t e = prepare_kernel(kernel, smem);
   if (e != cudaSuccess) return e;
   return launch_clusters(kernel, blocks, dim3((unsigned)(a.batch * blocks)), kThreads, smem, st, a);

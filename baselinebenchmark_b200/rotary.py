@@ -114,15 +114,6 @@ def _strides(x) -> Tuple[int, int]:
     return t if tokens > 1 else 0, h if heads > 1 else 0
 
 
-def _launch(q, k, positions, table, inverse, qo, ko, shape, index, dtype, q_heads_k) -> None:
-    """The call itself; everything has been looked at."""
-    (tokens, heads, dim), (heads_k, qs, ks) = shape, q_heads_k
-    call = _CALL.pack(tokens, heads, heads_k, dim, table.rotary_dim, table.interleaved, inverse, _DTYPES[dtype], 0, table.magnitude, 0, *qs, *ks,
-                      *_strides(qo), *((0, 0) if ko is None else _strides(ko)))
-    _run_on(index, _lib.lib().moba_rotary, call, q.data_ptr(), None if k is None else k.data_ptr(), positions.data_ptr(), table.turns.data_ptr(),
-            qo.data_ptr(), None if k is None else ko.data_ptr())
-
-
 def _turn(q, k, positions, table, inverse, out=None):
     """(q, k) turned, in `out` or in new tensors; looks at q, k, positions and the table first, each attribute once."""
     shape, index, dtype = q.shape, q.get_device(), q.dtype
@@ -144,11 +135,18 @@ def _turn(q, k, positions, table, inverse, out=None):
         _check_rotary(q, k, positions, table)
         raise ValueError("q, k, positions and the table do not describe a call")
     if out is None:
-        out = (torch.empty(shape, dtype=dtype, device=q.device), None if k is None else torch.empty(other, dtype=dtype, device=q.device))
+        device = q.device
+        out = (torch.empty(shape, dtype=dtype, device=device), None if k is None else torch.empty(other, dtype=dtype, device=device))
+        strides = (heads * dim, dim, heads_k * dim, dim)
     else:
         _check_out(q, k, out)
+        strides = (*_strides(out[0]), *((0, 0) if k is None else _strides(out[1])))
     if tokens > 0:
-        _launch(q, k, positions, table, inverse, *out, shape, index, dtype, (heads_k, (qt if tokens > 1 else 0, qh if heads > 1 else 0), ks))
+        call = _CALL.pack(tokens, heads, heads_k, dim, table.rotary_dim, table.interleaved, inverse, _DTYPES[dtype], 0, table.magnitude, 0,
+                          qt if tokens > 1 else 0, qh if heads > 1 else 0, *ks, *strides)
+        qo, ko = out
+        _run_on(index, _lib.lib().moba_rotary, call, q.data_ptr(), None if k is None else k.data_ptr(), positions.data_ptr(), table.turns.data_ptr(),
+                qo.data_ptr(), None if k is None else ko.data_ptr())
     return out
 
 
@@ -168,8 +166,8 @@ def _check_out(q, k, out) -> None:
 
 def _kernel_rows(x):
     """A gradient or tangent as the kernel takes it: whatever autograd makes of it is not the caller's to lay out."""
-    good = x.stride(2) == 1 and not (x.data_ptr() & 15) and all(s % 8 == 0 for s in _strides(x))
-    return x if good else x.contiguous()
+    t, h, d = x.stride()
+    return x if d == 1 and not (t | h) & 7 and not x.data_ptr() & 15 else x.contiguous()
 
 
 class _Rotary(torch.autograd.Function):
@@ -179,10 +177,11 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, q, k, positions, table, inverse):
         qo, ko = _turn(q, k, positions, table, inverse)
         ctx.save_for_backward(positions)
-        ctx.save_for_forward(positions)
         ctx.table, ctx.inverse, ctx.alone = table, inverse, k is None
         ctx.set_materialize_grads(False)
-        ctx.like = tuple((x.shape, x.dtype, x.device) for x in (q, k) if x is not None)
+        if getattr(forward_ad, "_current_level", 0) >= 0:
+            ctx.save_for_forward(positions)
+            ctx.like = tuple((x.shape, x.dtype, x.device) for x in (q, k) if x is not None)
         return qo if k is None else (qo, ko)
 
     @staticmethod
