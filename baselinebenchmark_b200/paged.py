@@ -368,7 +368,7 @@ def paged_keep(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
     """Moves the rows of an accepted branch together: of the packed tokens of sequence b, which the pages hold, rows path[b, 0] < path[b, 1]
     < .. (count[b] of them; `verify_drafts` gives both) go to the places of rows 0, 1, ..  Returns the sequences' lengths then, int32 [batch]: the tokens in
     front of the packed ones and the kept ones; what is behind them is no longer the sequence's.  8-bit rows are moved as they are, with
-    their powers of two.  A path ends in front of an entry that is no later row of the sequence than the one before it.  Each layer's pages are
+    their powers of two; a slot that two sequences' tables have is undefined.  A path ends in front of an entry that is no later row of the sequence than the one before it.  Each layer's pages are
     moved with the same seq_lens, those with the drafted tokens."""
     g = _Pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
     if path.ndim != 2 or path.shape[1] == 0:

@@ -167,7 +167,7 @@ def _check_out(q, k, out) -> None:
 def _kernel_rows(x):
     """A gradient or tangent as the kernel takes it: whatever autograd makes of it is not the caller's to lay out."""
     t, h, d = x.stride()
-    return x if d == 1 and not (t | h) & 7 and not x.data_ptr() & 15 else x.contiguous()
+    return x if d == 1 and not (t | h) & 7 and not x.data_ptr() & 15 else x.clone(memory_format=torch.contiguous_format)
 
 
 class _Rotary(torch.autograd.Function):
@@ -201,7 +201,8 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
-        dq, *dk = _Rotary._each(ctx, grads, not ctx.inverse)
+        wanted = [g if need else None for g, need in zip(grads, ctx.needs_input_grad)]
+        dq, *dk = _Rotary._each(ctx, wanted, not ctx.inverse)
         return dq, dk[0] if dk else None, None, None, None
 
     @staticmethod

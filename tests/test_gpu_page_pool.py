@@ -184,6 +184,48 @@ def test_a_captured_step_takes_and_gives_back():
         assert slots.tolist() == want[2] and positions.tolist() == want[3] and int(missing) == want[4]
 
 
+def test_no_rows():
+    """Nothing to place, or no sequence with a row: pages stay where they are."""
+    table, free, count = _start([20, 3], 16, 4, 9)
+    for rows, cu in ((0, [0, 0, 0]), (3, [0, 0, 0]), (0, [0, 2, 2])):
+        t, c = _i32(table), _i32([count])
+        slots, positions, missing = paged_reserve(t, _i32(cu), _i32([20, 3]), _i32(free), c, 16, rows)
+        assert t.tolist() == table and c.tolist() == [count] and missing.tolist() == [0]
+        assert slots.tolist() == [-1] * rows and positions.tolist() == [-1] * rows
+
+
+def test_pool_refusals():
+    table, free, count, cu, lens = _i32([[-1] * 4] * 2), _i32([0, 1, 2]), _i32([3]), _i32([0, 1, 2]), _i32([1, 1])
+    reserve = lambda **kw: paged_reserve(*{**dict(table=table, cu=cu, lens=lens, free=free, count=count, size=16, rows=2), **kw}.values())  # noqa: E731
+    for error, kw in ((ValueError, dict(table=table[0])), (TypeError, dict(table=table.long())), (NotImplementedError, dict(table=_i32([[-1] * 2] * 4).t())),
+                      (ValueError, dict(table=table[:1].expand(2, 4))), (ValueError, dict(cu=cu[:2])), (TypeError, dict(cu=cu.long())),
+                      (ValueError, dict(lens=lens[:1])), (TypeError, dict(lens=lens.cpu())), (ValueError, dict(free=free[:0])), (TypeError, dict(free=free.long())),
+                      (ValueError, dict(count=_i32([3, 3]))), (NotImplementedError, dict(size=24)), (ValueError, dict(size=0)), (ValueError, dict(rows=-1))):
+        with pytest.raises(error):
+            reserve(**kw)
+    with pytest.raises(ValueError, match="parents"):
+        paged_reserve(table, cu, lens, free, count, 16, 2, parents=_i32([0]))
+    with pytest.raises(RuntimeError, match="error -2"):                   # more sequences than a call takes
+        paged_release(_i32([[-1]]).repeat(16385, 1), _i32([0]).repeat(16385), free, count, 16)
+    with pytest.raises(ValueError, match="keep_lens"):
+        paged_release(table, lens[:1], free, count, 16)
+    assert table.tolist() == [[-1] * 4] * 2 and count.tolist() == [3]
+    with torch.inference_mode():
+        made = _i32([[-1] * 4] * 2)
+    with pytest.raises(RuntimeError, match="inference"):
+        paged_release(made, lens, free, count, 16)
+
+
+def test_many_sequences():
+    news, before = [1] * 16384, [(7 * i) % 50 for i in range(16384)]
+    lens = [n + b for n, b in zip(news, before)]
+    table, free, count = _start(before, 16, 4, 70000, seed=3)
+    want = reserve_rule(table, news, lens, free, count, 16, 16384)
+    t, c = _i32(table), _i32([count])
+    slots, positions, missing = paged_reserve(t, _i32(list(range(16385))), _i32(lens), _i32(free), c, 16, 16384)
+    assert t.tolist() == want[0] and c.tolist() == [want[1]] and slots.tolist() == want[2] and positions.tolist() == want[3]
+
+
 def test_pool_of_a_cache():
     pool = PagePool(7, 32)
     table = torch.full((2, 4), -1, dtype=torch.int32, device="cuda")

@@ -127,6 +127,18 @@ def test_gradients(turn, interleaved, dtype):
     assert ((total.double() - want.sum(0)).abs() <= (want.abs().sum(0) + size.sum(0) * 2.0 ** -20) * 2 * u + 1e-6).all()
 
 
+def test_gradients_of_one_of_two_and_at_odd_addresses():
+    q, k, pos = _rows(9, 4, 64, torch.bfloat16), _rows(9, 2, 64, torch.bfloat16, 3), _positions(9, 900)
+    table, f = RotaryTable(rotary_frequencies(64)), rotary_frequencies(64)
+    odd = torch.zeros(9 * 2 * 64 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(9, 2, 64)   # contiguous, 2 bytes behind a vector's boundary
+    odd.copy_(_rows(9, 2, 64, torch.bfloat16, 4))
+    leaf = k.clone().requires_grad_()
+    tq, tk = rotary(q, leaf, pos, table)
+    assert tq.requires_grad and tk.requires_grad
+    (grad,) = torch.autograd.grad(tk, leaf, odd)
+    close(grad, *turned(odd, pos, f, False, inverse=True))
+
+
 def test_differences_and_second_order():
     """(f(x + h e) - f(x - h e)) / 2h is exact for a linear operator but for the roundings: fp16 rows, h = 1, half a step of each value."""
     q, pos = _rows(4, 1, 64, torch.float16), _positions(4, 50)
