@@ -72,6 +72,8 @@ int tree_slots(const PagedParams& p) {
 }
 constexpr float kLn2 = 0.6931471805599453f;
 
+constexpr int kMostLine = 256;             // CTAs that share a line, at most
+
 // ---- the plan ------------------------------------------------------------------
 // In the workspace, one for each launch.
 struct RowsPlan {
@@ -83,6 +85,8 @@ struct RowsPlan {
   int32_t slot0[kPagedBatch];              // first result slot of a sequence whose items are cut
   int32_t piece[kPagedBatch];              // key tiles of a piece
   int32_t order[kPagedBatch];              // of trees: the sequences, those with the longest pieces first; `begin` is in this order
+  int4 shared[kMostLine];                  // of trees on a line, from each CTA: the item that it began and others end: pieces (0: there is none),
+                                           // first packed row, rows, kv head
 };
 
 __device__ __forceinline__ int rows_tiles(const PagedParams& p, int n) {
@@ -290,7 +294,7 @@ __global__ void __launch_bounds__(1024) paged_tree_plan_kernel(const PagedParams
       if (lane == 31) scan_s[0][warp] = x;
       __syncthreads();
       const int all = __reduce_add_sync(0xffffffffu, scan_s[0][lane]), before = __reduce_add_sync(0xffffffffu, lane < warp ? scan_s[0][lane] : 0);
-      const int ctas = max(min(min(sms, most_slots / 2), all / kTreeLeast), 1);
+      const int ctas = max(min(min(min(sms, kMostLine), most_slots / 2), all / kTreeLeast), 1);
       if (b < p.B) {
         plan->begin[b] = before + x - mine;
         if (b == p.B - 1) {
@@ -455,14 +459,15 @@ __device__ __forceinline__ bool rows_twice(int D, const RowsItem& it) { return D
 
 // A CTA's stretch of the line, from `u` on; `ctas` 0: items are drawn.
 struct RowsLine {
-  int ctas, u, last;
+  int ctas, u, last, each, rest;
+  bool told;                               // what others end
 };
 __device__ __forceinline__ RowsLine rows_line(const RowsArgs& a) {
-  RowsLine line{__ldcg(&a.plan->ctas), 0, 0};
+  RowsLine line{__ldcg(&a.plan->ctas), 0, 0, __ldcg(&a.plan->each), __ldcg(&a.plan->rest), false};
   if (line.ctas > 0) {
-    const int each = __ldcg(&a.plan->each), rest = __ldcg(&a.plan->rest), c = (int)blockIdx.x;
-    line.u = line_first(each, rest, min(c, line.ctas));
-    line.last = c < line.ctas ? line_first(each, rest, c + 1) : line.u;
+    const int c = (int)blockIdx.x;
+    line.u = line_first(line.each, line.rest, min(c, line.ctas));
+    line.last = c < line.ctas ? line_first(line.each, line.rest, c + 1) : line.u;
   }
   return line;
 }
@@ -475,15 +480,19 @@ __device__ __forceinline__ void rows_prefetch(const PagedParams& p, const RowsAr
   bool done = false;
   for (;;) {
     if (kTree && line.ctas > 0) {
-      if (line.u >= line.last || c.abort) { done = true; break; }
+      if (line.u >= line.last || c.abort) {
+        if (lane == 0 && !line.told && blockIdx.x < kMostLine) a.plan->shared[blockIdx.x] = make_int4(0, 0, 0, 0);
+        done = true;
+        break;
+      }
       it.b = search_warp(p.B, line.u, [&](int k) { return __ldcg(a.plan->begin + k); });
       const PagedSeq s = paged_seq(p, it.b);
       const int begin = __ldcg(a.plan->begin + it.b), tiles = key_tiles(rows_end(p, s, 0)), length = tiles + kTreeItem;
       it.h = (line.u - begin) / length;
-      const int on = line.u - begin - it.h * length - kTreeItem;
+      const int on = line.u - begin - it.h * length - kTreeItem, end = line.u + tiles - on;
       it.j0 = max(on, 0);
       it.ntiles = min(tiles, on + (line.last - line.u)) - it.j0;
-      line.u += tiles - on;
+      line.u = end;
       if (it.ntiles <= 0) continue;                         // (what is left of the stretch is not a key tile: the next CTA's item)
       it.tile = 0;
       it.nrows = (int)min((int64_t)s.n * p.G, (int64_t)item_rows(p.D));
@@ -491,6 +500,10 @@ __device__ __forceinline__ void rows_prefetch(const PagedParams& p, const RowsAr
       it.pos0 = s.pos0;
       it.len = s.len;
       it.slot = it.ntiles == tiles ? -1 : 2 * (int)blockIdx.x + (it.j0 == 0 ? 1 : 0);
+      if (it.j0 == 0 && it.slot >= 0) {                     // (the stretch ends here)
+        line.told = true;
+        if (lane == 0) a.plan->shared[blockIdx.x] = make_int4(line_cta(line.each, line.rest, end - 1) - (int)blockIdx.x + 1, it.row0, it.nrows, it.h);
+      }
       break;
     }
     int idx = 0;
@@ -1605,27 +1618,21 @@ __device__ __forceinline__ void join_row(const PagedParams& p, const RowsArgs& a
   if (a.lse != nullptr && lane == 0) a.lse[(int64_t)head * p.T + token] = (mx + log2f(sum)) * kLn2;
 }
 
-// Items on a line: jobs of kLineRows rows of the item that CTA c began and others end, if it is there.  (With a look at every packed row 148 uncut
+// Items on a line: jobs of kLineRows rows of the item that CTA c began and others end, if it did.  (With a look at every packed row 148 uncut
 // items of 256 rows cost 15 us.)
-constexpr int kLineRows = 32;
+constexpr int kLineRows = 16;
 template <bool kHalf, int D>
 __device__ __forceinline__ void join_line(const PagedParams& p, const RowsArgs& a, int ctas) {
   constexpr int kJobs = item_rows(D) / kLineRows;
   const int warp = threadIdx.x >> 5;
-  const int each = __ldcg(&a.plan->each), rest = __ldcg(&a.plan->rest);
-  for (int job = blockIdx.x; job < (ctas - 1) * kJobs; job += gridDim.x) {
-    const int c = job / kJobs, end = line_first(each, rest, c + 1);
-    const int b = search_warp(p.B, end, [&](int k) { return __ldcg(a.plan->begin + k); });
-    const PagedSeq s = paged_seq(p, b);
-    const int keys = key_tiles(rows_end(p, s, 0)), begin = __ldcg(a.plan->begin + b), length = keys + kTreeItem;
-    const int h = (end - begin) / length, from = begin + h * length + kTreeItem;
-    if (end <= from || line_cta(each, rest, from) != c) continue;
-    const RowsPieces pieces{2 * (int64_t)c + 1, 2 * (int64_t)c, 2, line_cta(each, rest, from + keys - 1) - c + 1};
-    const int rows = (int)min((int64_t)s.n * p.G, (int64_t)item_rows(D));
-    const int r0 = (job - c * kJobs) * kLineRows;
-    for (int r = r0 + warp; r < min(r0 + kLineRows, rows); r += kJoinThreads / 32) {
+  for (int job = blockIdx.x; job < ctas * kJobs; job += gridDim.x) {
+    const int c = job / kJobs;
+    const int4 it = __ldcg(&a.plan->shared[c]);             // pieces, first packed row, rows, kv head
+    const RowsPieces pieces{2 * (int64_t)c + 1, 2 * (int64_t)c, 2, it.x};
+    const int r0 = (job - c * kJobs) * kLineRows, end = it.x > 0 ? min(r0 + kLineRows, it.z) : 0;
+    for (int r = r0 + warp; r < end; r += kJoinThreads / 32) {
       const int i = r / a.by_group;
-      join_row<kHalf, D>(p, a, pieces, r, (int64_t)s.row0 + i, h * p.G + r - i * p.G, false);
+      join_row<kHalf, D>(p, a, pieces, r, (int64_t)it.y + i, it.w * p.G + r - i * p.G, false);
     }
   }
 }
