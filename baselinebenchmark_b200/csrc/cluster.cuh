@@ -20,6 +20,8 @@ __device__ __forceinline__ uint32_t cluster_size() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// In front of the first access to another block's shared memory (which exists once that block runs) lies a cluster_sync; so does one behind the last
+// access, before a block ends.
 // The place in block `rank` of what lies at `p` in this block's shared memory.
 __device__ __forceinline__ uint32_t cluster_place(const void* p, uint32_t rank) {
   uint32_t at;

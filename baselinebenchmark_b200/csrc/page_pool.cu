@@ -109,6 +109,7 @@ __global__ void __launch_bounds__(kThreads) pool_kernel(const PoolParams p) {
   __shared__ int32_t scan[kWarps], counts[kWarps], block_total[kBlocks];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = kRows ? 0 : cluster_rank(), blocks = kRows ? 1 : cluster_size();
+  if (!kRows) cluster_sync();                               // (all blocks are there)
   pdl_wait();
   pdl_trigger();
   const int have = min(max(__ldcg(p.count), 0), p.pages);
@@ -231,6 +232,7 @@ __global__ void __launch_bounds__(kThreads) pool_cut_kernel(const PoolParams p) 
   __shared__ int32_t counts[kWarps], block_total[kBlocks];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = kOne ? 0 : cluster_rank(), blocks = kOne ? 1 : cluster_size();
+  if (!kOne) cluster_sync();                                // (all blocks are there)
   pdl_wait();
   pdl_trigger();
   const int have = min(max(__ldcg(p.count), 0), p.pages);

@@ -161,7 +161,7 @@ static int check_pool(const moba_page_pool_t* p) {
   if (p->batch <= 0 || p->pages_per_seq <= 0 || p->num_pages <= 0 || p->page_size <= 0 || p->total_tokens < 0) return MOBA_E_SHAPE;
   if (p->page_size < 16 || (p->page_size & (p->page_size - 1)) != 0 || p->reserved != 0) return MOBA_E_UNSUPPORTED;
   if (p->batch > kPoolMostBatch || p->total_tokens >= ((int64_t)1 << 31)) return MOBA_E_UNSUPPORTED;
-  if ((int64_t)p->batch * p->pages_per_seq >= ((int64_t)1 << 31) || (int64_t)p->pages_per_seq * p->page_size >= ((int64_t)1 << 30))
+  if ((int64_t)p->batch * p->pages_per_seq >= ((int64_t)1 << 30) || (int64_t)p->pages_per_seq * p->page_size >= ((int64_t)1 << 30))
     return MOBA_E_UNSUPPORTED;
   if (p->table_stride < (p->batch > 1 ? p->pages_per_seq : 0)) return MOBA_E_SHAPE;
   return MOBA_OK;

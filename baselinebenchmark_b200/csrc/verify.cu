@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const VerifyParams 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank(), blocks = cluster_size();
   const int b = blockIdx.x / blocks;
+  cluster_sync();                                           // (all blocks are there)
   pdl_wait();
   pdl_trigger();
   const int64_t row0 = min(max((int64_t)__ldg(a.cu + b), (int64_t)0), a.rows), end = min((int64_t)__ldg(a.cu + b + 1), a.rows);

@@ -11,9 +11,10 @@ import struct
 from typing import Optional, Tuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _lib
-from .paged import _check_not_followed, _check_parents, _i32_rows, _run_on
+from .paged import _check_parents, _i32_rows, _run_on
 
 __all__ = ["verify_drafts"]
 
@@ -101,7 +102,10 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: t
         raise ValueError("target, draft, tokens, cu_seqlens, accept and sample do not describe a call")
     if parents is not None:
         _check_parents(parents, rows, index)
-    _check_not_followed(target=target, draft=draft, accept=accept, sample=sample)
+    for x in (target, draft, accept, sample):
+        if x is not None and ((x.requires_grad and torch.is_grad_enabled())
+                              or (getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(x).tangent is not None)):
+            raise NotImplementedError("whole numbers have no derivatives: verify_drafts takes no tensors that autograd follows")
     path = torch.empty((batch, max_new), dtype=i32, device=target.device)
     count, following = torch.empty(batch, dtype=i32, device=target.device), torch.empty(batch, dtype=token, device=target.device)
     if rows == 0:

@@ -255,3 +255,25 @@ def test_the_tokens_are_distributed_as_the_targets():
         behind = after[count > 1]                             # and the token behind an accepted one
         share = torch.bincount(behind, minlength=v).double() / behind.numel()
         assert ((share - p.double()).abs() <= 5 * (p.double() * (1 - p.double()) / behind.numel()).sqrt() + 1e-9).all()
+
+
+def test_refusals():
+    d = Drafts([3, 2], 20, torch.float32, spread=2, seed=15)
+    cu, tokens = _i32([0, 3, 5]), torch.tensor(d.tokens, device="cuda")
+    base = dict(target=d.target.cuda(), draft=d.draft.cuda(), tokens=tokens, cu_seqlens=cu, accept=d.accept.cuda(), sample=d.sample.cuda(), max_new=3)
+    for error, kw in ((ValueError, dict(target=base["target"][0])), (TypeError, dict(target=base["target"].double())), (ValueError, dict(draft=base["draft"][:2])),
+                      (TypeError, dict(draft=base["draft"].half())), (ValueError, dict(tokens=tokens[:2])), (TypeError, dict(tokens=tokens.short())),
+                      (TypeError, dict(cu_seqlens=cu.long())), (ValueError, dict(cu_seqlens=cu[:1])), (TypeError, dict(accept=base["accept"].half())),
+                      (ValueError, dict(sample=base["accept"])), (ValueError, dict(max_new=0)), (NotImplementedError, dict(max_new=1025)),
+                      (NotImplementedError, dict(target=base["target"].t().contiguous().t())), (TypeError, dict(accept=d.accept)),
+                      (ValueError, dict(parents=_i32([0])), ), (TypeError, dict(parents=torch.zeros(5, device="cuda"))),
+                      (NotImplementedError, dict(target=base["target"].clone().requires_grad_()))):
+        with pytest.raises(error):
+            verify_drafts(**{**base, **kw})
+    with torch.no_grad():
+        verify_drafts(**{**base, "target": base["target"].clone().requires_grad_()})
+    with torch.inference_mode():
+        path, count, after = verify_drafts(**base)
+    assert path.shape == (2, 3) and count.shape == after.shape == (2,)
+    path, count, after = verify_drafts(**{**base, "target": base["target"][:0], "draft": None, "tokens": tokens[:0], "accept": base["accept"][:0]})
+    assert (path == -1).all() and count.tolist() == [0, 0] and after.tolist() == [-1, -1]
