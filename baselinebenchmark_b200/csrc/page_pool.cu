@@ -7,6 +7,9 @@
 // Slots and positions follow row by row; the depth of a row in a tree of drafted tokens by doubling, d(i) += d(up(i)), up(i) <- up(up(i)), which takes
 // as many rounds as the depth has bits.
 // All of it is a few KB: what bounds it is the chain of dependent loads and barriers, and the launches.  Small calls are one block, one launch.
+// Measured (replayed from a graph, us): 64 sequences of one new token 6.3, their pages back 6.2; 40000 new tokens of 1000 sequences 10.3; 200000 in 32 sequences,
+// prompts and trees 24.7 (four launches; 118 more with a sequence's rows in one block); 1.9 million entries looked through for pages to give back 33
+// (300 entry by entry, in one cluster as now).
 #include "page_pool.cuh"
 
 #include "cluster.cuh"

@@ -281,7 +281,8 @@ cudaError_t launch_rows(bool load, const PagedParams& p, RowArgs a, cudaStream_t
 
 // Rows path[0] < path[1] < .. of a sequence's packed ones go to its places 0, 1, ...  A thread has 16 bytes of a head's rows (or their bytes of scale), from
 // the first row of the path to the last, several loads ahead of the stores: row j is written when path[0 .. j], which may lie there, have been read,
-// and no thread touches another's bytes.  Bound by the chain path -> page -> row -> store.
+// and no thread touches another's bytes.  Bound by the chain path -> page -> row -> store: 6 trees of 8 rows over 4 kv heads 4.3 us, 64 of 64 over 8
+// kv heads of e4m3 10.4 (16 rows under way at a time 10.5).
 constexpr int kKeepThreads = 128, kKeepAhead = 8;
 template <bool kCodes>
 __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedParams p, const KeepArgs a, int pieces) {

@@ -31,6 +31,7 @@
 //   one token of 16 requests of 8000, 16/4 heads, head dim 256, e4m3      77; int8, fp16 88                                     [40]
 //   five tokens of 12 requests of 338 to 20016, int8, 16/4 heads, fp16    92 -> 52                                              [14]
 //   one token behind 20011, 16/4 heads, head dim 64, fp16                 64 -> 19 (pieces joined in parallel) -> 16            [3]
+//   a tree of 8 tokens behind 4001, 16/4 heads, head dim 64, fp16         (the form for trees; with the rows stored) 16.4; on tcgen05 25
 // The last is a chain of latencies, and much of the one before it: the plan of the line, a page's number, its rows, four warps joined, the second kernel.
 #pragma once
 

@@ -28,6 +28,11 @@
 //                                                        -> 1.28 (next to nothing in local memory), 830 TFLOP/s [648 us]: 4600 cycles a tile
 //   prompts of 1023, 4096 and 200, 16 heads, head dim 256   3.8 ms (mma.sync) -> 0.22 [89 us]
 //   4 tokens of 16 requests of 8000 over 8 kv heads      127 us (one row tile at work) -> 95 (both, key tiles by turns) [80 us of bytes]
+// Trees of drafted tokens (a form of their own: kTree; in brackets bytes or products at the measured rates):
+//   24 of 64 rows behind 1K to 16K tokens                 275 us (as any rows, the branch walked in the softmax) -> 269 (items longest first) -> 267 (an even line)
+//                                                         -> 231 (branches written down ahead) -> 222 (CTAs tell the join)   [115]: 2.3 us a key tile of 256 rows
+//                                                         in each SM, half of which are its MMAs, and some 9 us an item for Q, output and the pipeline's ends
+//   12 of 32 rows behind 333 to 20011, e4m3               147 -> 138 -> 131 -> 128 -> 120   [29]: codes turned into operand tiles, 2.3 us a tile
 #pragma once
 
 #include "attend_rows.cuh"

@@ -14,7 +14,15 @@
 // it tells the others what sum is needed next (so that no block takes another way than its neighbours, whatever the tensors hold), all blocks add up
 // their part of the vocabulary and tell one another.  A walk needs one pass over one row of p and q, one more for each drafted
 // sibling beyond the first that is not accepted; the token is found in the one block, warp and thread whose sums the random number falls to.
+// The sums are quick where no child or one was rejected: max(p - q, 0) = max(p, q) - q takes the maximum in 32 bits, exactly, and two
+// conversions; a sum that is not finite tells of infinities, and is taken again the careful way.
 // Bound by the bytes of that row where there are many sequences, else by the chain of loads and barriers.
+// Measured (replayed from a graph, us; in brackets the bytes at the measured copy bandwidth):
+//   5 rows of 64 sequences over 128000 tokens, fp32      35.4 -> 28.8 (four blocks an SM in place of one) -> 20.6 (quick sums)   [10.0]
+//   6 rows of one sequence over 32000, fp32              10.3                                                                [0.04]
+//   40 rows of 16 over 100003, bf16, no draft            18.5 -> 14.4 (the rejected tokens' bits looked at a vector at a time) [0.5]
+//   32 rows of 24 over 64000, many siblings              141 (divided by S) -> 56 (by 1 / S, and quick sums)
+// The second is: launch 2.5, tokens and their probabilities (three dependent loads), the walk, three barriers of the cluster, one pass, one look for the token.
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 
