@@ -22,7 +22,6 @@ struct PagedParams {
   const int32_t* cu;
   const int32_t* lens;
   const int32_t* table;
-  const int32_t* parents;                  // of the packed rows, within their sequences; null: each row sees all before it
 };
 
 // A sequence of the batch: its packed rows [row0, row0 + n), of which row i is at position pos0 + i.  Numbers that make no
@@ -105,7 +104,7 @@ inline bool paged_few_rows(const PagedParams& p) {
   return (int64_t)p.max_new * p.G <= most;
 }
 
-// Both kernels have a form for trees of drafted tokens (PagedParams::parents), each in a source file of its own.
+// Both kernels have a form for trees of drafted tokens, each in a source file of its own; `parents`: of the packed rows, within their sequences.
 // Of trees over 16-bit pages up to 64 rows also where they are so few, before keys so few, that the other kernel's launches and items cost more than reading
 // the keys again for each 16 rows.  The lengths are on the device: what the tables have room for stands for them.  (rows: this kernel / tcgen05, us)
 //   head dim 64           1 sequence of 4000, 4 kv heads  32: 15 / 27, 64: 17 / 27     8 of 8000, 8  32: 56 / 60, 48: 72 / 61     48 of 500, 8  64: 51 / 62
@@ -127,9 +126,9 @@ cudaError_t launch_paged_rows(const PagedParams& p, const void* q, const void* k
 size_t paged_few_workspace(const PagedParams& p);
 cudaError_t launch_paged_few(const PagedParams& p, const void* q, const void* kp, const void* vp, const uint8_t* ks,
                              const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st);
-cudaError_t launch_paged_rows_tree(const PagedParams& p, const void* q, const void* kp, const void* vp, const uint8_t* ks,
+cudaError_t launch_paged_rows_tree(const PagedParams& p, const int32_t* parents, const void* q, const void* kp, const void* vp, const uint8_t* ks,
                                    const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st);
-cudaError_t launch_paged_few_tree(const PagedParams& p, const void* q, const void* kp, const void* vp, const uint8_t* ks,
+cudaError_t launch_paged_few_tree(const PagedParams& p, const int32_t* parents, const void* q, const void* kp, const void* vp, const uint8_t* ks,
                                   const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st);
 
 }  // namespace moba

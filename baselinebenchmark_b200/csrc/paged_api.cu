@@ -61,7 +61,6 @@ PagedParams paged_params(const moba_paged_t* p, const int32_t* cu, const int32_t
   r.cu = cu;
   r.lens = lens;
   r.table = table;
-  r.parents = nullptr;
   return r;
 }
 
@@ -134,12 +133,12 @@ int moba_paged_tree_attention(const moba_paged_t* p, const void* q, const int32_
   if (rc != MOBA_OK) return rc;
   if (!apart(p, p->o_stride_token, p->o_stride_head, p->num_q_heads)) return MOBA_E_SHAPE;
   if (((uintptr_t)lse_out | (uintptr_t)parents) & 3) return MOBA_E_ALIGN;
-  PagedParams r = paged_params(p, cu, lens, table);
-  r.parents = parents;
+  const PagedParams r = paged_params(p, cu, lens, table);
   if (workspace == nullptr || workspace_bytes < workspace_of(r, parents != nullptr)) return MOBA_E_WORKSPACE;
   if ((uintptr_t)workspace & 31) return MOBA_E_ALIGN;
-  const auto launch = parents ? (paged_few_tree(r) ? launch_paged_few_tree : launch_paged_rows_tree) : paged_few_rows(r) ? launch_paged_few : launch_paged_rows;
-  return (int)launch(r, q, kp, vp, ks, vs, out, lse_out, workspace, (cudaStream_t)stream);
+  if (parents != nullptr)
+    return (int)(paged_few_tree(r) ? launch_paged_few_tree : launch_paged_rows_tree)(r, parents, q, kp, vp, ks, vs, out, lse_out, workspace, (cudaStream_t)stream);
+  return (int)(paged_few_rows(r) ? launch_paged_few : launch_paged_rows)(r, q, kp, vp, ks, vs, out, lse_out, workspace, (cudaStream_t)stream);
 }
 
 int moba_paged_keep(const moba_paged_t* p, const int32_t* cu, const int32_t* lens, const int32_t* table, const int32_t* path,

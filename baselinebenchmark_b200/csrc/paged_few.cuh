@@ -268,6 +268,7 @@ struct FewArgs {
   float* part;                             // [2 * CTAs][kM][D]: outputs of shared items, by CTA: 0 one that others began, 1 one that others end
   float2* part_ml;                         // [2 * CTAs][kM]: {maximum, sum}
   FewShared* shared;                       // [CTAs]
+  const int32_t* parents;                  // of trees
 };
 
 // Packed row (token, head) of row r of a tile, or -1.
@@ -603,7 +604,7 @@ paged_few_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_k
         uint32_t see[kE];
         if (kTree) {
 #pragma unroll
-          for (int e = 0; e < kE; ++e) see[e] = tree_keys(p.parents + s.row0, node[e], s.pos0, key0);
+          for (int e = 0; e < kE; ++e) see[e] = tree_keys(a.parents + s.row0, node[e], s.pos0, key0);
         }
 #pragma unroll
         for (int n = 0; n < kBlocksN; ++n)
@@ -933,13 +934,13 @@ constexpr size_t kSharedBytes = (kFewMaxCtas * sizeof(FewShared) + 255) / 256 * 
 size_t few_workspace(const PagedParams& p) { return kSharedBytes + (size_t)2 * kFewMaxCtas * 16 * (p.D * sizeof(float) + sizeof(float2)); }
 
 template <bool kTree>
-cudaError_t launch_few(const PagedParams& all, const void* q, const void* kp, const void* vp, const uint8_t* ks,
+cudaError_t launch_few(const PagedParams& all, const int32_t* parents, const void* q, const void* kp, const void* vp, const uint8_t* ks,
                              const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st) {
   const bool eight = (int64_t)all.max_new * all.G <= 8;
   const int tile_rows = eight ? 8 : 16;
   const FewKernels k = all.fp16 ? (eight ? pick_few_dim<kTree, true, 8>(all.D, all.store) : pick_few_dim<kTree, true, 16>(all.D, all.store))
                                 : (eight ? pick_few_dim<kTree, false, 8>(all.D, all.store) : pick_few_dim<kTree, false, 16>(all.D, all.store));
-  FewArgs a{q, kp, vp, ks, vs, out, lse, nullptr, nullptr, nullptr};
+  FewArgs a{q, kp, vp, ks, vs, out, lse, nullptr, nullptr, nullptr, parents};
   a.shared = static_cast<FewShared*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + kSharedBytes);
   a.part = reinterpret_cast<float*>(a.part_ml + 2 * kFewMaxCtas * 16);

@@ -7,7 +7,7 @@ size_t paged_rows_workspace(const PagedParams& p) { return rows_workspace(p, fal
 
 cudaError_t launch_paged_rows(const PagedParams& p, const void* q, const void* kp, const void* vp, const uint8_t* ks,
                               const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st) {
-  return launch_rows<false>(p, q, kp, vp, ks, vs, out, lse, workspace, st);
+  return launch_rows<false>(p, nullptr, q, kp, vp, ks, vs, out, lse, workspace, st);
 }
 
 }  // namespace moba

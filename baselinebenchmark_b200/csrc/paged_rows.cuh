@@ -210,7 +210,7 @@ struct alignas(32) TreeMask {
   int32_t pad[3];
 };
 // Of 1024 packed rows from `base` on; all threads of a block.
-__device__ __forceinline__ void tree_masks(const PagedParams& p, TreeMask* masks, int64_t base, int* up) {
+__device__ __forceinline__ void tree_masks(const PagedParams& p, const int32_t* parents, TreeMask* masks, int64_t base, int* up) {
   const int64_t t = base + threadIdx.x;
   int parent = -1;
   bool on = false;
@@ -226,7 +226,7 @@ __device__ __forceinline__ void tree_masks(const PagedParams& p, TreeMask* masks
     const int64_t i = t - s.row0;
     on = i >= 0 && i < s.n;
     if (on) {
-      const int of = __ldg(p.parents + t);
+      const int of = __ldg(parents + t);
       if (of >= 0 && of < i) parent = s.row0 + of;          // (rows are counted in 32 bits)
     }
   }
@@ -259,14 +259,14 @@ static_assert(1024 % kTreeGroup == 0, "groups do not lie in two blocks");
 // sequence in even steps of a ratio.
 // Behind the plan's block, others write down what each packed row sees of the rows around it (see TreeMask).
 constexpr int kTreeSorted = 128;           // sequences up to which it is worth looking at their order
-__global__ void __launch_bounds__(1024) paged_tree_plan_kernel(const PagedParams p, RowsPlan* plan, TreeMask* masks, int sms, int most_slots) {
+__global__ void __launch_bounds__(1024) paged_tree_plan_kernel(const PagedParams p, const int32_t* parents, RowsPlan* plan, TreeMask* masks, int sms, int most_slots) {
   __shared__ int rows_s[kPagedBatch], most_s[kPagedBatch], least_s[kPagedBatch];
   __shared__ float cost_s[32];
   __shared__ int piece_s[32], scan_s[2][32];
   pdl_wait();
   pdl_trigger();
   if (blockIdx.x > 0) {
-    tree_masks(p, masks, (int64_t)(blockIdx.x - 1) * 1024, rows_s);
+    tree_masks(p, parents, masks, (int64_t)(blockIdx.x - 1) * 1024, rows_s);
     return;
   }
   const int b = threadIdx.x, warp = b >> 5, lane = b & 31;
@@ -1678,14 +1678,14 @@ __global__ void __launch_bounds__(kJoinThreads) paged_rows_join_kernel(const Pag
 }
 
 template <bool kTree, bool kHalf, int D>
-cudaError_t launch_rows_dim(const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, const RowsArgs& a, int sms, int slots, cudaStream_t st) {
+cudaError_t launch_rows_dim(const PagedParams& p, const int32_t* parents, const CUtensorMap& mk, const CUtensorMap& mv, const RowsArgs& a, int sms, int slots, cudaStream_t st) {
   auto kernel = p.store == MOBA_STORE_SAME ? paged_rows_kernel<kHalf, D, MOBA_STORE_SAME, kTree>
               : p.store == MOBA_STORE_E4M3 ? paged_rows_kernel<kHalf, D, MOBA_STORE_E4M3, kTree> : paged_rows_kernel<kHalf, D, MOBA_STORE_INT8, kTree>;
   const int threads = p.store == MOBA_STORE_SAME ? kRowsThreads<MOBA_STORE_SAME> : kRowsThreads<MOBA_STORE_E4M3>;
   cudaError_t e = prepare_kernel(kernel, kRowsSmem);
   if (e != cudaSuccess) return e;
   if constexpr (kTree) {
-    e = launch_pdl(paged_tree_plan_kernel, dim3((unsigned)(1 + (p.T + 1023) / 1024)), kPagedBatch, 0, st, p, a.plan, const_cast<TreeMask*>(a.masks), sms, slots);
+    e = launch_pdl(paged_tree_plan_kernel, dim3((unsigned)(1 + (p.T + 1023) / 1024)), kPagedBatch, 0, st, p, parents, a.plan, const_cast<TreeMask*>(a.masks), sms, slots);
   } else {
     e = launch_pdl(paged_plan_kernel, dim3(1), kPagedBatch, 0, st, p, a.plan, sms, slots);
   }
@@ -1705,7 +1705,7 @@ size_t rows_workspace(const PagedParams& p, bool tree) {
 }
 
 template <bool kTree>
-cudaError_t launch_rows(const PagedParams& all, const void* q, const void* kp, const void* vp, const uint8_t* ks,
+cudaError_t launch_rows(const PagedParams& all, const int32_t* parents, const void* q, const void* kp, const void* vp, const uint8_t* ks,
                               const uint8_t* vs, void* out, float* lse, void* workspace, cudaStream_t st) {
   RowsArgs a;
   a.q = static_cast<const __nv_bfloat16*>(q);
@@ -1735,10 +1735,10 @@ cudaError_t launch_rows(const PagedParams& all, const void* q, const void* kp, c
     p.cu += b;
     p.lens += b;
     p.table += b * all.table_stride;
-    const cudaError_t e = p.D == 64 ? (p.fp16 ? launch_rows_dim<kTree, true, 64>(p, mk, mv, a, sms, slots_of_results, st) : launch_rows_dim<kTree, false, 64>(p, mk, mv, a, sms, slots_of_results, st))
-                        : p.D == 96 ? (p.fp16 ? launch_rows_dim<kTree, true, 96>(p, mk, mv, a, sms, slots_of_results, st) : launch_rows_dim<kTree, false, 96>(p, mk, mv, a, sms, slots_of_results, st))
-                        : p.D == 128 ? (p.fp16 ? launch_rows_dim<kTree, true, 128>(p, mk, mv, a, sms, slots_of_results, st) : launch_rows_dim<kTree, false, 128>(p, mk, mv, a, sms, slots_of_results, st))
-                                     : (p.fp16 ? launch_rows_dim<kTree, true, 256>(p, mk, mv, a, sms, slots_of_results, st) : launch_rows_dim<kTree, false, 256>(p, mk, mv, a, sms, slots_of_results, st));
+    const cudaError_t e = p.D == 64 ? (p.fp16 ? launch_rows_dim<kTree, true, 64>(p, parents, mk, mv, a, sms, slots_of_results, st) : launch_rows_dim<kTree, false, 64>(p, parents, mk, mv, a, sms, slots_of_results, st))
+                        : p.D == 96 ? (p.fp16 ? launch_rows_dim<kTree, true, 96>(p, parents, mk, mv, a, sms, slots_of_results, st) : launch_rows_dim<kTree, false, 96>(p, parents, mk, mv, a, sms, slots_of_results, st))
+                        : p.D == 128 ? (p.fp16 ? launch_rows_dim<kTree, true, 128>(p, parents, mk, mv, a, sms, slots_of_results, st) : launch_rows_dim<kTree, false, 128>(p, parents, mk, mv, a, sms, slots_of_results, st))
+                                     : (p.fp16 ? launch_rows_dim<kTree, true, 256>(p, parents, mk, mv, a, sms, slots_of_results, st) : launch_rows_dim<kTree, false, 256>(p, parents, mk, mv, a, sms, slots_of_results, st));
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
