@@ -443,7 +443,8 @@ int moba_paged_attention(const moba_paged_t* p, const void* q, const int32_t* cu
                          void* stream);
 /* The same for packed rows that are trees of drafted tokens.  parents: int32[total_tokens] on the device; parents[cu[b] + i] is the row of
  * sequence b, counted from cu[b], that row i follows.  A row sees the positions in front of the sequence's packed rows, its own and those of its
- * ancestors; a parent that is not in 0 .. i-1 is none.  Positions of the table are by row, as in every call: the branches lie one behind
+ * ancestors; a parent that is not in 0 .. i-1 is none.  What is said above of infinities and NaN in a token behind holds for one of another
+ * branch.  Positions of the table are by row, as in every call: the branches lie one behind
  * another in the pages.  parents == NULL: moba_paged_attention, with its workspace. */
 int moba_paged_tree_workspace_size(const moba_paged_t* p, size_t* bytes);
 int moba_paged_tree_attention(const moba_paged_t* p, const void* q, const int32_t* parents, const int32_t* cu_seqlens,
