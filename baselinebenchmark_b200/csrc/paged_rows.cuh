@@ -29,9 +29,9 @@
 //   prompts of 1023, 4096 and 200, 16 heads, head dim 256   3.8 ms (mma.sync) -> 0.22 [89 us]
 //   4 tokens of 16 requests of 8000 over 8 kv heads      127 us (one row tile at work) -> 95 (both, key tiles by turns) [80 us of bytes]
 // Trees of drafted tokens (a form of their own: kTree; in brackets bytes or products at the measured rates):
-//   24 of 64 rows behind 1K to 16K tokens                 275 us (as any rows, the branch walked in the softmax) -> 269 (items longest first) -> 267 (an even line)
-//                                                         -> 231 (branches written down ahead) -> 222 (CTAs tell the join)   [115]: 2.3 us a key tile of 256 rows
-//                                                         in each SM, half of which are its MMAs, and some 9 us an item for Q, output and the pipeline's ends
+//   24 of 64 rows behind 1K to 16K tokens                 275 us (as any rows, the branch walked in the softmax) -> 267 (an even line) -> 231 (branches
+//                                                         written down ahead) -> 222 (CTAs tell the join)   [115]: 2.3 us a key tile of 256 rows in each
+//                                                         SM, half of which are its MMAs, and some 9 us an item for Q, output and the pipeline's ends
 //   12 of 32 rows behind 333 to 20011, e4m3               147 -> 138 -> 131 -> 128 -> 120   [29]: codes turned into operand tiles, 2.3 us a tile
 #pragma once
 
@@ -67,7 +67,7 @@ int rows_slots(const PagedParams& p) {
 }
 // Trees on a line (see paged_tree_plan_kernel): two slots for each CTA that has a stretch of it.
 constexpr int kTreeLeast = 8;              // units of a stretch, at least
-constexpr int kTreeItem = 4, kTreePiece = 2;   // what an item costs besides its key tiles, in tiles, and what more when it is cut
+constexpr int kTreeItem = 4;               // what an item costs besides its key tiles, in tiles
 int tree_slots(const PagedParams& p) {
   const int64_t keys = ((int64_t)p.per_seq << p.page_shift), units = (keys + kBN - 1) / kBN + kTreeItem;
   const int64_t items = (p.T < p.B ? p.T : p.B) * (int64_t)p.Hkv;
@@ -89,7 +89,6 @@ struct RowsPlan {
   int32_t begin[kPagedBatch + 1];          // first item of a sequence
   int32_t slot0[kPagedBatch];              // first result slot of a sequence whose items are cut
   int32_t piece[kPagedBatch];              // key tiles of a piece
-  int32_t order[kPagedBatch];              // of trees: the sequences, those with the longest pieces first; `begin` is in this order
   int4 shared[kMostLine];                  // of trees on a line, from each CTA: the item that it began and others end: pieces (0: there is none),
                                            // first packed row, rows, kv head
 };
@@ -117,13 +116,11 @@ __device__ __forceinline__ int even_piece(int tiles, int piece) {
 
 // Candidate k cuts the batch into about k / 4 pieces a CTA, candidate 0 not at all.  With equal pieces the time is that of the waves;
 // longer ones than the average may come last.
-__global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p, RowsPlan* plan, int sms, int most_slots) {
+__device__ __forceinline__ void plan_pieces(const PagedParams& p, RowsPlan* plan, int sms, int most_slots) {
   __shared__ int rows_s[kPagedBatch], most_s[kPagedBatch], least_s[kPagedBatch];
   __shared__ float cost_s[32];
   __shared__ int piece_s[32];
   __shared__ int scan_s[2][32];
-  pdl_wait();
-  pdl_trigger();
   const int b = threadIdx.x, warp = b >> 5, lane = b & 31;
   int rows = 0, most = 1, least = 1;
   if (b < p.B) {
@@ -199,6 +196,11 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p, R
     }
   }
 }
+__global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p, RowsPlan* plan, int sms, int most_slots) {
+  pdl_wait();
+  pdl_trigger();
+  plan_pieces(p, plan, sms, most_slots);
+}
 
 // What packed row t sees of the kTreeGroup packed rows of its group (those with the same t / kTreeGroup), and the nearest ancestor in front of it (-1:
 // none).  A row's branch is a walk along its ancestors, a load from L2 each where shared memory leaves no L1: with the walk in the softmax of
@@ -250,153 +252,52 @@ __device__ __forceinline__ void tree_masks(const PagedParams& p, const int32_t* 
 static_assert(1024 % kTreeGroup == 0, "groups do not lie in two blocks");
 
 // Trees: few rows behind keys of any number, so that a batch is a few hundred items of all lengths, and what counts is that no CTA is left with a long
-// one at the end.
-// Where no sequence has more than one row tile, the items are a line of units, kTreeItem in front of each for what it costs besides its key
-// tiles, and every CTA has an equal stretch of it: the end of an item, whole ones, the beginning of one.  Its two parts of items
-// go to two slots of results of its own, and the join finds an item's parts by where it lies on the line.
-// Otherwise row tiles see different numbers of keys, and those of one head read the same ones: items are drawn longest first, and a candidate's time is the largest of what no order can beat: the work of all, evenly; the
-// longest item; and k items of the length of number (k - 1) * SMs + 1, of which some CTA has k.  Candidates go down from the longest
-// sequence in even steps of a ratio.
+// one at the end.  Where no sequence has more than one row tile, the items are a line of units, kTreeItem in front of each for what it costs besides its key
+// tiles, and every CTA has an equal stretch of it: the end of an item, whole ones, the beginning of one.  Its two parts of items go to two slots of
+// results of its own.  Otherwise row tiles see different numbers of keys, and those of one head read the same ones: pieces as above.
 // Behind the plan's block, others write down what each packed row sees of the rows around it (see TreeMask).
-constexpr int kTreeSorted = 128;           // sequences up to which it is worth looking at their order
 __global__ void __launch_bounds__(1024) paged_tree_plan_kernel(const PagedParams p, const int32_t* parents, RowsPlan* plan, TreeMask* masks, int sms, int most_slots) {
-  __shared__ int rows_s[kPagedBatch], most_s[kPagedBatch], least_s[kPagedBatch];
-  __shared__ float cost_s[32];
-  __shared__ int piece_s[32], scan_s[2][32];
+  __shared__ int scan_s[32], up_s[1024];
   pdl_wait();
   pdl_trigger();
   if (blockIdx.x > 0) {
-    tree_masks(p, parents, masks, (int64_t)(blockIdx.x - 1) * 1024, rows_s);
+    tree_masks(p, parents, masks, (int64_t)(blockIdx.x - 1) * 1024, up_s);
     return;
   }
   const int b = threadIdx.x, warp = b >> 5, lane = b & 31;
-  int rows = 0, most = 1, least = 1;
+  int units = 0;                                            // of an item; none without rows
+  bool good = true;
   if (b < p.B) {
     const PagedSeq s = paged_seq(p, b);
     const int tiles = rows_tiles(p, s.n);
-    rows = tiles * p.Hkv;
-    if (tiles > 0) {
-      most = key_tiles(rows_end(p, s, tiles - 1));
-      least = key_tiles(rows_end(p, s, 0));
-    }
+    if (tiles > 0) units = key_tiles(rows_end(p, s, tiles - 1)) + kTreeItem;
+    good = tiles <= 1 && (int64_t)units * p.Hkv < ((int64_t)1 << 20);
   }
-  rows_s[b] = rows;
-  most_s[b] = most;
-  least_s[b] = least;
-  // ---- a line?
-  {
-    const int units = rows > 0 ? most + kTreeItem : 0;
-    // (rows: kv heads of the one row tile)
-    const bool good = rows <= p.Hkv && (int64_t)units * p.Hkv < ((int64_t)1 << 20);
-    const int mine = rows > 0 ? units * p.Hkv : 0;
-    if (__syncthreads_and(good)) {
-      int x = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += u;
-      }
-      if (lane == 31) scan_s[0][warp] = x;
-      __syncthreads();
-      const int all = __reduce_add_sync(0xffffffffu, scan_s[0][lane]), before = __reduce_add_sync(0xffffffffu, lane < warp ? scan_s[0][lane] : 0);
-      const int ctas = max(min(min(min(sms, kMostLine), most_slots / 2), all / kTreeLeast), 1);
-      if (b < p.B) {
-        plan->begin[b] = before + x - mine;
-        if (b == p.B - 1) {
-          plan->begin[p.B] = all;
-          plan->ctas = ctas;
-          plan->each = all / ctas;
-          plan->rest = all % ctas;
-          plan->status = 0;
-          plan->items = 0;
-        }
-      }
-      return;
-    }
+  if (!__syncthreads_and(good)) {
+    if (b == 0) plan->ctas = 0;
+    plan_pieces(p, plan, sms, most_slots);
+    return;
   }
-  int longest = 1;
-  for (int i = lane; i < p.B; i += 32)
-    if (rows_s[i] > 0) longest = max(longest, most_s[i]);
-  longest = __reduce_max_sync(0xffffffffu, longest);
-  const int piece = warp == 0 ? longest : max((int)ceilf((float)longest * exp2f(log2f((float)kLeastPiece / (float)max(longest, kLeastPiece)) * (float)warp / 31.f)), kLeastPiece);
-  float work = 0.f;
-  int slots = 0, top = 1, items = 0;
-  int size[2] = {0, 0}, count[2] = {0, 0};                  // of this lane's sequences, where there are up to 64
-  for (int i = lane, k = 0; i < p.B; i += 32, ++k) {
-    if (rows_s[i] == 0) continue;
-    const int even = even_piece(most_s[i], piece), cuts = (most_s[i] + even - 1) / even, mine = min(rows_s[i], 1 << 15) * min(cuts, 1 << 10);
-    const int cost = even + kTreeItem + (cuts > 1 ? kTreePiece : 0);
-    work += (float)rows_s[i] * (0.5f * (float)(most_s[i] + least_s[i]) + (float)cuts * (float)(cost - even));
-    if (cuts > 1) slots += (int)min((int64_t)rows_s[i] * cuts, (int64_t)(1 << 20));
-    top = max(top, cost);
-    items += min(mine, 1 << 20);
-    if (k < 2) {
-      if (k == 0) { size[0] = cost; count[0] = mine; } else { size[1] = cost; count[1] = mine; }
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
-  slots = __reduce_add_sync(0xffffffffu, min(slots, 1 << 25));
-  items = __reduce_add_sync(0xffffffffu, min(items, 1 << 25));
-  top = __reduce_max_sync(0xffffffffu, top);
-  float cost = fmaxf(work / (float)sms, (float)top);
-  if (p.B <= 64) {
-    for (int k = 2; k <= 4 && items > (k - 1) * sms; ++k) {
-      int lo = 1, hi = top;                                 // the largest size that as many items have
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        const int n = __reduce_add_sync(0xffffffffu, (size[0] >= mid ? count[0] : 0) + (size[1] >= mid ? count[1] : 0));
-        if (n > (k - 1) * sms) lo = mid; else hi = mid - 1;
-      }
-      cost = fmaxf(cost, (float)(k * lo));
-    }
-  }
-  if (lane == 0) {
-    cost_s[warp] = slots > most_slots ? INFINITY : cost;
-    piece_s[warp] = piece;
-  }
-  __syncthreads();
-  // every warp for itself: the cheapest, of equal ones the first (costs are not negative: they compare as integers)
-  const uint32_t mine = __float_as_uint(cost_s[lane]);
-  const int best = piece_s[__ffs(__ballot_sync(0xffffffffu, mine == __reduce_min_sync(0xffffffffu, mine))) - 1];
-  const int even = even_piece(most, best), cuts = (most + even - 1) / even;
-  // the sequences' places in the order
-  int place = b;
-  if (p.B <= kTreeSorted) {
-    least_s[b] = rows > 0 ? even : 0;
-    __syncthreads();
-    if (b < p.B) {
-      place = 0;
-      for (int i = 0; i < p.B; ++i) place += least_s[i] > least_s[b] || (least_s[i] == least_s[b] && i < b);
-    }
-    __syncthreads();
-  }
-  most_s[place] = rows * cuts;                              // (a thread without a sequence has its own place)
-  rows_s[place] = b;
-  __syncthreads();
-  // first items of the places, first slots of the sequences
-  const int n = b < p.B ? most_s[b] : 0, m = cuts > 1 && b < p.B ? rows * cuts : 0;
-  int x = n, y = m;
+  const int mine = units * p.Hkv;
+  int x = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
-    if (lane >= o) { x += u; y += v; }
+    const int u = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += u;
   }
-  if (lane == 31) { scan_s[0][warp] = x; scan_s[1][warp] = y; }
+  if (lane == 31) scan_s[warp] = x;
   __syncthreads();
-  const int bx = __reduce_add_sync(0xffffffffu, lane < warp ? scan_s[0][lane] : 0);
-  const int by = __reduce_add_sync(0xffffffffu, lane < warp ? scan_s[1][lane] : 0);
+  const int all = __reduce_add_sync(0xffffffffu, scan_s[lane]), before = __reduce_add_sync(0xffffffffu, lane < warp ? scan_s[lane] : 0);
   if (b < p.B) {
-    plan->begin[b] = bx + x - n;
-    plan->order[b] = rows_s[b];
-    plan->slot0[b] = m > 0 ? by + y - m : -1;
-    plan->piece[b] = even;
+    plan->begin[b] = before + x - mine;
     if (b == p.B - 1) {
-      plan->begin[p.B] = bx + x;
-      plan->items = bx + x;
-      plan->counter = 0;
+      const int ctas = max(min(min(min(sms, kMostLine), most_slots / 2), all / kTreeLeast), 1);
+      plan->begin[p.B] = all;
+      plan->ctas = ctas;
+      plan->each = all / ctas;
+      plan->rest = all % ctas;
       plan->status = 0;
-      plan->ctas = 0;
+      plan->items = 0;
     }
   }
 }
@@ -414,6 +315,7 @@ struct RowsItem {
   int j0, ntiles;                          // key tiles [j0, j0 + ntiles) of the sequence
   int row0, pos0, len;                     // the sequence's (PagedSeq)
   int slot;                                // of its results; -1: not cut
+  bool line;                               // of trees: no branches, each row sees all before it
 };
 
 // Where the codes of a key tile lie: for its eight groups of 16 keys, which have a page each.
@@ -452,7 +354,8 @@ struct RowsArgs {
   float* part;                             // [slots][rows of an item][D]
   float2* part_ml;                         // the same rows: {maximum, sum}
   FastDiv by_group;
-  const TreeMask* masks;                   // of trees: a packed row each
+  const int32_t* parents;                  // of trees
+  const TreeMask* masks;                   // the same: a packed row each
 };
 
 // Items that are not cut come longest first, all heads by turns, where the K and V of all heads stay in L2 together; otherwise head by head, so that
@@ -515,12 +418,11 @@ __device__ __forceinline__ void rows_prefetch(const PagedParams& p, const RowsAr
     if (lane == 0) idx = c.abort ? 0x7fffffff : atomicAdd(&a.plan->counter, 1);
     idx = __shfl_sync(0xffffffffu, idx, 0);
     if (idx >= c.items) { done = true; break; }
-    const int place = search_warp(p.B, idx, [&](int k) { return __ldcg(a.plan->begin + k); });
-    it.b = kTree ? __ldcg(a.plan->order + place) : place;
+    it.b = search_warp(p.B, idx, [&](int k) { return __ldcg(a.plan->begin + k); });
     const PagedSeq s = paged_seq(p, it.b);
     const int tiles = rows_tiles(p, s.n), piece = __ldcg(a.plan->piece + it.b);
     const int most = key_tiles(rows_end(p, s, tiles - 1)), cuts = (most + piece - 1) / piece;
-    const int i = idx - __ldcg(a.plan->begin + place);      // kv head, piece, row tile, the last one first
+    const int i = idx - __ldcg(a.plan->begin + it.b);      // kv head, piece, row tile, the last one first
     int cut = 0;
     if (cuts == 1 && (int64_t)s.len * p.Hkv * p.D * 4 <= kAllHeadsBytes) {
       it.tile = tiles - 1 - i / p.Hkv;
@@ -541,6 +443,23 @@ __device__ __forceinline__ void rows_prefetch(const PagedParams& p, const RowsAr
     it.len = s.len;
     it.slot = cuts > 1 ? __ldcg(a.plan->slot0 + it.b) + i : -1;
     break;
+  }
+  if (kTree && !done) {
+    // A batch may hold blocks of prompts beside trees, thousands of rows of which each follows the one before.  They need no masks but the causal one
+    // (one prompt of 8192 rows, 32/8 heads of 128: 0.68 ms; its branches put together from groups of rows, tile by tile, 1.7 ms; without parents 0.61).
+    const int last = min((int)(((int64_t)(it.tile + 1) * item_rows(p.D) - 1) / p.G), (int)((int64_t)it.tile * item_rows(p.D) + it.nrows - 1) / p.G);
+    const int32_t* up = a.parents + it.row0;
+    it.line = true;
+    constexpr int kAbreast = 8;
+    for (int base = 1; it.line && base <= last; base += 32 * kAbreast) {
+      bool good = true;
+#pragma unroll
+      for (int k = 0; k < kAbreast; ++k) {
+        const int i = base + 32 * k + lane;
+        if (i <= last) good &= __ldg(up + i) == i - 1;
+      }
+      it.line = __all_sync(0xffffffffu, good);
+    }
   }
   if (lane == 0) { c.item[at] = it; c.done[at] = done; }
   if (!done) {
@@ -902,6 +821,7 @@ __device__ __forceinline__ void zero_rows(unsigned char* tile, const RowsItem& i
 // The branch of a row in the key tile from key0 on, whatever pages there are: the keys in front of the packed rows, and of those the ones that
 // packed row t's masks say.  The tile's packed rows lie in two groups; farther groups are passed by their exits.
 __device__ __forceinline__ RowSees<true> branch_keys(const TreeMask* masks, const RowsItem& it, int i, int key0) {
+  if (it.line) return RowSees<true>{{0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu}};
   const int64_t front = (int64_t)it.pos0 - key0;            // keys of the tile in front of the packed rows
   const int64_t first = it.row0 - front;                    // packed row of the tile's first key (below row0 in front)
   const int64_t group = first >> 7;
@@ -1325,7 +1245,7 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
       const int i_row = (at + row) / a.by_group, i_first = at / a.by_group;
       const bool on = base + row < it.nrows;
       const int lim = on ? min(max(it.pos0 + i_row + 1, 0), it.len) : 0;
-      const int lim_first = min(max(it.pos0 + (kTree ? 0 : i_first + 1), 0), it.len);
+      const int lim_first = min(max(it.pos0 + (kTree && !it.line ? 0 : i_first + 1), 0), it.len);
       RowRef rr{-INFINITY, -INFINITY, 0.f};
       bool ok = true;
       if constexpr (kWide) {
@@ -1720,6 +1640,7 @@ cudaError_t launch_rows(const PagedParams& all, const int32_t* parents, const vo
   const int slots_of_results = kTree ? tree_slots(all) : rows_slots(all);
   a.part = reinterpret_cast<float*>(a.part_ml + (size_t)slots_of_results * item_rows(all.D));
   a.by_group = fast_div(all.G);
+  a.parents = parents;
   a.masks = reinterpret_cast<const TreeMask*>(static_cast<const char*>(workspace) + rows_results(all, slots_of_results));
   CUtensorMap mk{}, mv{};
   if (all.store == MOBA_STORE_SAME) {

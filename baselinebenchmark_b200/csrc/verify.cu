@@ -410,10 +410,11 @@ cudaError_t launch_verify(VerifyParams a, int dtype, cudaStream_t st) {
   int blocks = 0;
   int64_t least = 0;
   for (int n = kMostBlocks; n >= 1; n /= 2) {
+    const int64_t part = (a.vocabulary + n * step - 1) / (n * step) * step;
+    if (blocks != 0 && a.draft == nullptr && part / 8 > (128 << 10)) break;   // (the bits of a part lie in shared memory)
     const int64_t cost = (a.batch * (int64_t)n + round - 1) / round * (16000 + a.vocabulary / n);
-    if (blocks == 0 || cost < least) { blocks = n; least = cost; }
+    if (blocks == 0 || cost < least) { blocks = n; least = cost; a.part = part; }
   }
-  a.part = (a.vocabulary + blocks * step - 1) / (blocks * step) * step;
   const size_t smem = (size_t)a.max_new * (sizeof(double) + sizeof(Node)) + (size_t)((a.max_new + 1) & ~1) * sizeof(int16_t) +
                       (a.draft == nullptr ? (size_t)((a.part + 16 + 31) / 32) * 4 : 0);
   cudaError_t e = prepare_kernel(kernel, smem);

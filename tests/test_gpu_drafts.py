@@ -204,6 +204,23 @@ def test_a_wide_vocabulary():
         d.check()
 
 
+def test_the_widest_vocabulary_and_many_sequences():
+    """All rows have the same distribution, over 2**22 tokens; given tokens, rejected one after another."""
+    v, n = 2 ** 22, 600
+    g = torch.Generator(device="cuda").manual_seed(16)
+    row = torch.rand(v, device="cuda", generator=g)
+    row /= row.sum()
+    sample = torch.rand(n, device="cuda", generator=g)
+    tokens = torch.tensor([0, 5, v - 1, 70], device="cuda").repeat(n)
+    cu = torch.arange(0, 4 * n + 1, 4, dtype=torch.int32, device="cuda")
+    path, count, after = verify_drafts(row.expand(4 * n, v), None, tokens, cu, torch.ones(4 * n, device="cuda"), sample, 4, parents=_i32([-1, 0, 0, 0]).repeat(n))
+    assert (count == 1).all() and (path[:, 0] == 0).all() and (path[:, 1:] == -1).all()
+    left = row.double()
+    left[[5, v - 1, 70]] = 0.0
+    ends = left.cumsum(0)
+    assert torch.equal(after, torch.searchsorted(ends, sample.double() * ends[-1], right=True))
+
+
 def test_captured_and_on_two_streams():
     a, b = Drafts([5, 4], 5000, torch.float32, seed=12, spread=2), Drafts([5, 4], 5000, torch.float32, seed=13, spread=3)
     tensors = lambda d: [d.target.cuda(), d.draft.cuda(), torch.tensor(d.tokens, device="cuda"), d.accept.cuda(), d.sample.cuda(), _i32(d.parents)]  # noqa: E731

@@ -179,3 +179,25 @@ def test_even_and_uneven_batches_of_one_row_tile():
         table = torch.full((len(seqs), 8000), -1, dtype=torch.int32, device="cuda")
         table[:, :b.table.shape[1]] = b.table
         b.check(*paged_attention(b.q, b.k, b.v, table, b.cu, b.lens, 64, parents=b.parents, return_lse=True))
+
+
+@pytest.mark.parametrize("store", [None, E4M3])
+@pytest.mark.parametrize("dim", [128, 256])
+def test_prompts_beside_trees(dim, store):
+    """Blocks without branches, one that has a single branch late, trees and decode steps in one call; and a prompt alone, with parents and without."""
+    seqs = [(700, 900), (1, 300), (530, 530), (40, 100), (0, 9), (300, 800)]
+    b = TreeBatch(seqs, 4, 2, dim, 32, store=store, seed=14, spread=5)
+    ends, parents = b.cu_list, b.parent_list
+    for i in (0, 2, 5):
+        parents[ends[i]:ends[i + 1]] = range(-1, seqs[i][0] - 1)
+    parents[ends[2] + 511] = 400
+    b.parents.copy_(torch.tensor(parents, dtype=torch.int32))
+    b.fill()
+    b.check(*_attend(b))
+    one = TreeBatch([(700, 900)], 4, 2, dim, 32, store=store, seed=14, spread=1)
+    one.fill()
+    got, lse = _attend(one)
+    want, want_lse = paged_attention(one.q, one.k, one.v, *one.where, 700, return_lse=True, **one.scales)
+    # (pieces of an item may be cut elsewhere: sums of other parts)
+    one.check(got, lse)
+    one.check(want, want_lse)
