@@ -21,11 +21,20 @@ from .parallel import HEAD_DIMS
 
 __all__ = ["RotaryTable", "rotary", "rotary_frequencies"]
 
-_TURN = 2 * Fraction(314159265358979323846264338327950288419716939937510, 10 ** 50)
+#: 2 ** 160 units of a turn in a radian
+_PER_RADIAN = round(2 ** 160 / (2 * Fraction(314159265358979323846264338327950288419716939937510, 10 ** 50)))
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 #: struct moba_rotary, field by field (filling a ctypes structure by name takes ten times as long)
 _CALL = struct.Struct("@q8ifi8q")
 assert _CALL.size == C.sizeof(_lib.Rotary)
+
+
+def _turns(x: float) -> int:
+    """x radians as a part of a turn in units of 2 ** -64, whole turns dropped, as a signed 64-bit number."""
+    m, e = math.frexp(x)
+    n, shift = int(m * 2 ** 53) * _PER_RADIAN, 149 - e       # x = m * 2 ** 53 * 2 ** (e - 53)
+    n = ((n + (1 << (shift - 1))) >> shift if shift > 0 else n << -shift) % 2 ** 64
+    return n - 2 ** 64 if n >= 2 ** 63 else n
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str = "none", factor: float = 1.0,
@@ -66,17 +75,14 @@ class RotaryTable:
         f = torch.as_tensor(frequencies, dtype=torch.float64).detach().cpu()
         if f.ndim != 1 or f.numel() == 0:
             raise ValueError(f"frequencies must have shape [rotary_dim / 2], got {tuple(f.shape)}")
-        if not bool(torch.isfinite(f).all()):
+        radians = f.tolist()
+        if not all(map(math.isfinite, radians)):
             raise ValueError("frequencies must be finite")
         if not 0.0 < C.c_float(float(magnitude)).value <= 3.0e38:
             raise ValueError(f"magnitude must be a positive number of 32 bits, got {magnitude}")
-        turns = []
-        for x in f.tolist():
-            n = round(Fraction(x) / _TURN * 2 ** 64) % 2 ** 64      # (exact to half a unit: whole turns do not count)
-            turns.append(n - 2 ** 64 if n >= 2 ** 63 else n)
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self.rotary_dim, self.interleaved, self.magnitude = 2 * f.numel(), bool(interleaved), float(magnitude)
-        self.turns = torch.tensor(turns, dtype=torch.int64).to(device)
+        self.turns = torch.tensor([_turns(x) for x in radians], dtype=torch.int64).to(device)
         self.index = self.turns.get_device()
 
 
