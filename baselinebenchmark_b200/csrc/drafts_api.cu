@@ -37,6 +37,11 @@ int moba_rotary(const moba_rotary_t* p, const void* q, const void* k, const int3
   if (!q || !q_out || !positions || !turns || (p->num_kv_heads > 0 && (!k || !k_out))) return MOBA_E_NULL;
   if (((uintptr_t)q | (uintptr_t)q_out | (p->num_kv_heads > 0 ? (uintptr_t)k | (uintptr_t)k_out : 0)) & 15) return MOBA_E_ALIGN;
   if (((uintptr_t)positions & 3) || ((uintptr_t)turns & 7)) return MOBA_E_ALIGN;
+  // rows that are turned where they are lie there the same way (a single token or head is never stepped over)
+  auto apart = [&](int64_t t, int64_t h, int64_t to, int64_t ho, int heads) { return (p->total_tokens > 1 && t != to) || (heads > 1 && h != ho); };
+  if (q == q_out && apart(p->q_stride_token, p->q_stride_head, p->qo_stride_token, p->qo_stride_head, p->num_q_heads)) return MOBA_E_SHAPE;
+  if (p->num_kv_heads > 0 && k == k_out && apart(p->k_stride_token, p->k_stride_head, p->ko_stride_token, p->ko_stride_head, p->num_kv_heads))
+    return MOBA_E_SHAPE;
   RotaryParams r{};
   r.rows = p->total_tokens;
   r.heads_q = p->num_q_heads;

@@ -217,6 +217,9 @@ def test_refusals():
         rotary(q, k, pos, table, out=(q[:2], k))
     with pytest.raises(RuntimeError, match="error -1"):                   # rows on one another
         rotary(q, None, pos, table, out=(q[:1].expand(3, 2, 64), None))
+    other = torch.zeros(3, 4, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="error -1"):                   # where the rows are, but not the same way
+        rotary(other[:, ::2], None, pos, table, out=(other[:, :2], None))
     with pytest.raises(RuntimeError, match="error -6"):
         rotary(torch.zeros(3 * 130, dtype=torch.bfloat16, device="cuda").as_strided((3, 2, 64), (130, 65, 1)), None, pos, table)
     leaf = q.clone().requires_grad_()
