@@ -823,6 +823,8 @@ __device__ __forceinline__ void zero_rows(unsigned char* tile, const RowsItem& i
 __device__ __forceinline__ RowSees<true> branch_keys(const TreeMask* masks, const RowsItem& it, int i, int key0) {
   if (it.line) return RowSees<true>{{0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu}};
   const int64_t front = (int64_t)it.pos0 - key0;            // keys of the tile in front of the packed rows
+  // (all of them where a sequence's length is beyond what its table has room for: its packed rows lie behind the last tile)
+  if (front >= kBN) return RowSees<true>{{0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu}};
   const int64_t first = it.row0 - front;                    // packed row of the tile's first key (below row0 in front)
   const int64_t group = first >> 7;
   const int off = (int)(first & 127);
@@ -835,7 +837,7 @@ __device__ __forceinline__ RowSees<true> branch_keys(const TreeMask* masks, cons
   };
   uint64_t a0 = 0, a1 = 0, b0 = 0, b1 = 0;
   int64_t at = (int64_t)it.row0 + i;
-  while ((at >> 7) > group + 1) at = __ldcg(&masks[at].exit);   // (each in front of the last; -1 ends it)
+  while (at >= 0 && (at >> 7) > group + 1) at = __ldcg(&masks[at].exit);   // (each in front of the last; -1: there is none)
   if (at >= 0 && (at >> 7) == group + 1) at = load(at, b0, b1);
   if (at >= 0 && (at >> 7) == group) load(at, a0, a1);
   // 128 bits from bit `off` of the two groups' 256 on
@@ -844,7 +846,7 @@ __device__ __forceinline__ RowSees<true> branch_keys(const TreeMask* masks, cons
   uint64_t lo = s ? x0 >> s | x1 << (64 - s) : x0, hi = s ? x1 >> s | x2 << (64 - s) : x1;
   if (front > 0) {
     lo |= front >= 64 ? ~0ull : (1ull << front) - 1;
-    if (front > 64) hi |= front >= 128 ? ~0ull : (1ull << (front - 64)) - 1;
+    if (front > 64) hi |= (1ull << (front - 64)) - 1;
   }
   return RowSees<true>{{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)}};
 }
