@@ -818,13 +818,19 @@ __device__ __forceinline__ void zero_rows(unsigned char* tile, const RowsItem& i
   }
 }
 
+// All keys of a tile, whatever pages there are.
+template <bool kTree>
+__device__ __forceinline__ RowSees<kTree> every_key() {
+  if constexpr (kTree) return RowSees<true>{{0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu}};
+  else return RowSees<false>{};                             // (a causal row's keys are counted: see row_sees)
+}
 // The branch of a row in the key tile from key0 on, whatever pages there are: the keys in front of the packed rows, and of those the ones that
 // packed row t's masks say.  The tile's packed rows lie in two groups; farther groups are passed by their exits.
 __device__ __forceinline__ RowSees<true> branch_keys(const TreeMask* masks, const RowsItem& it, int i, int key0) {
-  if (it.line) return RowSees<true>{{0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu}};
+  if (it.line) return every_key<true>();
   const int64_t front = (int64_t)it.pos0 - key0;            // keys of the tile in front of the packed rows
   // (all of them where a sequence's length is beyond what its table has room for: its packed rows lie behind the last tile)
-  if (front >= kBN) return RowSees<true>{{0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu}};
+  if (front >= kBN) return every_key<true>();
   const int64_t first = it.row0 - front;                    // packed row of the tile's first key (below row0 in front)
   const int64_t group = first >> 7;
   const int off = (int)(first & 127);
@@ -1209,7 +1215,8 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
       if (x == 0) {
         for (int j = 0; ok && j < ntiles; ++j, ++g) {
           const int key0 = (j0 + j) * kBN;
-          RowSees<kTree> branch{};
+          // (a tile in front of the packed rows is masked too where it lacks a page or its scores are large)
+          RowSees<kTree> branch = every_key<kTree>();
           if constexpr (kTree) { if (lim > 0 && key0 + kBN > lim_first) branch = branch_keys(a.masks, it, i_row, key0); }
           ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&c.s_full[g & 1]), (g >> 1) & 1));
           if (!ok) break;
@@ -1256,7 +1263,7 @@ paged_rows_kernel(const PagedParams p, const __grid_constant__ CUtensorMap tmap_
         const int j1 = twice ? x : 0, by = twice ? 2 : 1;
         for (int j = j1; ok && j < ntiles; j += by) {
           const int key0 = (j0 + j) * kBN;
-          RowSees<kTree> branch{};                          // (asked for before the scores are waited for)
+          RowSees<kTree> branch = every_key<kTree>();       // (asked for before the scores are waited for)
           if constexpr (kTree) { if (lim > 0 && key0 + kBN > lim_first) branch = branch_keys(a.masks, it, i_row, key0); }
           ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&c.s_full[x]), sph));
           if (!ok) break;
