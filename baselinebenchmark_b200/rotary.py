@@ -45,7 +45,9 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str =
         "linear"  every frequency divided by the factor
         "base"    the base times factor ** (rotary_dim / (rotary_dim - 2)): the slowest pair is divided by the factor, the fastest stays
         "parts"   pairs that turn `fast` times or more within the `original` context stay, those that turn `slow` times or less are divided by the
-                  factor, those between are mixed in proportion"""
+                  factor; of those between a part stays that is linear in their turns, (original f / (2 pi) - slow) / (fast - slow): f times
+                  the part, and f / factor times the rest.  (Another rule in use is linear in the pair's index: its frequencies go to
+                  `RotaryTable` as they are.)"""
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be a positive even int, got {rotary_dim}")
     if scaling not in ("none", "linear", "base", "parts"):
