@@ -106,7 +106,9 @@ inline bool paged_few_rows(const PagedParams& p) {
 
 // Both kernels have a form for trees of drafted tokens, each in a source file of its own; `parents`: of the packed rows, within their sequences.
 // Of trees over 16-bit pages up to 64 rows also where they are so few, before keys so few, that the other kernel's launches and items cost more than reading
-// the keys again for each 16 rows.  The lengths are on the device: what the tables have room for stands for them.  (rows: this kernel / tcgen05, us)
+// the keys again for each 16 rows.  The lengths are on the device: what the tables have room for stands for them, so that a table much wider than
+// its sequences takes the other kernel (1 sequence of 4000, 8 kv heads of 128, 32 rows, us: room for 32K tokens 18.9, for 64K 30.9; 4 kv heads of 64,
+// 64 rows, 32K 13.8, 64K 27.1).  All figures below are of tables that fit.  (rows: this kernel / tcgen05, us)
 //   head dim 64           1 sequence of 4000, 4 kv heads  32: 15 / 27, 64: 17 / 27     8 of 8000, 8  32: 56 / 60, 48: 72 / 61     48 of 500, 8  64: 51 / 62
 //   head dim 128          1 sequence of 4000, 8 kv heads  32: 22 / 31, 64: 25 / 31     4 of 8000, 8  32: 45 / 60, 48: 65 / 60     8 of 8000, 8  32: 103 / 78
 //                         2 of 8000, 8                    48: 38 / 43, 64: 43 / 43     1 of 40000, 8  48: 69 / 71

@@ -403,7 +403,8 @@ cudaError_t launch_verify(VerifyParams a, int dtype, cudaStream_t st) {
   const VerifyKernel kernel = dtype == MOBA_DTYPE_FP32 ? pick_kernel<float>(a.draft != nullptr)
                             : dtype == MOBA_DTYPE_FP16 ? pick_kernel<__half>(a.draft != nullptr) : pick_kernel<__nv_bfloat16>(a.draft != nullptr);
   const int64_t step = (int64_t)kWarps * 32 * (dtype == MOBA_DTYPE_FP32 ? 4 : 8);   // whole vectors of all warps
-  // Blocks of a cluster: a round of them (four an SM) takes 8 us and 0.5 us for each 1000 tokens of a part.  (sequences x tokens, us with 8 / 4 / 2 / 1 blocks:
+  // Blocks of a cluster: a round of them (four an SM, as many as fit of fp32 rows with a draft and few new ones; the bits of a wide part and max_new of 1024 leave
+  // fewer, which costs time only) takes 8 us and 0.5 us for each 1000 tokens of a part.  (fp32 with a draft, sequences x tokens, us with 8 / 4 / 2 / 1 blocks:
   // 1 x 32000 10 / 12 / 16 / 23, 100 x 32000 19 / 14 / 18 / 25, 300 x 32000 44 / 32 / 29 / 31, 64 x 128000 21 / 29 / 51 / 93, 300 x 128000 86 / 83 / 107 / 124,
   // 600 x 1000 65 / 37 / 23 / 16)
   const int64_t round = 4 * (int64_t)device_info().sms;

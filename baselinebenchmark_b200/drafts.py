@@ -78,7 +78,8 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: t
     sequence, at most 1024; rows beyond are not looked at.
 
     A child with token x of row r is accepted where accept * draft[r, x] < target[r, x]; after one that is not, its siblings are tried against what is
-    left, max(target[r] - draft[r], 0) over its sum (draft = None: target[r] without x over its sum), and so on; the walk goes on from an accepted one.
+    left, max(target[r] - draft[r], 0) over its sum (draft = None: target[r] without x over 1 - target[r, x]: its rows are taken to add up to 1), and so on;
+    the walk goes on from an accepted one.
     The next token is drawn from what is left of the last row's target by `sample`.
 
     Returns (path, count, next): path int32 [batch, max_new], the accepted rows counted from the sequence's first (row 0 among them), -1 behind

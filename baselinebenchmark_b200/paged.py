@@ -336,7 +336,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     `parents` [T] int32: the packed tokens are trees of drafted ones.  parents[row] is the row of the same sequence, counted from its
     first packed one, that the token follows; what is not an earlier row (-1) is none.  A token then sees the tokens in front of
-    the packed ones, its ancestors and itself.  Rows keep their places in the pages, whatever branch they are of."""
+    the packed ones, its ancestors and itself.  Rows keep their places in the pages, whatever branch they are of.  Small trees are fastest with
+    no more columns of the table than the longest sequence needs (a view, page_table[:, :n], will do): which kernel takes them goes by its room."""
     g = _Pages(k_pages, v_pages, page_table, cu_seqlens, seq_lens, k_scales, v_scales)
     return _attention(g, q, None, k_pages, v_pages, max_new, scale, return_lse, out, parents)
 

@@ -435,7 +435,8 @@ int moba_paged_load(const moba_paged_t* p, const int32_t* cu_seqlens, const int3
  * token sees makes that token's output NaN, one in V of 16-bit pages in its own channel at least; so does an infinity in 8-bit pages, which
  * reads back as NaN.  In 16-bit pages a score of +infinity makes the output NaN, one of -infinity is a weight of 0, and an infinity in V
  * makes its channel infinite or NaN.  Any of them in a token behind, in the same tile of at most 128 positions, may do the same.
- * Over 8-bit pages a key whose weight times its V row's power of two is less than 2^-126 of the largest such product may count for nothing. */
+ * Over 8-bit pages a key whose weight times its V row's power of two is less than 2^-126 of the largest such product may count for nothing.
+ * A key whose weight is less than 2^-126 of the row's largest may count as 2^-126 of it (or as nothing). */
 int moba_paged_workspace_size(const moba_paged_t* p, size_t* bytes);
 int moba_paged_attention(const moba_paged_t* p, const void* q, const int32_t* cu_seqlens, const int32_t* seq_lens,
                          const int32_t* page_table, const void* k_pages, const void* v_pages, const uint8_t* k_scales,
@@ -445,7 +446,10 @@ int moba_paged_attention(const moba_paged_t* p, const void* q, const int32_t* cu
  * sequence b, counted from cu[b], that row i follows.  A row sees the positions in front of the sequence's packed rows, its own and those of its
  * ancestors; a parent that is not in 0 .. i-1 is none.  What is said above of infinities and NaN in a token behind holds for one of another
  * branch.  Positions of the table are by row, as in every call: the branches lie one behind
- * another in the pages.  parents == NULL: moba_paged_attention, with its workspace. */
+ * another in the pages.  parents == NULL: moba_paged_attention, with its workspace.
+ * For trees of up to 64 rows (tokens times query heads of a kv head) over 16-bit pages the kernel is chosen by the room in the table, pages_per_seq: the results
+ * are right either way, but a table much wider than its sequences may cost a third of the speed.  pages_per_seq may be fewer columns than
+ * table_stride: those that the longest sequence needs. */
 int moba_paged_tree_workspace_size(const moba_paged_t* p, size_t* bytes);
 int moba_paged_tree_attention(const moba_paged_t* p, const void* q, const int32_t* parents, const int32_t* cu_seqlens,
                               const int32_t* seq_lens, const int32_t* page_table, const void* k_pages, const void* v_pages,
